@@ -108,6 +108,22 @@ SIGNATURES = {
                                            _i32, _i32, _i32, _i32, _i32, _f32,
                                            ctypes.POINTER(_vp), _i32, _i32, _i32, _vp, _vp, _sz,
                                            _vp, ctypes.POINTER(_vp)]),
+    "dcr_paged_workspace_bytes": (_sz, [_i32] * 6),
+    "dcr_paged_attend": (_i32, [_vp, _i64, _i64, _vp, _vp, _i32] + [_i64] * 6 + [
+        _i32, _i32, _vp, _i64, _i32, _vp, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _vp, _vp, _i64,
+        _i64, _vp, _sz, _vp]),
+    "dcr_paged_append": (_i32, [_vp, _i64, _i64] * 3 + [_vp, _vp, _f32, _vp, _vp, _i32, _i32, _vp,
+                                                        _vp, _vp, _i32, _i32, _i32, _i32, _i32,
+                                                        _vp, _vp, _vp] + [_i64] * 6 + [
+        _i32, _i32, _vp, _i64, _i32, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp]),
+    "dcr_paged_evict_workspace_bytes": (_sz, [_i32] * 3),
+    "dcr_paged_evict": (_i32, [_vp, _vp, _i32] + [_i64] * 6 + [
+        _i32, _i32, _vp, _i64, _i32, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _i32, _i32,
+        _i32, _i32, _i32, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _sz, _vp]),
+    "dcr_logits_workspace_bytes": (_sz, [_i32] * 3),
+    "dcr_process_logits": (_i32, [_vp, _i64, _i32, _i32, _i32, _vp, _i32, _i64, _i32, _vp, _vp,
+                                  _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _sz,
+                                  _vp]),
     "dcr_read_device_status": (_i32, [ctypes.POINTER(_i32), _i32]),
     "dcr_binary_version": (_i32, [ctypes.POINTER(_i32)]),
 }

@@ -420,6 +420,104 @@ int dcr_silu_mul(const void* gate, const void* up, int dtype, int64_t n, void* o
 int dcr_silu_mul_packed(const void* gate_up, int dtype, int rows, int inter, void* out,
                         void* stream);
 
+/* ---- paged serving (dcr_paged_attend.cu, dcr_paged_append.cu, dcr_paged_evict.cu) ---------
+ * A decode step over a paged key-value cache. No counterpart in the reference, whose cache is
+ * one contiguous tensor per layer (dcr_attention/models/llama/compat.py:208-254).
+ *
+ * A pool is num_pages pages of page_size slots (any size >= 1); element d of slot s of KV head
+ * h in page p is pages[p * stride_p + h * stride_h + s * stride_s + d] (strides in elements,
+ * multiples of 16 bytes, for K and V separately; rows contiguous). Sequence b's slot i is in
+ * page page_table[b * table_stride + i / page_size] at i % page_size; a negative entry is a
+ * page that is not mapped. D is 64 or 128 and H any multiple of H_kv here. Nothing outside the
+ * pool is read or written whatever lengths, tables, slots, positions and tokens hold on the
+ * device: an entry out of range is skipped and sets DCR_ERR_DEVICE_INDEX in the device status
+ * (a length beyond max_pages * page_size is taken as that, a negative one as 0).
+ * Attended slots must be finite for finite results: slots past the length, before the window
+ * or in unmapped pages may hold anything. */
+
+/* Bytes of workspace dcr_paged_attend needs; it need not be initialised. 0: invalid shape. */
+size_t dcr_paged_workspace_bytes(int B, int H, int H_kv, int D, int max_slots, int with_weights);
+
+/* O [B, H, D] = softmax(scale * q . K) V over the lengths[b] slots of each sequence (the last
+ * `window` of them when window > 0), for one new token per sequence: q [B, H, D] with strides.
+ * fp32 softmax statistics and sums, one rounding. lse [B, H] (or NULL) receives the natural
+ * log of the softmax denominators. weights (or NULL; fp32, weights[b * w_stride_b +
+ * h_kv * w_stride_h + slot], max_pages * page_size slots) is increased by every slot's
+ * softmax weight, summed over the KV head's query heads in a fixed order. A row with no valid
+ * slot gets O = 0 and lse = -inf; a score of -inf counts as a masked slot. */
+int dcr_paged_attend(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k_pages,
+                     const void* v_pages, int dtype, int64_t k_stride_p, int64_t k_stride_h,
+                     int64_t k_stride_s, int64_t v_stride_p, int64_t v_stride_h,
+                     int64_t v_stride_s, int num_pages, int page_size, const int32_t* page_table,
+                     int64_t table_stride, int max_pages, const int32_t* lengths, int B, int H,
+                     int H_kv, int D, float scale, int window, void* o, float* lse,
+                     float* weights, int64_t w_stride_b, int64_t w_stride_h, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* For T tokens: q_out [T, H, D] and the pages' new key rows get rotate(norm(x)), with norm(x) =
+ * x * rsqrt(mean(x^2) + eps) * weight (a NULL weight: x itself) and rotate as HF
+ * apply_rotary_pos_emb with row positions[t] of cos and sin [n_pos, D] (dtype or fp32), in
+ * fp32, rounded once; the value rows are copied. q [T, H, D], k and v [T, H_kv, D] have token
+ * and head strides (multiples of 16 bytes). Token t's key and value go to slot slots[t] of
+ * sequence seq[t] (seq NULL: sequence t) of the n_seq rows of page_table; a negative slot
+ * means nowhere. weights / pos (or NULL) get 0 / positions[t] at that slot for every KV head.
+ * No two tokens may name the same slot. A position outside [0, n_pos) gives a zero query and
+ * appends nothing (device status). */
+int dcr_paged_append(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+                     int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
+                     int64_t v_stride_h, const void* q_weight, const void* k_weight, float eps,
+                     const void* cos, const void* sin, int table_dtype, int n_pos,
+                     const int32_t* positions, const int32_t* seq, const int32_t* slots, int dtype,
+                     int T, int H, int H_kv, int D, void* q_out, void* k_pages, void* v_pages,
+                     int64_t kp_stride_p, int64_t kp_stride_h, int64_t kp_stride_s,
+                     int64_t vp_stride_p, int64_t vp_stride_h, int64_t vp_stride_s, int num_pages,
+                     int page_size, const int32_t* page_table, int64_t table_stride, int n_seq,
+                     int max_pages, float* weights, int64_t w_stride_b, int64_t w_stride_h,
+                     int32_t* pos, int64_t p_stride_b, int64_t p_stride_h, void* stream);
+
+size_t dcr_paged_evict_workspace_bytes(int B, int H_kv, int budget);
+
+/* Per sequence and KV head, keeps `budget` of the lengths[b] slots: the protected ones first
+ * (pos < sinks, or pos >= seen[b] - recent), then those of the largest weight, equal ones by
+ * the lower slot (-0 equals +0, NaN ranks highest). Kept slots at or past the budget move, in
+ * slot order, into the evicted slots before it, K and V rows included, in place. src_out
+ * [B, H_kv, budget] int32: the slot each one's row came from (its own for a row that stayed,
+ * -1 past the new length). weights_out and pos_out (first `budget` slots; other tensors than
+ * weights and pos) receive the kept slots' entries, 0 and -1 past the new length; lengths_out
+ * [B] = min(lengths, budget) (another tensor than lengths). */
+int dcr_paged_evict(void* k_pages, void* v_pages, int dtype, int64_t k_stride_p,
+                    int64_t k_stride_h, int64_t k_stride_s, int64_t v_stride_p,
+                    int64_t v_stride_h, int64_t v_stride_s, int num_pages, int page_size,
+                    const int32_t* page_table, int64_t table_stride, int max_pages,
+                    const int32_t* lengths, const float* weights, int64_t w_stride_b,
+                    int64_t w_stride_h, const int32_t* pos, int64_t p_stride_b,
+                    int64_t p_stride_h, const int32_t* seen, int B, int H_kv, int D, int budget,
+                    int sinks, int recent, int32_t* src_out, float* weights_out,
+                    int64_t wo_stride_b, int64_t wo_stride_h, int32_t* pos_out,
+                    int64_t po_stride_b, int64_t po_stride_h, int32_t* lengths_out,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- logits of a decode step (dcr_logits.cu) ------------------------------------------ */
+size_t dcr_logits_workspace_bytes(int B, int V, int L);
+
+/* Per row of logits [B, V], in fp32 and in this order, rounded once to dtype: x > 0 ?
+ * x / repetition : x * repetition for tokens in the row's history; x - count * frequency and
+ * x - presence for those that occur after its prompt; x + bias; -inf where `allowed` (32
+ * tokens a word, token t in bit t % 32 of word t / 32, 1 = allowed) has a clear bit.
+ * next_token [B]: the lowest index of the largest returned value among the allowed tokens
+ * (NaN is the largest), -1 where none is allowed. tokens [B, L] int32 or int64 (negative:
+ * padding; >= V: skipped, device status), of which a row's first token_lengths[b] count (NULL:
+ * L) and of these the first prompt_lengths[b] are its prompt (NULL: 0). repetition, presence,
+ * frequency [B], bias (row stride 0: one for all rows) and allowed may be NULL. out may be
+ * logits itself (same strides). */
+int dcr_process_logits(const void* logits, int64_t l_stride_b, int dtype, int B, int V,
+                       const void* tokens, int tokens_are_int64, int64_t t_stride_b, int L,
+                       const int32_t* token_lengths, const int32_t* prompt_lengths,
+                       const float* repetition, const float* presence, const float* frequency,
+                       const float* bias, int64_t bias_stride_b, const uint32_t* allowed,
+                       int64_t a_stride_b, void* out, int64_t o_stride_b, int64_t* next_token,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif
