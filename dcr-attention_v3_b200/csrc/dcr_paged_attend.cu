@@ -9,17 +9,51 @@
 // (dcr_attention/models/llama/attention.py:436); pages, windows and weights have no
 // counterpart there.
 //
-// One CTA per (sequence, KV head), a warp per slot: online softmax in base 2, sums in fp32,
-// the warps' states merged in shared memory, one rounding to the output type.
+// Bound: the K and V rows, read once (2 * D * element bytes per slot and KV head). The
+// arithmetic is 4 * G * D per row, a few per cent of the matrix units, so what matters is how
+// many bytes are in flight and that no SM runs dry.
+//
+// Split. A unit is (sequence, KV head, block of HB = 8 or 16 of its query heads); its slots
+// are cut into tiles of R slots on multiples of R. All tiles of all units, in order, are one
+// line that the CTAs share out evenly, and each CTA's share its warps: lengths on the device
+// may be as unequal as they like. A warp walks its share alone, without barriers: it loads
+// rows with 16-byte cp.async into a ring of its own (NH half tiles, K and V in turn; slots
+// that are not valid are zero-filled, never read), and keeps the running maximum, sum and
+// output (m, l, o) of the unit it is in. Where a unit lies wholly inside a warp's share the
+// warp writes O itself. Otherwise it leaves a piece (m, l, o); the CTA folds its pieces, and
+// units that span CTAs are folded from the CTAs' partials in the workspace by a second kernel
+// (launched as a programmatic dependent), in a fixed order. Weights take a third kernel: the
+// first leaves the scores in the workspace, which costs 8 * G bytes a slot instead of reading
+// K again (2 * D bytes).
+//
+// 16-bit rows go through the tensor cores (mma.sync m16n8k16, A = the query heads as rows): one
+// token has at most 16 rows a KV head, so the tile of a tcgen05.mma (64 or 128 rows) would be
+// mostly padding and its round trip through TMEM longer than the work. P enters the second
+// product as two 16-bit parts (hi = rn(p), lo = rn(p - hi)), which keeps 16 bits of every
+// weight; with HB = 8 the parts are the two row halves of one MMA. fp32 rows use fp32 FMAs.
 #include <math.h>
+
+#include <type_traits>
 
 #include "dcr_internal.h"
 #include "dcr_paged.cuh"
 
 namespace dcr {
 
-constexpr int kPaThreads = 256;
-constexpr int kPaWarps = kPaThreads / 32;
+constexpr int kPaWarps = 8;
+constexpr int kPaThreads = kPaWarps * 32;
+// Fewest tiles a CTA takes: below it, spreading further costs more in folding than it gains.
+constexpr int kPaMinTiles = 8;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// What a CTA's first open unit needs of the fold kernel: the unit and the last CTA of it.
+struct PaRecord {
+  int32_t b;
+  int32_t u;     // -1: nothing begins in this CTA that ends in a later one
+  int32_t last;
+  int32_t pad;
+};
 
 struct PagedAttendParams {
   PagePool c;
@@ -27,101 +61,906 @@ struct PagedAttendParams {
   int64_t qsb, qsh;
   const int32_t* lengths;
   int B, H, H_kv, G;
-  float scale2;  // scale * log2(e)
+  int units;      // per sequence: H_kv * blocks of query heads
+  int hblocks;    // blocks of query heads per KV head
+  float scale2;   // scale * log2(e)
   int window;
+  int page16;     // page_size is a multiple of R: a tile lies in one page
   void* o;        // [B][H][D]
-  float* lse;     // [B][H] or null
-  float* weights; // [B][H_kv][...] or null
-  int64_t wsb, wsh;
+  float* lse;     // [B][H] natural log, or null
+  float2* stats;  // [B][H] (maximum in base 2, 1 / sum), with scores
+  float* part;    // [CTAs][2][HB][D + 2]: o, m, l of the open units
+  PaRecord* rec;  // [CTAs]
+  float* scores;  // [B][H][s_stride] base-2 scores, or null
+  int64_t s_stride;
 };
 
-template <typename T>
-__device__ __forceinline__ float pa_elem(const void* p, int64_t i) {
-  if constexpr (sizeof(T) == 4)
-    return static_cast<const float*>(p)[i];
-  else
-    return ElemTraits<T>::widen1(static_cast<const uint16_t*>(p)[i]);
+// Geometry of a variant: T's element bytes, D and the rows of a head block.
+template <typename T, int D, int HB>
+struct PaShape {
+  static constexpr bool k16 = sizeof(T) == 2;
+  static constexpr int R = k16 ? 16 : 8;                  // slots per tile
+  static constexpr int kRow = D * static_cast<int>(sizeof(T));
+  static constexpr int kChunks = kRow / 16;               // 16-byte chunks per row: 8, 16 or 32
+  static constexpr int kHalf = R * kRow;                  // bytes of a K or V half tile
+  static constexpr int kRowsPer = 32 / kChunks;           // rows a warp copies per instruction
+  static constexpr int kCopies = R / kRowsPer;
+  static constexpr int kPiece = HB * (D + 2) * 4;         // a piece (o, m, l)
+  static constexpr int kQ = k16 ? 0 : HB * D * 4;         // fp32: the queries, read as broadcasts
+  static constexpr int kP = k16 ? 0 : HB * R * 4;         // fp32: the tile's weights
+  // ring: an odd number of half tiles (the last half prefetched is of the kind just consumed)
+  static constexpr int kFree = (227 * 1024 - 1024) / kPaWarps - kPiece - kQ - kP - 64;
+  static constexpr int NHraw = kFree / kHalf;
+  static constexpr int NHodd = (NHraw % 2) ? NHraw : NHraw - 1;
+  static constexpr int NH = NHodd > 13 ? 13 : NHodd;
+  static constexpr int kWarpBytes = NH * kHalf + kPiece + kQ + kP + 64;
+  static constexpr int kSmem = kWarpBytes * kPaWarps;
+  static_assert(NH >= 3, "the ring holds at least K, V and K");
+  static_assert(NH * kHalf >= kPiece, "the ring is reused for the last piece");
+};
+
+__device__ __forceinline__ float pa_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kPaThreads) paged_attend_kernel(const PagedAttendParams p) {
-  constexpr int E = D / 32;
-  __shared__ float m_s[kPaWarps], l_s[kPaWarps], o_s[kPaWarps][D];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int b = blockIdx.y, hk = blockIdx.x;
-  const int n = checked_length(p.c, p.lengths[b]);
-  const int lo = p.window > 0 && n > p.window ? n - p.window : 0;
-  // z (base 2) of one slot for the query held in q; false if the slot's page is not mapped
-  auto score = [&](const float (&q)[E], int i, int& pg, int& in) {
-    const uint32_t pi = p.c.page.div(i);
-    pg = page_of(p.c, b, pi);
-    in = i - pi * p.c.page.d;
-    if (pg < 0) return -INFINITY;
-    const int64_t at = pg * p.c.ksp + hk * p.c.ksh + in * p.c.ksr;
-    float s = 0.0f;
+// A row's statistics: lse = (m + log2 l) ln 2, and what the weights need. Weights are
+// exp2(z - m) / l: the difference of two near scores is exact, where lse would be rounded once.
+__device__ __forceinline__ void pa_store_stats(const PagedAttendParams& p, int64_t row, float m,
+                                               float l) {
+  if (p.lse != nullptr) p.lse[row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+  if (p.stats != nullptr) p.stats[row] = l == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(m, 1.0f / l);
+}
+
+template <typename T>
+__device__ __forceinline__ void pa_store2(T* dst, float a, float b) {
+  if constexpr (std::is_same<T, __half>::value)
+    *reinterpret_cast<__half2*>(dst) = __floats2half2_rn(a, b);
+  else
+    *reinterpret_cast<__nv_bfloat162*>(dst) = __floats2bfloat162_rn(a, b);
+}
+
+// Tiles of sequence b: its length, first valid slot and tile range.
+template <int R>
+__device__ __forceinline__ void pa_sequence(const PagedAttendParams& p, int b, int& len, int& lo,
+                                            int& t_lo, int& t_hi) {
+  len = checked_length(p.c, __ldg(p.lengths + b));
+  lo = p.window > 0 && len > p.window ? len - p.window : 0;
+  t_lo = lo / R;
+  t_hi = (len + R - 1) / R;
+}
+
+// A place on the line of tiles.
+struct PaCursor {
+  int b, u, t, t_lo, t_hi, len, lo;
+};
+
+template <int R>
+__device__ __forceinline__ void pa_next(const PagedAttendParams& p, PaCursor& c) {
+  if (++c.t < c.t_hi) return;
+  if (++c.u == p.units) {
+    c.u = 0;
+    do {
+      if (++c.b >= p.B) return;  // past the end: the caller's count stops here
+      pa_sequence<R>(p, c.b, c.len, c.lo, c.t_lo, c.t_hi);
+    } while (c.t_lo >= c.t_hi);
+  }
+  c.t = c.t_lo;
+}
+
+// Sum over the sequences of their tiles (all lanes get it).
+template <int R>
+__device__ __forceinline__ int64_t pa_total(const PagedAttendParams& p) {
+  const int lane = threadIdx.x & 31;
+  int64_t n = 0;
+  for (int b = lane; b < p.B; b += 32) {
+    int len, lo, t_lo, t_hi;
+    pa_sequence<R>(p, b, len, lo, t_lo, t_hi);
+    n += t_hi - t_lo;
+  }
 #pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(q[e], pa_elem<T>(p.c.k, at + lane + 32 * e), s);
+  for (int o = 16; o >= 1; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  return n * p.units;
+}
+
+// The cursor at place s (< total) of the line.
+template <int R>
+__device__ __forceinline__ PaCursor pa_seek(const PagedAttendParams& p, int64_t s) {
+  const int lane = threadIdx.x & 31;
+  int64_t before = 0;
+  for (int b0 = 0;; b0 += 32) {
+    const int b = b0 + lane;
+    int n = 0;
+    if (b < p.B) {
+      int len, lo, t_lo, t_hi;
+      pa_sequence<R>(p, b, len, lo, t_lo, t_hi);
+      n = t_hi - t_lo;
+    }
+    int64_t incl = n;
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    return s * p.scale2;
-  };
-  for (int pass = 0; pass < (p.weights != nullptr ? 2 : 1); ++pass) {
-    for (int g = 0; g < p.G; ++g) {
-      const int h = hk * p.G + g;
-      float q[E], o[E];
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, s < before + incl * p.units);
+    if (hit != 0 || b0 + 32 >= p.B) {
+      const int src = hit != 0 ? __ffs(hit) - 1 : 31;
+      PaCursor c;
+      c.b = b0 + src < p.B ? b0 + src : p.B - 1;
+      pa_sequence<R>(p, c.b, c.len, c.lo, c.t_lo, c.t_hi);
+      const int64_t base = before + __shfl_sync(0xffffffffu, incl - n, src) * p.units;
+      const int nt = c.t_hi - c.t_lo;
+      const int64_t off = s - base;
+      c.u = nt > 0 ? static_cast<int>(off / nt) : 0;
+      c.t = c.t_lo + static_cast<int>(off - static_cast<int64_t>(c.u) * nt);
+      return c;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31) * p.units;
+  }
+}
+
+// The copies of one tile: K's then V's, from the same rows.
+template <typename T, int D, int HB>
+struct PaLoader {
+  using S = PaShape<T, D, HB>;
+  int64_t row_v[S::kCopies];  // V offsets (elements) of the rows this lane copies
+  uint32_t ok;                // bit i: this lane's i-th row is valid
+
+  // Issues the tile's K half into `dst` and returns its mask of valid slots.
+  __device__ __forceinline__ uint32_t keys(const PagedAttendParams& p, const PaCursor& c,
+                                           uint8_t* dst) {
+    const int lane = threadIdx.x & 31;
+    const int ch = lane % S::kChunks, r0 = lane / S::kChunks;
+    const int hk = c.u / p.hblocks;
+    const int slot0 = c.t * S::R;
+    const int from = c.lo > slot0 ? c.lo - slot0 : 0;
+    const int to = c.len - slot0 < S::R ? c.len - slot0 : S::R;
+    uint32_t mask = (0xffffffffu >> (32 - to)) & (0xffffffffu << from);
+    const T* kbase = static_cast<const T*>(p.c.k) + hk * p.c.ksh + ch * (16 / sizeof(T));
+    const int64_t vbase = hk * p.c.vsh + ch * (16 / static_cast<int>(sizeof(T)));
+    ok = 0;
+    if (p.page16) {
+      const uint32_t pi = p.c.page.div(slot0);
+      const int pg = page_of(p.c, c.b, pi);
+      if (pg < 0) mask = 0;
+      const int in = slot0 - static_cast<int>(pi * p.c.page.d);
+      const int64_t pgk = pg < 0 ? 0 : pg * p.c.ksp, pgv = pg < 0 ? 0 : pg * p.c.vsp;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        q[e] = pa_elem<T>(p.q, b * p.qsb + h * p.qsh + lane + 32 * e);
-        o[e] = 0.0f;
+      for (int i = 0; i < S::kCopies; ++i) {
+        const int r = r0 + i * S::kRowsPer;
+        const bool v = (mask >> r) & 1u;
+        row_v[i] = v ? vbase + pgv + (in + r) * p.c.vsr : 0;
+        ok |= static_cast<uint32_t>(v) << i;
+        copy(dst, r, ch, v ? kbase + pgk + (in + r) * p.c.ksr : static_cast<const T*>(p.c.k), v);
       }
-      float m = -INFINITY, l = 0.0f;
-      const float lse2 = pass == 1 ? p.lse[static_cast<int64_t>(b) * p.H + h] : 0.0f;
-      for (int i = lo + warp; i < n; i += kPaWarps) {
-        int pg, in;
-        const float z = score(q, i, pg, in);
-        if (z == -INFINITY) continue;
-        if (pass == 1) {  // the same warp adds every head's share of its slots, in head order
-          if (lane == 0)
-            p.weights[b * p.wsb + hk * p.wsh + i] += exp2f(z - lse2 * 1.4426950408889634f);
-          continue;
+      return mask;
+    }
+    uint32_t held = 0;
+#pragma unroll
+    for (int i = 0; i < S::kCopies; ++i) {
+      const int r = r0 + i * S::kRowsPer;
+      bool v = (mask >> r) & 1u;
+      int64_t pgk = 0, pgv = 0;
+      int in = 0;
+      if (v) {
+        const uint32_t pi = p.c.page.div(slot0 + r);
+        const int pg = page_of(p.c, c.b, pi);
+        in = slot0 + r - static_cast<int>(pi * p.c.page.d);
+        v = pg >= 0;
+        pgk = v ? pg * p.c.ksp : 0;
+        pgv = v ? pg * p.c.vsp : 0;
+      }
+      row_v[i] = v ? vbase + pgv + in * p.c.vsr : 0;
+      ok |= static_cast<uint32_t>(v) << i;
+      copy(dst, r, ch, v ? kbase + pgk + in * p.c.ksr : static_cast<const T*>(p.c.k), v);
+      const unsigned bal = __ballot_sync(0xffffffffu, v);
+#pragma unroll
+      for (int j = 0; j < S::kRowsPer; ++j)
+        held |= ((bal >> (j * S::kChunks)) & 1u) << (i * S::kRowsPer + j);
+    }
+    return held;
+  }
+
+  __device__ __forceinline__ void values(const PagedAttendParams& p, uint8_t* dst) const {
+    const int lane = threadIdx.x & 31;
+    const int ch = lane % S::kChunks, r0 = lane / S::kChunks;
+#pragma unroll
+    for (int i = 0; i < S::kCopies; ++i)
+      copy(dst, r0 + i * S::kRowsPer, ch, static_cast<const T*>(p.c.v) + row_v[i], (ok >> i) & 1u);
+  }
+
+  // Chunk ch of row r: 16-bit rows by ldmatrix (8 rows of one chunk column at once), fp32 rows
+  // by 16-byte reads of two rows' quarters; the swizzles keep both free of bank conflicts.
+  __device__ __forceinline__ static uint32_t at(int r, int ch) {
+    const int sw = S::k16 ? (ch ^ (r & 7)) : (ch ^ ((r & 1) << 2));
+    return static_cast<uint32_t>(r * S::kRow + sw * 16);
+  }
+  __device__ __forceinline__ static void copy(uint8_t* dst, int r, int ch, const T* src, bool v) {
+    cp_async_16(dst + at(r, ch), src, v ? 16u : 0u);
+  }
+};
+
+// The running state of the unit a warp is in. 16-bit: row g of the head block is the MMA row
+// lane / 4 (and lane / 4 + 8 when HB = 16), and o holds its dims 8 j + 2 (lane % 4) + {0, 1}.
+template <typename T, int D, int HB>
+struct PaState16 {
+  using S = PaShape<T, D, HB>;
+  static constexpr int M = HB / 8;  // row halves in use
+  uint32_t qf[D / 16][2 * M];
+  float o[D / 8][4];
+  float m[M], l[M];
+  uint32_t ph[2][M], pl[2][M];  // the tile's weights, hi and lo parts, per 8 slots
+
+  __device__ __forceinline__ void begin(const PagedAttendParams& p, const PaCursor& c, uint8_t*) {
+    const int lane = threadIdx.x & 31;
+    const int hk = c.u / p.hblocks, h0 = (c.u - hk * p.hblocks) * HB;
+    const uint16_t* q = static_cast<const uint16_t*>(p.q) + c.b * p.qsb;
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      const int g = h0 + lane / 4 + 8 * i;
+      const bool in = g < p.G;
+      const uint16_t* row = q + (hk * p.G + (in ? g : 0)) * p.qsh + 2 * (lane % 4);
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        qf[ks][i] = in ? *reinterpret_cast<const uint32_t*>(row + ks * 16) : 0u;
+        qf[ks][M + i] = in ? *reinterpret_cast<const uint32_t*>(row + ks * 16 + 8) : 0u;
+      }
+      m[i] = -INFINITY;
+      l[i] = 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
+  }
+
+  __device__ __forceinline__ void scores(const PagedAttendParams& p, const PaCursor& c,
+                                         const uint8_t* tile, uint32_t mask, uint8_t*) {
+    const int lane = threadIdx.x & 31;
+    float z[2][4] = {};
+    const int mat = lane >> 3, r8 = lane & 7;
+    const int row = (mat >> 1) * 8 + r8;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      uint32_t k0, k1, k2, k3;
+      ldsm_x4(smem_u32(tile + PaLoader<T, D, HB>::at(row, 2 * ks + (mat & 1))), k0, k1, k2, k3);
+      const uint32_t a[4] = {qf[ks][0], M == 2 ? qf[ks][M - 1] : 0u, qf[ks][M],
+                             M == 2 ? qf[ks][2 * M - 1] : 0u};
+      UnionMma<T>::mma(z[0], a, k0, k1);
+      UnionMma<T>::mma(z[1], a, k2, k3);
+    }
+    const int pos = 2 * (lane & 3);
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      float s[2][2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          s[j][e] = z[j][2 * i + e] * p.scale2;
+          if (mask != 0xffffu && !((mask >> (8 * j + pos + e)) & 1u)) s[j][e] = -INFINITY;
         }
-        const float mn = fmaxf(m, z);
-        const float a = m == -INFINITY ? 0.0f : exp2f(m - mn);
-        const float w = exp2f(z - mn);
-        m = mn;
-        l = fmaf(l, a, w);
-        const int64_t at = pg * p.c.vsp + hk * p.c.vsh + in * p.c.vsr;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = fmaf(o[e], a, w * pa_elem<T>(p.c.v, at + lane + 32 * e));
-      }
-      if (pass == 1) continue;
-      if (lane == 0) {
-        m_s[warp] = m;
-        l_s[warp] = l;
-      }
-#pragma unroll
-      for (int e = 0; e < E; ++e) o_s[warp][lane + 32 * e] = o[e];
-      __syncthreads();
-      if (warp == 0) {
-        float M = -INFINITY, L = 0.0f, acc[E] = {};
-        for (int w = 0; w < kPaWarps; ++w) M = fmaxf(M, m_s[w]);
-        for (int w = 0; w < kPaWarps; ++w) {
-          const float a = m_s[w] == -INFINITY ? 0.0f : exp2f(m_s[w] - M);
-          L = fmaf(a, l_s[w], L);
-#pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] = fmaf(a, o_s[w][lane + 32 * e], acc[e]);
+      if (p.scores != nullptr) {
+        const int hk = c.u / p.hblocks;
+        const int g = (c.u - hk * p.hblocks) * HB + (lane >> 2) + 8 * i;
+        if (g < p.G) {
+          float* dst = p.scores + (static_cast<int64_t>(c.b) * p.H + hk * p.G + g) * p.s_stride +
+                       c.t * S::R + pos;
+          *reinterpret_cast<float2*>(dst) = make_float2(s[0][0], s[0][1]);
+          *reinterpret_cast<float2*>(dst + 8) = make_float2(s[1][0], s[1][1]);
         }
-        const int64_t row = static_cast<int64_t>(b) * p.H + h;
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          ElemTraits<T>::store(static_cast<T*>(p.o) + row * D, lane + 32 * e,
-                               L > 0.0f || L != L ? acc[e] / L : 0.0f);
-        if (lane == 0 && p.lse != nullptr)
-          p.lse[row] = M == -INFINITY ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
       }
-      __syncthreads();
+      // The maximum is raised only when some score is 2^8 above it: weights stay below 2^8,
+      // and most tiles need no rescaling. A NaN score raises nothing and spreads by itself.
+      float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+      if (__any_sync(0xffffffffu, top > m[i] + 8.0f)) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float mn = fmaxf(m[i], top);
+        const float a = m[i] == -INFINITY ? 0.0f : pa_exp2(m[i] - mn);
+        m[i] = mn;
+        l[i] *= a;
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) {
+          o[j][2 * i] *= a;
+          o[j][2 * i + 1] *= a;
+          if (M == 1) {
+            o[j][2] *= a;
+            o[j][3] *= a;
+          }
+        }
+      }
+      const float ms = m[i] == -INFINITY ? 0.0f : m[i];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float w0 = pa_exp2(s[j][0] - ms), w1 = pa_exp2(s[j][1] - ms);
+        l[i] += w0 + w1;
+        UnionMma<T>::split(w0, w1, ph[j][i], pl[j][i]);
+      }
     }
   }
+
+  __device__ __forceinline__ void values(const uint8_t* tile, uint32_t, uint8_t*) {
+    const int lane = threadIdx.x & 31;
+    const int mat = lane >> 3, r8 = lane & 7;
+    const int row = (mat & 1) * 8 + r8;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+      uint32_t v0, v1, v2, v3;
+      ldsm_x4_t(smem_u32(tile + PaLoader<T, D, HB>::at(row, 2 * j + (mat >> 1))), v0, v1, v2, v3);
+      if constexpr (M == 1) {
+        const uint32_t a[4] = {ph[0][0], pl[0][0], ph[1][0], pl[1][0]};
+        UnionMma<T>::mma(o[2 * j], a, v0, v1);
+        UnionMma<T>::mma(o[2 * j + 1], a, v2, v3);
+      } else {
+        const uint32_t ah[4] = {ph[0][0], ph[0][M - 1], ph[1][0], ph[1][M - 1]};
+        const uint32_t al[4] = {pl[0][0], pl[0][M - 1], pl[1][0], pl[1][M - 1]};
+        UnionMma<T>::mma(o[2 * j], ah, v0, v1);
+        UnionMma<T>::mma(o[2 * j + 1], ah, v2, v3);
+        UnionMma<T>::mma(o[2 * j], al, v0, v1);
+        UnionMma<T>::mma(o[2 * j + 1], al, v2, v3);
+      }
+    }
+  }
+
+  // The unit's (or share's) end: sums over the lanes of a row.
+  __device__ __forceinline__ void close() {
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    }
+    if (M == 1) {
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j) {
+        o[j][0] += o[j][2];
+        o[j][1] += o[j][3];
+      }
+    }
+  }
+
+  __device__ __forceinline__ void write(const PagedAttendParams& p, const PaCursor& c) const {
+    const int lane = threadIdx.x & 31;
+    const int hk = c.u / p.hblocks;
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      const int g = (c.u - hk * p.hblocks) * HB + (lane >> 2) + 8 * i;
+      if (g >= p.G) continue;
+      const int64_t row = static_cast<int64_t>(c.b) * p.H + hk * p.G + g;
+      const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
+      T* out = static_cast<T*>(p.o) + row * D + 2 * (lane & 3);
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j)
+        pa_store2(out + 8 * j, o[j][2 * i] * inv, o[j][2 * i + 1] * inv);
+      if ((lane & 3) == 0) pa_store_stats(p, row, m[i], l[i]);
+    }
+  }
+
+  __device__ __forceinline__ void piece(float* dst) const {  // [HB][D + 2]
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      float* r = dst + ((lane >> 2) + 8 * i) * (D + 2);
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j)
+        *reinterpret_cast<float2*>(r + 8 * j + 2 * (lane & 3)) =
+            make_float2(o[j][2 * i], o[j][2 * i + 1]);
+      if ((lane & 3) == 0) {
+        r[D] = m[i];
+        r[D + 1] = l[i];
+      }
+    }
+  }
+};
+
+// fp32 rows. Scores: lane = (slot lane / 4, quarter lane % 4), which takes every fourth chunk
+// of the row; the four partial sums meet by shuffles. Values: a lane holds D / 32 dims of all
+// HB rows. m and l are kept by every lane (all lanes agree).
+template <typename T, int D, int HB>
+struct PaState32 {
+  using S = PaShape<T, D, HB>;
+  static constexpr int E = D / 32;
+  float o[HB][E];
+  float m[HB], l[HB];
+  int rows;
+
+  __device__ __forceinline__ static float* q_of(uint8_t* own) { return reinterpret_cast<float*>(own); }
+  __device__ __forceinline__ static float* p_of(uint8_t* own) {
+    return reinterpret_cast<float*>(own + S::kQ);
+  }
+
+  __device__ __forceinline__ void begin(const PagedAttendParams& p, const PaCursor& c, uint8_t* own) {
+    const int lane = threadIdx.x & 31;
+    const int hk = c.u / p.hblocks, h0 = (c.u - hk * p.hblocks) * HB;
+    rows = p.G - h0 < HB ? p.G - h0 : HB;
+    const float* q = static_cast<const float*>(p.q) + c.b * p.qsb + (hk * p.G + h0) * p.qsh;
+    __syncwarp();
+    for (int g = 0; g < rows; ++g)
+#pragma unroll
+      for (int e = 0; e < E; ++e) q_of(own)[g * D + lane + 32 * e] = q[g * p.qsh + lane + 32 * e];
+    __syncwarp();
+#pragma unroll
+    for (int g = 0; g < HB; ++g) {
+      m[g] = -INFINITY;
+      l[g] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[g][e] = 0.0f;
+    }
+  }
+
+  __device__ __forceinline__ void scores(const PagedAttendParams& p, const PaCursor& c,
+                                         const uint8_t* tile, uint32_t mask, uint8_t* own) {
+    const int lane = threadIdx.x & 31;
+    const int r = lane >> 2, qd = lane & 3;
+    float4 k[S::kChunks / 4];
+#pragma unroll
+    for (int i = 0; i < S::kChunks / 4; ++i)
+      k[i] = *reinterpret_cast<const float4*>(tile + PaLoader<T, D, HB>::at(r, 4 * i + qd));
+    const bool valid = (mask >> r) & 1u;
+    const int hk = c.u / p.hblocks;
+    const int64_t row0 = static_cast<int64_t>(c.b) * p.H + hk * p.G + (c.u - hk * p.hblocks) * HB;
+#pragma unroll
+    for (int g = 0; g < HB; ++g) {
+      if (g >= rows) break;
+      const float4* q = reinterpret_cast<const float4*>(q_of(own) + g * D);
+      float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+      for (int i = 0; i < S::kChunks / 4; ++i) {
+        const float4 x = q[4 * i + qd];
+        s0 = fmaf(k[i].x, x.x, s0);
+        s1 = fmaf(k[i].y, x.y, s1);
+        s0 = fmaf(k[i].z, x.z, s0);
+        s1 = fmaf(k[i].w, x.w, s1);
+      }
+      float s = s0 + s1;
+      s += __shfl_xor_sync(0xffffffffu, s, 1);
+      s += __shfl_xor_sync(0xffffffffu, s, 2);
+      s = valid ? s * p.scale2 : -INFINITY;
+      if (p.scores != nullptr && qd == 0) p.scores[(row0 + g) * p.s_stride + c.t * S::R + r] = s;
+      if (__any_sync(0xffffffffu, s > m[g] + 8.0f)) {
+        float top = s;
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        const float mn = fmaxf(m[g], top);
+        const float a = m[g] == -INFINITY ? 0.0f : pa_exp2(m[g] - mn);
+        m[g] = mn;
+        l[g] *= a;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[g][e] *= a;
+      }
+      const float w = pa_exp2(s - (m[g] == -INFINITY ? 0.0f : m[g]));
+      l[g] += qd == 0 ? w : 0.0f;
+      if (qd == 0) p_of(own)[g * S::R + r] = w;
+    }
+    __syncwarp();
+  }
+
+  __device__ __forceinline__ void values(const uint8_t* tile, uint32_t, uint8_t* own) {
+    const int lane = threadIdx.x & 31;
+    float v[S::R][E];
+#pragma unroll
+    for (int r = 0; r < S::R; ++r) {
+      const uint8_t* at = tile + PaLoader<T, D, HB>::at(r, lane * E / 4) + (lane * E % 4) * 4;
+      if constexpr (E == 2) {
+        const float2 x = *reinterpret_cast<const float2*>(at);
+        v[r][0] = x.x;
+        v[r][1] = x.y;
+      } else {
+        const float4 x = *reinterpret_cast<const float4*>(at);
+        v[r][0] = x.x;
+        v[r][1] = x.y;
+        v[r][2] = x.z;
+        v[r][3] = x.w;
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < HB; ++g) {
+      if (g >= rows) break;
+      const float4* w = reinterpret_cast<const float4*>(p_of(own) + g * S::R);
+#pragma unroll
+      for (int i = 0; i < S::R / 4; ++i) {
+        const float4 x = w[i];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          o[g][e] = fmaf(x.x, v[4 * i][e], o[g][e]);
+          o[g][e] = fmaf(x.y, v[4 * i + 1][e], o[g][e]);
+          o[g][e] = fmaf(x.z, v[4 * i + 2][e], o[g][e]);
+          o[g][e] = fmaf(x.w, v[4 * i + 3][e], o[g][e]);
+        }
+      }
+    }
+    __syncwarp();
+  }
+
+  __device__ __forceinline__ void close() {
+#pragma unroll
+    for (int g = 0; g < HB; ++g)
+#pragma unroll
+      for (int off = 16; off >= 1; off >>= 1) l[g] += __shfl_xor_sync(0xffffffffu, l[g], off);
+  }
+
+  __device__ __forceinline__ void write(const PagedAttendParams& p, const PaCursor& c) const {
+    const int lane = threadIdx.x & 31;
+    const int hk = c.u / p.hblocks;
+    const int64_t row0 = static_cast<int64_t>(c.b) * p.H + hk * p.G + (c.u - hk * p.hblocks) * HB;
+#pragma unroll
+    for (int g = 0; g < HB; ++g) {
+      if (g >= rows) break;
+      float* out = static_cast<float*>(p.o) + (row0 + g) * D + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) out[e] = l[g] == 0.0f ? 0.0f : o[g][e] / l[g];
+      if (lane == 0) pa_store_stats(p, row0 + g, m[g], l[g]);
+    }
+  }
+
+  __device__ __forceinline__ void piece(float* dst) const {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int g = 0; g < HB; ++g) {
+      float* r = dst + g * (D + 2);
+#pragma unroll
+      for (int e = 0; e < E; ++e) r[lane * E + e] = o[g][e];
+      if (lane == 0) {
+        r[D] = m[g];
+        r[D + 1] = l[g];
+      }
+    }
+  }
+};
+
+// A warp's piece: which unit, and whether the unit's tiles go on before or after it.
+struct PaPiece {
+  int b, u;          // u < 0: none
+  int before, after;
+  int64_t end;       // the unit's end on the line
+};
+
+template <typename T, int D, int HB>
+__global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const PagedAttendParams p) {
+  using S = PaShape<T, D, HB>;
+  using State = typename std::conditional<S::k16, PaState16<T, D, HB>, PaState32<T, D, HB>>::type;
+  extern __shared__ __align__(128) uint8_t pa_smem[];
+  __shared__ PaPiece pieces[2 * kPaWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  asm volatile("griddepcontrol.launch_dependents;");
+  uint8_t* ring = pa_smem + warp * (S::NH * S::kHalf);
+  uint8_t* own = pa_smem + kPaWarps * (S::NH * S::kHalf) + warp * (S::kPiece + S::kQ + S::kP + 64);
+  float* kept = reinterpret_cast<float*>(own);            // the piece that came first
+  uint8_t* extra = own + S::kPiece;                       // fp32: queries and weights
+  uint32_t* masks = reinterpret_cast<uint32_t*>(own + S::kPiece + S::kQ + S::kP);  // [16]
+
+  // rows of empty sequences
+  for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
+    int len, lo, t_lo, t_hi;
+    pa_sequence<S::R>(p, b, len, lo, t_lo, t_hi);
+    if (t_lo < t_hi) continue;
+    const int64_t row0 = static_cast<int64_t>(b) * p.H;
+    for (int i = threadIdx.x; i < p.H * D; i += kPaThreads)
+      ElemTraits<T>::store(static_cast<T*>(p.o) + row0 * D, i, 0.0f);
+    if (p.lse != nullptr)
+      for (int i = threadIdx.x; i < p.H; i += kPaThreads) p.lse[row0 + i] = -INFINITY;
+  }
+
+  const int64_t total = pa_total<S::R>(p);
+  int64_t ctas = (total + kPaMinTiles - 1) / kPaMinTiles;
+  if (ctas > gridDim.x) ctas = gridDim.x;
+  if (blockIdx.x >= ctas) {
+    if (threadIdx.x == 0) p.rec[blockIdx.x].u = -1;
+    return;
+  }
+  const int64_t c0 = blockIdx.x * total / ctas, c1 = (blockIdx.x + 1) * total / ctas;
+  const int64_t s0 = c0 + warp * (c1 - c0) / kPaWarps, s1 = c0 + (warp + 1) * (c1 - c0) / kPaWarps;
+  const int n = static_cast<int>(s1 - s0);
+  if (lane == 0) pieces[2 * warp].u = pieces[2 * warp + 1].u = -1;
+
+  if (n > 0) {
+    PaCursor in = pa_seek<S::R>(p, s0);  // where loads are
+    PaCursor at = in;                    // where the arithmetic is
+    PaLoader<T, D, HB> load;
+    State st;
+    constexpr int kAhead = S::NH - 1;    // half tiles in flight, an even number
+    int hs_in = 0, t_in = 0;             // ring place and tile count of the loads
+    auto issue_keys = [&]() {
+      if (t_in < n) {
+        const uint32_t mask = load.keys(p, in, ring + hs_in * S::kHalf);
+        if (lane == 0) masks[t_in & 15] = mask;
+      }
+      cp_async_commit();
+      hs_in = hs_in + 1 == S::NH ? 0 : hs_in + 1;
+    };
+    auto issue_values = [&]() {
+      if (t_in < n) {
+        load.values(p, ring + hs_in * S::kHalf);
+        ++t_in;
+        if (t_in < n) pa_next<S::R>(p, in);
+      }
+      cp_async_commit();
+      hs_in = hs_in + 1 == S::NH ? 0 : hs_in + 1;
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead / 2; ++i) {
+      issue_keys();
+      issue_values();
+    }
+    int64_t g0 = s0 - (at.t - at.t_lo);  // the unit's begin on the line
+    int first = at.t;                    // its first tile in this share
+    st.begin(p, at, extra);
+    int hs = 0;
+    for (int i = 0; i < n; ++i) {
+      cp_async_wait<kAhead - 1>();
+      __syncwarp();
+      issue_keys();
+      const uint32_t mask = masks[i & 15];
+      st.scores(p, at, ring + hs * S::kHalf, mask, extra);
+      hs = hs + 1 == S::NH ? 0 : hs + 1;
+      cp_async_wait<kAhead - 1>();
+      __syncwarp();
+      issue_values();
+      st.values(ring + hs * S::kHalf, mask, extra);
+      hs = hs + 1 == S::NH ? 0 : hs + 1;
+      const bool ends = at.t + 1 == at.t_hi;
+      if (ends || i + 1 == n) {
+        st.close();
+        const bool before = first > at.t_lo;
+        if (!before && ends) {
+          st.write(p, at);
+        } else {
+          // before: the only piece that can be followed by others, so it has its own place;
+          // a piece that goes on after the share is the last, and the ring is free then
+          float* dst = kept;
+          if (!before) {
+            cp_async_wait<0>();
+            __syncwarp();
+            dst = reinterpret_cast<float*>(ring);
+          }
+          st.piece(dst);
+          if (lane == 0) {
+            PaPiece& pc = pieces[2 * warp + (before ? 0 : 1)];
+            pc.b = at.b;
+            pc.u = at.u;
+            pc.before = before;
+            pc.after = !ends;
+            pc.end = g0 + (at.t_hi - at.t_lo);
+          }
+        }
+        if (i + 1 < n) {
+          pa_next<S::R>(p, at);
+          first = at.t;
+          g0 = s0 + i + 1;
+          st.begin(p, at, extra);
+        }
+      } else {
+        ++at.t;
+      }
+    }
+    cp_async_wait<0>();
+  }
+  __syncthreads();
+
+  // Fold the CTA's pieces: runs of pieces of one unit, row by row over the warps.
+  bool opens = false;
+  for (int i = 0; i < 2 * kPaWarps;) {
+    const PaPiece lead = pieces[i];
+    if (lead.u < 0) {
+      ++i;
+      continue;
+    }
+    int j = i + 1, last = i;
+    while (j < 2 * kPaWarps && (pieces[j].u < 0 || (pieces[j].u == lead.u && pieces[j].b == lead.b))) {
+      if (pieces[j].u >= 0) last = j;
+      ++j;
+    }
+    const bool before = lead.before, after = pieces[last].after;
+    const int hk = lead.u / p.hblocks, h0 = (lead.u - hk * p.hblocks) * HB;
+    const int rows = p.G - h0 < HB ? p.G - h0 : HB;
+    for (int g = warp; g < rows; g += kPaWarps) {
+      float M = -INFINITY;
+      for (int x = i; x <= last; ++x) {
+        if (pieces[x].u < 0) continue;
+        const float* src = (x & 1) ? reinterpret_cast<const float*>(pa_smem + (x >> 1) * (S::NH * S::kHalf))
+                                   : reinterpret_cast<const float*>(
+                                         pa_smem + kPaWarps * (S::NH * S::kHalf) +
+                                         (x >> 1) * (S::kPiece + S::kQ + S::kP + 64));
+        M = fmaxf(M, src[g * (D + 2) + D]);
+      }
+      float L = 0.0f, acc[D / 32] = {};
+      for (int x = i; x <= last; ++x) {
+        if (pieces[x].u < 0) continue;
+        const float* src = (x & 1) ? reinterpret_cast<const float*>(pa_smem + (x >> 1) * (S::NH * S::kHalf))
+                                   : reinterpret_cast<const float*>(
+                                         pa_smem + kPaWarps * (S::NH * S::kHalf) +
+                                         (x >> 1) * (S::kPiece + S::kQ + S::kP + 64));
+        const float mm = src[g * (D + 2) + D];
+        const float a = mm == -INFINITY ? 0.0f : pa_exp2(mm - M);
+        const float ll = src[g * (D + 2) + D + 1];
+        L += ll != ll ? ll : a * ll;
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) {
+          const float v = src[g * (D + 2) + lane + 32 * e];
+          acc[e] = mm == -INFINITY ? (v != v ? v : acc[e]) : fmaf(a, v, acc[e]);
+        }
+      }
+      if (!before && !after) {
+        const int64_t row = static_cast<int64_t>(lead.b) * p.H + hk * p.G + h0 + g;
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e)
+          ElemTraits<T>::store(static_cast<T*>(p.o) + row * D, lane + 32 * e,
+                               L == 0.0f ? 0.0f : acc[e] / L);
+        if (lane == 0) pa_store_stats(p, row, M, L);
+      } else {
+        float* dst = p.part + ((2 * static_cast<int64_t>(blockIdx.x) + (before ? 0 : 1)) * HB + g) * (D + 2);
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) dst[lane + 32 * e] = acc[e];
+        if (lane == 0) {
+          dst[D] = M;
+          dst[D + 1] = L;
+        }
+      }
+    }
+    if (!before && after) {
+      opens = true;
+      if (threadIdx.x == 0) {
+        PaRecord r;
+        r.b = lead.b;
+        r.u = lead.u;
+        // the CTA whose share holds the unit's last tile: the largest c with c*total/ctas < end
+        r.last = static_cast<int32_t>((lead.end * ctas - 1) / total);
+        r.pad = 0;
+        p.rec[blockIdx.x] = r;
+      }
+    }
+    i = j;
+  }
+  if (!opens && threadIdx.x == 0) p.rec[blockIdx.x].u = -1;
+}
+
+// Folds the partials of the unit that begins in CTA blockIdx.x of the first kernel and ends in
+// a later one; blockIdx.y is the row of the head block. Thread groups of D take every
+// (128 / D)-th partial.
+template <typename T, int D, int HB>
+__global__ void __launch_bounds__(128) paged_fold_kernel(const PagedAttendParams p) {
+  constexpr int N = 128 / D;
+  __shared__ float m_s[4], acc_s[128], l_s[2];
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const PaRecord r = p.rec[blockIdx.x];
+  if (r.u < 0) return;
+  const int hk = r.u / p.hblocks;
+  const int g = blockIdx.y, h = (r.u - hk * p.hblocks) * HB + g;
+  if (h >= p.G) return;
+  const int c0 = blockIdx.x;
+  auto part = [&](int c) {
+    return p.part + ((2 * static_cast<int64_t>(c) + (c == c0 ? 1 : 0)) * HB + g) * (D + 2);
+  };
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float M = -INFINITY;
+  for (int c = c0 + threadIdx.x; c <= r.last; c += 128) M = fmaxf(M, part(c)[D]);
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  if (lane == 0) m_s[warp] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(m_s[0], m_s[1]), fmaxf(m_s[2], m_s[3]));
+  const int d = threadIdx.x % D, k = threadIdx.x / D;
+  float acc = 0.0f, L = 0.0f;
+#pragma unroll 4
+  for (int c = c0 + k; c <= r.last; c += N) {
+    const float* s = part(c);
+    const float mm = s[D], ll = s[D + 1], v = s[d];
+    const float a = mm == -INFINITY ? 0.0f : pa_exp2(mm - M);
+    L += ll != ll ? ll : a * ll;
+    acc = mm == -INFINITY ? (v != v ? v : acc) : fmaf(a, v, acc);
+  }
+  if (N > 1) {
+    acc_s[threadIdx.x] = acc;
+    if (d == 0) l_s[k] = L;
+    __syncthreads();
+    if (k > 0) return;
+#pragma unroll
+    for (int i = 1; i < N; ++i) {
+      acc += acc_s[i * D + d];
+      L += l_s[i];
+    }
+  }
+  const int64_t row = static_cast<int64_t>(r.b) * p.H + hk * p.G + h;
+  ElemTraits<T>::store(static_cast<T*>(p.o) + row * D, d, L == 0.0f ? 0.0f : acc / L);
+  if (d == 0) pa_store_stats(p, row, M, L);
+}
+
+// weights[b][h_kv][i] += sum over the G heads of exp2(score - m) / l, in head order.
+__global__ void __launch_bounds__(256) paged_weights_kernel(const PagedAttendParams p,
+                                                            float* weights, int64_t wsb,
+                                                            int64_t wsh, int chunk) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int hk = blockIdx.y;
+  for (int b = blockIdx.z; b < p.B; b += gridDim.z) {
+    const int n = checked_length(p.c, __ldg(p.lengths + b));
+    const int lo = p.window > 0 && n > p.window ? n - p.window : 0;
+    const int from = max(lo, static_cast<int>(blockIdx.x) * chunk);
+    const int to = min(n, (static_cast<int>(blockIdx.x) + 1) * chunk);
+    const int64_t row0 = static_cast<int64_t>(b) * p.H + hk * p.G;
+    for (int i = from + threadIdx.x; i < to; i += 256) {
+      float w = 0.0f;
+      for (int g = 0; g < p.G; ++g) {
+        const float2 ml = p.stats[row0 + g];
+        const float s = p.scores[(row0 + g) * p.s_stride + i];
+        w += s == -INFINITY ? 0.0f : pa_exp2(s - ml.x) * ml.y;
+      }
+      float* dst = weights + b * wsb + hk * wsh + i;
+      *dst += w;
+    }
+  }
+}
+
+// Workspace sections.
+struct PagedAttendLayout {
+  size_t rec, part, stats, scores, total;
+  int64_t s_stride;
+  int ctas;
+};
+
+// Query heads per block: all of a KV head's up to 16, so that its rows are read once. Single
+// precision with D = 128 keeps to 8: the queries and pieces of 16 would leave no ring.
+static int pa_head_block(int G, int D, int dtype) {
+  return G <= 8 || (D == 128 && dtype == DCR_DTYPE_F32) ? 8 : 16;
+}
+
+static PagedAttendLayout pa_layout(int B, int H, int G, int D, int max_slots, bool weights) {
+  PagedAttendLayout w;
+  w.ctas = device_sm_count();
+  size_t off = 0;
+  auto take = [&](size_t n) {
+    const size_t at = off;
+    off = (off + n + 255) / 256 * 256;
+    return at;
+  };
+  w.rec = take(sizeof(PaRecord) * w.ctas);
+  w.part = take(sizeof(float) * 2 * w.ctas * (G <= 8 ? 8 : 16) * (D + 2));
+  w.stats = weights ? take(sizeof(float2) * static_cast<size_t>(B) * H) : 0;
+  w.s_stride = (static_cast<int64_t>(max_slots) + 15) / 16 * 16;
+  w.scores = weights ? take(sizeof(float) * static_cast<size_t>(B) * H * w.s_stride) : 0;
+  w.total = off;
+  return w;
+}
+
+template <typename... Args>
+static cudaError_t pa_launch_dependent(void (*kernel)(Args...), dim3 grid, dim3 block,
+                                       cudaStream_t s, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <typename T, int D, int HB>
+static int pa_launch(const PagedAttendParams& p, int ctas, cudaStream_t s) {
+  using S = PaShape<T, D, HB>;
+  auto kernel = paged_attend_kernel<T, D, HB>;
+  if (ensure_smem_attr(reinterpret_cast<const void*>(kernel), S::kSmem) != cudaSuccess)
+    return DCR_ERR_CUDA;
+  PagedAttendParams q = p;
+  q.page16 = p.c.page.d % S::R == 0;
+  kernel<<<ctas, kPaThreads, S::kSmem, s>>>(q);
+  if (cudaGetLastError() != cudaSuccess) return DCR_ERR_CUDA;
+  const int rows = p.G < HB ? p.G : HB;
+  if (pa_launch_dependent(paged_fold_kernel<T, D, HB>, dim3(ctas, rows), dim3(128), s, q) != cudaSuccess)
+    return DCR_ERR_CUDA;
+  return DCR_OK;
+}
+
+template <typename T>
+static int pa_launch_t(const PagedAttendParams& p, int D, int HB, int ctas, cudaStream_t s) {
+  if (D == 64) return HB == 8 ? pa_launch<T, 64, 8>(p, ctas, s) : pa_launch<T, 64, 16>(p, ctas, s);
+  if constexpr (sizeof(T) == 2) {
+    if (HB == 16) return pa_launch<T, 128, 16>(p, ctas, s);
+  }
+  return pa_launch<T, 128, 8>(p, ctas, s);
 }
 
 }  // namespace dcr
@@ -133,7 +972,7 @@ extern "C" {
 size_t dcr_paged_workspace_bytes(int B, int H, int H_kv, int D, int max_slots, int with_weights) {
   if (B <= 0 || H_kv <= 0 || H <= 0 || H % H_kv != 0 || (D != 64 && D != 128) || max_slots <= 0)
     return 0;
-  return with_weights ? sizeof(float) * static_cast<size_t>(B) * H : 16;
+  return pa_layout(B, H, H / H_kv, D, max_slots, with_weights != 0).total;
 }
 
 int dcr_paged_attend(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k_pages,
@@ -145,7 +984,8 @@ int dcr_paged_attend(const void* q, int64_t q_stride_b, int64_t q_stride_h, cons
                      float* weights, int64_t w_stride_b, int64_t w_stride_h, void* workspace,
                      size_t workspace_bytes, void* stream) {
   if (q == nullptr || lengths == nullptr || o == nullptr) return DCR_ERR_NULL;
-  if (B <= 0 || B > 65535 || H <= 0 || H_kv <= 0 || H % H_kv != 0 || window < 0) return DCR_ERR_SHAPE;
+  if (B <= 0 || H <= 0 || H_kv <= 0 || H_kv > 65535 || H % H_kv != 0 || window < 0)
+    return DCR_ERR_SHAPE;
   const int st = check_pool(k_pages, v_pages, dtype, k_stride_p, k_stride_h, k_stride_s,
                             v_stride_p, v_stride_h, v_stride_s, num_pages, page_size, page_table,
                             table_stride, max_pages, H_kv, D);
@@ -157,9 +997,13 @@ int dcr_paged_attend(const void* q, int64_t q_stride_b, int64_t q_stride_h, cons
   if (q_stride_b < 0 || q_stride_h < 0) return DCR_ERR_SHAPE;
   const int max_slots = max_pages * page_size;
   if (weights != nullptr && (w_stride_h < 0 || w_stride_b < 0)) return DCR_ERR_SHAPE;
-  if (workspace == nullptr ||
-      workspace_bytes < dcr_paged_workspace_bytes(B, H, H_kv, D, max_slots, weights != nullptr))
+  const int G = H / H_kv;
+  const PagedAttendLayout w = pa_layout(B, H, G, D, max_slots, weights != nullptr);
+  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15u) ||
+      workspace_bytes < w.total)
     return DCR_ERR_WORKSPACE;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const int HB = pa_head_block(G, D, dtype);
   PagedAttendParams p;
   p.c = make_pool(k_pages, v_pages, k_stride_p, k_stride_h, k_stride_s, v_stride_p, v_stride_h,
                   v_stride_s, num_pages, page_size, page_table, table_stride, max_pages);
@@ -170,25 +1014,33 @@ int dcr_paged_attend(const void* q, int64_t q_stride_b, int64_t q_stride_h, cons
   p.B = B;
   p.H = H;
   p.H_kv = H_kv;
-  p.G = H / H_kv;
-  p.scale2 = scale * 1.4426950408889634f;
+  p.G = G;
+  p.hblocks = (G + HB - 1) / HB;
+  p.units = H_kv * p.hblocks;
+  p.scale2 = scale * kLog2e;
   p.window = window;
+  p.page16 = 0;
   p.o = o;
-  p.lse = lse != nullptr ? lse : weights != nullptr ? static_cast<float*>(workspace) : nullptr;
-  p.weights = weights;
-  p.wsb = w_stride_b;
-  p.wsh = w_stride_h;
+  p.lse = lse;
+  p.stats = weights != nullptr ? reinterpret_cast<float2*>(ws + w.stats) : nullptr;
+  p.part = reinterpret_cast<float*>(ws + w.part);
+  p.rec = reinterpret_cast<PaRecord*>(ws + w.rec);
+  p.scores = weights != nullptr ? reinterpret_cast<float*>(ws + w.scores) : nullptr;
+  p.s_stride = w.s_stride;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const dim3 grid(H_kv, B);
-  switch (dtype * 2 + (D == 128)) {
-    case 0: paged_attend_kernel<__nv_bfloat16, 64><<<grid, kPaThreads, 0, s>>>(p); break;
-    case 1: paged_attend_kernel<__nv_bfloat16, 128><<<grid, kPaThreads, 0, s>>>(p); break;
-    case 2: paged_attend_kernel<__half, 64><<<grid, kPaThreads, 0, s>>>(p); break;
-    case 3: paged_attend_kernel<__half, 128><<<grid, kPaThreads, 0, s>>>(p); break;
-    case 4: paged_attend_kernel<float, 64><<<grid, kPaThreads, 0, s>>>(p); break;
-    default: paged_attend_kernel<float, 128><<<grid, kPaThreads, 0, s>>>(p); break;
+  int rc;
+  switch (dtype) {
+    case DCR_DTYPE_BF16: rc = pa_launch_t<__nv_bfloat16>(p, D, HB, w.ctas, s); break;
+    case DCR_DTYPE_F16: rc = pa_launch_t<__half>(p, D, HB, w.ctas, s); break;
+    default: rc = pa_launch_t<float>(p, D, HB, w.ctas, s); break;
   }
-  return cudaGetLastError() == cudaSuccess ? DCR_OK : DCR_ERR_CUDA;
+  if (rc != DCR_OK || weights == nullptr) return rc;
+  const int chunk = 1024;
+  const dim3 grid((max_slots + chunk - 1) / chunk, H_kv, B < 65535 ? B : 65535);
+  return pa_launch_dependent(paged_weights_kernel, grid, dim3(256), s, p, weights, w_stride_b,
+                             w_stride_h, chunk) == cudaSuccess
+             ? DCR_OK
+             : DCR_ERR_CUDA;
 }
 
 }  // extern "C"
