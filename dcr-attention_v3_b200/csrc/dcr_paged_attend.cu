@@ -65,7 +65,7 @@ struct PagedAttendParams {
   int hblocks;    // blocks of query heads per KV head
   float scale2;   // scale * log2(e)
   int window;
-  int page16;     // page_size is a multiple of R: a tile lies in one page
+  int page16;     // page_size is a multiple of a group: a group lies in one page
   void* o;        // [B][H][D]
   float* lse;     // [B][H] natural log, or null
   float2* stats;  // [B][H] (maximum in base 2, 1 / sum), with scores
@@ -79,12 +79,14 @@ struct PagedAttendParams {
 template <typename T, int D, int HB>
 struct PaShape {
   static constexpr bool k16 = sizeof(T) == 2;
-  static constexpr int R = k16 ? 16 : 8;                  // slots per tile
   static constexpr int kRow = D * static_cast<int>(sizeof(T));
+  static constexpr int R = 4096 / kRow;                   // slots per tile: 32, 16 or 8
   static constexpr int kChunks = kRow / 16;               // 16-byte chunks per row: 8, 16 or 32
   static constexpr int kHalf = R * kRow;                  // bytes of a K or V half tile
   static constexpr int kRowsPer = 32 / kChunks;           // rows a warp copies per instruction
   static constexpr int kCopies = R / kRowsPer;
+  static constexpr int kGroup = R < 16 ? R : 16;          // slots per page lookup
+  static constexpr int kGroups = R / kGroup;
   static constexpr int kPiece = HB * (D + 2) * 4;         // a piece (o, m, l)
   static constexpr int kQ = k16 ? 0 : HB * D * 4;         // fp32: the queries, read as broadcasts
   static constexpr int kP = k16 ? 0 : HB * R * 4;         // fp32: the tile's weights
@@ -200,60 +202,94 @@ __device__ __forceinline__ PaCursor pa_seek(const PagedAttendParams& p, int64_t 
   }
 }
 
-// The copies of one tile: K's then V's, from the same rows.
+// The copies of one tile: K's rows, then V's. Where pages hold whole groups of 16 slots (or R,
+// if that is less), a tile of valid slots, which is all but the ends of a sequence, looks a
+// page up per group and takes its rows by a fixed stride; any other looks every row up, and
+// fills the slots that are not valid with zeros.
 template <typename T, int D, int HB>
 struct PaLoader {
   using S = PaShape<T, D, HB>;
-  int64_t row_v[S::kCopies];  // V offsets (elements) of the rows this lane copies
-  uint32_t ok;                // bit i: this lane's i-th row is valid
+  static constexpr uint32_t kAll = 0xffffffffu >> (32 - S::R);
+  const char* next_v[S::kGroups];  // this lane's first V row of each group, when `whole`
+  bool whole;
+  int b, hk, slot0;
+  uint32_t mask;
 
   // Issues the tile's K half into `dst` and returns its mask of valid slots.
   __device__ __forceinline__ uint32_t keys(const PagedAttendParams& p, const PaCursor& c,
                                            uint8_t* dst) {
     const int lane = threadIdx.x & 31;
     const int ch = lane % S::kChunks, r0 = lane / S::kChunks;
-    const int hk = c.u / p.hblocks;
-    const int slot0 = c.t * S::R;
+    b = c.b;
+    hk = c.u / p.hblocks;
+    slot0 = c.t * S::R;
     const int from = c.lo > slot0 ? c.lo - slot0 : 0;
     const int to = c.len - slot0 < S::R ? c.len - slot0 : S::R;
-    uint32_t mask = (0xffffffffu >> (32 - to)) & (0xffffffffu << from);
-    const T* kbase = static_cast<const T*>(p.c.k) + hk * p.c.ksh + ch * (16 / sizeof(T));
-    const int64_t vbase = hk * p.c.vsh + ch * (16 / static_cast<int>(sizeof(T)));
-    ok = 0;
-    if (p.page16) {
-      const uint32_t pi = p.c.page.div(slot0);
-      const int pg = page_of(p.c, c.b, pi);
-      if (pg < 0) mask = 0;
-      const int in = slot0 - static_cast<int>(pi * p.c.page.d);
-      const int64_t pgk = pg < 0 ? 0 : pg * p.c.ksp, pgv = pg < 0 ? 0 : pg * p.c.vsp;
+    mask = (0xffffffffu >> (32 - to)) & (0xffffffffu << from);
+    whole = p.page16 && mask == kAll;
+    if (whole) {
+      const char* src[S::kGroups];
 #pragma unroll
-      for (int i = 0; i < S::kCopies; ++i) {
-        const int r = r0 + i * S::kRowsPer;
-        const bool v = (mask >> r) & 1u;
-        row_v[i] = v ? vbase + pgv + (in + r) * p.c.vsr : 0;
-        ok |= static_cast<uint32_t>(v) << i;
-        copy(dst, r, ch, v ? kbase + pgk + (in + r) * p.c.ksr : static_cast<const T*>(p.c.k), v);
+      for (int g = 0; g < S::kGroups; ++g) {
+        const int s0 = slot0 + g * S::kGroup;
+        const uint32_t pi = p.c.page.div(s0);
+        const int pg = page_of(p.c, b, pi);
+        const int in = s0 - static_cast<int>(pi * p.c.page.d) + r0;
+        whole = whole && pg >= 0;
+        src[g] = static_cast<const char*>(p.c.k) + ch * 16 +
+                 (pg * p.c.ksp + hk * p.c.ksh + in * p.c.ksr) * static_cast<int64_t>(sizeof(T));
+        next_v[g] = static_cast<const char*>(p.c.v) + ch * 16 +
+                    (pg * p.c.vsp + hk * p.c.vsh + in * p.c.vsr) * static_cast<int64_t>(sizeof(T));
       }
-      return mask;
+      if (whole) {
+        copy_whole(dst, src, p.c.ksr * static_cast<int64_t>(S::kRowsPer * sizeof(T)));
+        return mask;
+      }
     }
-    uint32_t held = 0;
+    mask = copy_each(p, p.c.k, p.c.ksp, p.c.ksh, p.c.ksr, dst);
+    return mask;
+  }
+
+  __device__ __forceinline__ void values(const PagedAttendParams& p, uint8_t* dst) const {
+    if (whole)
+      copy_whole(dst, next_v, p.c.vsr * static_cast<int64_t>(S::kRowsPer * sizeof(T)));
+    else
+      copy_each(p, p.c.v, p.c.vsp, p.c.vsh, p.c.vsr, dst);
+  }
+
+  __device__ __forceinline__ static void copy_whole(uint8_t* dst, const char* const (&src)[S::kGroups],
+                                                    int64_t step) {
+    const int lane = threadIdx.x & 31;
+    constexpr int kPer = S::kCopies / S::kGroups;
 #pragma unroll
+    for (int g = 0; g < S::kGroups; ++g) {
+      const char* at_g = src[g];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        cp_async_16(dst + at(lane / S::kChunks + (g * kPer + i) * S::kRowsPer, lane % S::kChunks), at_g, 16u);
+        at_g += step;
+      }
+    }
+  }
+
+  __device__ __forceinline__ uint32_t copy_each(const PagedAttendParams& p, const void* base,
+                                                int64_t sp, int64_t sh, int64_t sr,
+                                                uint8_t* dst) const {
+    const int lane = threadIdx.x & 31;
+    const int ch = lane % S::kChunks;
+    uint32_t held = 0;
+#pragma unroll 1
     for (int i = 0; i < S::kCopies; ++i) {
-      const int r = r0 + i * S::kRowsPer;
+      const int r = lane / S::kChunks + i * S::kRowsPer;
       bool v = (mask >> r) & 1u;
-      int64_t pgk = 0, pgv = 0;
-      int in = 0;
+      int64_t off = 0;
       if (v) {
         const uint32_t pi = p.c.page.div(slot0 + r);
-        const int pg = page_of(p.c, c.b, pi);
-        in = slot0 + r - static_cast<int>(pi * p.c.page.d);
+        const int pg = page_of(p.c, b, pi);
         v = pg >= 0;
-        pgk = v ? pg * p.c.ksp : 0;
-        pgv = v ? pg * p.c.vsp : 0;
+        if (v) off = pg * sp + hk * sh + (slot0 + r - static_cast<int>(pi * p.c.page.d)) * sr + ch * (16 / static_cast<int>(sizeof(T)));
       }
-      row_v[i] = v ? vbase + pgv + in * p.c.vsr : 0;
-      ok |= static_cast<uint32_t>(v) << i;
-      copy(dst, r, ch, v ? kbase + pgk + in * p.c.ksr : static_cast<const T*>(p.c.k), v);
+      cp_async_16(dst + at(r, ch), static_cast<const T*>(base) + off, v ? 16u : 0u);
       const unsigned bal = __ballot_sync(0xffffffffu, v);
 #pragma unroll
       for (int j = 0; j < S::kRowsPer; ++j)
@@ -262,22 +298,11 @@ struct PaLoader {
     return held;
   }
 
-  __device__ __forceinline__ void values(const PagedAttendParams& p, uint8_t* dst) const {
-    const int lane = threadIdx.x & 31;
-    const int ch = lane % S::kChunks, r0 = lane / S::kChunks;
-#pragma unroll
-    for (int i = 0; i < S::kCopies; ++i)
-      copy(dst, r0 + i * S::kRowsPer, ch, static_cast<const T*>(p.c.v) + row_v[i], (ok >> i) & 1u);
-  }
-
   // Chunk ch of row r: 16-bit rows by ldmatrix (8 rows of one chunk column at once), fp32 rows
   // by 16-byte reads of two rows' quarters; the swizzles keep both free of bank conflicts.
   __device__ __forceinline__ static uint32_t at(int r, int ch) {
     const int sw = S::k16 ? (ch ^ (r & 7)) : (ch ^ ((r & 1) << 2));
     return static_cast<uint32_t>(r * S::kRow + sw * 16);
-  }
-  __device__ __forceinline__ static void copy(uint8_t* dst, int r, int ch, const T* src, bool v) {
-    cp_async_16(dst + at(r, ch), src, v ? 16u : 0u);
   }
 };
 
@@ -290,7 +315,8 @@ struct PaState16 {
   uint32_t qf[D / 16][2 * M];
   float o[D / 8][4];
   float m[M], l[M];
-  uint32_t ph[2][M], pl[2][M];  // the tile's weights, hi and lo parts, per 8 slots
+  static constexpr int NT = S::R / 8;
+  uint32_t ph[NT][M], pl[NT][M];  // the tile's weights, hi and lo parts, per 8 slots
 
   __device__ __forceinline__ void begin(const PagedAttendParams& p, const PaCursor& c, uint8_t*) {
     const int lane = threadIdx.x & 31;
@@ -318,42 +344,53 @@ struct PaState16 {
   __device__ __forceinline__ void scores(const PagedAttendParams& p, const PaCursor& c,
                                          const uint8_t* tile, uint32_t mask, uint8_t*) {
     const int lane = threadIdx.x & 31;
-    float z[2][4] = {};
+    float z[NT][4] = {};
     const int mat = lane >> 3, r8 = lane & 7;
     const int row = (mat >> 1) * 8 + r8;
+    const uint32_t base = smem_u32(tile);
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
-      uint32_t k0, k1, k2, k3;
-      ldsm_x4(smem_u32(tile + PaLoader<T, D, HB>::at(row, 2 * ks + (mat & 1))), k0, k1, k2, k3);
       const uint32_t a[4] = {qf[ks][0], M == 2 ? qf[ks][M - 1] : 0u, qf[ks][M],
                              M == 2 ? qf[ks][2 * M - 1] : 0u};
-      UnionMma<T>::mma(z[0], a, k0, k1);
-      UnionMma<T>::mma(z[1], a, k2, k3);
+#pragma unroll
+      for (int j = 0; j < NT / 2; ++j) {
+        uint32_t k0, k1, k2, k3;
+        ldsm_x4(base + PaLoader<T, D, HB>::at(row, 2 * ks + (mat & 1)) + j * 16 * S::kRow, k0, k1, k2, k3);
+        UnionMma<T>::mma(z[2 * j], a, k0, k1);
+        UnionMma<T>::mma(z[2 * j + 1], a, k2, k3);
+      }
     }
     const int pos = 2 * (lane & 3);
 #pragma unroll
     for (int i = 0; i < M; ++i) {
-      float s[2][2];
+      float s[NT][2];
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          s[j][e] = z[j][2 * i + e] * p.scale2;
-          if (mask != 0xffffu && !((mask >> (8 * j + pos + e)) & 1u)) s[j][e] = -INFINITY;
-        }
+        for (int e = 0; e < 2; ++e) s[j][e] = z[j][2 * i + e] * p.scale2;
+      if (mask != PaLoader<T, D, HB>::kAll) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (!((mask >> (8 * j + pos + e)) & 1u)) s[j][e] = -INFINITY;
+      }
       if (p.scores != nullptr) {
         const int hk = c.u / p.hblocks;
         const int g = (c.u - hk * p.hblocks) * HB + (lane >> 2) + 8 * i;
         if (g < p.G) {
           float* dst = p.scores + (static_cast<int64_t>(c.b) * p.H + hk * p.G + g) * p.s_stride +
                        c.t * S::R + pos;
-          *reinterpret_cast<float2*>(dst) = make_float2(s[0][0], s[0][1]);
-          *reinterpret_cast<float2*>(dst + 8) = make_float2(s[1][0], s[1][1]);
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+            *reinterpret_cast<float2*>(dst + 8 * j) = make_float2(s[j][0], s[j][1]);
         }
       }
       // The maximum is raised only when some score is 2^8 above it: weights stay below 2^8,
       // and most tiles need no rescaling. A NaN score raises nothing and spreads by itself.
-      float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+      float top = fmaxf(s[0][0], s[0][1]);
+#pragma unroll
+      for (int j = 1; j < NT; ++j) top = fmaxf(top, fmaxf(s[j][0], s[j][1]));
       if (__any_sync(0xffffffffu, top > m[i] + 8.0f)) {
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -373,7 +410,7 @@ struct PaState16 {
       }
       const float ms = m[i] == -INFINITY ? 0.0f : m[i];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < NT; ++j) {
         const float w0 = pa_exp2(s[j][0] - ms), w1 = pa_exp2(s[j][1] - ms);
         l[i] += w0 + w1;
         UnionMma<T>::split(w0, w1, ph[j][i], pl[j][i]);
@@ -385,21 +422,25 @@ struct PaState16 {
     const int lane = threadIdx.x & 31;
     const int mat = lane >> 3, r8 = lane & 7;
     const int row = (mat & 1) * 8 + r8;
+    const uint32_t base = smem_u32(tile);
 #pragma unroll
-    for (int j = 0; j < D / 16; ++j) {
-      uint32_t v0, v1, v2, v3;
-      ldsm_x4_t(smem_u32(tile + PaLoader<T, D, HB>::at(row, 2 * j + (mat >> 1))), v0, v1, v2, v3);
-      if constexpr (M == 1) {
-        const uint32_t a[4] = {ph[0][0], pl[0][0], ph[1][0], pl[1][0]};
-        UnionMma<T>::mma(o[2 * j], a, v0, v1);
-        UnionMma<T>::mma(o[2 * j + 1], a, v2, v3);
-      } else {
-        const uint32_t ah[4] = {ph[0][0], ph[0][M - 1], ph[1][0], ph[1][M - 1]};
-        const uint32_t al[4] = {pl[0][0], pl[0][M - 1], pl[1][0], pl[1][M - 1]};
-        UnionMma<T>::mma(o[2 * j], ah, v0, v1);
-        UnionMma<T>::mma(o[2 * j + 1], ah, v2, v3);
-        UnionMma<T>::mma(o[2 * j], al, v0, v1);
-        UnionMma<T>::mma(o[2 * j + 1], al, v2, v3);
+    for (int t = 0; t < NT; t += 2) {
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        uint32_t v0, v1, v2, v3;
+        ldsm_x4_t(base + PaLoader<T, D, HB>::at(row, 2 * j + (mat >> 1)) + t * 8 * S::kRow, v0, v1, v2, v3);
+        if constexpr (M == 1) {
+          const uint32_t a[4] = {ph[t][0], pl[t][0], ph[t + 1][0], pl[t + 1][0]};
+          UnionMma<T>::mma(o[2 * j], a, v0, v1);
+          UnionMma<T>::mma(o[2 * j + 1], a, v2, v3);
+        } else {
+          const uint32_t ah[4] = {ph[t][0], ph[t][M - 1], ph[t + 1][0], ph[t + 1][M - 1]};
+          const uint32_t al[4] = {pl[t][0], pl[t][M - 1], pl[t + 1][0], pl[t + 1][M - 1]};
+          UnionMma<T>::mma(o[2 * j], ah, v0, v1);
+          UnionMma<T>::mma(o[2 * j + 1], ah, v2, v3);
+          UnionMma<T>::mma(o[2 * j], al, v0, v1);
+          UnionMma<T>::mma(o[2 * j + 1], al, v2, v3);
+        }
       }
     }
   }
@@ -493,33 +534,40 @@ struct PaState32 {
                                          const uint8_t* tile, uint32_t mask, uint8_t* own) {
     const int lane = threadIdx.x & 31;
     const int r = lane >> 2, qd = lane & 3;
-    float4 k[S::kChunks / 4];
-#pragma unroll
-    for (int i = 0; i < S::kChunks / 4; ++i)
-      k[i] = *reinterpret_cast<const float4*>(tile + PaLoader<T, D, HB>::at(r, 4 * i + qd));
-    const bool valid = (mask >> r) & 1u;
     const int hk = c.u / p.hblocks;
     const int64_t row0 = static_cast<int64_t>(c.b) * p.H + hk * p.G + (c.u - hk * p.hblocks) * HB;
+    float4 k[S::R / 8][S::kChunks / 4];
+#pragma unroll
+    for (int t = 0; t < S::R / 8; ++t)
+#pragma unroll
+      for (int i = 0; i < S::kChunks / 4; ++i)
+        k[t][i] = *reinterpret_cast<const float4*>(tile + PaLoader<T, D, HB>::at(r + 8 * t, 4 * i + qd));
 #pragma unroll
     for (int g = 0; g < HB; ++g) {
       if (g >= rows) break;
       const float4* q = reinterpret_cast<const float4*>(q_of(own) + g * D);
-      float s0 = 0.0f, s1 = 0.0f;
+      float s[S::R / 8];
+      float top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < S::kChunks / 4; ++i) {
-        const float4 x = q[4 * i + qd];
-        s0 = fmaf(k[i].x, x.x, s0);
-        s1 = fmaf(k[i].y, x.y, s1);
-        s0 = fmaf(k[i].z, x.z, s0);
-        s1 = fmaf(k[i].w, x.w, s1);
+      for (int t = 0; t < S::R / 8; ++t) {
+        float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < S::kChunks / 4; ++i) {
+          const float4 x = q[4 * i + qd];
+          s0 = fmaf(k[t][i].x, x.x, s0);
+          s1 = fmaf(k[t][i].y, x.y, s1);
+          s0 = fmaf(k[t][i].z, x.z, s0);
+          s1 = fmaf(k[t][i].w, x.w, s1);
+        }
+        s[t] = s0 + s1;
+        s[t] += __shfl_xor_sync(0xffffffffu, s[t], 1);
+        s[t] += __shfl_xor_sync(0xffffffffu, s[t], 2);
+        s[t] = (mask >> (r + 8 * t)) & 1u ? s[t] * p.scale2 : -INFINITY;
+        if (p.scores != nullptr && qd == 0)
+          p.scores[(row0 + g) * p.s_stride + c.t * S::R + r + 8 * t] = s[t];
+        top = fmaxf(top, s[t]);
       }
-      float s = s0 + s1;
-      s += __shfl_xor_sync(0xffffffffu, s, 1);
-      s += __shfl_xor_sync(0xffffffffu, s, 2);
-      s = valid ? s * p.scale2 : -INFINITY;
-      if (p.scores != nullptr && qd == 0) p.scores[(row0 + g) * p.s_stride + c.t * S::R + r] = s;
-      if (__any_sync(0xffffffffu, s > m[g] + 8.0f)) {
-        float top = s;
+      if (__any_sync(0xffffffffu, top > m[g] + 8.0f)) {
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
         const float mn = fmaxf(m[g], top);
@@ -529,9 +577,12 @@ struct PaState32 {
 #pragma unroll
         for (int e = 0; e < E; ++e) o[g][e] *= a;
       }
-      const float w = pa_exp2(s - (m[g] == -INFINITY ? 0.0f : m[g]));
-      l[g] += qd == 0 ? w : 0.0f;
-      if (qd == 0) p_of(own)[g * S::R + r] = w;
+#pragma unroll
+      for (int t = 0; t < S::R / 8; ++t) {
+        const float w = pa_exp2(s[t] - (m[g] == -INFINITY ? 0.0f : m[g]));
+        l[g] += qd == 0 ? w : 0.0f;
+        if (qd == 0) p_of(own)[g * S::R + r + 8 * t] = w;
+      }
     }
     __syncwarp();
   }
@@ -917,7 +968,7 @@ static PagedAttendLayout pa_layout(int B, int H, int G, int D, int max_slots, bo
   w.rec = take(sizeof(PaRecord) * w.ctas);
   w.part = take(sizeof(float) * 2 * w.ctas * (G <= 8 ? 8 : 16) * (D + 2));
   w.stats = weights ? take(sizeof(float2) * static_cast<size_t>(B) * H) : 0;
-  w.s_stride = (static_cast<int64_t>(max_slots) + 15) / 16 * 16;
+  w.s_stride = (static_cast<int64_t>(max_slots) + 31) / 32 * 32;  // whole tiles are stored
   w.scores = weights ? take(sizeof(float) * static_cast<size_t>(B) * H * w.s_stride) : 0;
   w.total = off;
   return w;
@@ -945,7 +996,7 @@ static int pa_launch(const PagedAttendParams& p, int ctas, cudaStream_t s) {
   if (ensure_smem_attr(reinterpret_cast<const void*>(kernel), S::kSmem) != cudaSuccess)
     return DCR_ERR_CUDA;
   PagedAttendParams q = p;
-  q.page16 = p.c.page.d % S::R == 0;
+  q.page16 = p.c.page.d % S::kGroup == 0;
   kernel<<<ctas, kPaThreads, S::kSmem, s>>>(q);
   if (cudaGetLastError() != cudaSuccess) return DCR_ERR_CUDA;
   const int rows = p.G < HB ? p.G : HB;
