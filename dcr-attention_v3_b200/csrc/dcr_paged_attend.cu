@@ -47,14 +47,6 @@ constexpr int kPaMinTiles = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// What a CTA's first open unit needs of the fold kernel: the unit and the last CTA of it.
-struct PaRecord {
-  int32_t b;
-  int32_t u;     // -1: nothing begins in this CTA that ends in a later one
-  int32_t last;
-  int32_t pad;
-};
-
 struct PagedAttendParams {
   PagePool c;
   const void* q;
@@ -70,7 +62,6 @@ struct PagedAttendParams {
   float* lse;     // [B][H] natural log, or null
   float2* stats;  // [B][H] (maximum in base 2, 1 / sum), with scores
   float* part;    // [CTAs][2][HB][D + 2]: o, m, l of the open units
-  PaRecord* rec;  // [CTAs]
   float* scores;  // [B][H][s_stride] base-2 scores, or null
   int64_t s_stride;
 };
@@ -115,6 +106,12 @@ __device__ __forceinline__ void pa_store_stats(const PagedAttendParams& p, int64
   if (p.stats != nullptr) p.stats[row] = l == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(m, 1.0f / l);
 }
 
+// Adds a state's sum x (with maximum m) to one with maximum M >= m. A state without any valid
+// slot (m = -inf) adds nothing; a NaN goes through.
+__device__ __forceinline__ void pa_fold_sum(float M, float m, float x, float& sum) {
+  sum = m == -INFINITY ? (x != x ? x : sum) : fmaf(pa_exp2(m - M), x, sum);
+}
+
 template <typename T>
 __device__ __forceinline__ void pa_store2(T* dst, float a, float b) {
   if constexpr (std::is_same<T, __half>::value)
@@ -151,33 +148,63 @@ __device__ __forceinline__ void pa_next(const PagedAttendParams& p, PaCursor& c)
   c.t = c.t_lo;
 }
 
-// Sum over the sequences of their tiles (all lanes get it).
+__device__ __forceinline__ uint64_t pa_div(uint64_t a, uint32_t b) {
+  return (a >> 32) == 0 ? static_cast<uint32_t>(a) / b : a / b;
+}
+
+// How the line is shared out: every CTA gets `each` tiles, the first `more` one more.
+struct PaLine {
+  int64_t total, each;
+  int ctas, more;
+  int n_lane;  // tiles of sequence `lane`, for the search that follows
+
+  __device__ __forceinline__ int64_t begin(int c) const { return c * each + (c < more ? c : more); }
+  __device__ __forceinline__ int cta_of(int64_t place) const {
+    const int64_t big = more * (each + 1);
+    return place < big ? static_cast<int>(place / (each + 1))
+                       : more + static_cast<int>((place - big) / each);
+  }
+};
+
 template <int R>
-__device__ __forceinline__ int64_t pa_total(const PagedAttendParams& p) {
+__device__ __forceinline__ PaLine pa_line(const PagedAttendParams& p, int ctas) {
   const int lane = threadIdx.x & 31;
+  PaLine a;
+  a.n_lane = 0;
   int64_t n = 0;
   for (int b = lane; b < p.B; b += 32) {
     int len, lo, t_lo, t_hi;
     pa_sequence<R>(p, b, len, lo, t_lo, t_hi);
+    if (b == lane) a.n_lane = t_hi - t_lo;
     n += t_hi - t_lo;
   }
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-  return n * p.units;
+  a.total = n * p.units;
+  const int64_t want = (a.total + kPaMinTiles - 1) / kPaMinTiles;
+  a.ctas = want < ctas ? static_cast<int>(want) : ctas;
+  a.each = a.ctas > 0 ? pa_div(a.total, a.ctas) : 0;
+  a.more = static_cast<int>(a.total - a.each * a.ctas);
+  return a;
 }
 
 // The cursor at place s (< total) of the line.
 template <int R>
-__device__ __forceinline__ PaCursor pa_seek(const PagedAttendParams& p, int64_t s) {
+__device__ __forceinline__ PaCursor pa_seek(const PagedAttendParams& p, const PaLine& line,
+                                            int64_t s) {
   const int lane = threadIdx.x & 31;
   int64_t before = 0;
+#pragma unroll 1
   for (int b0 = 0;; b0 += 32) {
     const int b = b0 + lane;
-    int n = 0;
-    if (b < p.B) {
-      int len, lo, t_lo, t_hi;
-      pa_sequence<R>(p, b, len, lo, t_lo, t_hi);
-      n = t_hi - t_lo;
+    int n = line.n_lane;
+    if (b0 > 0) {
+      n = 0;
+      if (b < p.B) {
+        int len, lo, t_lo, t_hi;
+        pa_sequence<R>(p, b, len, lo, t_lo, t_hi);
+        n = t_hi - t_lo;
+      }
     }
     int64_t incl = n;
 #pragma unroll
@@ -191,10 +218,9 @@ __device__ __forceinline__ PaCursor pa_seek(const PagedAttendParams& p, int64_t 
       PaCursor c;
       c.b = b0 + src < p.B ? b0 + src : p.B - 1;
       pa_sequence<R>(p, c.b, c.len, c.lo, c.t_lo, c.t_hi);
-      const int64_t base = before + __shfl_sync(0xffffffffu, incl - n, src) * p.units;
+      const int64_t off = s - (before + __shfl_sync(0xffffffffu, incl - n, src) * p.units);
       const int nt = c.t_hi - c.t_lo;
-      const int64_t off = s - base;
-      c.u = nt > 0 ? static_cast<int>(off / nt) : 0;
+      c.u = nt > 0 ? static_cast<int>(pa_div(off, nt)) : 0;
       c.t = c.t_lo + static_cast<int>(off - static_cast<int64_t>(c.u) * nt);
       return c;
     }
@@ -664,7 +690,6 @@ struct PaState32 {
 struct PaPiece {
   int b, u;          // u < 0: none
   int before, after;
-  int64_t end;       // the unit's end on the line
 };
 
 template <typename T, int D, int HB>
@@ -681,73 +706,51 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const Paged
   uint8_t* extra = own + S::kPiece;                       // fp32: queries and weights
   uint32_t* masks = reinterpret_cast<uint32_t*>(own + S::kPiece + S::kQ + S::kP);  // [16]
 
-  // rows of empty sequences
-  for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
-    int len, lo, t_lo, t_hi;
-    pa_sequence<S::R>(p, b, len, lo, t_lo, t_hi);
-    if (t_lo < t_hi) continue;
-    const int64_t row0 = static_cast<int64_t>(b) * p.H;
-    for (int i = threadIdx.x; i < p.H * D; i += kPaThreads)
-      ElemTraits<T>::store(static_cast<T*>(p.o) + row0 * D, i, 0.0f);
-    if (p.lse != nullptr)
-      for (int i = threadIdx.x; i < p.H; i += kPaThreads) p.lse[row0 + i] = -INFINITY;
-  }
-
-  const int64_t total = pa_total<S::R>(p);
-  int64_t ctas = (total + kPaMinTiles - 1) / kPaMinTiles;
-  if (ctas > gridDim.x) ctas = gridDim.x;
-  if (blockIdx.x >= ctas) {
-    if (threadIdx.x == 0) p.rec[blockIdx.x].u = -1;
-    return;
-  }
-  const int64_t c0 = blockIdx.x * total / ctas, c1 = (blockIdx.x + 1) * total / ctas;
-  const int64_t s0 = c0 + warp * (c1 - c0) / kPaWarps, s1 = c0 + (warp + 1) * (c1 - c0) / kPaWarps;
-  const int n = static_cast<int>(s1 - s0);
+  const PaLine line = pa_line<S::R>(p, gridDim.x);
+  const bool works = static_cast<int>(blockIdx.x) < line.ctas;
+  const int64_t c0 = line.begin(blockIdx.x);
+  const int n_cta = works ? static_cast<int>(line.each) + (static_cast<int>(blockIdx.x) < line.more) : 0;
+  const int rest = n_cta % kPaWarps;
+  const int n = n_cta / kPaWarps + (warp < rest);
+  const int64_t s0 = c0 + warp * (n_cta / kPaWarps) + (warp < rest ? warp : rest);
   if (lane == 0) pieces[2 * warp].u = pieces[2 * warp + 1].u = -1;
 
   if (n > 0) {
-    PaCursor in = pa_seek<S::R>(p, s0);  // where loads are
-    PaCursor at = in;                    // where the arithmetic is
+    PaCursor in = pa_seek<S::R>(p, line, s0);  // where loads are
+    PaCursor at = in;                          // where the arithmetic is
     PaLoader<T, D, HB> load;
     State st;
-    constexpr int kAhead = S::NH - 1;    // half tiles in flight, an even number
-    int hs_in = 0, t_in = 0;             // ring place and tile count of the loads
-    auto issue_keys = [&]() {
-      if (t_in < n) {
-        const uint32_t mask = load.keys(p, in, ring + hs_in * S::kHalf);
-        if (lane == 0) masks[t_in & 15] = mask;
-      }
-      cp_async_commit();
-      hs_in = hs_in + 1 == S::NH ? 0 : hs_in + 1;
-    };
-    auto issue_values = [&]() {
-      if (t_in < n) {
-        load.values(p, ring + hs_in * S::kHalf);
-        ++t_in;
-        if (t_in < n) pa_next<S::R>(p, in);
-      }
-      cp_async_commit();
-      hs_in = hs_in + 1 == S::NH ? 0 : hs_in + 1;
-    };
-#pragma unroll
-    for (int i = 0; i < kAhead / 2; ++i) {
-      issue_keys();
-      issue_values();
-    }
-    int64_t g0 = s0 - (at.t - at.t_lo);  // the unit's begin on the line
-    int first = at.t;                    // its first tile in this share
-    st.begin(p, at, extra);
+    constexpr int kAhead = (S::NH - 1) / 2;  // tiles in flight
+    int hs_in = 0;                           // ring places of the loads and of the arithmetic
     int hs = 0;
-    for (int i = 0; i < n; ++i) {
-      cp_async_wait<kAhead - 1>();
+    int first = at.t;                        // its first tile in this share
+    st.begin(p, at, extra);
+    // the first kAhead turns only load; every turn's loads are kAhead tiles ahead
+#pragma unroll 1
+    for (int i = -kAhead; i < n; ++i) {
+      const int j = i + kAhead;
+      cp_async_wait<2 * kAhead - 1>();
       __syncwarp();
-      issue_keys();
+      if (j < n) {
+        const uint32_t m = load.keys(p, in, ring + hs_in * S::kHalf);
+        if (lane == 0) masks[j & 15] = m;
+      }
+      cp_async_commit();
+      hs_in = hs_in + 1 == S::NH ? 0 : hs_in + 1;
       const uint32_t mask = masks[i & 15];
-      st.scores(p, at, ring + hs * S::kHalf, mask, extra);
-      hs = hs + 1 == S::NH ? 0 : hs + 1;
-      cp_async_wait<kAhead - 1>();
-      __syncwarp();
-      issue_values();
+      if (i >= 0) {
+        st.scores(p, at, ring + hs * S::kHalf, mask, extra);
+        hs = hs + 1 == S::NH ? 0 : hs + 1;
+        cp_async_wait<2 * kAhead - 1>();
+        __syncwarp();
+      }
+      if (j < n) {
+        load.values(p, ring + hs_in * S::kHalf);
+        if (j + 1 < n) pa_next<S::R>(p, in);
+      }
+      cp_async_commit();
+      hs_in = hs_in + 1 == S::NH ? 0 : hs_in + 1;
+      if (i < 0) continue;
       st.values(ring + hs * S::kHalf, mask, extra);
       hs = hs + 1 == S::NH ? 0 : hs + 1;
       const bool ends = at.t + 1 == at.t_hi;
@@ -772,13 +775,11 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const Paged
             pc.u = at.u;
             pc.before = before;
             pc.after = !ends;
-            pc.end = g0 + (at.t_hi - at.t_lo);
           }
         }
         if (i + 1 < n) {
           pa_next<S::R>(p, at);
           first = at.t;
-          g0 = s0 + i + 1;
           st.begin(p, at, extra);
         }
       } else {
@@ -789,8 +790,14 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const Paged
   }
   __syncthreads();
 
-  // Fold the CTA's pieces: runs of pieces of one unit, row by row over the warps.
-  bool opens = false;
+  // Fold the CTA's pieces: runs of pieces of one unit, row by row over the warps. Odd pieces
+  // are in the rings, even ones in the warps' own places.
+  auto piece_at = [&](int x) {
+    return reinterpret_cast<const float*>(
+        (x & 1) ? pa_smem + (x >> 1) * (S::NH * S::kHalf)
+                : pa_smem + kPaWarps * (S::NH * S::kHalf) + (x >> 1) * (S::kPiece + S::kQ + S::kP + 64));
+  };
+#pragma unroll 1
   for (int i = 0; i < 2 * kPaWarps;) {
     const PaPiece lead = pieces[i];
     if (lead.u < 0) {
@@ -805,32 +812,18 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const Paged
     const bool before = lead.before, after = pieces[last].after;
     const int hk = lead.u / p.hblocks, h0 = (lead.u - hk * p.hblocks) * HB;
     const int rows = p.G - h0 < HB ? p.G - h0 : HB;
+#pragma unroll 1
     for (int g = warp; g < rows; g += kPaWarps) {
       float M = -INFINITY;
-      for (int x = i; x <= last; ++x) {
-        if (pieces[x].u < 0) continue;
-        const float* src = (x & 1) ? reinterpret_cast<const float*>(pa_smem + (x >> 1) * (S::NH * S::kHalf))
-                                   : reinterpret_cast<const float*>(
-                                         pa_smem + kPaWarps * (S::NH * S::kHalf) +
-                                         (x >> 1) * (S::kPiece + S::kQ + S::kP + 64));
-        M = fmaxf(M, src[g * (D + 2) + D]);
-      }
+      for (int x = i; x <= last; ++x)
+        if (pieces[x].u >= 0) M = fmaxf(M, piece_at(x)[g * (D + 2) + D]);
       float L = 0.0f, acc[D / 32] = {};
       for (int x = i; x <= last; ++x) {
         if (pieces[x].u < 0) continue;
-        const float* src = (x & 1) ? reinterpret_cast<const float*>(pa_smem + (x >> 1) * (S::NH * S::kHalf))
-                                   : reinterpret_cast<const float*>(
-                                         pa_smem + kPaWarps * (S::NH * S::kHalf) +
-                                         (x >> 1) * (S::kPiece + S::kQ + S::kP + 64));
-        const float mm = src[g * (D + 2) + D];
-        const float a = mm == -INFINITY ? 0.0f : pa_exp2(mm - M);
-        const float ll = src[g * (D + 2) + D + 1];
-        L += ll != ll ? ll : a * ll;
+        const float* src = piece_at(x) + g * (D + 2);
+        pa_fold_sum(M, src[D], src[D + 1], L);
 #pragma unroll
-        for (int e = 0; e < D / 32; ++e) {
-          const float v = src[g * (D + 2) + lane + 32 * e];
-          acc[e] = mm == -INFINITY ? (v != v ? v : acc[e]) : fmaf(a, v, acc[e]);
-        }
+        for (int e = 0; e < D / 32; ++e) pa_fold_sum(M, src[D], src[lane + 32 * e], acc[e]);
       }
       if (!before && !after) {
         const int64_t row = static_cast<int64_t>(lead.b) * p.H + hk * p.G + h0 + g;
@@ -849,73 +842,92 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const Paged
         }
       }
     }
-    if (!before && after) {
-      opens = true;
-      if (threadIdx.x == 0) {
-        PaRecord r;
-        r.b = lead.b;
-        r.u = lead.u;
-        // the CTA whose share holds the unit's last tile: the largest c with c*total/ctas < end
-        r.last = static_cast<int32_t>((lead.end * ctas - 1) / total);
-        r.pad = 0;
-        p.rec[blockIdx.x] = r;
-      }
-    }
     i = j;
   }
-  if (!opens && threadIdx.x == 0) p.rec[blockIdx.x].u = -1;
+
+  // rows of empty sequences
+#pragma unroll 1
+  for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
+    int len, lo, t_lo, t_hi;
+    pa_sequence<S::R>(p, b, len, lo, t_lo, t_hi);
+    if (t_lo < t_hi) continue;
+    const int64_t row0 = static_cast<int64_t>(b) * p.H;
+    for (int i = threadIdx.x; i < p.H * D; i += kPaThreads)
+      ElemTraits<T>::store(static_cast<T*>(p.o) + row0 * D, i, 0.0f);
+    for (int i = threadIdx.x; i < p.H; i += kPaThreads) pa_store_stats(p, row0 + i, 0.0f, 0.0f);
+  }
 }
 
 // Folds the partials of the unit that begins in CTA blockIdx.x of the first kernel and ends in
-// a later one; blockIdx.y is the row of the head block. Thread groups of D take every
-// (128 / D)-th partial.
+// a later one; blockIdx.y is the row of the head block. What there is to fold follows from the
+// lengths, so it is known before the first kernel is done; then one round of loads is left.
+// Thread groups of D take every (256 / D)-th partial.
 template <typename T, int D, int HB>
-__global__ void __launch_bounds__(128) paged_fold_kernel(const PagedAttendParams p) {
-  constexpr int N = 128 / D;
-  __shared__ float m_s[4], acc_s[128], l_s[2];
+__global__ void __launch_bounds__(256) paged_fold_kernel(const PagedAttendParams p) {
+  using S = PaShape<T, D, HB>;
+  constexpr int N = 256 / D, kBatch = 8;
+  __shared__ float m_s[N], l_s[N], acc_s[256];
   asm volatile("griddepcontrol.launch_dependents;");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const PaRecord r = p.rec[blockIdx.x];
-  if (r.u < 0) return;
-  const int hk = r.u / p.hblocks;
-  const int g = blockIdx.y, h = (r.u - hk * p.hblocks) * HB + g;
-  if (h >= p.G) return;
+  const PaLine line = pa_line<S::R>(p, gridDim.x);
   const int c0 = blockIdx.x;
-  auto part = [&](int c) {
-    return p.part + ((2 * static_cast<int64_t>(c) + (c == c0 ? 1 : 0)) * HB + g) * (D + 2);
-  };
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float M = -INFINITY;
-  for (int c = c0 + threadIdx.x; c <= r.last; c += 128) M = fmaxf(M, part(c)[D]);
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  if (lane == 0) m_s[warp] = M;
-  __syncthreads();
-  M = fmaxf(fmaxf(m_s[0], m_s[1]), fmaxf(m_s[2], m_s[3]));
-  const int d = threadIdx.x % D, k = threadIdx.x / D;
-  float acc = 0.0f, L = 0.0f;
-#pragma unroll 4
-  for (int c = c0 + k; c <= r.last; c += N) {
-    const float* s = part(c);
-    const float mm = s[D], ll = s[D + 1], v = s[d];
-    const float a = mm == -INFINITY ? 0.0f : pa_exp2(mm - M);
-    L += ll != ll ? ll : a * ll;
-    acc = mm == -INFINITY ? (v != v ? v : acc) : fmaf(a, v, acc);
+  const int64_t end_cta = line.begin(c0 + 1);
+  bool open = c0 + 1 < line.ctas;
+  PaCursor c;
+  int last = 0, hk = 0, h = 0;
+  if (open) {
+    c = pa_seek<S::R>(p, line, end_cta - 1);
+    const int64_t begin = end_cta - 1 - (c.t - c.t_lo), end = begin + (c.t_hi - c.t_lo);
+    hk = c.u / p.hblocks;
+    h = (c.u - hk * p.hblocks) * HB + blockIdx.y;
+    open = begin >= line.begin(c0) && end > end_cta && h < p.G;
+    if (open) last = line.cta_of(end - 1);
   }
-  if (N > 1) {
-    acc_s[threadIdx.x] = acc;
-    if (d == 0) l_s[k] = L;
-    __syncthreads();
-    if (k > 0) return;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!open) return;
+  const int d = threadIdx.x % D, k = threadIdx.x / D;
+  float M = -INFINITY, L = 0.0f, acc = 0.0f;
+  for (int c1 = c0 + k; c1 <= last; c1 += N * kBatch) {
+    float m[kBatch], l[kBatch], v[kBatch];
 #pragma unroll
-    for (int i = 1; i < N; ++i) {
-      acc += acc_s[i * D + d];
-      L += l_s[i];
+    for (int i = 0; i < kBatch; ++i) {
+      const int x = c1 + N * i;
+      const float* src = p.part + ((2 * static_cast<int64_t>(x) + (x == c0 ? 1 : 0)) * HB + blockIdx.y) * (D + 2);
+      m[i] = x <= last ? src[D] : -INFINITY;
+      l[i] = x <= last ? src[D + 1] : 0.0f;
+      v[i] = x <= last ? src[d] : 0.0f;
+    }
+    float top = M;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) top = fmaxf(top, m[i]);
+    const float a = M == -INFINITY ? 0.0f : pa_exp2(M - top);
+    L = M == -INFINITY ? L : L * a;
+    acc = M == -INFINITY ? acc : acc * a;
+    M = top;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      pa_fold_sum(M, m[i], l[i], L);
+      pa_fold_sum(M, m[i], v[i], acc);
     }
   }
-  const int64_t row = static_cast<int64_t>(r.b) * p.H + hk * p.G + h;
-  ElemTraits<T>::store(static_cast<T*>(p.o) + row * D, d, L == 0.0f ? 0.0f : acc / L);
-  if (d == 0) pa_store_stats(p, row, M, L);
+  acc_s[threadIdx.x] = acc;
+  if (d == 0) {
+    m_s[k] = M;
+    l_s[k] = L;
+  }
+  __syncthreads();
+  if (k > 0) return;
+  float top = M;
+#pragma unroll
+  for (int i = 1; i < N; ++i) top = fmaxf(top, m_s[i]);
+  float sl = 0.0f, sa = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    pa_fold_sum(top, m_s[i], l_s[i], sl);
+    pa_fold_sum(top, m_s[i], acc_s[i * D + d], sa);
+  }
+  const int64_t row = static_cast<int64_t>(c.b) * p.H + hk * p.G + h;
+  ElemTraits<T>::store(static_cast<T*>(p.o) + row * D, d, sl == 0.0f ? 0.0f : sa / sl);
+  if (d == 0) pa_store_stats(p, row, top, sl);
 }
 
 // weights[b][h_kv][i] += sum over the G heads of exp2(score - m) / l, in head order.
@@ -945,7 +957,7 @@ __global__ void __launch_bounds__(256) paged_weights_kernel(const PagedAttendPar
 
 // Workspace sections.
 struct PagedAttendLayout {
-  size_t rec, part, stats, scores, total;
+  size_t part, stats, scores, total;
   int64_t s_stride;
   int ctas;
 };
@@ -965,7 +977,6 @@ static PagedAttendLayout pa_layout(int B, int H, int G, int D, int max_slots, bo
     off = (off + n + 255) / 256 * 256;
     return at;
   };
-  w.rec = take(sizeof(PaRecord) * w.ctas);
   w.part = take(sizeof(float) * 2 * w.ctas * (G <= 8 ? 8 : 16) * (D + 2));
   w.stats = weights ? take(sizeof(float2) * static_cast<size_t>(B) * H) : 0;
   w.s_stride = (static_cast<int64_t>(max_slots) + 31) / 32 * 32;  // whole tiles are stored
@@ -1000,7 +1011,7 @@ static int pa_launch(const PagedAttendParams& p, int ctas, cudaStream_t s) {
   kernel<<<ctas, kPaThreads, S::kSmem, s>>>(q);
   if (cudaGetLastError() != cudaSuccess) return DCR_ERR_CUDA;
   const int rows = p.G < HB ? p.G : HB;
-  if (pa_launch_dependent(paged_fold_kernel<T, D, HB>, dim3(ctas, rows), dim3(128), s, q) != cudaSuccess)
+  if (pa_launch_dependent(paged_fold_kernel<T, D, HB>, dim3(ctas, rows), dim3(256), s, q) != cudaSuccess)
     return DCR_ERR_CUDA;
   return DCR_OK;
 }
@@ -1075,7 +1086,6 @@ int dcr_paged_attend(const void* q, int64_t q_stride_b, int64_t q_stride_h, cons
   p.lse = lse;
   p.stats = weights != nullptr ? reinterpret_cast<float2*>(ws + w.stats) : nullptr;
   p.part = reinterpret_cast<float*>(ws + w.part);
-  p.rec = reinterpret_cast<PaRecord*>(ws + w.rec);
   p.scores = weights != nullptr ? reinterpret_cast<float*>(ws + w.scores) : nullptr;
   p.s_stride = w.s_stride;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
