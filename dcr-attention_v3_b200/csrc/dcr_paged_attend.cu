@@ -229,15 +229,14 @@ __device__ __forceinline__ PaCursor pa_seek(const PagedAttendParams& p, const Pa
 }
 
 // The copies of one tile: K's rows, then V's. Where pages hold whole groups of 16 slots (or R,
-// if that is less), a tile of valid slots, which is all but the ends of a sequence, looks a
-// page up per group and takes its rows by a fixed stride; any other looks every row up, and
-// fills the slots that are not valid with zeros.
+// if that is less) a page is looked up per group and its rows are a fixed stride apart;
+// otherwise every row is looked up. Slots that are not valid are filled with zeros: a copy of
+// no bytes reads nothing, whatever its address.
 template <typename T, int D, int HB>
 struct PaLoader {
   using S = PaShape<T, D, HB>;
   static constexpr uint32_t kAll = 0xffffffffu >> (32 - S::R);
-  const char* next_v[S::kGroups];  // this lane's first V row of each group, when `whole`
-  bool whole;
+  const char* next_v[S::kGroups];  // this lane's first V row of each group of the tile under way
   int b, hk, slot0;
   uint32_t mask;
 
@@ -252,48 +251,51 @@ struct PaLoader {
     const int from = c.lo > slot0 ? c.lo - slot0 : 0;
     const int to = c.len - slot0 < S::R ? c.len - slot0 : S::R;
     mask = (0xffffffffu >> (32 - to)) & (0xffffffffu << from);
-    whole = p.page16 && mask == kAll;
-    if (whole) {
-      const char* src[S::kGroups];
-#pragma unroll
-      for (int g = 0; g < S::kGroups; ++g) {
-        const int s0 = slot0 + g * S::kGroup;
-        const uint32_t pi = p.c.page.div(s0);
-        const int pg = page_of(p.c, b, pi);
-        const int in = s0 - static_cast<int>(pi * p.c.page.d) + r0;
-        whole = whole && pg >= 0;
-        src[g] = static_cast<const char*>(p.c.k) + ch * 16 +
-                 (pg * p.c.ksp + hk * p.c.ksh + in * p.c.ksr) * static_cast<int64_t>(sizeof(T));
-        next_v[g] = static_cast<const char*>(p.c.v) + ch * 16 +
-                    (pg * p.c.vsp + hk * p.c.vsh + in * p.c.vsr) * static_cast<int64_t>(sizeof(T));
-      }
-      if (whole) {
-        copy_whole(dst, src, p.c.ksr * static_cast<int64_t>(S::kRowsPer * sizeof(T)));
-        return mask;
-      }
+    if (!p.page16) {
+      mask = copy_each(p, p.c.k, p.c.ksp, p.c.ksh, p.c.ksr, dst);
+      return mask;
     }
-    mask = copy_each(p, p.c.k, p.c.ksp, p.c.ksh, p.c.ksr, dst);
+    const char* src[S::kGroups];
+#pragma unroll
+    for (int g = 0; g < S::kGroups; ++g) {
+      const uint32_t of_group = (0xffffffffu >> (32 - S::kGroup)) << (g * S::kGroup);
+      const int s0 = slot0 + g * S::kGroup;
+      const uint32_t pi = p.c.page.div(s0);
+      const int in = s0 - static_cast<int>(pi * p.c.page.d) + r0;
+      int pg = mask & of_group ? page_of(p.c, b, pi) : -1;
+      if (pg < 0) {
+        mask &= ~of_group;
+        pg = 0;
+      }
+      src[g] = static_cast<const char*>(p.c.k) + ch * 16 +
+               (pg * p.c.ksp + hk * p.c.ksh + in * p.c.ksr) * static_cast<int64_t>(sizeof(T));
+      next_v[g] = static_cast<const char*>(p.c.v) + ch * 16 +
+                  (pg * p.c.vsp + hk * p.c.vsh + in * p.c.vsr) * static_cast<int64_t>(sizeof(T));
+    }
+    copy_groups(dst, src, p.c.ksr * static_cast<int64_t>(S::kRowsPer * sizeof(T)));
     return mask;
   }
 
   __device__ __forceinline__ void values(const PagedAttendParams& p, uint8_t* dst) const {
-    if (whole)
-      copy_whole(dst, next_v, p.c.vsr * static_cast<int64_t>(S::kRowsPer * sizeof(T)));
+    if (p.page16)
+      copy_groups(dst, next_v, p.c.vsr * static_cast<int64_t>(S::kRowsPer * sizeof(T)));
     else
       copy_each(p, p.c.v, p.c.vsp, p.c.vsh, p.c.vsr, dst);
   }
 
-  __device__ __forceinline__ static void copy_whole(uint8_t* dst, const char* const (&src)[S::kGroups],
-                                                    int64_t step) {
+  __device__ __forceinline__ void copy_groups(uint8_t* dst, const char* const (&src)[S::kGroups],
+                                              int64_t step) const {
     const int lane = threadIdx.x & 31;
+    const uint32_t bits = mask >> (lane / S::kChunks);
     constexpr int kPer = S::kCopies / S::kGroups;
 #pragma unroll
     for (int g = 0; g < S::kGroups; ++g) {
-      const char* at_g = src[g];
+      const char* from = src[g];
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        cp_async_16(dst + at(lane / S::kChunks + (g * kPer + i) * S::kRowsPer, lane % S::kChunks), at_g, 16u);
-        at_g += step;
+        const int r = (g * kPer + i) * S::kRowsPer;
+        cp_async_16(dst + at(lane / S::kChunks + r, lane % S::kChunks), from, ((bits >> r) & 1u) * 16u);
+        from += step;
       }
     }
   }
@@ -790,47 +792,49 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const Paged
   }
   __syncthreads();
 
-  // Fold the CTA's pieces: runs of pieces of one unit, row by row over the warps. Odd pieces
-  // are in the rings, even ones in the warps' own places.
-  auto piece_at = [&](int x) {
-    return reinterpret_cast<const float*>(
-        (x & 1) ? pa_smem + (x >> 1) * (S::NH * S::kHalf)
-                : pa_smem + kPaWarps * (S::NH * S::kHalf) + (x >> 1) * (S::kPiece + S::kQ + S::kP + 64));
-  };
-#pragma unroll 1
-  for (int i = 0; i < 2 * kPaWarps;) {
-    const PaPiece lead = pieces[i];
-    if (lead.u < 0) {
-      ++i;
-      continue;
-    }
-    int j = i + 1, last = i;
-    while (j < 2 * kPaWarps && (pieces[j].u < 0 || (pieces[j].u == lead.u && pieces[j].b == lead.b))) {
-      if (pieces[j].u >= 0) last = j;
-      ++j;
-    }
-    const bool before = lead.before, after = pieces[last].after;
-    const int hk = lead.u / p.hblocks, h0 = (lead.u - hk * p.hblocks) * HB;
+  // Fold the CTA's pieces, row by row over the warps; lane x holds piece x. The pieces of a
+  // unit are neighbours. Odd pieces are in the rings, even ones in the warps' own places.
+  const PaPiece mine = pieces[lane % (2 * kPaWarps)];
+  const bool have = lane < 2 * kPaWarps && mine.u >= 0;
+  const float* own_piece = reinterpret_cast<const float*>(
+      (lane & 1) ? pa_smem + (lane >> 1) % kPaWarps * (S::NH * S::kHalf)
+                 : pa_smem + kPaWarps * (S::NH * S::kHalf) +
+                       (lane >> 1) % kPaWarps * (S::kPiece + S::kQ + S::kP + 64));
+  unsigned todo = __ballot_sync(0xffffffffu, have);
+  while (todo != 0) {
+    const int lead = __ffs(todo) - 1;
+    const int b = __shfl_sync(0xffffffffu, mine.b, lead), u = __shfl_sync(0xffffffffu, mine.u, lead);
+    const bool in = have && mine.b == b && mine.u == u;
+    const unsigned run = __ballot_sync(0xffffffffu, in);
+    todo &= ~run;
+    const bool before = __shfl_sync(0xffffffffu, mine.before, lead);
+    const bool after = __shfl_sync(0xffffffffu, mine.after, 31 - __clz(run));
+    const int hk = u / p.hblocks, h0 = (u - hk * p.hblocks) * HB;
     const int rows = p.G - h0 < HB ? p.G - h0 : HB;
-#pragma unroll 1
     for (int g = warp; g < rows; g += kPaWarps) {
-      float M = -INFINITY;
-      for (int x = i; x <= last; ++x)
-        if (pieces[x].u >= 0) M = fmaxf(M, piece_at(x)[g * (D + 2) + D]);
-      float L = 0.0f, acc[D / 32] = {};
-      for (int x = i; x <= last; ++x) {
-        if (pieces[x].u < 0) continue;
-        const float* src = piece_at(x) + g * (D + 2);
-        pa_fold_sum(M, src[D], src[D + 1], L);
+      const float m = in ? own_piece[g * (D + 2) + D] : -INFINITY;
+      float M = m;
 #pragma unroll
-        for (int e = 0; e < D / 32; ++e) pa_fold_sum(M, src[D], src[lane + 32 * e], acc[e]);
+      for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+      float L = 0.0f;
+      if (in) pa_fold_sum(M, m, own_piece[g * (D + 2) + D + 1], L);
+#pragma unroll
+      for (int o = 16; o >= 1; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+      float acc[D / 32] = {};
+      for (unsigned left = run; left != 0; left &= left - 1) {
+        const int x = __ffs(left) - 1;
+        const float mx = __shfl_sync(0xffffffffu, m, x);
+        const float* src = reinterpret_cast<const float*>(
+            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(own_piece), x));
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) pa_fold_sum(M, mx, src[g * (D + 2) + lane + 32 * e], acc[e]);
       }
       if (!before && !after) {
-        const int64_t row = static_cast<int64_t>(lead.b) * p.H + hk * p.G + h0 + g;
+        const int64_t row = static_cast<int64_t>(b) * p.H + hk * p.G + h0 + g;
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
         for (int e = 0; e < D / 32; ++e)
-          ElemTraits<T>::store(static_cast<T*>(p.o) + row * D, lane + 32 * e,
-                               L == 0.0f ? 0.0f : acc[e] / L);
+          ElemTraits<T>::store(static_cast<T*>(p.o) + row * D, lane + 32 * e, acc[e] * inv);
         if (lane == 0) pa_store_stats(p, row, M, L);
       } else {
         float* dst = p.part + ((2 * static_cast<int64_t>(blockIdx.x) + (before ? 0 : 1)) * HB + g) * (D + 2);
@@ -842,7 +846,6 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const Paged
         }
       }
     }
-    i = j;
   }
 
   // rows of empty sequences
