@@ -988,21 +988,6 @@ static PagedAttendLayout pa_layout(int B, int H, int G, int D, int max_slots, bo
   return w;
 }
 
-template <typename... Args>
-static cudaError_t pa_launch_dependent(void (*kernel)(Args...), dim3 grid, dim3 block,
-                                       cudaStream_t s, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 template <typename T, int D, int HB>
 static int pa_launch(const PagedAttendParams& p, int ctas, cudaStream_t s) {
   using S = PaShape<T, D, HB>;
@@ -1014,7 +999,7 @@ static int pa_launch(const PagedAttendParams& p, int ctas, cudaStream_t s) {
   kernel<<<ctas, kPaThreads, S::kSmem, s>>>(q);
   if (cudaGetLastError() != cudaSuccess) return DCR_ERR_CUDA;
   const int rows = p.G < HB ? p.G : HB;
-  if (pa_launch_dependent(paged_fold_kernel<T, D, HB>, dim3(ctas, rows), dim3(256), s, q) != cudaSuccess)
+  if (launch_dependent(paged_fold_kernel<T, D, HB>, dim3(ctas, rows), dim3(256), s, q) != cudaSuccess)
     return DCR_ERR_CUDA;
   return DCR_OK;
 }
@@ -1101,7 +1086,7 @@ int dcr_paged_attend(const void* q, int64_t q_stride_b, int64_t q_stride_h, cons
   if (rc != DCR_OK || weights == nullptr) return rc;
   const int chunk = 1024;
   const dim3 grid((max_slots + chunk - 1) / chunk, H_kv, B < 65535 ? B : 65535);
-  return pa_launch_dependent(paged_weights_kernel, grid, dim3(256), s, p, weights, w_stride_b,
+  return launch_dependent(paged_weights_kernel, grid, dim3(256), s, p, weights, w_stride_b,
                              w_stride_h, chunk) == cudaSuccess
              ? DCR_OK
              : DCR_ERR_CUDA;

@@ -10,18 +10,31 @@
 // the slot its row came from; weights and positions are gathered to new tables. The reference
 // has no counterpart (its cache only grows).
 //
-// Kernel 1, one CTA a row: the budget-th largest 32-bit order key by four 8-bit histogram
-// levels in shared memory, then one pass in slot order that matches holes and movers.
-// Kernel 2: gathers the tables and moves the K and V rows.
+// Bound: 8 bytes a slot for the selection and the moved rows' 2 * 2 * D * element bytes; with
+// few slots, latency.
+//
+// Kernel 1, a cluster of C CTAs a row: every thread keeps its slots' 32-bit order keys in
+// registers (a warp's slots are consecutive, 32 at a time); the budget-th largest key by three
+// histogram levels (12, 10 and 10 bits) in shared memory, added up in CTA 0; then one exchange
+// of per-warp counts gives every warp the ranks of its holes and movers, which ballots spread
+// over its slots in slot order. A table of a size that registers cannot hold is read again at
+// every level. Kernel 2 (a programmatic dependent) pairs the i-th hole with the i-th mover and
+// copies the rows, 16 bytes a lane.
+#include <cooperative_groups.h>
+
 #include "dcr_internal.h"
 #include "dcr_paged.cuh"
 
 namespace dcr {
 
+namespace cg = cooperative_groups;
+
 constexpr int kEvThreads = 1024;
+constexpr int kEvWarps = kEvThreads / 32;
+constexpr int kEvBins = 4096;
 
 struct PagedEvictParams {
-  PagePool c;
+  PagePool c;           // strides in 16-byte chunks
   void* k_pages;
   void* v_pages;
   const int32_t* lengths;
@@ -38,9 +51,11 @@ struct PagedEvictParams {
   int64_t posb, posh;
   int32_t* len_out;     // [B]
   int32_t* holes;       // [B * H_kv][budget]
+  int32_t* movers;      // [B * H_kv][budget]
+  int32_t* n_moves;     // [B * H_kv]
 };
 
-// Order of a slot's claim to stay, as an unsigned key: larger stays first.
+// Order of a slot's claim to stay, as an unsigned key (never 0): larger stays first.
 __device__ __forceinline__ uint32_t ev_key(float w, int pos, int sinks, int from) {
   if (pos < sinks || pos >= from) return 0xffffffffu;
   uint32_t u = __float_as_uint(w);
@@ -49,120 +64,279 @@ __device__ __forceinline__ uint32_t ev_key(float w, int pos, int sinks, int from
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Exclusive sum of a flag over the CTA's threads in order, and the total.
-__device__ __forceinline__ int ev_block_rank(bool f, int* warp_sums, int& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const unsigned b = __ballot_sync(0xffffffffu, f);
-  if (lane == 0) warp_sums[warp] = __popc(b);
-  __syncthreads();
-  const int mine = warp_sums[lane];  // kEvThreads / 32 = 32 warps
-  int incl = mine;
+// The whole CTA finds, from the top, the bin in which the k-th largest key of a histogram of
+// 1024 * Q bins lies: *bin, the number of keys above it and in it.
+template <int Q>
+__device__ __forceinline__ void ev_find(const uint32_t* hist, uint32_t k, uint32_t* sums,
+                                        uint32_t* res) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint32_t c[Q], s = 0;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += y;
+  for (int i = 0; i < Q; ++i) {  // descending bins
+    c[i] = hist[kEvThreads * Q - 1 - (tid * Q + i)];
+    s += c[i];
   }
-  total = __shfl_sync(0xffffffffu, incl, 31);
-  const int before = __shfl_sync(0xffffffffu, incl - mine, warp);
+  const uint32_t incl = warp_incl_scan(s);
+  if (lane == 31) sums[warp] = incl;
   __syncthreads();
-  return before + __popc(b & ((1u << lane) - 1u));
+  uint32_t before = lane < warp ? sums[lane] : 0u;
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  uint32_t above = before + incl - s;
+  if (above < k && k <= above + s) {
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+      if (above < k && k <= above + c[i]) {
+        res[0] = static_cast<uint32_t>(kEvThreads * Q - 1 - (tid * Q + i));
+        res[1] = above;
+      }
+      above += c[i];
+    }
+  }
 }
 
+template <int VPT>
 __global__ void __launch_bounds__(kEvThreads) paged_evict_select_kernel(const PagedEvictParams p) {
-  __shared__ uint32_t hist[256];
-  __shared__ int sums[32];
-  __shared__ uint32_t found_s[2];
-  const int tid = threadIdx.x;
-  const int h = blockIdx.x, b = blockIdx.y;
-  const int64_t row = static_cast<int64_t>(b) * p.H_kv + h;
-  const int n = checked_length(p.c, p.lengths[b]);
-  const int from = p.seen[b] - p.recent;
+  __shared__ uint32_t hist[kEvBins + 2048];  // the three levels' bins
+  __shared__ uint32_t sums[kEvWarps];
+  __shared__ uint32_t res[2];
+  __shared__ int4 counts[kEvWarps];          // per warp, then the sums before it
+  __shared__ int4 totals[8];                 // per CTA of the cluster
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = static_cast<int>(cluster.num_blocks());
+  const int rank = static_cast<int>(cluster.block_rank());
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int64_t row = blockIdx.x / C;
+  const int b = static_cast<int>(row / p.H_kv), h = static_cast<int>(row - static_cast<int64_t>(b) * p.H_kv);
+  const int n = checked_length(p.c, __ldg(p.lengths + b));
+  const int from = __ldg(p.seen + b) - p.recent;
   const float* w = p.weights + b * p.wsb + h * p.wsh;
   const int32_t* ps = p.pos + b * p.psb + h * p.psh;
   int32_t* src = p.src + row * p.budget;
-  if (h == 0 && tid == 0) p.len_out[b] = n < p.budget ? n : p.budget;
-  if (n <= p.budget) {
-    for (int i = tid; i < p.budget; i += kEvThreads) src[i] = i < n ? i : -1;
+  float* wo = p.w_out + b * p.wosb + h * p.wosh;
+  int32_t* po = p.pos_out + b * p.posb + h * p.posh;
+  if (h == 0 && rank == 0 && tid == 0) p.len_out[b] = n < p.budget ? n : p.budget;
+  if (n <= p.budget) {  // nothing to evict: all CTAs of the cluster return
+    for (int i = rank * kEvThreads + tid; i < p.budget; i += C * kEvThreads) {
+      src[i] = i < n ? i : -1;
+      wo[i] = i < n ? w[i] : 0.0f;
+      po[i] = i < n ? ps[i] : -1;
+    }
+    if (rank == 0 && tid == 0) p.n_moves[row] = 0;
     return;
   }
-  uint32_t prefix = 0, mask = 0, left = p.budget;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
-    __syncthreads();
-    for (int i = tid; i < n; i += kEvThreads) {
-      const uint32_t key = ev_key(w[i], ps[i], p.sinks, from);
-      if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1u);
-    }
-    __syncthreads();
-    if (tid < 32) {
-      int bin;
-      uint32_t above;
-      warp_find_bin(hist, left, bin, above);
-      if (tid == 0) {
-        found_s[0] = static_cast<uint32_t>(bin);
-        found_s[1] = above;
-      }
-    }
-    __syncthreads();
-    prefix |= found_s[0] << shift;
-    mask |= 255u << shift;
-    left -= found_s[1];
-    __syncthreads();
+
+  const int used = (n + C * kEvThreads - 1) / (C * kEvThreads);  // slots per thread
+  const int base = (rank * kEvWarps + warp) * 32 * used + lane;  // slot j of this lane: + 32 j
+  auto load = [&](int j) {
+    const int i = base + 32 * j;
+    return i < n ? ev_key(w[i], ps[i], p.sinks, from) : 0u;
+  };
+  uint32_t keys[VPT > 0 ? VPT : 1];
+  if constexpr (VPT > 0) {
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) keys[j] = j < used ? load(j) : 0u;
   }
-  // keys above `prefix` stay, and the first `left` that equal it
+  auto each = [&](auto&& f) {
+    if constexpr (VPT > 0) {
+#pragma unroll
+      for (int j = 0; j < VPT; ++j)
+        if (j < used) f(j, keys[j]);
+    } else {
+      for (int j = 0; j < used; ++j) f(j, load(j));
+    }
+  };
+  for (int i = tid; i < kEvBins + 2048; i += kEvThreads) hist[i] = 0;
+  __syncthreads();
+
+  // the threshold T = prefix, level by level: `left` counts from the top within the prefix
+  uint32_t prefix = 0, left = p.budget;
+  auto level = [&](int shift, int bits, uint32_t* bins, auto q) {
+    constexpr int Q = decltype(q)::value;
+    const uint32_t above_mask = bits + shift == 32 ? 0u : 0xffffffffu << (bits + shift);
+    each([&](int, uint32_t key) {
+      if (key != 0u && ((key ^ prefix) & above_mask) == 0u)
+        atomicAdd(bins + ((key >> shift) & ((1u << bits) - 1u)), 1u);
+    });
+    if (C > 1) {
+      cluster.sync();  // the bins of CTA 0 are zeroed and this CTA's are full
+      if (rank > 0) {
+        uint32_t* bins0 = cluster.map_shared_rank(bins, 0);
+        for (int i = tid; i < (1 << bits); i += kEvThreads)
+          if (bins[i] != 0u) atomicAdd(bins0 + i, bins[i]);
+      }
+      cluster.sync();
+      if (rank == 0) {
+        ev_find<Q>(bins, left, sums, res);
+        __syncthreads();
+        if (tid >= 1 && tid < C) {
+          uint32_t* r = cluster.map_shared_rank(res, tid);
+          r[0] = res[0];
+          r[1] = res[1];
+        }
+      }
+      cluster.sync();
+    } else {
+      __syncthreads();
+      ev_find<Q>(bins, left, sums, res);
+      __syncthreads();
+    }
+    prefix |= res[0] << shift;
+    left -= res[1];
+  };
+  level(20, 12, hist, std::integral_constant<int, 4>());
+  level(10, 10, hist + kEvBins, std::integral_constant<int, 1>());
+  level(0, 10, hist + kEvBins + 1024, std::integral_constant<int, 1>());
+
+  // Keys above T stay, and the first `left` that equal it. Per warp: evicted slots below the
+  // budget and kept ones past it, ties aside (x, y), and ties below and past the budget (z, w).
+  int4 mine = make_int4(0, 0, 0, 0);
+  each([&](int j, uint32_t key) {
+    const bool lo = base + 32 * j < p.budget, tie = key == prefix;
+    mine.x += __popc(__ballot_sync(0xffffffffu, key != 0u && lo && key < prefix));
+    mine.y += __popc(__ballot_sync(0xffffffffu, !lo && key > prefix));
+    mine.z += __popc(__ballot_sync(0xffffffffu, lo && tie));
+    mine.w += __popc(__ballot_sync(0xffffffffu, !lo && tie));
+  });
+  if (lane == 0) counts[warp] = mine;
+  __syncthreads();
+  if (warp == 0) {
+    const int4 c = counts[lane];
+    int4 s;
+    s.x = static_cast<int>(warp_incl_scan(c.x));
+    s.y = static_cast<int>(warp_incl_scan(c.y));
+    s.z = static_cast<int>(warp_incl_scan(c.z));
+    s.w = static_cast<int>(warp_incl_scan(c.w));
+    counts[lane] = make_int4(s.x - c.x, s.y - c.y, s.z - c.z, s.w - c.w);
+    int4 t;
+    t.x = __shfl_sync(0xffffffffu, s.x, 31);
+    t.y = __shfl_sync(0xffffffffu, s.y, 31);
+    t.z = __shfl_sync(0xffffffffu, s.z, 31);
+    t.w = __shfl_sync(0xffffffffu, s.w, 31);
+    if (lane < C) *cluster.map_shared_rank(&totals[rank], lane) = t;
+  }
+  if (C > 1)
+    cluster.sync();
+  else
+    __syncthreads();
+  int4 at = counts[warp];
+  int past_total = 0, ties_below = 0;
+  for (int r = 0; r < C; ++r) {
+    const int4 t = totals[r];
+    past_total += t.y;
+    ties_below += t.z;
+    if (r < rank) {
+      at.x += t.x;
+      at.y += t.y;
+      at.z += t.z;
+      at.w += t.w;
+    }
+  }
+  const int quota = static_cast<int>(left);
+  if (rank == 0 && tid == 0) p.n_moves[row] = past_total + quota - min(quota, ties_below);
+  int tie0 = at.z + at.w;                                       // ties before this warp
+  int hole0 = at.x + at.z - min(at.z, quota);                   // evicted slots below the budget
+  int move0 = at.y + min(quota, tie0) - min(quota, at.z);       // kept slots past it
   int32_t* holes = p.holes + row * p.budget;
-  int ties = 0, n_holes = 0, n_moves = 0;
-  for (int base = 0; base < n; base += kEvThreads) {
-    const int i = base + tid;
-    const bool in = i < n;
-    const uint32_t key = in ? ev_key(w[i], ps[i], p.sinks, from) : 0u;
-    int total;
-    const int tie = ties + ev_block_rank(in && key == prefix, sums, total);
-    ties += total;
-    const bool keep = in && (key > prefix || (key == prefix && tie < static_cast<int>(left)));
-    const bool hole = in && !keep && i < p.budget;
-    const int rank_h = n_holes + ev_block_rank(hole, sums, total);
-    n_holes += total;
-    if (hole) holes[rank_h] = i;
-    if (keep && i < p.budget) src[i] = i;
-    __syncthreads();  // the holes of this chunk and before are visible to its movers
-    const bool move = keep && i >= p.budget;
-    const int rank_m = n_moves + ev_block_rank(move, sums, total);
-    n_moves += total;
-    if (move) src[holes[rank_m]] = i;
+  int32_t* movers = p.movers + row * p.budget;
+  const unsigned below = (1u << lane) - 1u;
+  each([&](int j, uint32_t key) {
+    const int i = base + 32 * j;
+    const bool lo = i < p.budget, tie = key == prefix;
+    const unsigned bt = __ballot_sync(0xffffffffu, tie);
+    const bool keep = key > prefix || (tie && tie0 + __popc(bt & below) < quota);
+    const bool hole = key != 0u && lo && !keep, move = keep && !lo;
+    const unsigned bh = __ballot_sync(0xffffffffu, hole), bm = __ballot_sync(0xffffffffu, move);
+    if (hole) holes[hole0 + __popc(bh & below)] = i;
+    if (move) movers[move0 + __popc(bm & below)] = i;
+    if (keep && lo) {
+      src[i] = i;
+      wo[i] = w[i];
+      po[i] = ps[i];
+    }
+    tie0 += __popc(bt);
+    hole0 += __popc(bh);
+    move0 += __popc(bm);
+  });
+}
+
+// The i-th mover of a row goes to its i-th hole. kUnroll pairs per lane group are in flight.
+template <int RowBytes>
+__global__ void __launch_bounds__(256) paged_evict_move_kernel(const PagedEvictParams p) {
+  constexpr int L = RowBytes / 16, RW = 32 / L, kUnroll = 2;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const int ch = lane % L;
+  const int64_t row = blockIdx.y;
+  const int b = static_cast<int>(row / p.H_kv), h = static_cast<int>(row - static_cast<int64_t>(b) * p.H_kv);
+  const int n = __ldg(p.n_moves + row);
+  uint4* k = static_cast<uint4*>(p.k_pages) + h * p.c.ksh + ch;
+  uint4* v = static_cast<uint4*>(p.v_pages) + h * p.c.vsh + ch;
+  const int first = (blockIdx.x * 8 + (threadIdx.x >> 5)) * RW * kUnroll + lane / L;
+  for (int r0 = first; r0 < n; r0 += gridDim.x * 8 * RW * kUnroll) {
+    uint4 kx[kUnroll], vx[kUnroll];
+    int to[kUnroll];
+    int64_t tk[kUnroll], tv[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const int r = r0 + i * RW;
+      to[i] = -1;
+      if (r >= n) continue;
+      const int d = p.holes[row * p.budget + r], s = p.movers[row * p.budget + r];
+      if (ch == 0) {
+        p.src[row * p.budget + d] = s;
+        p.w_out[b * p.wosb + h * p.wosh + d] = p.weights[b * p.wsb + h * p.wsh + s];
+        p.pos_out[b * p.posb + h * p.posh + d] = p.pos[b * p.psb + h * p.psh + s];
+      }
+      const uint32_t fi = p.c.page.div(s), ti = p.c.page.div(d);
+      const int fp = page_of(p.c, b, fi), tp = page_of(p.c, b, ti);
+      if (fp < 0 || tp < 0) {  // a row without a mapped page on either side
+        raise_status(DCR_ERR_DEVICE_INDEX);
+        continue;
+      }
+      const int64_t fs = s - static_cast<int>(fi * p.c.page.d), ts = d - static_cast<int>(ti * p.c.page.d);
+      to[i] = d;
+      tk[i] = tp * p.c.ksp + ts * p.c.ksr;
+      tv[i] = tp * p.c.vsp + ts * p.c.vsr;
+      kx[i] = k[fp * p.c.ksp + fs * p.c.ksr];
+      vx[i] = v[fp * p.c.vsp + fs * p.c.vsr];
+    }
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      if (to[i] < 0) continue;
+      k[tk[i]] = kx[i];
+      v[tv[i]] = vx[i];
+    }
   }
 }
 
-// One warp per destination slot.
+// Cluster size and register keys per thread: clusters grow while all rows' CTAs still fit the
+// GPU at once and a CTA keeps 2048 slots, or as far as it takes to hold a row in registers.
+static int ev_launch_select(const PagedEvictParams& p, int rows, int slots, cudaStream_t s) {
+  const int sms = device_sm_count();
+  int C = 1;
+  while (C < 8 && ((rows * 2 * C <= sms && slots > 2048 * C) || slots > 32 * kEvThreads * C)) C *= 2;
+  const int need = (slots + C * kEvThreads - 1) / (C * kEvThreads);
+  const dim3 grid(static_cast<unsigned>(rows) * C), block(kEvThreads);
+  cudaError_t e;
+  if (need <= 4) e = launch_cluster(paged_evict_select_kernel<4>, grid, block, 0, s, C, p);
+  else if (need <= 8) e = launch_cluster(paged_evict_select_kernel<8>, grid, block, 0, s, C, p);
+  else if (need <= 32) e = launch_cluster(paged_evict_select_kernel<32>, grid, block, 0, s, C, p);
+  else e = launch_cluster(paged_evict_select_kernel<0>, grid, block, 0, s, C, p);
+  return e == cudaSuccess ? DCR_OK : DCR_ERR_CUDA;
+}
+
 template <int RowBytes>
-__global__ void __launch_bounds__(256) paged_evict_move_kernel(const PagedEvictParams p) {
-  const int lane = threadIdx.x & 31;
-  const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int h = blockIdx.y, b = blockIdx.z;
-  if (i >= p.budget) return;
-  const int64_t row = static_cast<int64_t>(b) * p.H_kv + h;
-  const int s = p.src[row * p.budget + i];
-  if (lane == 0) {
-    p.w_out[b * p.wosb + h * p.wosh + i] = s < 0 ? 0.0f : p.weights[b * p.wsb + h * p.wsh + s];
-    p.pos_out[b * p.posb + h * p.posh + i] = s < 0 ? -1 : p.pos[b * p.psb + h * p.psh + s];
-  }
-  if (s < 0 || s == i) return;
-  const uint32_t fi = p.c.page.div(s), ti = p.c.page.div(i);
-  const int fp = page_of(p.c, b, fi), tp = page_of(p.c, b, ti);
-  if (fp < 0 || tp < 0) {
-    raise_status(DCR_ERR_DEVICE_INDEX);
-    return;
-  }
-  const int64_t fs = s - static_cast<int64_t>(fi) * p.c.page.d, ts = i - static_cast<int64_t>(ti) * p.c.page.d;
-  constexpr int kC = RowBytes / 16;  // strides below are in 16-byte chunks
-  uint4* k = static_cast<uint4*>(p.k_pages);
-  uint4* v = static_cast<uint4*>(p.v_pages);
-  if (lane < kC) {
-    k[tp * p.c.ksp + h * p.c.ksh + ts * p.c.ksr + lane] =
-        k[fp * p.c.ksp + h * p.c.ksh + fs * p.c.ksr + lane];
-    v[tp * p.c.vsp + h * p.c.vsh + ts * p.c.vsr + lane] =
-        v[fp * p.c.vsp + h * p.c.vsh + fs * p.c.vsr + lane];
-  }
+static int ev_launch_move(const PagedEvictParams& p, int rows, int most, cudaStream_t s) {
+  constexpr int kPer = 8 * (32 * 16 / RowBytes) * 2;  // pairs a CTA takes at once
+  int x = (most + kPer - 1) / kPer;
+  const int cap = (device_sm_count() * 8 + rows - 1) / rows;  // the GPU full once
+  if (x > cap) x = cap;
+  return launch_dependent(paged_evict_move_kernel<RowBytes>, dim3(x, rows), dim3(256), s, p) ==
+                 cudaSuccess
+             ? DCR_OK
+             : DCR_ERR_CUDA;
 }
 
 }  // namespace dcr
@@ -173,7 +347,7 @@ extern "C" {
 
 size_t dcr_paged_evict_workspace_bytes(int B, int H_kv, int budget) {
   if (B <= 0 || H_kv <= 0 || budget <= 0) return 0;
-  return sizeof(int32_t) * static_cast<size_t>(B) * H_kv * budget;
+  return sizeof(int32_t) * static_cast<size_t>(B) * H_kv * (2 * static_cast<size_t>(budget) + 1);
 }
 
 int dcr_paged_evict(void* k_pages, void* v_pages, int dtype, int64_t k_stride_p,
@@ -190,7 +364,7 @@ int dcr_paged_evict(void* k_pages, void* v_pages, int dtype, int64_t k_stride_p,
   if (lengths == nullptr || weights == nullptr || pos == nullptr || seen == nullptr ||
       src_out == nullptr || weights_out == nullptr || pos_out == nullptr || lengths_out == nullptr)
     return DCR_ERR_NULL;
-  if (B <= 0 || B > 65535 || H_kv > 65535 || budget <= 0 || sinks < 0 || recent < 0)
+  if (B <= 0 || static_cast<int64_t>(B) * H_kv > 65535 || budget <= 0 || sinks < 0 || recent < 0)
     return DCR_ERR_SHAPE;
   const int st = check_pool(k_pages, v_pages, dtype, k_stride_p, k_stride_h, k_stride_s,
                             v_stride_p, v_stride_h, v_stride_s, num_pages, page_size, page_table,
@@ -232,16 +406,18 @@ int dcr_paged_evict(void* k_pages, void* v_pages, int dtype, int64_t k_stride_p,
   p.posb = po_stride_b;
   p.posh = po_stride_h;
   p.len_out = lengths_out;
+  const int rows = B * H_kv, slots = max_pages * page_size;
   p.holes = static_cast<int32_t*>(workspace);
+  p.movers = p.holes + static_cast<int64_t>(rows) * budget;
+  p.n_moves = p.movers + static_cast<int64_t>(rows) * budget;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  paged_evict_select_kernel<<<dim3(H_kv, B), kEvThreads, 0, s>>>(p);
-  if (cudaGetLastError() != cudaSuccess) return DCR_ERR_CUDA;
-  const dim3 grid((budget + 7) / 8, H_kv, B);
+  const int rc = ev_launch_select(p, rows, slots, s);
+  if (rc != DCR_OK || slots == budget) return rc;  // no row holds more than the budget
+  const int most = budget < slots - budget ? budget : slots - budget;
   const int bytes = D * (dtype == DCR_DTYPE_F32 ? 4 : 2);
-  if (bytes == 128) paged_evict_move_kernel<128><<<grid, 256, 0, s>>>(p);
-  else if (bytes == 256) paged_evict_move_kernel<256><<<grid, 256, 0, s>>>(p);
-  else paged_evict_move_kernel<512><<<grid, 256, 0, s>>>(p);
-  return cudaGetLastError() == cudaSuccess ? DCR_OK : DCR_ERR_CUDA;
+  if (bytes == 128) return ev_launch_move<128>(p, rows, most, s);
+  if (bytes == 256) return ev_launch_move<256>(p, rows, most, s);
+  return ev_launch_move<512>(p, rows, most, s);
 }
 
 }  // extern "C"
