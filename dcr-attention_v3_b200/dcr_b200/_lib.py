@@ -120,10 +120,8 @@ SIGNATURES = {
     "dcr_paged_evict": (_i32, [_vp, _vp, _i32] + [_i64] * 6 + [
         _i32, _i32, _vp, _i64, _i32, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _i32, _i32,
         _i32, _i32, _i32, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _sz, _vp]),
-    "dcr_logits_workspace_bytes": (_sz, [_i32] * 3),
     "dcr_process_logits": (_i32, [_vp, _i64, _i32, _i32, _i32, _vp, _i32, _i64, _i32, _vp, _vp,
-                                  _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _sz,
-                                  _vp]),
+                                  _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp]),
     "dcr_read_device_status": (_i32, [ctypes.POINTER(_i32), _i32]),
     "dcr_binary_version": (_i32, [ctypes.POINTER(_i32)]),
 }

@@ -12,7 +12,7 @@ import torch
 
 from dcr_b200 import _lib
 from dcr_b200.kernel.cuda._common import check_dtype
-from dcr_b200.kernel.cuda.paged import _bytes, _call, _on_cuda, _refuse, _scratch
+from dcr_b200.kernel.cuda.paged import _call, _on_cuda, _refuse
 
 
 def _per_row(t: Optional[torch.Tensor], B: int, dtype: torch.dtype, name: str, device):
@@ -30,9 +30,7 @@ def process_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = Non
                    presence: Optional[torch.Tensor] = None,
                    frequency: Optional[torch.Tensor] = None,
                    bias: Optional[torch.Tensor] = None, allowed: Optional[torch.Tensor] = None,
-                   out: Optional[torch.Tensor] = None,
-                   workspace_buf: Optional[torch.Tensor] = None
-                   ) -> Tuple[torch.Tensor, torch.Tensor]:
+                   out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """(processed logits ``[B, V]`` in the logits' dtype, next token ``[B]`` int64).
 
     In fp32 and in this order, rounded once: ``x / repetition`` (``x * repetition`` for x <= 0)
@@ -92,8 +90,7 @@ def process_logits(logits: torch.Tensor, *, tokens: Optional[torch.Tensor] = Non
             _refuse("logits processed in place must keep their strides")
     token = torch.empty((B,), dtype=torch.int64, device=dev)
     if B > 0:
-        ws = _scratch(dev, _bytes("dcr_logits_workspace_bytes", dev.index, B, V, L), workspace_buf)
         _call(dev, "dcr_process_logits", logits.data_ptr(), logits.stride(0), dt, B, V, t_ptr, tok64,
               t_stride, L, n_ptr, m_ptr, r_ptr, p_ptr, f_ptr, b_ptr, b_stride, a_ptr, a_stride,
-              out.data_ptr(), out.stride(0), token.data_ptr(), ws.data_ptr(), ws.numel())
+              out.data_ptr(), out.stride(0), token.data_ptr())
     return out, token

@@ -498,8 +498,6 @@ int dcr_paged_evict(void* k_pages, void* v_pages, int dtype, int64_t k_stride_p,
                     void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- logits of a decode step (dcr_logits.cu) ------------------------------------------ */
-size_t dcr_logits_workspace_bytes(int B, int V, int L);
-
 /* Per row of logits [B, V], in fp32 and in this order, rounded once to dtype: x > 0 ?
  * x / repetition : x * repetition for tokens in the row's history; x - count * frequency and
  * x - presence for those that occur after its prompt; x + bias; -inf where `allowed` (32
@@ -516,7 +514,7 @@ int dcr_process_logits(const void* logits, int64_t l_stride_b, int dtype, int B,
                        const float* repetition, const float* presence, const float* frequency,
                        const float* bias, int64_t bias_stride_b, const uint32_t* allowed,
                        int64_t a_stride_b, void* out, int64_t o_stride_b, int64_t* next_token,
-                       void* workspace, size_t workspace_bytes, void* stream);
+                       void* stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */
