@@ -15,9 +15,10 @@
 //
 // Kernel 1, a cluster of C CTAs a row: every thread keeps its slots' 32-bit order keys in
 // registers (a warp's slots are consecutive, 32 at a time); the budget-th largest key by three
-// histogram levels (12, 10 and 10 bits) in shared memory, added up in CTA 0; then one exchange
-// of per-warp counts gives every warp the ranks of its holes and movers, which ballots spread
-// over its slots in slot order. A table of a size that registers cannot hold is read again at
+// histogram levels (12, 10 and 10 bits) in shared memory, added up in CTA 0 (only bins that
+// hold anything travel; reading all bins of all CTAs in each of them was 1.3 to 10 times
+// slower); then one exchange of per-warp counts gives every warp the ranks of its holes and
+// movers, which ballots spread over its slots in slot order. A table of a size that registers cannot hold is read again at
 // every level. Kernel 2 (a programmatic dependent) pairs the i-th hole with the i-th mover and
 // copies the rows, 16 bytes a lane.
 #include <cooperative_groups.h>
@@ -65,7 +66,7 @@ __device__ __forceinline__ uint32_t ev_key(float w, int pos, int sinks, int from
 }
 
 // The whole CTA finds, from the top, the bin in which the k-th largest key of a histogram of
-// 1024 * Q bins lies: *bin, the number of keys above it and in it.
+// 1024 * Q bins lies: res = (bin, number of keys above it).
 template <int Q>
 __device__ __forceinline__ void ev_find(const uint32_t* hist, uint32_t k, uint32_t* sums,
                                         uint32_t* res) {
@@ -73,7 +74,7 @@ __device__ __forceinline__ void ev_find(const uint32_t* hist, uint32_t k, uint32
   uint32_t c[Q], s = 0;
 #pragma unroll
   for (int i = 0; i < Q; ++i) {  // descending bins
-    c[i] = hist[kEvThreads * Q - 1 - (tid * Q + i)];
+    c[i] = hist[(kEvThreads - tid) * Q - 1 - i];
     s += c[i];
   }
   const uint32_t incl = warp_incl_scan(s);
@@ -131,12 +132,40 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_select_kernel(const Pa
   const int base = (rank * kEvWarps + warp) * 32 * used + lane;  // slot j of this lane: + 32 j
   auto load = [&](int j) {
     const int i = base + 32 * j;
-    return i < n ? ev_key(w[i], ps[i], p.sinks, from) : 0u;
+    return i < n ? ev_key(__ldg(w + i), __ldg(ps + i), p.sinks, from) : 0u;
   };
+  // Every slot below the budget keeps its place at first; the second kernel fills the holes.
+  // Batches of loads, so that no load waits for a store.
+  constexpr int kBatch = VPT == 0 ? 8 : VPT < 8 ? VPT : 8;
   uint32_t keys[VPT > 0 ? VPT : 1];
-  if constexpr (VPT > 0) {
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) keys[j] = j < used ? load(j) : 0u;
+  for (int j0 = 0; j0 < (VPT > 0 ? VPT : used); j0 += kBatch) {
+    if (j0 >= used) {
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (VPT > 0) keys[VPT > 0 ? j0 + j : 0] = 0u;
+      continue;
+    }
+    float wj[kBatch];
+    int pj[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int i = base + 32 * (j0 + j);
+      const bool in = j0 + j < used && i < n;
+      wj[j] = in ? __ldg(w + i) : 0.0f;
+      pj[j] = in ? __ldg(ps + i) : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int i = base + 32 * (j0 + j);
+      const bool in = j0 + j < used && i < n;
+      if (VPT > 0) keys[VPT > 0 ? j0 + j : 0] = in ? ev_key(wj[j], pj[j], p.sinks, from) : 0u;
+      if (in && i < p.budget) {
+        src[i] = i;
+        wo[i] = wj[j];
+        po[i] = pj[j];
+      }
+    }
   }
   auto each = [&](auto&& f) {
     if constexpr (VPT > 0) {
@@ -160,7 +189,7 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_select_kernel(const Pa
         atomicAdd(bins + ((key >> shift) & ((1u << bits) - 1u)), 1u);
     });
     if (C > 1) {
-      cluster.sync();  // the bins of CTA 0 are zeroed and this CTA's are full
+      cluster.sync();  // CTA 0's bins are zeroed, and this CTA's are full
       if (rank > 0) {
         uint32_t* bins0 = cluster.map_shared_rank(bins, 0);
         for (int i = tid; i < (1 << bits); i += kEvThreads)
@@ -250,11 +279,6 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_select_kernel(const Pa
     const unsigned bh = __ballot_sync(0xffffffffu, hole), bm = __ballot_sync(0xffffffffu, move);
     if (hole) holes[hole0 + __popc(bh & below)] = i;
     if (move) movers[move0 + __popc(bm & below)] = i;
-    if (keep && lo) {
-      src[i] = i;
-      wo[i] = w[i];
-      po[i] = ps[i];
-    }
     tie0 += __popc(bt);
     hole0 += __popc(bh);
     move0 += __popc(bm);
@@ -273,50 +297,66 @@ __global__ void __launch_bounds__(256) paged_evict_move_kernel(const PagedEvictP
   const int n = __ldg(p.n_moves + row);
   uint4* k = static_cast<uint4*>(p.k_pages) + h * p.c.ksh + ch;
   uint4* v = static_cast<uint4*>(p.v_pages) + h * p.c.vsh + ch;
+  const float* w = p.weights + b * p.wsb + h * p.wsh;
+  const int32_t* ps = p.pos + b * p.psb + h * p.psh;
   const int first = (blockIdx.x * 8 + (threadIdx.x >> 5)) * RW * kUnroll + lane / L;
   for (int r0 = first; r0 < n; r0 += gridDim.x * 8 * RW * kUnroll) {
+    // all loads of one kind before the next kind, and all before the stores
     uint4 kx[kUnroll], vx[kUnroll];
-    int to[kUnroll];
-    int64_t tk[kUnroll], tv[kUnroll];
+    int d[kUnroll], f[kUnroll], fp[kUnroll], tp[kUnroll];
+    float wx[kUnroll];
+    int px[kUnroll];
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
       const int r = r0 + i * RW;
-      to[i] = -1;
-      if (r >= n) continue;
-      const int d = p.holes[row * p.budget + r], s = p.movers[row * p.budget + r];
-      if (ch == 0) {
-        p.src[row * p.budget + d] = s;
-        p.w_out[b * p.wosb + h * p.wosh + d] = p.weights[b * p.wsb + h * p.wsh + s];
-        p.pos_out[b * p.posb + h * p.posh + d] = p.pos[b * p.psb + h * p.psh + s];
-      }
-      const uint32_t fi = p.c.page.div(s), ti = p.c.page.div(d);
-      const int fp = page_of(p.c, b, fi), tp = page_of(p.c, b, ti);
-      if (fp < 0 || tp < 0) {  // a row without a mapped page on either side
-        raise_status(DCR_ERR_DEVICE_INDEX);
-        continue;
-      }
-      const int64_t fs = s - static_cast<int>(fi * p.c.page.d), ts = d - static_cast<int>(ti * p.c.page.d);
-      to[i] = d;
-      tk[i] = tp * p.c.ksp + ts * p.c.ksr;
-      tv[i] = tp * p.c.vsp + ts * p.c.vsr;
-      kx[i] = k[fp * p.c.ksp + fs * p.c.ksr];
-      vx[i] = v[fp * p.c.vsp + fs * p.c.vsr];
+      d[i] = r < n ? p.holes[row * p.budget + r] : -1;
+      f[i] = r < n ? p.movers[row * p.budget + r] : 0;
     }
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
-      if (to[i] < 0) continue;
-      k[tk[i]] = kx[i];
-      v[tv[i]] = vx[i];
+      if (d[i] < 0) continue;
+      fp[i] = page_of(p.c, b, p.c.page.div(f[i]));
+      tp[i] = page_of(p.c, b, p.c.page.div(d[i]));
+      if (ch == 0) {
+        wx[i] = __ldg(w + f[i]);
+        px[i] = __ldg(ps + f[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      if (d[i] < 0 || fp[i] < 0 || tp[i] < 0) continue;
+      const int64_t in = f[i] - static_cast<int>(p.c.page.div(f[i]) * p.c.page.d);
+      kx[i] = k[fp[i] * p.c.ksp + in * p.c.ksr];
+      vx[i] = v[fp[i] * p.c.vsp + in * p.c.vsr];
+    }
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      if (d[i] < 0) continue;
+      if (ch == 0) {
+        p.src[row * p.budget + d[i]] = f[i];
+        p.w_out[b * p.wosb + h * p.wosh + d[i]] = wx[i];
+        p.pos_out[b * p.posb + h * p.posh + d[i]] = px[i];
+      }
+      if (fp[i] < 0 || tp[i] < 0) {  // a row without a mapped page on either side
+        raise_status(DCR_ERR_DEVICE_INDEX);
+        continue;
+      }
+      const int64_t in = d[i] - static_cast<int>(p.c.page.div(d[i]) * p.c.page.d);
+      k[tp[i] * p.c.ksp + in * p.c.ksr] = kx[i];
+      v[tp[i] * p.c.vsp + in * p.c.vsr] = vx[i];
     }
   }
 }
 
-// Cluster size and register keys per thread: clusters grow while all rows' CTAs still fit the
-// GPU at once and a CTA keeps 2048 slots, or as far as it takes to hold a row in registers.
+// Cluster size and register keys per thread: one CTA takes 8192 slots, since the levels'
+// cluster barriers cost more than longer loops up to there (rows x slots, C = 1 / 2 / 4 / 8:
+// 32 x 8192 15.3 / 16.3 / 15.5 / 19.7 us, 32 x 32768 40.9 / 37.3 / 29.0 / 32.0, 8 x 32769 88.1 /
+// 28.1 / 25.3 / 18.7, 128 x 8192 47.8 / 52.3 / 64.3 / 92.3, with the moves); clusters grow past it
+// while all rows' CTAs still fit the GPU at once, or as far as registers need it.
 static int ev_launch_select(const PagedEvictParams& p, int rows, int slots, cudaStream_t s) {
   const int sms = device_sm_count();
   int C = 1;
-  while (C < 8 && ((rows * 2 * C <= sms && slots > 2048 * C) || slots > 32 * kEvThreads * C)) C *= 2;
+  while (C < 8 && ((rows * 2 * C <= sms && slots > 8192 * C) || slots > 32 * kEvThreads * C)) C *= 2;
   const int need = (slots + C * kEvThreads - 1) / (C * kEvThreads);
   const dim3 grid(static_cast<unsigned>(rows) * C), block(kEvThreads);
   cudaError_t e;
