@@ -7,11 +7,13 @@ available, every entry point raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 
 import torch
 
-from dcr_b200.build import LIB_PATH
+from dcr_b200.build import LIB_PATH, TORCH_PATH
 
 DTYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
@@ -153,6 +155,28 @@ def load() -> ctypes.CDLL:
             fn.argtypes = args
         _lib = lib
     return _lib
+
+
+_torch_ops = None
+
+
+def torch_ops():
+    """The paged operators' torch binding (dcr_b200_torch.so, csrc/dcr_torch.cpp), loaded once:
+    it calls the same libdcr_b200.so and has no fallback either."""
+    global _torch_ops
+    if _torch_ops is None:
+        load()
+        if not os.path.exists(TORCH_PATH):
+            raise RuntimeError(
+                f"dcr_b200_torch.so not found at {TORCH_PATH}; build it with "
+                "`python -c 'import __graft_entry__ as g; g.build()'` (or python -m "
+                "dcr_b200.build). There is no CPU fallback.")
+        loader = importlib.machinery.ExtensionFileLoader("dcr_b200_torch", TORCH_PATH)
+        spec = importlib.util.spec_from_file_location("dcr_b200_torch", TORCH_PATH, loader=loader)
+        module = importlib.util.module_from_spec(spec)
+        loader.exec_module(module)
+        _torch_ops = module
+    return _torch_ops
 
 
 def status_string(status: int) -> str:

@@ -1,4 +1,5 @@
-"""Build libdcr_b200.so (the sm_100a CUDA library behind the C ABI in include/dcr_b200.h).
+"""Build libdcr_b200.so (the sm_100a CUDA library behind the C ABI in include/dcr_b200.h) and
+dcr_b200_torch.so (the paged operators' binding to torch tensors, csrc/dcr_torch.cpp).
 
 The library is one nvcc translation unit (csrc/dcr_b200_lib.cu) built in-tree into
 ``dcr_b200/lib/libdcr_b200.so`` with ``-gencode arch=compute_100a,code=sm_100a``.
@@ -23,6 +24,8 @@ CSRC = os.path.join(SRC_ROOT, "csrc")
 INCLUDE = os.path.join(REPO_ROOT, "include")
 LIB_DIR = os.path.join(PKG_DIR, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libdcr_b200.so")
+TORCH_PATH = os.path.join(LIB_DIR, "dcr_b200_torch.so")
+TORCH_SOURCE = os.path.join(CSRC, "dcr_torch.cpp")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-shared",
@@ -48,10 +51,43 @@ def up_to_date() -> bool:
     return all(os.path.getmtime(s) <= t for s in _sources())
 
 
+def build_torch(force: bool = False, verbose: bool = False) -> str:
+    """Compile the torch binding (host code only) if a source is newer than it."""
+    sources = [TORCH_SOURCE, os.path.join(INCLUDE, "dcr_b200.h")]
+    if not force and os.path.exists(TORCH_PATH) and all(
+            os.path.getmtime(s) <= os.path.getmtime(TORCH_PATH) for s in sources):
+        return TORCH_PATH
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    cuda_include = os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include")
+    includes = [INCLUDE, *include_paths(), cuda_include, sysconfig.get_path("include")]
+    tmp = TORCH_PATH + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-isystem{i}" for i in includes), TORCH_SOURCE, "-o", tmp, f"-L{LIB_DIR}",
+           "-l:libdcr_b200.so", *(f"-L{d}" for d in library_paths()), "-lc10", "-lc10_cuda",
+           "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"the torch binding failed to build ({r.returncode}):\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, TORCH_PATH)
+    return TORCH_PATH
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile the library if any source is newer than it; return its path."""
-    if not force and up_to_date():
-        return LIB_PATH
+    """Compile the libraries if any of their sources is newer; return libdcr_b200.so's path."""
+    if force or not up_to_date():
+        _build_library(verbose)
+    build_torch(force, verbose)
+    return LIB_PATH
+
+
+def _build_library(verbose: bool) -> None:
     os.makedirs(LIB_DIR, exist_ok=True)
     tmp = LIB_PATH + ".tmp"
     cmd = [nvcc_path(), *ARCH_FLAGS, *NVCC_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}",
@@ -64,7 +100,6 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if "spill" in (r.stderr or "") and verbose:
         print(r.stderr, file=sys.stderr)
     os.replace(tmp, LIB_PATH)
-    return LIB_PATH
 
 
 if __name__ == "__main__":
