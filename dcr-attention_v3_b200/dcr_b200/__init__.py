@@ -13,6 +13,11 @@ Beyond the reference's API:
 
 * ``dcr_b200.kernel.cuda.projected`` - projected-score mode (rank-16 keys written at append)
 * ``dcr_b200.kv_cache``              - ``StaticKVCache``: preallocated K/V/KP, in-place append
+* ``dcr_b200.kernel.cuda.paged``     - a decode step over pages: attention of one token, query/key
+  norms with rotation and append, eviction by accumulated attention weight
+* ``dcr_b200.kernel.cuda.logits``    - penalties, bias, grammar mask and the greedy token
+* ``dcr_b200.paged_cache``           - ``PagedKVCache``: pages for a batch of unequal sequences
+* ``dcr_b200.models.llama.paged``    - ``PagedLlamaDecoder``: these together, in a model
 * ``dcr_b200.sharded``               - the decode step over several GPUs (KV-head split;
   sequence split with an exact global top-K over NCCL or NVLink peer memory)
 
