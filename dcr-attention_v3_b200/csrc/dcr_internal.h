@@ -51,6 +51,31 @@ cudaError_t launch_cluster(Kernel kernel, dim3 grid, dim3 block, size_t smem, cu
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// Launches a kernel as a programmatic dependent of the one before it on the stream (with
+// cluster > 1, as clusters of that many CTAs): its CTAs may be placed while that kernel drains.
+// Every such kernel begins with griddepcontrol.wait in all its threads, before it reads or
+// writes anything a kernel before it may touch; so kernels of a stream still follow one another,
+// whatever came before, and only the launch itself overlaps.
+template <typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Args...), dim3 grid, dim3 block, size_t smem,
+                             cudaStream_t st, int cluster, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // Split-K factor used by Pass 3 for this shape (1 = no split, no workspace partials).
 int attend_splits(int rows, int k_eff);
 

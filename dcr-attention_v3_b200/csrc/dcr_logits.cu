@@ -166,6 +166,8 @@ __global__ void __launch_bounds__(kLgThreads) logits_kernel(const LogitsParams p
   const int C = static_cast<int>(cluster.num_blocks());
   const int rank = static_cast<int>(cluster.block_rank());
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
   // arrives here, waits before the first access to another CTA's shared memory
   asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
   const int b = blockIdx.x / C;
@@ -485,7 +487,7 @@ static int lg_launch(LogitsParams p, int B, cudaStream_t s) {
   auto kernel = logits_kernel<T, kBias>;
   if (ensure_smem_attr(reinterpret_cast<const void*>(kernel), static_cast<int>(smem)) != cudaSuccess)
     return DCR_ERR_CUDA;
-  return launch_cluster(kernel, dim3(static_cast<unsigned>(B) * C), dim3(kLgThreads), smem, s, C, p) ==
+  return launch_dependent(kernel, dim3(static_cast<unsigned>(B) * C), dim3(kLgThreads), smem, s, C, p) ==
                  cudaSuccess
              ? DCR_OK
              : DCR_ERR_CUDA;

@@ -97,23 +97,6 @@ inline int check_pool(const void* k, const void* v, int dtype, int64_t ksp, int6
   return DCR_OK;
 }
 
-// Launches a kernel as a programmatic dependent of the one before it on the stream: its CTAs
-// may start early and wait (griddepcontrol.wait) before they read that kernel's results.
-template <typename... Args>
-inline cudaError_t launch_dependent(void (*kernel)(Args...), dim3 grid, dim3 block,
-                                    cudaStream_t s, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 inline PagePool make_pool(const void* k, const void* v, int64_t ksp, int64_t ksh, int64_t ksr,
                           int64_t vsp, int64_t vsh, int64_t vsr, int num_pages, int page_size,
                           const int32_t* table, int64_t table_stride, int max_pages) {

@@ -83,6 +83,8 @@ __global__ void __launch_bounds__(kApWarps * 32) paged_append_kernel(const Paged
   constexpr int N = ElemTraits<T>::kPerChunk;  // elements per lane
   constexpr int L = D / N;                     // lanes per row
   constexpr int RW = 32 / L;                   // rows per step
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
   const int lane = threadIdx.x & 31;
   const int ch = lane % L, sub = lane / L;
   const int nq = (p.H + RW * kApSteps - 1) / (RW * kApSteps);
@@ -216,14 +218,12 @@ __global__ void __launch_bounds__(kApWarps * 32) paged_append_kernel(const Paged
 }
 
 template <typename T, typename TC>
-static void launch_paged_append(const PagedAppendParams& p, int D, cudaStream_t s) {
+static cudaError_t launch_paged_append(const PagedAppendParams& p, int D, cudaStream_t s) {
   const int per = kApSteps * 32 * ElemTraits<T>::kPerChunk / D;  // heads per warp
   const int64_t warps = static_cast<int64_t>(p.T) * ((p.H + per - 1) / per + 2 * ((p.H_kv + per - 1) / per));
   const unsigned grid = static_cast<unsigned>((warps + kApWarps - 1) / kApWarps);
-  if (D == 64)
-    paged_append_kernel<T, TC, 64><<<grid, kApWarps * 32, 0, s>>>(p);
-  else
-    paged_append_kernel<T, TC, 128><<<grid, kApWarps * 32, 0, s>>>(p);
+  return launch_dependent(D == 64 ? paged_append_kernel<T, TC, 64> : paged_append_kernel<T, TC, 128>,
+                          dim3(grid), dim3(kApWarps * 32), 0, s, 1, p);
 }
 
 }  // namespace dcr
@@ -305,14 +305,14 @@ extern "C" int dcr_paged_append(
   p.psh = p_stride_h;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool f32_tables = table_dtype == DCR_DTYPE_F32;
-  if (dtype == DCR_DTYPE_BF16) {
-    if (f32_tables) launch_paged_append<__nv_bfloat16, float>(p, D, s);
-    else launch_paged_append<__nv_bfloat16, __nv_bfloat16>(p, D, s);
-  } else if (dtype == DCR_DTYPE_F16) {
-    if (f32_tables) launch_paged_append<__half, float>(p, D, s);
-    else launch_paged_append<__half, __half>(p, D, s);
-  } else {
-    launch_paged_append<float, float>(p, D, s);
-  }
-  return cudaGetLastError() == cudaSuccess ? DCR_OK : DCR_ERR_CUDA;
+  cudaError_t e;
+  if (dtype == DCR_DTYPE_BF16)
+    e = f32_tables ? launch_paged_append<__nv_bfloat16, float>(p, D, s)
+                   : launch_paged_append<__nv_bfloat16, __nv_bfloat16>(p, D, s);
+  else if (dtype == DCR_DTYPE_F16)
+    e = f32_tables ? launch_paged_append<__half, float>(p, D, s)
+                   : launch_paged_append<__half, __half>(p, D, s);
+  else
+    e = launch_paged_append<float, float>(p, D, s);
+  return e == cudaSuccess ? DCR_OK : DCR_ERR_CUDA;
 }

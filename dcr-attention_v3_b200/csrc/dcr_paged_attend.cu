@@ -701,6 +701,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const Paged
   extern __shared__ __align__(128) uint8_t pa_smem[];
   __shared__ PaPiece pieces[2 * kPaWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
   uint8_t* ring = pa_smem + warp * (S::NH * S::kHalf);
   uint8_t* own = pa_smem + kPaWarps * (S::NH * S::kHalf) + warp * (S::kPiece + S::kQ + S::kP + 64);
@@ -996,10 +997,9 @@ static int pa_launch(const PagedAttendParams& p, int ctas, cudaStream_t s) {
     return DCR_ERR_CUDA;
   PagedAttendParams q = p;
   q.page16 = p.c.page.d % S::kGroup == 0;
-  kernel<<<ctas, kPaThreads, S::kSmem, s>>>(q);
-  if (cudaGetLastError() != cudaSuccess) return DCR_ERR_CUDA;
   const int rows = p.G < HB ? p.G : HB;
-  if (launch_dependent(paged_fold_kernel<T, D, HB>, dim3(ctas, rows), dim3(256), s, q) != cudaSuccess)
+  if (launch_dependent(kernel, dim3(ctas), dim3(kPaThreads), S::kSmem, s, 1, q) != cudaSuccess ||
+      launch_dependent(paged_fold_kernel<T, D, HB>, dim3(ctas, rows), dim3(256), 0, s, 1, q) != cudaSuccess)
     return DCR_ERR_CUDA;
   return DCR_OK;
 }
@@ -1086,7 +1086,7 @@ int dcr_paged_attend(const void* q, int64_t q_stride_b, int64_t q_stride_h, cons
   if (rc != DCR_OK || weights == nullptr) return rc;
   const int chunk = 1024;
   const dim3 grid((max_slots + chunk - 1) / chunk, H_kv, B < 65535 ? B : 65535);
-  return launch_dependent(paged_weights_kernel, grid, dim3(256), s, p, weights, w_stride_b,
+  return launch_dependent(paged_weights_kernel, grid, dim3(256), 0, s, 1, p, weights, w_stride_b,
                              w_stride_h, chunk) == cudaSuccess
              ? DCR_OK
              : DCR_ERR_CUDA;

@@ -107,6 +107,7 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_select_kernel(const Pa
   const int C = static_cast<int>(cluster.num_blocks());
   const int rank = static_cast<int>(cluster.block_rank());
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
   const int64_t row = blockIdx.x / C;
   const int b = static_cast<int>(row / p.H_kv), h = static_cast<int>(row - static_cast<int64_t>(b) * p.H_kv);
@@ -360,10 +361,10 @@ static int ev_launch_select(const PagedEvictParams& p, int rows, int slots, cuda
   const int need = (slots + C * kEvThreads - 1) / (C * kEvThreads);
   const dim3 grid(static_cast<unsigned>(rows) * C), block(kEvThreads);
   cudaError_t e;
-  if (need <= 4) e = launch_cluster(paged_evict_select_kernel<4>, grid, block, 0, s, C, p);
-  else if (need <= 8) e = launch_cluster(paged_evict_select_kernel<8>, grid, block, 0, s, C, p);
-  else if (need <= 32) e = launch_cluster(paged_evict_select_kernel<32>, grid, block, 0, s, C, p);
-  else e = launch_cluster(paged_evict_select_kernel<0>, grid, block, 0, s, C, p);
+  if (need <= 4) e = launch_dependent(paged_evict_select_kernel<4>, grid, block, 0, s, C, p);
+  else if (need <= 8) e = launch_dependent(paged_evict_select_kernel<8>, grid, block, 0, s, C, p);
+  else if (need <= 32) e = launch_dependent(paged_evict_select_kernel<32>, grid, block, 0, s, C, p);
+  else e = launch_dependent(paged_evict_select_kernel<0>, grid, block, 0, s, C, p);
   return e == cudaSuccess ? DCR_OK : DCR_ERR_CUDA;
 }
 
@@ -373,7 +374,7 @@ static int ev_launch_move(const PagedEvictParams& p, int rows, int most, cudaStr
   int x = (most + kPer - 1) / kPer;
   const int cap = (device_sm_count() * 8 + rows - 1) / rows;  // the GPU full once
   if (x > cap) x = cap;
-  return launch_dependent(paged_evict_move_kernel<RowBytes>, dim3(x, rows), dim3(256), s, p) ==
+  return launch_dependent(paged_evict_move_kernel<RowBytes>, dim3(x, rows), dim3(256), 0, s, 1, p) ==
                  cudaSuccess
              ? DCR_OK
              : DCR_ERR_CUDA;
