@@ -865,12 +865,15 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const Paged
 // Folds the partials of the unit that begins in CTA blockIdx.x of the first kernel and ends in
 // a later one; blockIdx.y is the row of the head block. What there is to fold follows from the
 // lengths, so it is known before the first kernel is done; then one round of loads is left.
-// Thread groups of D take every (256 / D)-th partial.
+// Thread groups of D take every (128 / D)-th partial. (CTAs with nothing to fold leave at once,
+// all but the first: the kernel must not end before the one it waits for.)
+constexpr int kFoldThreads = 128;
+
 template <typename T, int D, int HB>
-__global__ void __launch_bounds__(256) paged_fold_kernel(const PagedAttendParams p) {
+__global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const PagedAttendParams p) {
   using S = PaShape<T, D, HB>;
-  constexpr int N = 256 / D, kBatch = 8;
-  __shared__ float m_s[N], l_s[N], acc_s[256];
+  constexpr int N = kFoldThreads / D, kBatch = 8;
+  __shared__ float m_s[N], l_s[N], acc_s[kFoldThreads];
   asm volatile("griddepcontrol.launch_dependents;");
   const PaLine line = pa_line<S::R>(p, gridDim.x);
   const int c0 = blockIdx.x;
@@ -886,6 +889,7 @@ __global__ void __launch_bounds__(256) paged_fold_kernel(const PagedAttendParams
     open = begin >= line.begin(c0) && end > end_cta && h < p.G;
     if (open) last = line.cta_of(end - 1);
   }
+  if (!open && blockIdx.x + blockIdx.y > 0) return;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!open) return;
   const int d = threadIdx.x % D, k = threadIdx.x / D;
@@ -934,28 +938,41 @@ __global__ void __launch_bounds__(256) paged_fold_kernel(const PagedAttendParams
   if (d == 0) pa_store_stats(p, row, top, sl);
 }
 
-// weights[b][h_kv][i] += sum over the G heads of exp2(score - m) / l, in head order.
-__global__ void __launch_bounds__(256) paged_weights_kernel(const PagedAttendParams p,
-                                                            float* weights, int64_t wsb,
-                                                            int64_t wsh, int chunk) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+// weights[b][h_kv][i] += sum over the G heads of exp2(score - m) / l, in head order. A thread
+// takes kWeightSlots neighbouring slots; the old weights, which no kernel before this one of the
+// call touches, are loaded while those still run.
+constexpr int kWeightThreads = 256, kWeightSlots = 4;
+
+__global__ void __launch_bounds__(kWeightThreads) paged_weights_kernel(const PagedAttendParams p,
+                                                                       float* weights, int64_t wsb,
+                                                                       int64_t wsh) {
   const int hk = blockIdx.y;
+  const int i0 = (blockIdx.x * kWeightThreads + threadIdx.x) * kWeightSlots;
+  bool waited = false;
   for (int b = blockIdx.z; b < p.B; b += gridDim.z) {
     const int n = checked_length(p.c, __ldg(p.lengths + b));
     const int lo = p.window > 0 && n > p.window ? n - p.window : 0;
-    const int from = max(lo, static_cast<int>(blockIdx.x) * chunk);
-    const int to = min(n, (static_cast<int>(blockIdx.x) + 1) * chunk);
+    float* dst = weights + b * wsb + hk * wsh + i0;
+    float w[kWeightSlots], add[kWeightSlots] = {};
+#pragma unroll
+    for (int e = 0; e < kWeightSlots; ++e) w[e] = i0 + e >= lo && i0 + e < n ? dst[e] : 0.0f;
+    if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+    waited = true;
+    if (i0 >= n || i0 + kWeightSlots <= lo) continue;
     const int64_t row0 = static_cast<int64_t>(b) * p.H + hk * p.G;
-    for (int i = from + threadIdx.x; i < to; i += 256) {
-      float w = 0.0f;
-      for (int g = 0; g < p.G; ++g) {
-        const float2 ml = p.stats[row0 + g];
-        const float s = p.scores[(row0 + g) * p.s_stride + i];
-        w += s == -INFINITY ? 0.0f : pa_exp2(s - ml.x) * ml.y;
-      }
-      float* dst = weights + b * wsb + hk * wsh + i;
-      *dst += w;
+    const float* src = p.scores + row0 * p.s_stride + i0;
+#pragma unroll 4
+    for (int g = 0; g < p.G; ++g) {
+      const float2 ml = p.stats[row0 + g];
+      const float4 s4 = *reinterpret_cast<const float4*>(src + g * p.s_stride);
+      const float s[kWeightSlots] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+      for (int e = 0; e < kWeightSlots; ++e)
+        add[e] += s[e] == -INFINITY ? 0.0f : pa_exp2(s[e] - ml.x) * ml.y;
     }
+#pragma unroll
+    for (int e = 0; e < kWeightSlots; ++e)
+      if (i0 + e >= lo && i0 + e < n) dst[e] = w[e] + add[e];
   }
 }
 
@@ -999,7 +1016,7 @@ static int pa_launch(const PagedAttendParams& p, int ctas, cudaStream_t s) {
   q.page16 = p.c.page.d % S::kGroup == 0;
   const int rows = p.G < HB ? p.G : HB;
   if (launch_dependent(kernel, dim3(ctas), dim3(kPaThreads), S::kSmem, s, 1, q) != cudaSuccess ||
-      launch_dependent(paged_fold_kernel<T, D, HB>, dim3(ctas, rows), dim3(256), 0, s, 1, q) != cudaSuccess)
+      launch_dependent(paged_fold_kernel<T, D, HB>, dim3(ctas, rows), dim3(kFoldThreads), 0, s, 1, q) != cudaSuccess)
     return DCR_ERR_CUDA;
   return DCR_OK;
 }
@@ -1084,10 +1101,10 @@ int dcr_paged_attend(const void* q, int64_t q_stride_b, int64_t q_stride_h, cons
     default: rc = pa_launch_t<float>(p, D, HB, w.ctas, s); break;
   }
   if (rc != DCR_OK || weights == nullptr) return rc;
-  const int chunk = 1024;
+  const int chunk = kWeightThreads * kWeightSlots;
   const dim3 grid((max_slots + chunk - 1) / chunk, H_kv, B < 65535 ? B : 65535);
-  return launch_dependent(paged_weights_kernel, grid, dim3(256), 0, s, 1, p, weights, w_stride_b,
-                             w_stride_h, chunk) == cudaSuccess
+  return launch_dependent(paged_weights_kernel, grid, dim3(kWeightThreads), 0, s, 1, p, weights,
+                          w_stride_b, w_stride_h) == cudaSuccess
              ? DCR_OK
              : DCR_ERR_CUDA;
 }
