@@ -15,9 +15,9 @@
 //
 // Kernel 1, a cluster of C CTAs a row: every thread keeps its slots' 32-bit order keys in
 // registers (a warp's slots are consecutive, 32 at a time); the budget-th largest key by three
-// histogram levels (12, 10 and 10 bits) in shared memory, added up in CTA 0 (only bins that
-// hold anything travel; reading all bins of all CTAs in each of them was 1.3 to 10 times
-// slower); then one exchange of per-warp counts gives every warp the ranks of its holes and
+// histogram levels (12, 10 and 10 bits) in shared memory, whose bins every CTA adds to the sums
+// of all CTAs of its cluster (only bins that hold anything travel; reading all bins of all CTAs
+// instead was 1.3 to 10 times slower); then one exchange of per-warp counts gives every warp the ranks of its holes and
 // movers, which ballots spread over its slots in slot order. A table of a size that registers cannot hold is read again at
 // every level. Kernel 2 (a programmatic dependent) pairs the i-th hole with the i-th mover and
 // copies the rows, 16 bytes a lane.
@@ -33,6 +33,7 @@ namespace cg = cooperative_groups;
 constexpr int kEvThreads = 1024;
 constexpr int kEvWarps = kEvThreads / 32;
 constexpr int kEvBins = 4096;
+constexpr int kEvAllBins = kEvBins + 2048;  // of the three levels
 
 struct PagedEvictParams {
   PagePool c;           // strides in 16-byte chunks
@@ -98,7 +99,7 @@ __device__ __forceinline__ void ev_find(const uint32_t* hist, uint32_t k, uint32
 
 template <int VPT>
 __global__ void __launch_bounds__(kEvThreads) paged_evict_select_kernel(const PagedEvictParams p) {
-  __shared__ uint32_t hist[kEvBins + 2048];  // the three levels' bins
+  extern __shared__ uint32_t hist[];         // the three levels' bins; clusters: and their sums
   __shared__ uint32_t sums[kEvWarps];
   __shared__ uint32_t res[2];
   __shared__ int4 counts[kEvWarps];          // per warp, then the sums before it
@@ -177,8 +178,11 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_select_kernel(const Pa
       for (int j = 0; j < used; ++j) f(j, load(j));
     }
   };
-  for (int i = tid; i < kEvBins + 2048; i += kEvThreads) hist[i] = 0;
-  __syncthreads();
+  for (int i = tid; i < (C > 1 ? 2 : 1) * kEvAllBins; i += kEvThreads) hist[i] = 0;
+  if (C > 1)
+    cluster.sync();
+  else
+    __syncthreads();
 
   // the threshold T = prefix, level by level: `left` counts from the top within the prefix
   uint32_t prefix = 0, left = p.budget;
@@ -189,29 +193,17 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_select_kernel(const Pa
       if (key != 0u && ((key ^ prefix) & above_mask) == 0u)
         atomicAdd(bins + ((key >> shift) & ((1u << bits) - 1u)), 1u);
     });
+    __syncthreads();
     if (C > 1) {
-      cluster.sync();  // CTA 0's bins are zeroed, and this CTA's are full
-      if (rank > 0) {
-        uint32_t* bins0 = cluster.map_shared_rank(bins, 0);
-        for (int i = tid; i < (1 << bits); i += kEvThreads)
-          if (bins[i] != 0u) atomicAdd(bins0 + i, bins[i]);
+      for (int i = tid; i < (1 << bits); i += kEvThreads) {
+        const uint32_t c = bins[i];
+        if (c == 0u) continue;
+        for (int r = 0; r < C; ++r) atomicAdd(cluster.map_shared_rank(bins + kEvAllBins + i, r), c);
       }
       cluster.sync();
-      if (rank == 0) {
-        ev_find<Q>(bins, left, sums, res);
-        __syncthreads();
-        if (tid >= 1 && tid < C) {
-          uint32_t* r = cluster.map_shared_rank(res, tid);
-          r[0] = res[0];
-          r[1] = res[1];
-        }
-      }
-      cluster.sync();
-    } else {
-      __syncthreads();
-      ev_find<Q>(bins, left, sums, res);
-      __syncthreads();
     }
+    ev_find<Q>(C > 1 ? bins + kEvAllBins : bins, left, sums, res);
+    __syncthreads();
     prefix |= res[0] << shift;
     left -= res[1];
   };
@@ -286,73 +278,96 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_select_kernel(const Pa
   });
 }
 
-// The i-th mover of a row goes to its i-th hole. kUnroll pairs per lane group are in flight.
+// The i-th mover of a row goes to its i-th hole, kUnroll pairs per lane group at a time. The
+// sequence's page table is read into shared memory before the first kernel is done (where it
+// fits), and a round's pairs while the round before is on its way, so that a round waits for one
+// read of the rows (with three dependent reads a round and three waves of CTAs, the call for
+// 134,000 pairs of 128-byte rows took 34.0 us instead of 31.9).
+constexpr int kEvPages = 4096;
+
 template <int RowBytes>
 __global__ void __launch_bounds__(256) paged_evict_move_kernel(const PagedEvictParams p) {
   constexpr int L = RowBytes / 16, RW = 32 / L, kUnroll = 2;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  __shared__ int32_t pages[kEvPages];
   const int lane = threadIdx.x & 31;
   const int ch = lane % L;
   const int64_t row = blockIdx.y;
   const int b = static_cast<int>(row / p.H_kv), h = static_cast<int>(row - static_cast<int64_t>(b) * p.H_kv);
-  const int n = __ldg(p.n_moves + row);
+  const bool local = p.c.max_pages <= kEvPages;
+  if (local)
+    for (int i = threadIdx.x; i < p.c.max_pages; i += 256) pages[i] = page_of(p.c, b, i);
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int n = p.n_moves[row];
+  const int32_t* holes = p.holes + row * p.budget;
+  const int32_t* movers = p.movers + row * p.budget;
   uint4* k = static_cast<uint4*>(p.k_pages) + h * p.c.ksh + ch;
   uint4* v = static_cast<uint4*>(p.v_pages) + h * p.c.vsh + ch;
   const float* w = p.weights + b * p.wsb + h * p.wsh;
   const int32_t* ps = p.pos + b * p.psb + h * p.psh;
-  const int first = (blockIdx.x * 8 + (threadIdx.x >> 5)) * RW * kUnroll + lane / L;
-  for (int r0 = first; r0 < n; r0 += gridDim.x * 8 * RW * kUnroll) {
-    // all loads of one kind before the next kind, and all before the stores
+  const int step = gridDim.x * 8 * RW * kUnroll;
+  int r0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * RW * kUnroll + lane / L;
+  int d[kUnroll], f[kUnroll];
+  auto pairs = [&](int r) {  // asked for before n is known; what lies past n is not used
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const int at = r + i * RW;
+      d[i] = at < p.budget ? holes[at] : 0;
+      f[i] = at < p.budget ? movers[at] : 0;
+    }
+  };
+  pairs(r0);
+  while (r0 < n) {
     uint4 kx[kUnroll], vx[kUnroll];
-    int d[kUnroll], f[kUnroll], fp[kUnroll], tp[kUnroll];
+    int64_t tk[kUnroll], tv[kUnroll];
+    int to[kUnroll], from[kUnroll];
+    bool moves[kUnroll];
     float wx[kUnroll];
     int px[kUnroll];
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
-      const int r = r0 + i * RW;
-      d[i] = r < n ? p.holes[row * p.budget + r] : -1;
-      f[i] = r < n ? p.movers[row * p.budget + r] : 0;
-    }
-#pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      if (d[i] < 0) continue;
-      fp[i] = page_of(p.c, b, p.c.page.div(f[i]));
-      tp[i] = page_of(p.c, b, p.c.page.div(d[i]));
+      to[i] = r0 + i * RW < n ? d[i] : -1;
+      from[i] = f[i];
+      moves[i] = false;
+      if (to[i] < 0) continue;
+      const uint32_t fi = p.c.page.div(from[i]), ti = p.c.page.div(to[i]);
+      const int fp = local ? pages[fi] : page_of(p.c, b, fi), tp = local ? pages[ti] : page_of(p.c, b, ti);
       if (ch == 0) {
-        wx[i] = __ldg(w + f[i]);
-        px[i] = __ldg(ps + f[i]);
+        wx[i] = __ldg(w + from[i]);
+        px[i] = __ldg(ps + from[i]);
       }
-    }
-#pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      if (d[i] < 0 || fp[i] < 0 || tp[i] < 0) continue;
-      const int64_t in = f[i] - static_cast<int>(p.c.page.div(f[i]) * p.c.page.d);
-      kx[i] = k[fp[i] * p.c.ksp + in * p.c.ksr];
-      vx[i] = v[fp[i] * p.c.vsp + in * p.c.vsr];
-    }
-#pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      if (d[i] < 0) continue;
-      if (ch == 0) {
-        p.src[row * p.budget + d[i]] = f[i];
-        p.w_out[b * p.wosb + h * p.wosh + d[i]] = wx[i];
-        p.pos_out[b * p.posb + h * p.posh + d[i]] = px[i];
-      }
-      if (fp[i] < 0 || tp[i] < 0) {  // a row without a mapped page on either side
+      if (fp < 0 || tp < 0) {  // a row without a mapped page on either side
         raise_status(DCR_ERR_DEVICE_INDEX);
         continue;
       }
-      const int64_t in = d[i] - static_cast<int>(p.c.page.div(d[i]) * p.c.page.d);
-      k[tp[i] * p.c.ksp + in * p.c.ksr] = kx[i];
-      v[tp[i] * p.c.vsp + in * p.c.vsr] = vx[i];
+      moves[i] = true;
+      const int64_t fs = from[i] - static_cast<int>(fi * p.c.page.d), ts = to[i] - static_cast<int>(ti * p.c.page.d);
+      kx[i] = k[fp * p.c.ksp + fs * p.c.ksr];
+      vx[i] = v[fp * p.c.vsp + fs * p.c.vsr];
+      tk[i] = tp * p.c.ksp + ts * p.c.ksr;
+      tv[i] = tp * p.c.vsp + ts * p.c.vsr;
+    }
+    r0 += step;
+    pairs(r0);
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      if (to[i] < 0) continue;
+      if (ch == 0) {
+        p.src[row * p.budget + to[i]] = from[i];
+        p.w_out[b * p.wosb + h * p.wosh + to[i]] = wx[i];
+        p.pos_out[b * p.posb + h * p.posh + to[i]] = px[i];
+      }
+      if (!moves[i]) continue;
+      k[tk[i]] = kx[i];
+      v[tv[i]] = vx[i];
     }
   }
 }
 
 // Cluster size and register keys per thread: one CTA takes 8192 slots, since the levels'
-// cluster barriers cost more than longer loops up to there (rows x slots, C = 1 / 2 / 4 / 8:
-// 32 x 8192 15.3 / 16.3 / 15.5 / 19.7 us, 32 x 32768 40.9 / 37.3 / 29.0 / 32.0, 8 x 32769 88.1 /
-// 28.1 / 25.3 / 18.7, 128 x 8192 47.8 / 52.3 / 64.3 / 92.3, with the moves); clusters grow past it
+// cluster barriers cost more than longer loops up to there (whole calls for rows x slots, C = 1 /
+// 2 / 4 / 8: 32 x 8192 14.5 / 14.7 / 13.9 / 19.0 us, 128 x 8192 39.7 / 43.2 / 54.8 / 80.4, 32 x 32768
+// 39.5 / 33.8 / 25.3 / 30.8, 8 x 32769 89.4 / 26.3 / 23.6 / 18.0); clusters grow past it
 // while all rows' CTAs still fit the GPU at once, or as far as registers need it.
 static int ev_launch_select(const PagedEvictParams& p, int rows, int slots, cudaStream_t s) {
   const int sms = device_sm_count();
@@ -360,11 +375,13 @@ static int ev_launch_select(const PagedEvictParams& p, int rows, int slots, cuda
   while (C < 8 && ((rows * 2 * C <= sms && slots > 8192 * C) || slots > 32 * kEvThreads * C)) C *= 2;
   const int need = (slots + C * kEvThreads - 1) / (C * kEvThreads);
   const dim3 grid(static_cast<unsigned>(rows) * C), block(kEvThreads);
-  cudaError_t e;
-  if (need <= 4) e = launch_dependent(paged_evict_select_kernel<4>, grid, block, 0, s, C, p);
-  else if (need <= 8) e = launch_dependent(paged_evict_select_kernel<8>, grid, block, 0, s, C, p);
-  else if (need <= 32) e = launch_dependent(paged_evict_select_kernel<32>, grid, block, 0, s, C, p);
-  else e = launch_dependent(paged_evict_select_kernel<0>, grid, block, 0, s, C, p);
+  auto kernel = need <= 4    ? paged_evict_select_kernel<4>
+                : need <= 8  ? paged_evict_select_kernel<8>
+                : need <= 32 ? paged_evict_select_kernel<32>
+                             : paged_evict_select_kernel<0>;
+  const size_t smem = sizeof(uint32_t) * kEvAllBins * (C > 1 ? 2 : 1);
+  cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kernel), 2 * 4 * kEvAllBins);
+  if (e == cudaSuccess) e = launch_dependent(kernel, grid, block, smem, s, C, p);
   return e == cudaSuccess ? DCR_OK : DCR_ERR_CUDA;
 }
 
@@ -372,7 +389,7 @@ template <int RowBytes>
 static int ev_launch_move(const PagedEvictParams& p, int rows, int most, cudaStream_t s) {
   constexpr int kPer = 8 * (32 * 16 / RowBytes) * 2;  // pairs a CTA takes at once
   int x = (most + kPer - 1) / kPer;
-  const int cap = (device_sm_count() * 8 + rows - 1) / rows;  // the GPU full once
+  const int cap = (device_sm_count() * 3 + rows - 1) / rows;  // the GPU full once
   if (x > cap) x = cap;
   return launch_dependent(paged_evict_move_kernel<RowBytes>, dim3(x, rows), dim3(256), 0, s, 1, p) ==
                  cudaSuccess
