@@ -11,12 +11,14 @@
 // cache under eviction). The reference's step is HF apply_rotary_pos_emb and a torch.cat
 // (dcr_attention/models/llama/attention.py:395-421); the norms have no counterpart there.
 //
-// Bound: the rows, read and written once. A row is spread over its 16-byte chunks' lanes (8, 16
-// or 32), so a warp takes 4, 2 or 1 rows at a time and every access is 16 bytes a lane; the
-// element D/2 away sits in the lane half a row away and comes by shuffle. A warp takes up to
-// kApSteps such steps of one token and kind (query, key, value): the token's table rows times
-// the norm weight are folded into two factors once, x' = rs * (x * (w c) + x_far * (w_far s)),
-// and all its rows are in flight before the first is used.
+// Bound: the rows, read and written once; and the issue slots, since a 16-bit element costs a
+// conversion, a square, two products and a rounding. A lane holds a 16-byte chunk of a row and the
+// chunk half a row further, which the rotation pairs with it, so no element is exchanged or
+// converted twice (by shuffles between the lanes of the two halves the prompts below took 78.7
+// us). A row takes 4 to 16 lanes, a warp kApSteps times 8 to 2 rows of one token and kind (query,
+// key, value): the token's table rows times the norm weights are folded into two factors once,
+// x' = rs * (x * (w c) + x_far * (w_far s)), and all its rows are in flight before the first is
+// used.
 #include <type_traits>
 
 #include "dcr_internal.h"
@@ -50,7 +52,7 @@ struct PagedAppendParams {
 };
 
 constexpr int kApWarps = 4;
-constexpr int kApSteps = 4;
+constexpr int kApSteps = 2;
 
 // N consecutive elements from a 16-byte (or wider) aligned address, widened.
 template <typename T, int N>
@@ -78,10 +80,20 @@ __device__ __forceinline__ uint32_t ap_pack(float a, float b) {
   }
 }
 
+template <typename T>
+__device__ __forceinline__ uint4 ap_round(const float2 (&f)[ElemTraits<T>::kPerChunk / 2]) {
+  if constexpr (sizeof(T) == 4)
+    return make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x),
+                      __float_as_uint(f[1].y));
+  else
+    return make_uint4(ap_pack<T>(f[0].x, f[0].y), ap_pack<T>(f[1].x, f[1].y),
+                      ap_pack<T>(f[2].x, f[2].y), ap_pack<T>(f[3].x, f[3].y));
+}
+
 template <typename T, typename TC, int D>
 __global__ void __launch_bounds__(kApWarps * 32) paged_append_kernel(const PagedAppendParams p) {
-  constexpr int N = ElemTraits<T>::kPerChunk;  // elements per lane
-  constexpr int L = D / N;                     // lanes per row
+  constexpr int N = ElemTraits<T>::kPerChunk;  // elements of a chunk
+  constexpr int L = D / (2 * N);               // lanes per row: chunks ch and ch + L
   constexpr int RW = 32 / L;                   // rows per step
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
@@ -100,13 +112,15 @@ __global__ void __launch_bounds__(kApWarps * 32) paged_append_kernel(const Paged
   const int h0 = blk * RW * kApSteps + sub;  // this lane's heads: h0, h0 + RW, ...
   const char* src = static_cast<const char*>(kind == 0 ? p.q : kind == 1 ? p.k : p.v) + ch * 16;
   const int64_t st = kind == 0 ? p.qst : kind == 1 ? p.kst : p.vst;
-  const int64_t sh = kind == 0 ? p.qsh : kind == 1 ? p.ksh : p.vsh;
-  uint4 x[kApSteps];
+  const int64_t sh = (kind == 0 ? p.qsh : kind == 1 ? p.ksh : p.vsh) * static_cast<int64_t>(sizeof(T));
+  src += t * st * static_cast<int64_t>(sizeof(T));
+  uint4 x[kApSteps][2];
 #pragma unroll
   for (int i = 0; i < kApSteps; ++i) {
     const int h = h0 + i * RW;
-    x[i] = h < heads ? __ldg(reinterpret_cast<const uint4*>(src + (t * st + h * sh) * static_cast<int64_t>(sizeof(T))))
-                     : make_uint4(0u, 0u, 0u, 0u);
+    const uint4* row = reinterpret_cast<const uint4*>(src + h * sh);
+    x[i][0] = h < heads ? __ldg(row) : make_uint4(0u, 0u, 0u, 0u);
+    x[i][1] = h < heads ? __ldg(row + L) : make_uint4(0u, 0u, 0u, 0u);
   }
   const int position = __ldg(p.positions + t);
   const bool fine = position >= 0 && position < p.n_pos;
@@ -148,78 +162,83 @@ __global__ void __launch_bounds__(kApWarps * 32) paged_append_kernel(const Paged
   dst += ch * 16;
   if (kind == 2) {
 #pragma unroll
-    for (int i = 0; i < kApSteps; ++i)
-      if (h0 + i * RW < heads) *reinterpret_cast<uint4*>(dst + (h0 + i * RW) * dh) = x[i];
+    for (int i = 0; i < kApSteps; ++i) {
+      if (h0 + i * RW >= heads) break;
+      uint4* row = reinterpret_cast<uint4*>(dst + (h0 + i * RW) * dh);
+      row[0] = x[i][0];
+      row[L] = x[i][1];
+    }
     return;
   }
 
-  // x' = rs * (x * near + x_far * far); the far half of a row enters the near one with a minus
-  float near[N], far[N];
+  // [half]: x'[half] = rs * (x[half] * near[half] + x[other half] * far[half]), where the first
+  // half's far factor has a minus
+  float2 near[2][N / 2], far[2][N / 2];
+  const void* w = kind == 0 ? p.qw : p.kw;
   {
     const int64_t row = static_cast<int64_t>(fine ? position : 0) * D + ch * N;
-    ap_load<TC, N>(p.cos, row, near);
-    ap_load<TC, N>(p.sin, row, far);
-    const float sign = ch < L / 2 ? -1.0f : 1.0f;
-    const void* w = kind == 0 ? p.qw : p.kw;
-    float wn[N], wf[N];
+    float wt[2][N];
     if (w != nullptr) {
-      ap_load<T, N>(w, ch * N, wn);
-      ap_load<T, N>(w, (ch ^ (L / 2)) * N, wf);
+      ap_load<T, N>(w, ch * N, wt[0]);
+      ap_load<T, N>(w, ch * N + D / 2, wt[1]);
     }
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      near[e] *= w != nullptr ? wn[e] : 1.0f;
-      far[e] *= sign * (w != nullptr ? wf[e] : 1.0f);
-    }
-  }
-  const bool norm = (kind == 0 ? p.qw : p.kw) != nullptr;
-#pragma unroll
-  for (int i = 0; i < kApSteps; ++i) {
-    float a[N], b[N];
-    ElemTraits<T>::widen(x[i], a);
-    uint4 y;
-    y.x = __shfl_xor_sync(0xffffffffu, x[i].x, L / 2);
-    y.y = __shfl_xor_sync(0xffffffffu, x[i].y, L / 2);
-    y.z = __shfl_xor_sync(0xffffffffu, x[i].z, L / 2);
-    y.w = __shfl_xor_sync(0xffffffffu, x[i].w, L / 2);
-    ElemTraits<T>::widen(y, b);
-    float rs = 1.0f;
-    if (norm) {
-      float2 s2 = make_float2(0.0f, 0.0f);
+    for (int half = 0; half < 2; ++half) {
+      float c[N], s[N];
+      ap_load<TC, N>(p.cos, row + half * (D / 2), c);
+      ap_load<TC, N>(p.sin, row + half * (D / 2), s);
 #pragma unroll
       for (int e = 0; e < N; e += 2) {
-        const float2 v = make_float2(a[e], a[e + 1]);
-        s2 = ffma2(v, v, s2);
+        near[half][e / 2] = w != nullptr ? make_float2(c[e] * wt[half][e], c[e + 1] * wt[half][e + 1])
+                                         : make_float2(c[e], c[e + 1]);
+        const float2 f = w != nullptr ? make_float2(s[e] * wt[1 - half][e], s[e + 1] * wt[1 - half][e + 1])
+                                      : make_float2(s[e], s[e + 1]);
+        far[half][e / 2] = half == 0 ? make_float2(-f.x, -f.y) : f;
       }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kApSteps; ++i) {
+    float2 a[2][N / 2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      float f[N];
+      ElemTraits<T>::widen(x[i][half], f);
+#pragma unroll
+      for (int e = 0; e < N; e += 2) a[half][e / 2] = make_float2(f[e], f[e + 1]);
+    }
+    const float2 zero = make_float2(0.0f, 0.0f);
+    float2 rs = make_float2(1.0f, 1.0f);
+    if (w != nullptr) {
+      float2 s2 = zero;
+#pragma unroll
+      for (int e = 0; e < N / 2; ++e) s2 = ffma2(a[1][e], a[1][e], ffma2(a[0][e], a[0][e], s2));
       float ss = s2.x + s2.y;
 #pragma unroll
       for (int o = L / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      rs = rsqrtf(ss * (1.0f / D) + p.eps);
+      rs.x = rs.y = rsqrtf(ss * (1.0f / D) + p.eps);
     }
-    const float2 rs2 = make_float2(rs, rs), zero = make_float2(0.0f, 0.0f);
-    float2 out[N / 2];
+    uint4 r[2];
 #pragma unroll
-    for (int e = 0; e < N; e += 2) {
-      const float2 f = ffma2(make_float2(b[e], b[e + 1]), make_float2(far[e], far[e + 1]), zero);
-      const float2 s = ffma2(make_float2(a[e], a[e + 1]), make_float2(near[e], near[e + 1]), f);
-      out[e / 2] = norm ? ffma2(s, rs2, zero) : s;
+    for (int half = 0; half < 2; ++half) {
+      float2 out[N / 2];
+#pragma unroll
+      for (int e = 0; e < N / 2; ++e) {
+        out[e] = ffma2(a[half][e], near[half][e], ffma2(a[1 - half][e], far[half][e], zero));
+        if (w != nullptr) out[e] = ffma2(out[e], rs, zero);
+      }
+      r[half] = ap_round<T>(out);
     }
     if (h0 + i * RW >= heads) continue;
-    uint4 r;
-    if constexpr (N == 8) {
-      r = make_uint4(ap_pack<T>(out[0].x, out[0].y), ap_pack<T>(out[1].x, out[1].y),
-                     ap_pack<T>(out[2].x, out[2].y), ap_pack<T>(out[3].x, out[3].y));
-    } else {
-      r = make_uint4(__float_as_uint(out[0].x), __float_as_uint(out[0].y),
-                     __float_as_uint(out[1].x), __float_as_uint(out[1].y));
-    }
-    *reinterpret_cast<uint4*>(dst + (h0 + i * RW) * dh) = fine ? r : make_uint4(0u, 0u, 0u, 0u);
+    uint4* row = reinterpret_cast<uint4*>(dst + (h0 + i * RW) * dh);
+    row[0] = fine ? r[0] : make_uint4(0u, 0u, 0u, 0u);
+    row[L] = fine ? r[1] : make_uint4(0u, 0u, 0u, 0u);
   }
 }
 
 template <typename T, typename TC>
 static cudaError_t launch_paged_append(const PagedAppendParams& p, int D, cudaStream_t s) {
-  const int per = kApSteps * 32 * ElemTraits<T>::kPerChunk / D;  // heads per warp
+  const int per = kApSteps * 64 * ElemTraits<T>::kPerChunk / D;  // heads per warp
   const int64_t warps = static_cast<int64_t>(p.T) * ((p.H + per - 1) / per + 2 * ((p.H_kv + per - 1) / per));
   const unsigned grid = static_cast<unsigned>((warps + kApWarps - 1) / kApWarps);
   return launch_dependent(D == 64 ? paged_append_kernel<T, TC, 64> : paged_append_kernel<T, TC, 128>,
