@@ -18,7 +18,10 @@
 // us). A row takes 4 to 16 lanes, a warp kApSteps times 8 to 2 rows of one token and kind (query,
 // key, value): the token's table rows times the norm weights are folded into two factors once,
 // x' = rs * (x * (w c) + x_far * (w_far s)), and all its rows are in flight before the first is
-// used.
+// used. Rows are read and written once, as streaming accesses (77.3 us without the hint on both
+// sides, 70.0 with it). Measured: 16381 tokens of 32 + 2 x 8 heads of 128 in f16, 404 MB, in 70.0
+// us, 5.77 TB/s, 88% of the measured copy bandwidth; a warp that took a whole token, the next rows
+// on their way meanwhile, needed 126 registers and 83 us.
 #include <type_traits>
 
 #include "dcr_internal.h"
@@ -119,8 +122,8 @@ __global__ void __launch_bounds__(kApWarps * 32) paged_append_kernel(const Paged
   for (int i = 0; i < kApSteps; ++i) {
     const int h = h0 + i * RW;
     const uint4* row = reinterpret_cast<const uint4*>(src + h * sh);
-    x[i][0] = h < heads ? __ldg(row) : make_uint4(0u, 0u, 0u, 0u);
-    x[i][1] = h < heads ? __ldg(row + L) : make_uint4(0u, 0u, 0u, 0u);
+    x[i][0] = h < heads ? __ldcs(row) : make_uint4(0u, 0u, 0u, 0u);
+    x[i][1] = h < heads ? __ldcs(row + L) : make_uint4(0u, 0u, 0u, 0u);
   }
   const int position = __ldg(p.positions + t);
   const bool fine = position >= 0 && position < p.n_pos;
@@ -165,8 +168,8 @@ __global__ void __launch_bounds__(kApWarps * 32) paged_append_kernel(const Paged
     for (int i = 0; i < kApSteps; ++i) {
       if (h0 + i * RW >= heads) break;
       uint4* row = reinterpret_cast<uint4*>(dst + (h0 + i * RW) * dh);
-      row[0] = x[i][0];
-      row[L] = x[i][1];
+      __stcs(row, x[i][0]);
+      __stcs(row + L, x[i][1]);
     }
     return;
   }
@@ -231,8 +234,8 @@ __global__ void __launch_bounds__(kApWarps * 32) paged_append_kernel(const Paged
     }
     if (h0 + i * RW >= heads) continue;
     uint4* row = reinterpret_cast<uint4*>(dst + (h0 + i * RW) * dh);
-    row[0] = fine ? r[0] : make_uint4(0u, 0u, 0u, 0u);
-    row[L] = fine ? r[1] : make_uint4(0u, 0u, 0u, 0u);
+    __stcs(row, fine ? r[0] : make_uint4(0u, 0u, 0u, 0u));
+    __stcs(row + L, fine ? r[1] : make_uint4(0u, 0u, 0u, 0u));
   }
 }
 
