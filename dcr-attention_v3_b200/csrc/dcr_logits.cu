@@ -228,9 +228,17 @@ __global__ void __launch_bounds__(kLgThreads) logits_kernel(const LogitsParams p
       for (int j = tid; j < count; j += kLgThreads) cp_async_4(mask + j, allowed + w0 + j);
     }
     cp_async_commit();
-    int ahead = va + tid;
+    // With a bias on 16-bit logits, whose bytes are twice the logits', the stream begins at
+    // another place in every row: rows that share a bias would all read the same part of it at
+    // the same time (128 rows of 128256 with mask and history 40.9 instead of 48.9 us; without a
+    // bias or in fp32 it costs 2 us and gains nothing).
+    constexpr bool kTurn = kBias && N == 8;
+    const int rounds = (vb - va + kLgStream - 1) / kLgStream;
+    const int begin = kTurn && rounds > 0 ? va + tid + b % rounds * kLgStream : va + tid;
+    const int turns = va + tid + rounds * kLgStream;  // past it, back to the first vector
+    int ahead = begin, left = rounds;
     auto fetch = [&](int slot) {
-      if (ahead < vb && streams) {
+      if (ahead < vb && streams && (!kTurn || left > 0)) {
         uint4* dst = ring + slot * (R::kParts * kLgStream) + tid;
         const int t = ahead * N - off;
         cp_async_16(dst, x + t, 16u);
@@ -248,6 +256,8 @@ __global__ void __launch_bounds__(kLgThreads) logits_kernel(const LogitsParams p
       }
       cp_async_commit();
       ahead += kLgStream;
+      if (kTurn && ahead == turns) ahead = va + tid;
+      --left;
     };
 #pragma unroll
     for (int i = 0; i < R::kAhead; ++i) fetch(i);
@@ -335,9 +345,12 @@ __global__ void __launch_bounds__(kLgThreads) logits_kernel(const LogitsParams p
         }
       }
     } else {
-      int slot = 0;
+      int slot = 0, v = begin - kLgStream;
 #pragma unroll 1
-      for (int v = va + tid; v < vb; v += kLgStream) {
+      for (int i = 0; i < rounds; ++i) {
+        v += kLgStream;
+        if (kTurn && v == turns) v = va + tid;
+        if (!kTurn && v >= vb) break;
         cp_async_wait<R::kAhead - 1>();
         float f[N];
         const uint4* src = ring + slot * (R::kParts * kLgStream) + tid;
@@ -355,6 +368,7 @@ __global__ void __launch_bounds__(kLgThreads) logits_kernel(const LogitsParams p
         }
         fetch(slot);  // the thread's own place, which it has just read
         slot = slot + 1 == R::kAhead ? 0 : slot + 1;
+        if (kTurn && v >= vb) continue;
         const int place = (v - v0) * N, t = v * N - off;
         const uint32_t marked = n > 0 ? (marks[place >> 5] >> (place & 31)) & ((1u << N) - 1u) : 0u;
         const uint32_t in = allowed_at(t) & ~marked;
