@@ -82,7 +82,7 @@ inline int check_pool(const void* k, const void* v, int dtype, int64_t ksp, int6
   }
   if (D != 64 && D != 128) return DCR_ERR_SHAPE;
   if (H_kv <= 0 || num_pages <= 0 || page_size <= 0 || max_pages <= 0) return DCR_ERR_SHAPE;
-  if (static_cast<int64_t>(max_pages) * page_size > 0x7fff0000ll) return DCR_ERR_SHAPE;
+  if (static_cast<int64_t>(max_pages) * page_size > (1ll << 29)) return DCR_ERR_SHAPE;
   if (table_stride < max_pages) return DCR_ERR_SHAPE;
   const int64_t st[6] = {ksp, ksh, ksr, vsp, vsh, vsr};
   for (int i = 0; i < 6; ++i) {

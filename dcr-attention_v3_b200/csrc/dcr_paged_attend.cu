@@ -106,6 +106,11 @@ __device__ __forceinline__ void pa_store_stats(const PagedAttendParams& p, int64
   if (p.stats != nullptr) p.stats[row] = l == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(m, 1.0f / l);
 }
 
+// 8-byte asynchronous global->shared copy.
+__device__ __forceinline__ void cp_async_8(void* smem_dst, const void* gsrc) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(smem_dst)), "l"(gsrc) : "memory");
+}
+
 // Adds a state's sum x (with maximum m) to one with maximum M >= m. A state without any valid
 // slot (m = -inf) adds nothing; a NaN goes through.
 __device__ __forceinline__ void pa_fold_sum(float M, float m, float x, float& sum) {
@@ -152,11 +157,13 @@ __device__ __forceinline__ uint64_t pa_div(uint64_t a, uint32_t b) {
   return (a >> 32) == 0 ? static_cast<uint32_t>(a) / b : a / b;
 }
 
-// How the line is shared out: every CTA gets `each` tiles, the first `more` one more.
+// How the line is shared out: every CTA gets `each` tiles, the first `more` one more. Lane l of
+// a warp sums up `per` neighbouring sequences for the search that follows.
 struct PaLine {
   int64_t total, each;
   int ctas, more;
-  int n_lane;  // tiles of sequence `lane`, for the search that follows
+  int per;
+  int64_t upto;  // tiles per unit of this lane's sequences and all before
 
   __device__ __forceinline__ int64_t begin(int c) const { return c * each + (c < more ? c : more); }
   __device__ __forceinline__ int cta_of(int64_t place) const {
@@ -170,17 +177,23 @@ template <int R>
 __device__ __forceinline__ PaLine pa_line(const PagedAttendParams& p, int ctas) {
   const int lane = threadIdx.x & 31;
   PaLine a;
-  a.n_lane = 0;
-  int64_t n = 0;
-  for (int b = lane; b < p.B; b += 32) {
-    int len, lo, t_lo, t_hi;
-    pa_sequence<R>(p, b, len, lo, t_lo, t_hi);
-    if (b == lane) a.n_lane = t_hi - t_lo;
-    n += t_hi - t_lo;
+  a.per = (p.B + 31) >> 5;
+  a.upto = 0;
+#pragma unroll 4
+  for (int j = 0; j < a.per; ++j) {
+    const int b = lane * a.per + j;
+    if (b < p.B) {
+      int len, lo, t_lo, t_hi;
+      pa_sequence<R>(p, b, len, lo, t_lo, t_hi);
+      a.upto += t_hi - t_lo;
+    }
   }
 #pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-  a.total = n * p.units;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, a.upto, o);
+    if (lane >= o) a.upto += y;
+  }
+  a.total = __shfl_sync(0xffffffffu, a.upto, 31) * p.units;
   const int64_t want = (a.total + kPaMinTiles - 1) / kPaMinTiles;
   a.ctas = want < ctas ? static_cast<int>(want) : ctas;
   a.each = a.ctas > 0 ? pa_div(a.total, a.ctas) : 0;
@@ -192,40 +205,26 @@ __device__ __forceinline__ PaLine pa_line(const PagedAttendParams& p, int ctas) 
 template <int R>
 __device__ __forceinline__ PaCursor pa_seek(const PagedAttendParams& p, const PaLine& line,
                                             int64_t s) {
-  const int lane = threadIdx.x & 31;
-  int64_t before = 0;
+  const unsigned hit = __ballot_sync(0xffffffffu, s < line.upto * p.units);
+  const int l = hit != 0 ? __ffs(hit) - 1 : 31;
+  int64_t before = __shfl_sync(0xffffffffu, line.upto, l > 0 ? l - 1 : 0);
+  before = l > 0 ? before * p.units : 0;
+  PaCursor c;
+  c.b = l * line.per;
+  pa_sequence<R>(p, c.b, c.len, c.lo, c.t_lo, c.t_hi);
 #pragma unroll 1
-  for (int b0 = 0;; b0 += 32) {
-    const int b = b0 + lane;
-    int n = line.n_lane;
-    if (b0 > 0) {
-      n = 0;
-      if (b < p.B) {
-        int len, lo, t_lo, t_hi;
-        pa_sequence<R>(p, b, len, lo, t_lo, t_hi);
-        n = t_hi - t_lo;
-      }
-    }
-    int64_t incl = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += y;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, s < before + incl * p.units);
-    if (hit != 0 || b0 + 32 >= p.B) {
-      const int src = hit != 0 ? __ffs(hit) - 1 : 31;
-      PaCursor c;
-      c.b = b0 + src < p.B ? b0 + src : p.B - 1;
-      pa_sequence<R>(p, c.b, c.len, c.lo, c.t_lo, c.t_hi);
-      const int64_t off = s - (before + __shfl_sync(0xffffffffu, incl - n, src) * p.units);
-      const int nt = c.t_hi - c.t_lo;
-      c.u = nt > 0 ? static_cast<int>(pa_div(off, nt)) : 0;
-      c.t = c.t_lo + static_cast<int>(off - static_cast<int64_t>(c.u) * nt);
-      return c;
-    }
-    before += __shfl_sync(0xffffffffu, incl, 31) * p.units;
+  while (c.b + 1 < p.B) {
+    const int64_t tiles = static_cast<int64_t>(c.t_hi - c.t_lo) * p.units;
+    if (s < before + tiles) break;
+    before += tiles;
+    ++c.b;
+    pa_sequence<R>(p, c.b, c.len, c.lo, c.t_lo, c.t_hi);
   }
+  const int nt = c.t_hi - c.t_lo;
+  const int64_t off = s - before;
+  c.u = nt > 0 ? static_cast<int>(pa_div(off, nt)) : 0;
+  c.t = c.t_lo + static_cast<int>(off - static_cast<int64_t>(c.u) * nt);
+  return c;
 }
 
 // The copies of one tile: K's rows, then V's. Where pages hold whole groups of 16 slots (or R,
@@ -793,42 +792,49 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const Paged
   }
   __syncthreads();
 
-  // Fold the CTA's pieces, row by row over the warps; lane x holds piece x. The pieces of a
-  // unit are neighbours. Odd pieces are in the rings, even ones in the warps' own places.
+  // Fold the CTA's pieces: the rows of all its units are dealt out to the warps. Lane x holds
+  // piece x; the pieces of a unit are neighbours. Odd pieces are in the rings, even ones in the
+  // warps' own places.
   const PaPiece mine = pieces[lane % (2 * kPaWarps)];
   const bool have = lane < 2 * kPaWarps && mine.u >= 0;
-  const float* own_piece = reinterpret_cast<const float*>(
-      (lane & 1) ? pa_smem + (lane >> 1) % kPaWarps * (S::NH * S::kHalf)
-                 : pa_smem + kPaWarps * (S::NH * S::kHalf) +
-                       (lane >> 1) % kPaWarps * (S::kPiece + S::kQ + S::kP + 64));
+  auto piece_at = [&](int x) {
+    return reinterpret_cast<const float*>(
+        (x & 1) ? pa_smem + (x >> 1) * (S::NH * S::kHalf)
+                : pa_smem + kPaWarps * (S::NH * S::kHalf) + (x >> 1) * (S::kPiece + S::kQ + S::kP + 64));
+  };
+  const float* own_piece = piece_at(lane % (2 * kPaWarps));
   unsigned todo = __ballot_sync(0xffffffffu, have);
+  int dealt = warp;  // rows until this warp's next one
   while (todo != 0) {
     const int lead = __ffs(todo) - 1;
     const int b = __shfl_sync(0xffffffffu, mine.b, lead), u = __shfl_sync(0xffffffffu, mine.u, lead);
-    const bool in = have && mine.b == b && mine.u == u;
-    const unsigned run = __ballot_sync(0xffffffffu, in);
+    const unsigned run = __ballot_sync(0xffffffffu, have && mine.b == b && mine.u == u);
     todo &= ~run;
     const bool before = __shfl_sync(0xffffffffu, mine.before, lead);
     const bool after = __shfl_sync(0xffffffffu, mine.after, 31 - __clz(run));
     const int hk = u / p.hblocks, h0 = (u - hk * p.hblocks) * HB;
     const int rows = p.G - h0 < HB ? p.G - h0 : HB;
-    for (int g = warp; g < rows; g += kPaWarps) {
+    for (; dealt < rows; dealt += kPaWarps) {
+      const int g = dealt;
+      const bool in = (run >> lane) & 1u;
       const float m = in ? own_piece[g * (D + 2) + D] : -INFINITY;
       float M = m;
 #pragma unroll
-      for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+      for (int o = kPaWarps; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+      M = __shfl_sync(0xffffffffu, M, lead);  // pieces are in the first 2 * kPaWarps lanes
       float L = 0.0f;
       if (in) pa_fold_sum(M, m, own_piece[g * (D + 2) + D + 1], L);
 #pragma unroll
-      for (int o = 16; o >= 1; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+      for (int o = kPaWarps; o >= 1; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+      L = __shfl_sync(0xffffffffu, L, lead);
       float acc[D / 32] = {};
+#pragma unroll 1
       for (unsigned left = run; left != 0; left &= left - 1) {
         const int x = __ffs(left) - 1;
         const float mx = __shfl_sync(0xffffffffu, m, x);
-        const float* src = reinterpret_cast<const float*>(
-            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(own_piece), x));
+        const float* src = piece_at(x) + g * (D + 2);
 #pragma unroll
-        for (int e = 0; e < D / 32; ++e) pa_fold_sum(M, mx, src[g * (D + 2) + lane + 32 * e], acc[e]);
+        for (int e = 0; e < D / 32; ++e) pa_fold_sum(M, mx, src[lane + 32 * e], acc[e]);
       }
       if (!before && !after) {
         const int64_t row = static_cast<int64_t>(b) * p.H + hk * p.G + h0 + g;
@@ -847,6 +853,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const Paged
         }
       }
     }
+    dealt -= rows;
   }
 
   // rows of empty sequences
@@ -864,16 +871,17 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const Paged
 
 // Folds the partials of the unit that begins in CTA blockIdx.x of the first kernel and ends in
 // a later one; blockIdx.y is the row of the head block. What there is to fold follows from the
-// lengths, so it is known before the first kernel is done; then one round of loads is left.
-// Thread groups of D take every (128 / D)-th partial. (CTAs with nothing to fold leave at once,
-// all but the first: the kernel must not end before the one it waits for.)
-constexpr int kFoldThreads = 128;
+// lengths, so it is known before the first kernel is done; then up to kFoldParts partials are
+// copied to shared memory at once and folded from there. The code is kept small and rolled up:
+// it runs once, from a cold instruction cache. (CTAs with nothing to fold leave at once, all but
+// the first: the kernel must not end before the one it waits for.)
+constexpr int kFoldThreads = 128, kFoldParts = 32;
 
 template <typename T, int D, int HB>
 __global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const PagedAttendParams p) {
   using S = PaShape<T, D, HB>;
-  constexpr int N = kFoldThreads / D, kBatch = 8;
-  __shared__ float m_s[N], l_s[N], acc_s[kFoldThreads];
+  constexpr int W = D + 2;              // o, m, l
+  __shared__ __align__(8) float part[kFoldParts * W];
   asm volatile("griddepcontrol.launch_dependents;");
   const PaLine line = pa_line<S::R>(p, gridDim.x);
   const int c0 = blockIdx.x;
@@ -892,50 +900,48 @@ __global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const PagedAtt
   if (!open && blockIdx.x + blockIdx.y > 0) return;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!open) return;
-  const int d = threadIdx.x % D, k = threadIdx.x / D;
+  const int d = threadIdx.x;
   float M = -INFINITY, L = 0.0f, acc = 0.0f;
-  for (int c1 = c0 + k; c1 <= last; c1 += N * kBatch) {
-    float m[kBatch], l[kBatch], v[kBatch];
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int x = c1 + N * i;
-      const float* src = p.part + ((2 * static_cast<int64_t>(x) + (x == c0 ? 1 : 0)) * HB + blockIdx.y) * (D + 2);
-      m[i] = x <= last ? src[D] : -INFINITY;
-      l[i] = x <= last ? src[D + 1] : 0.0f;
-      v[i] = x <= last ? src[d] : 0.0f;
+#pragma unroll 1
+  for (int c1 = c0; c1 <= last; c1 += kFoldParts) {
+    const int count = min(kFoldParts, last + 1 - c1);
+    if (c1 > c0) __syncthreads();
+#pragma unroll 1
+    for (int i = threadIdx.x; i < count * (W / 2); i += kFoldThreads) {
+      const int x = i / (W / 2), e = i - x * (W / 2);
+      const float* src = p.part + ((2 * static_cast<int64_t>(c1 + x) + (c1 + x == c0 ? 1 : 0)) * HB + blockIdx.y) * W;
+      cp_async_8(part + x * W + 2 * e, src + 2 * e);
     }
-    float top = M;
+    cp_async_commit();
+    cp_async_wait<0>();
+    __syncthreads();
+    // lane x holds partial x's statistics, in every warp
+    const int lane = threadIdx.x & 31;
+    const float m = lane < count ? part[lane * W + D] : -INFINITY;
+    float top = fmaxf(M, m);
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) top = fmaxf(top, m[i]);
-    const float a = M == -INFINITY ? 0.0f : pa_exp2(M - top);
-    L = M == -INFINITY ? L : L * a;
-    acc = M == -INFINITY ? acc : acc * a;
+    for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (M != -INFINITY) {
+      const float a = pa_exp2(M - top);
+      L *= a;
+      acc *= a;
+    }
     M = top;
+    float l = 0.0f;
+    if (lane < count) pa_fold_sum(M, m, part[lane * W + D + 1], l);
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      pa_fold_sum(M, m[i], l[i], L);
-      pa_fold_sum(M, m[i], v[i], acc);
+    for (int o = 16; o >= 1; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    L += l;
+#pragma unroll 4
+    for (int x = 0; x < count; ++x) {
+      const float mx = __shfl_sync(0xffffffffu, m, x);
+      pa_fold_sum(M, mx, part[x * W + (d < D ? d : 0)], acc);
     }
   }
-  acc_s[threadIdx.x] = acc;
-  if (d == 0) {
-    m_s[k] = M;
-    l_s[k] = L;
-  }
-  __syncthreads();
-  if (k > 0) return;
-  float top = M;
-#pragma unroll
-  for (int i = 1; i < N; ++i) top = fmaxf(top, m_s[i]);
-  float sl = 0.0f, sa = 0.0f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    pa_fold_sum(top, m_s[i], l_s[i], sl);
-    pa_fold_sum(top, m_s[i], acc_s[i * D + d], sa);
-  }
+  if (d >= D) return;
   const int64_t row = static_cast<int64_t>(c.b) * p.H + hk * p.G + h;
-  ElemTraits<T>::store(static_cast<T*>(p.o) + row * D, d, sl == 0.0f ? 0.0f : sa / sl);
-  if (d == 0) pa_store_stats(p, row, top, sl);
+  ElemTraits<T>::store(static_cast<T*>(p.o) + row * D, d, L == 0.0f ? 0.0f : acc / L);
+  if (d == 0) pa_store_stats(p, row, M, L);
 }
 
 // weights[b][h_kv][i] += sum over the G heads of exp2(score - m) / l, in head order. A thread

@@ -428,7 +428,8 @@ int dcr_silu_mul_packed(const void* gate_up, int dtype, int rows, int inter, voi
  * h in page p is pages[p * stride_p + h * stride_h + s * stride_s + d] (strides in elements,
  * multiples of 16 bytes, for K and V separately; rows contiguous). Sequence b's slot i is in
  * page page_table[b * table_stride + i / page_size] at i % page_size; a negative entry is a
- * page that is not mapped. D is 64 or 128 and H any multiple of H_kv here. Nothing outside the
+ * page that is not mapped; max_pages * page_size is at most 2^29. D is 64 or 128 and H any
+ * multiple of H_kv here. Nothing outside the
  * pool is read or written whatever lengths, tables, slots, positions and tokens hold on the
  * device: an entry out of range is skipped and sets DCR_ERR_DEVICE_INDEX in the device status
  * (a length beyond max_pages * page_size is taken as that, a negative one as 0).
