@@ -55,7 +55,9 @@ cudaError_t launch_cluster(Kernel kernel, dim3 grid, dim3 block, size_t smem, cu
 // cluster > 1, as clusters of that many CTAs): its CTAs may be placed while that kernel drains.
 // Every such kernel begins with griddepcontrol.wait in all its threads, before it reads or
 // writes anything a kernel before it may touch; so kernels of a stream still follow one another,
-// whatever came before, and only the launch itself overlaps.
+// whatever came before, and only the launch itself overlaps. They read what others may have
+// written by plain loads: a read-only (non-coherent) load promises that nothing writes the data
+// while the kernel exists, and it exists before its predecessor is done.
 template <typename... Args>
 cudaError_t launch_dependent(void (*kernel)(Args...), dim3 grid, dim3 block, size_t smem,
                              cudaStream_t st, int cluster, Args... args) {

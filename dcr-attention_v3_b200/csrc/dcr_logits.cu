@@ -110,8 +110,8 @@ __device__ __forceinline__ float lg_max(float a, float b) {
 // A history's token i, -1 past the first n.
 __device__ __forceinline__ int64_t lg_token(const LogitsParams& p, int b, int i, int n) {
   if (i >= n) return -1;
-  return p.tok64 ? static_cast<int64_t>(__ldg(static_cast<const long long*>(p.tokens) + b * p.tsb + i))
-                 : static_cast<int64_t>(__ldg(static_cast<const int*>(p.tokens) + b * p.tsb + i));
+  return p.tok64 ? static_cast<int64_t>(static_cast<const long long*>(p.tokens)[b * p.tsb + i])
+                 : static_cast<int64_t>(static_cast<const int*>(p.tokens)[b * p.tsb + i]);
 }
 
 // Its place in the chunk [t0, t0 + span); -1 elsewhere or padding, -2 past the vocabulary.
@@ -200,24 +200,24 @@ __global__ void __launch_bounds__(kLgThreads) logits_kernel(const LogitsParams p
 #pragma unroll
       for (int u = 0; u < kLgHeld; ++u) {
         const int i = tid + u * kLgThreads;
-        token[u] = i < p.L ? static_cast<int64_t>(__ldg(static_cast<const long long*>(p.tokens) + b * p.tsb + i)) : -1;
+        token[u] = i < p.L ? static_cast<int64_t>(static_cast<const long long*>(p.tokens)[b * p.tsb + i]) : -1;
       }
     } else {
 #pragma unroll
       for (int u = 0; u < kLgHeld; ++u) {
         const int i = tid + u * kLgThreads;
-        token[u] = i < p.L ? static_cast<int64_t>(__ldg(static_cast<const int*>(p.tokens) + b * p.tsb + i)) : -1;
+        token[u] = i < p.L ? static_cast<int64_t>(static_cast<const int*>(p.tokens)[b * p.tsb + i]) : -1;
       }
     }
     if (v0 == rank * each) {
       if (p.L > 0) {
-        n = p.n_tok != nullptr ? __ldg(p.n_tok + b) : p.L;
+        n = p.n_tok != nullptr ? p.n_tok[b] : p.L;
         n = n < 0 ? 0 : n > p.L ? p.L : n;
-        prompt = p.n_prompt != nullptr ? __ldg(p.n_prompt + b) : 0;
+        prompt = p.n_prompt != nullptr ? p.n_prompt[b] : 0;
       }
-      row.r = p.repetition != nullptr ? __ldg(p.repetition + b) : 1.0f;
-      row.pr = p.presence != nullptr ? __ldg(p.presence + b) : 0.0f;
-      row.fr = p.frequency != nullptr ? __ldg(p.frequency + b) : 0.0f;
+      row.r = p.repetition != nullptr ? p.repetition[b] : 1.0f;
+      row.pr = p.presence != nullptr ? p.presence[b] : 0.0f;
+      row.fr = p.frequency != nullptr ? p.frequency[b] : 0.0f;
     } else {
       __syncthreads();  // the chunk before is done with the tables
     }
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(kLgThreads) logits_kernel(const LogitsParams p
         float f;
         if constexpr (sizeof(T) == 4) f = x[t];
         else f = ElemTraits<T>::widen1(reinterpret_cast<const uint16_t*>(x)[t]);
-        if (kBias) f = __fadd_rn(f, __ldg(bias + t));
+        if (kBias) f = __fadd_rn(f, bias[t]);
         ElemTraits<T>::store(out, t, row.take(f, allowed_at(t) & 1u, t));
       }
     }
@@ -528,7 +528,7 @@ int dcr_process_logits(const void* logits, int64_t l_stride_b, int dtype, int B,
   if (logits == nullptr || out == nullptr || next_token == nullptr) return DCR_ERR_NULL;
   if (dtype != DCR_DTYPE_BF16 && dtype != DCR_DTYPE_F16 && dtype != DCR_DTYPE_F32)
     return DCR_ERR_DTYPE;
-  if (B <= 0 || B > (1 << 27) || V <= 0 || V > 0x7fffff00 || L < 0) return DCR_ERR_SHAPE;
+  if (B <= 0 || B > (1 << 27) || V <= 0 || V > (1 << 30) || L < 0) return DCR_ERR_SHAPE;
   if (L > 0 && tokens == nullptr) return DCR_ERR_NULL;
   if (l_stride_b < 0 || t_stride_b < 0 || bias_stride_b < 0 || a_stride_b < 0) return DCR_ERR_SHAPE;
   if (B > 1 && o_stride_b < V) return DCR_ERR_SHAPE;

@@ -49,7 +49,7 @@ struct PagePool {
 // The page that holds `slot` of sequence b, or -1 (unmapped, or out of range: raises the
 // status). slot must be below max_pages * page_size.
 __device__ __forceinline__ int page_of(const PagePool& c, int b, uint32_t page_index) {
-  const int pg = __ldg(c.table + b * c.tstride + page_index);
+  const int pg = c.table[b * c.tstride + page_index];
   if (pg >= c.num_pages) {
     raise_status(DCR_ERR_DEVICE_INDEX);
     return -1;

@@ -66,7 +66,7 @@ __device__ __forceinline__ void ap_load(const void* base, int64_t i, float (&f)[
 #pragma unroll
   for (int c = 0; c < N / kPer; ++c) {
     float x[kPer];
-    ElemTraits<T>::widen(__ldg(src + c), x);
+    ElemTraits<T>::widen(src[c], x);
 #pragma unroll
     for (int e = 0; e < kPer; ++e) f[c * kPer + e] = x[e];
   }
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kApWarps * 32) paged_append_kernel(const Paged
     x[i][0] = h < heads ? __ldcs(row) : make_uint4(0u, 0u, 0u, 0u);
     x[i][1] = h < heads ? __ldcs(row + L) : make_uint4(0u, 0u, 0u, 0u);
   }
-  const int position = __ldg(p.positions + t);
+  const int position = p.positions[t];
   const bool fine = position >= 0 && position < p.n_pos;
   if (!fine) raise_status(DCR_ERR_DEVICE_INDEX);
 
@@ -135,9 +135,9 @@ __global__ void __launch_bounds__(kApWarps * 32) paged_append_kernel(const Paged
     dst = static_cast<char*>(p.q_out) + static_cast<int64_t>(t) * p.H * (D * static_cast<int>(sizeof(T)));
     dh = D * static_cast<int>(sizeof(T));
   } else {
-    const int slot = __ldg(p.slots + t);
+    const int slot = p.slots[t];
     if (slot < 0 || !fine) return;
-    const int b = p.seq != nullptr ? __ldg(p.seq + t) : t;
+    const int b = p.seq != nullptr ? p.seq[t] : t;
     int pg = -1;
     uint32_t pi = 0;
     if (b >= 0 && b < p.n_seq && slot < p.c.max_pages * static_cast<int>(p.c.page.d)) {

@@ -129,7 +129,7 @@ __device__ __forceinline__ void pa_store2(T* dst, float a, float b) {
 template <int R>
 __device__ __forceinline__ void pa_sequence(const PagedAttendParams& p, int b, int& len, int& lo,
                                             int& t_lo, int& t_hi) {
-  len = checked_length(p.c, __ldg(p.lengths + b));
+  len = checked_length(p.c, p.lengths[b]);
   lo = p.window > 0 && len > p.window ? len - p.window : 0;
   t_lo = lo / R;
   t_hi = (len + R - 1) / R;
@@ -956,7 +956,7 @@ __global__ void __launch_bounds__(kWeightThreads) paged_weights_kernel(const Pag
   const int i0 = (blockIdx.x * kWeightThreads + threadIdx.x) * kWeightSlots;
   bool waited = false;
   for (int b = blockIdx.z; b < p.B; b += gridDim.z) {
-    const int n = checked_length(p.c, __ldg(p.lengths + b));
+    const int n = checked_length(p.c, p.lengths[b]);
     const int lo = p.window > 0 && n > p.window ? n - p.window : 0;
     float* dst = weights + b * wsb + hk * wsh + i0;
     float w[kWeightSlots], add[kWeightSlots] = {};

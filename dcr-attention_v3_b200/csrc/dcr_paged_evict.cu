@@ -112,8 +112,8 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_select_kernel(const Pa
   asm volatile("griddepcontrol.launch_dependents;");
   const int64_t row = blockIdx.x / C;
   const int b = static_cast<int>(row / p.H_kv), h = static_cast<int>(row - static_cast<int64_t>(b) * p.H_kv);
-  const int n = checked_length(p.c, __ldg(p.lengths + b));
-  const int from = __ldg(p.seen + b) - p.recent;
+  const int n = checked_length(p.c, p.lengths[b]);
+  const int from = p.seen[b] - p.recent;
   const float* w = p.weights + b * p.wsb + h * p.wsh;
   const int32_t* ps = p.pos + b * p.psb + h * p.psh;
   int32_t* src = p.src + row * p.budget;
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_select_kernel(const Pa
   const int base = (rank * kEvWarps + warp) * 32 * used + lane;  // slot j of this lane: + 32 j
   auto load = [&](int j) {
     const int i = base + 32 * j;
-    return i < n ? ev_key(__ldg(w + i), __ldg(ps + i), p.sinks, from) : 0u;
+    return i < n ? ev_key(w[i], ps[i], p.sinks, from) : 0u;
   };
   // Every slot below the budget keeps its place at first; the second kernel fills the holes.
   // Batches of loads, so that no load waits for a store.
@@ -154,8 +154,8 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_select_kernel(const Pa
     for (int j = 0; j < kBatch; ++j) {
       const int i = base + 32 * (j0 + j);
       const bool in = j0 + j < used && i < n;
-      wj[j] = in ? __ldg(w + i) : 0.0f;
-      pj[j] = in ? __ldg(ps + i) : 0;
+      wj[j] = in ? w[i] : 0.0f;
+      pj[j] = in ? ps[i] : 0;
     }
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
@@ -333,8 +333,8 @@ __global__ void __launch_bounds__(256) paged_evict_move_kernel(const PagedEvictP
       const uint32_t fi = p.c.page.div(from[i]), ti = p.c.page.div(to[i]);
       const int fp = local ? pages[fi] : page_of(p.c, b, fi), tp = local ? pages[ti] : page_of(p.c, b, ti);
       if (ch == 0) {
-        wx[i] = __ldg(w + from[i]);
-        px[i] = __ldg(ps + from[i]);
+        wx[i] = w[from[i]];
+        px[i] = ps[from[i]];
       }
       if (fp < 0 || tp < 0) {  // a row without a mapped page on either side
         raise_status(DCR_ERR_DEVICE_INDEX);

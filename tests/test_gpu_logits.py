@@ -87,6 +87,12 @@ def test_large_vocabularies(V):
     _check(2, V, 2000, "bf16", bias="one", mask="some")
 
 
+def test_history_longer_than_the_tables():
+    """The vocabulary is taken in chunks where the counts of a whole slice would not fit."""
+    _check(2, 200001, 40000, "f32", bias="one", mask="some")
+    _check(1, 3000, 70000, "bf16", tok=torch.int64)
+
+
 def test_many_rows():
     _check(200, 3001, 64, "bf16", mask="some")
 

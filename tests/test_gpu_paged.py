@@ -371,6 +371,10 @@ def test_evict_sizes(n, budget):
     _check_evict([n, max(1, n // 2)], 2, budget, 64, torch.bfloat16, sinks=4, recent=budget // 4, seed=n)
 
 
+def test_evict_rows_that_registers_cannot_hold():
+    _check_evict([300001], 1, 1000, 64, torch.bfloat16, sinks=1, recent=100)
+
+
 def _ties(w, pos):
     w.mul_(4).floor_()
 
