@@ -366,13 +366,22 @@ def test_evict_types_and_layouts(dt, D, layout, page):
 
 
 @pytest.mark.parametrize("n,budget", [(2, 1), (1000, 1), (1000, 999), (1025, 1024), (5000, 2500),
-                                      (20000, 3000), (40000, 39999), (1000, 1000)])
+                                      (20000, 3000), (40000, 39999), (9000, 8997), (1004, 1000), (1005, 1000), (36000, 35998), (1000, 1000)])
 def test_evict_sizes(n, budget):
     _check_evict([n, max(1, n // 2)], 2, budget, 64, torch.bfloat16, sinks=4, recent=budget // 4, seed=n)
 
 
 def test_evict_rows_that_registers_cannot_hold():
     _check_evict([300001], 1, 1000, 64, torch.bfloat16, sinks=1, recent=100)
+
+
+@pytest.mark.parametrize("few", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("n", [40, 3000, 20000])
+def test_evict_few(few, n):
+    """The evicted ones at the front, at the end (no move at all) and among ties."""
+    for make in (None, _ties, _zeros, _wild, lambda w, pos: w[..., -n:].copy_(-torch.arange(n, device=DEV)),
+                 lambda w, pos: w.copy_(torch.arange(w.shape[-1], device=DEV))):
+        _check_evict([n, n - 1], 2, n - few, 16, torch.bfloat16, make=make, recent=3, sinks=1)
 
 
 def _ties(w, pos):
