@@ -228,6 +228,10 @@ __global__ void __launch_bounds__(kLgThreads) logits_kernel(const LogitsParams p
       for (int j = tid; j < count; j += kLgThreads) cp_async_4(mask + j, allowed + w0 + j);
     }
     cp_async_commit();
+    if (p.L > 0) {
+      for (int j = tid; j < words; j += kLgThreads) marks[j] = 0u;
+      for (int i = tid; i < min(p.L, span); i += kLgThreads) counts[i] = 0u;
+    }
     // With a bias on 16-bit logits, whose bytes are twice the logits', the stream begins at
     // another place in every row: rows that share a bias would all read the same part of it at
     // the same time (128 rows of 128256 with mask and history 40.9 instead of 48.9 us; without a
@@ -273,8 +277,6 @@ __global__ void __launch_bounds__(kLgThreads) logits_kernel(const LogitsParams p
         for (int i = tid + kLgHeld * kLgThreads; i < n; i += kLgThreads)
           f(i, lg_place(p, lg_token(p, b, i, n), t0, span));
       };
-      for (int j = tid; j < words; j += kLgThreads) marks[j] = 0u;
-      for (int i = tid; i < min(n, span); i += kLgThreads) counts[i] = 0u;
       __syncthreads();
       each_token([&](int, int at) {
         if (at >= 0) atomicOr(marks + (at >> 5), 1u << (at & 31));
