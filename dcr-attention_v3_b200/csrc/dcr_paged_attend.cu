@@ -111,10 +111,10 @@ __device__ __forceinline__ void cp_async_8(void* smem_dst, const void* gsrc) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(smem_dst)), "l"(gsrc) : "memory");
 }
 
-// Adds a state's sum x (with maximum m) to one with maximum M >= m. A state without any valid
-// slot (m = -inf) adds nothing; a NaN goes through.
-__device__ __forceinline__ void pa_fold_sum(float M, float m, float x, float& sum) {
-  sum = m == -INFINITY ? (x != x ? x : sum) : fmaf(pa_exp2(m - M), x, sum);
+// What a state with maximum m counts for in one with maximum M >= m; a state without any valid
+// slot (m = -inf, sums of 0) counts for nothing.
+__device__ __forceinline__ float pa_share(float M, float m) {
+  return m == -INFINITY ? 0.0f : pa_exp2(m - M);
 }
 
 template <typename T>
@@ -822,8 +822,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const Paged
 #pragma unroll
       for (int o = kPaWarps; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
       M = __shfl_sync(0xffffffffu, M, lead);  // pieces are in the first 2 * kPaWarps lanes
-      float L = 0.0f;
-      if (in) pa_fold_sum(M, m, own_piece[g * (D + 2) + D + 1], L);
+      const float a = pa_share(M, m);
+      float L = in ? a * own_piece[g * (D + 2) + D + 1] : 0.0f;
 #pragma unroll
       for (int o = kPaWarps; o >= 1; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
       L = __shfl_sync(0xffffffffu, L, lead);
@@ -831,10 +831,10 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const Paged
 #pragma unroll 1
       for (unsigned left = run; left != 0; left &= left - 1) {
         const int x = __ffs(left) - 1;
-        const float mx = __shfl_sync(0xffffffffu, m, x);
+        const float ax = __shfl_sync(0xffffffffu, a, x);
         const float* src = piece_at(x) + g * (D + 2);
 #pragma unroll
-        for (int e = 0; e < D / 32; ++e) pa_fold_sum(M, mx, src[lane + 32 * e], acc[e]);
+        for (int e = 0; e < D / 32; ++e) acc[e] = fmaf(ax, src[lane + 32 * e], acc[e]);
       }
       if (!before && !after) {
         const int64_t row = static_cast<int64_t>(b) * p.H + hk * p.G + h0 + g;
@@ -921,22 +921,18 @@ __global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const PagedAtt
     float top = fmaxf(M, m);
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (M != -INFINITY) {
-      const float a = pa_exp2(M - top);
-      L *= a;
-      acc *= a;
-    }
+    const float old = pa_share(top, M);
+    L *= old;
+    acc *= old;
     M = top;
-    float l = 0.0f;
-    if (lane < count) pa_fold_sum(M, m, part[lane * W + D + 1], l);
+    const float a = pa_share(M, m);
+    float l = lane < count ? a * part[lane * W + D + 1] : 0.0f;
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     L += l;
-#pragma unroll 4
-    for (int x = 0; x < count; ++x) {
-      const float mx = __shfl_sync(0xffffffffu, m, x);
-      pa_fold_sum(M, mx, part[x * W + (d < D ? d : 0)], acc);
-    }
+#pragma unroll 8
+    for (int x = 0; x < count; ++x)
+      acc = fmaf(__shfl_sync(0xffffffffu, a, x), part[x * W + (d < D ? d : 0)], acc);
   }
   if (d >= D) return;
   const int64_t row = static_cast<int64_t>(c.b) * p.H + hk * p.G + h;
