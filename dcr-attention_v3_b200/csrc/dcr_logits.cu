@@ -25,6 +25,13 @@
 // memory, some 16-byte vectors ahead, the first of them on their way while the history is marked.
 // A vector is looked at for the best token only if its maximum reaches the CTA's so far; the
 // CTAs' best tokens meet in CTA 0.
+//
+// Measured (calls back to back): 128 rows of 128256 fp32 logits, 131 MB: 24.7 us with 16 tokens of
+// history (5.3 TB/s), 31.4 us with 6144 on average, 39.3 us with a bias and a mask too (3.5 TB/s);
+// one bf16 row with 1000 tokens of history 9.3 us, of which 3 us are the history's phases and 3 us
+// the launch and the cluster's barriers. Counts of all tokens in shared memory (a slice of 16032
+// tokens a CTA) took 78 us for the first case with bias, mask and history; finishing the marked
+// tokens by all warps before the stream 50.9 us.
 #include <cooperative_groups.h>
 #include <math.h>
 

@@ -31,6 +31,15 @@
 // mostly padding and its round trip through TMEM longer than the work. P enters the second
 // product as two 16-bit parts (hi = rn(p), lo = rn(p - hi)), which keeps 16 bits of every
 // weight; with HB = 8 the parts are the two row halves of one MMA. fp32 rows use fp32 FMAs.
+//
+// Measured (whole calls back to back in a CUDA graph; the measured copy bandwidth is 6.54 TB/s):
+// 4 x 8 KV heads of 64 over 32769 slots, bf16 (268 MB): 47.5 us, 5.65 TB/s, of which some 38 us are
+// the stream at 7 TB/s, 4 us its beginning (lengths, page table, first rows) and 5 us the folds; 48
+// sequences of 0 to 16000 slots, f16 (747 MB): 120 us, 6.2 TB/s; 16 x 8 heads of 128 in a window of
+// 8191, bf16 (537 MB): 92 us, 5.8 TB/s; 3 x 16 heads over 8195 slots in fp32 (201 MB): 38 us, 5.3
+// TB/s; 8 x 8 heads over 16385 slots with weights (277 MB): 58.7 us; one sequence of 1000: 7.8 us.
+// Tiles of 2 KB instead of 4 needed 453 instead of 261 instructions per 16 slots (66.8 instead of
+// 51.7 us for the first case at that step).
 #include <math.h>
 
 #include <type_traits>
@@ -42,7 +51,9 @@ namespace dcr {
 
 constexpr int kPaWarps = 8;
 constexpr int kPaThreads = kPaWarps * 32;
-// Fewest tiles a CTA takes: below it, spreading further costs more in folding than it gains.
+// Fewest tiles a CTA takes: below it, spreading further costs more in folding than it gains. With
+// 4 / 8 / 16 of them, 8 KV heads of 64 over 100 slots take 5.5 / 6.2 / 8.2 us, over 1000 7.1 / 7.6 /
+// 8.6, over 4000 9.8 / 8.2 / 9.5, and one KV head of 128 over 8000 14.1 / 10.8 / 10.3.
 constexpr int kPaMinTiles = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
