@@ -429,10 +429,10 @@ int dcr_silu_mul_packed(const void* gate_up, int dtype, int rows, int inter, voi
  * multiples of 16 bytes, for K and V separately; rows contiguous). Sequence b's slot i is in
  * page page_table[b * table_stride + i / page_size] at i % page_size; a negative entry is a
  * page that is not mapped; max_pages * page_size is at most 2^29. D is 64 or 128 and H any
- * multiple of H_kv here. Nothing outside the
- * pool is read or written whatever lengths, tables, slots, positions and tokens hold on the
- * device: an entry out of range is skipped and sets DCR_ERR_DEVICE_INDEX in the device status
- * (a length beyond max_pages * page_size is taken as that, a negative one as 0).
+ * multiple of H_kv here. Nothing outside the pool is read or written whatever lengths, tables,
+ * slots, positions and tokens hold on the device: an entry out of range is skipped and sets
+ * DCR_ERR_DEVICE_INDEX in the device status (a length beyond max_pages * page_size is taken as
+ * that, a negative one as 0).
  * Attended slots must be finite for finite results: slots past the length, before the window
  * or in unmapped pages may hold anything. */
 
@@ -485,7 +485,8 @@ size_t dcr_paged_evict_workspace_bytes(int B, int H_kv, int budget);
  * [B, H_kv, budget] int32: the slot each one's row came from (its own for a row that stayed,
  * -1 past the new length). weights_out and pos_out (first `budget` slots; other tensors than
  * weights and pos) receive the kept slots' entries, 0 and -1 past the new length; lengths_out
- * [B] = min(lengths, budget) (another tensor than lengths). */
+ * [B] = min(lengths, budget) (another tensor than lengths). The sequences' pages must not be
+ * shared with one another: a shared row would be moved for each of them. */
 int dcr_paged_evict(void* k_pages, void* v_pages, int dtype, int64_t k_stride_p,
                     int64_t k_stride_h, int64_t k_stride_s, int64_t v_stride_p,
                     int64_t v_stride_h, int64_t v_stride_s, int num_pages, int page_size,
