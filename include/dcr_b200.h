@@ -476,6 +476,8 @@ int dcr_paged_append(const void* q, int64_t q_stride_t, int64_t q_stride_h, cons
                      int max_pages, float* weights, int64_t w_stride_b, int64_t w_stride_h,
                      int32_t* pos, int64_t p_stride_b, int64_t p_stride_h, void* stream);
 
+/* Bytes of workspace dcr_paged_evict needs (16-byte aligned, like dcr_paged_attend's); it need
+ * not be initialised. 0: invalid shape. */
 size_t dcr_paged_evict_workspace_bytes(int B, int H_kv, int budget);
 
 /* Per sequence and KV head, keeps `budget` of the lengths[b] slots: the protected ones first
