@@ -18,7 +18,7 @@
 // line that the CTAs share out evenly, and each CTA's share its warps: lengths on the device
 // may be as unequal as they like. A warp walks its share alone, without barriers: it loads
 // rows with 16-byte cp.async into a ring of its own (NH half tiles, K and V in turn; slots
-// that are not valid are zero-filled, never read), and keeps the running maximum, sum and
+// that are not valid are zero-filled, never read), and keeps the running base, sum and
 // output (m, l, o) of the unit it is in. Where a unit lies wholly inside a warp's share the
 // warp writes O itself. Otherwise it leaves a piece (m, l, o); the CTA folds its pieces, and
 // units that span CTAs are folded from the CTAs' partials in the workspace by a second kernel
@@ -29,8 +29,11 @@
 // 16-bit rows go through the tensor cores (mma.sync m16n8k16, A = the query heads as rows): one
 // token has at most 16 rows a KV head, so the tile of a tcgen05.mma (64 or 128 rows) would be
 // mostly padding and its round trip through TMEM longer than the work. P enters the second
-// product as two 16-bit parts (hi = rn(p), lo = rn(p - hi)), which keeps 16 bits of every
-// weight; with HB = 8 the parts are the two row halves of one MMA. fp32 rows use fp32 FMAs.
+// product as two 16-bit parts (hi = rn(p), lo = rn(p - hi)); with HB = 8 the parts are the two
+// row halves of one MMA. In bf16 the parts keep 16 bits of every weight. In f16 they keep 21,
+// but end at 2^-24, so f16 weights are taken 2^7 larger (against a base 7 below the maximum):
+// they stay below 2^15, and what is lost of a weight is 2^-32 of the row's largest at most. fp32
+// rows use fp32 FMAs.
 //
 // Measured (whole calls back to back in a CUDA graph; the measured copy bandwidth is 6.54 TB/s):
 // 4 x 8 KV heads of 64 over 32769 slots, bf16 (268 MB): 47.5 us, 5.65 TB/s, of which some 38 us are
@@ -71,7 +74,7 @@ struct PagedAttendParams {
   int page16;     // page_size is a multiple of a group: a group lies in one page
   void* o;        // [B][H][D]
   float* lse;     // [B][H] natural log, or null
-  float2* stats;  // [B][H] (maximum in base 2, 1 / sum), with scores
+  float2* stats;  // [B][H] (base of the exponents, 1 / sum), with scores
   float* part;    // [CTAs][2][HB][D + 2]: o, m, l of the open units
   float* scores;  // [B][H][s_stride] base-2 scores, or null
   int64_t s_stride;
@@ -109,8 +112,9 @@ __device__ __forceinline__ float pa_exp2(float x) {
   return y;
 }
 
-// A row's statistics: lse = (m + log2 l) ln 2, and what the weights need. Weights are
-// exp2(z - m) / l: the difference of two near scores is exact, where lse would be rounded once.
+// A row's statistics, with l the sum of exp2(z - m): lse = (m + log2 l) ln 2, and what the
+// weights need. Weights are exp2(z - m) / l: a difference of near scores, where lse would be
+// rounded once.
 __device__ __forceinline__ void pa_store_stats(const PagedAttendParams& p, int64_t row, float m,
                                                float l) {
   if (p.lse != nullptr) p.lse[row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
@@ -122,7 +126,7 @@ __device__ __forceinline__ void cp_async_8(void* smem_dst, const void* gsrc) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(smem_dst)), "l"(gsrc) : "memory");
 }
 
-// What a state with maximum m counts for in one with maximum M >= m; a state without any valid
+// What a state with base m counts for in one with base M >= m; a state without any valid
 // slot (m = -inf, sums of 0) counts for nothing.
 __device__ __forceinline__ float pa_share(float M, float m) {
   return m == -INFINITY ? 0.0f : pa_exp2(m - M);
@@ -354,6 +358,8 @@ struct PaState16 {
   float o[D / 8][4];
   float m[M], l[M];
   static constexpr int NT = S::R / 8;
+  // m is a base: this much below the largest score so far when it was set
+  static constexpr float kBelow = std::is_same<T, __half>::value ? 7.0f : 0.0f;
   uint32_t ph[NT][M], pl[NT][M];  // the tile's weights, hi and lo parts, per 8 slots
 
   __device__ __forceinline__ void begin(const PagedAttendParams& p, const PaCursor& c, uint8_t*) {
@@ -424,15 +430,16 @@ struct PaState16 {
             *reinterpret_cast<float2*>(dst + 8 * j) = make_float2(s[j][0], s[j][1]);
         }
       }
-      // The maximum is raised only when some score is 2^8 above it: weights stay below 2^8,
-      // and most tiles need no rescaling. A NaN score raises nothing and spreads by itself.
+      // The base is raised only when some score is 8 above the largest it was set by: weights
+      // stay below 2^(8 + kBelow), and most tiles need no rescaling. A NaN score raises nothing
+      // and spreads by itself.
       float top = fmaxf(s[0][0], s[0][1]);
 #pragma unroll
       for (int j = 1; j < NT; ++j) top = fmaxf(top, fmaxf(s[j][0], s[j][1]));
-      if (__any_sync(0xffffffffu, top > m[i] + 8.0f)) {
+      if (__any_sync(0xffffffffu, top > m[i] + (8.0f + kBelow))) {
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float mn = fmaxf(m[i], top);
+        const float mn = fmaxf(m[i], top - kBelow);
         const float a = m[i] == -INFINITY ? 0.0f : pa_exp2(m[i] - mn);
         m[i] = mn;
         l[i] *= a;

@@ -1,0 +1,65 @@
+"""The paged serving operators on the GPU where they can go wrong by their surroundings: weights far
+below a row's largest, flags, table entries that no slot uses, pages that are not mapped."""
+from __future__ import annotations
+
+import math
+import os
+import sys
+
+import pytest
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+import paged_ref as ref  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+DEV = torch.device("cuda:0")
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def _status():
+    from dcr_b200 import _lib
+    return _lib.read_device_status(clear=True)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("G", [4, 16])
+@pytest.mark.parametrize("nats", [14.5, 16.0, 18.0, 20.0])
+def test_f16_weights_far_below_the_largest(D, G, nats):
+    """One slot far ahead of all others with a value row of zeros: O is the others' alone. The
+    sequences share their pages, and are so many that a warp walks whole rows."""
+    from dcr_b200.kernel.cuda.paged import paged_attention
+    n, page, B, H_kv = 8192, 64, 320, 8
+    pages = n // page
+    k = torch.zeros(pages, H_kv, page, D, dtype=torch.float16, device=DEV)
+    k[0, :, 3, 0] = nats
+    v = (0.5 + torch.rand(pages, H_kv, page, D, generator=_gen(1), device=DEV)).half()
+    v[0, :, 3] = 0
+    q = torch.zeros(B, G * H_kv, D, dtype=torch.float16, device=DEV)
+    q[:, :, 0] = 1
+    table = torch.arange(pages, dtype=torch.int32, device=DEV).expand(B, pages).contiguous()
+    o, lse = paged_attention(q, k, v, table, _i32([n] * B), scale=1.0, return_lse=True)
+    assert _status() == 0
+    # every row's maximum is nats, so all its weights are against e^nats
+    rest = v.double().sum((0, 2)) * math.exp(-nats)                  # [H_kv, D]
+    total = 1 + (n - 1) * math.exp(-nats)
+    want = (rest / total).repeat_interleave(G, 0)
+    # A weight enters in two fp16 parts on a scale where the row's largest is 2^7 at least: off by
+    # 2^-22 of itself or, among the subnormals, by 2^-25 of that scale, so 2^-32 of the largest. fp32
+    # sums of n terms; one rounding to fp16 (subnormal steps of 2^-24).
+    part = want.abs()
+    tol = n * 2.0 ** -32 * v.double().max() / total + part * (2.0 ** -21 + (n + 64) * 2 * ref.EPS)
+    tol = tol + 2.0 ** -11 * (want.abs() + tol) + 2.0 ** -25
+    off = ((o.double() - want).abs() / tol).max()
+    assert off <= 1, (float(off), float(((o.double() - want).abs() / want).max()))
+    # the denominators: fp32 sums of n terms, whatever their order
+    lse_tol = (n + 64) * 2 * ref.EPS + 64 * ref.EPS * nats
+    assert (lse.double() - (nats + math.log(total))).abs().max() <= lse_tol
