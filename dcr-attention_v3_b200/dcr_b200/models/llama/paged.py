@@ -72,8 +72,9 @@ class PagedLlamaDecoder(torch.nn.Module):
     def prefill(self, prompts: Sequence[Sequence[int]], cache: PagedKVCache) -> torch.Tensor:
         """Feeds one prompt per sequence into an empty cache (an empty prompt leaves its sequence
         idle); returns the logits [batch, vocab] after each prompt's last token (zeros for idle
-        sequences). Attention within a prompt is causal SDPA over its rows; attention weights of a
-        cache with a budget begin to accumulate with the decode steps."""
+        sequences). Attention within a prompt is causal SDPA over its rows. In a cache with a budget,
+        attention weights begin to accumulate with the decode steps; a prompt over the budget, which
+        is evicted before its first step attends, begins with those of its last token."""
         require(len(prompts) == cache.batch, f"{cache.batch} prompts expected")
         require(not any(cache.host_lengths), "prefill expects an empty cache")
         lengths = [len(p) for p in prompts]
@@ -81,8 +82,16 @@ class PagedLlamaDecoder(torch.nn.Module):
         cache.reserve(lengths)
         flat = torch.tensor([t for p in prompts for t in p], dtype=torch.int64).to(self.model.device)
         begins = [sum(lengths[:b]) for b in range(len(lengths))]
+        over = last_rows = None
+        if cache.budget is not None and max(lengths) > cache.budget:
+            over = torch.tensor([n if n > cache.budget else 0 for n in lengths],
+                                dtype=torch.int32).to(self.model.device)
+            last_rows = torch.tensor([begins[b] + n - 1 if n else 0
+                                      for b, n in enumerate(lengths)]).to(self.model.device)
 
         def attend(i, q):
+            if over is not None:
+                cache.weigh(i, q[last_rows], over)
             o = torch.empty_like(q)
             for b, n in enumerate(lengths):
                 if n:

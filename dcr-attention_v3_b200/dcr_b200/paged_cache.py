@@ -150,6 +150,13 @@ class PagedKVCache:
                                window=window,
                                weights=None if self.weights is None else self.weights[layer])
 
+    def weigh(self, layer: int, q: torch.Tensor, lengths: torch.Tensor) -> None:
+        """Accumulates the attention weights of one query row per sequence over its first
+        ``lengths[b]`` slots (int32 on the device; 0: none) in the layer's table, and nothing else."""
+        require(self.budget is not None, "this cache has no budget")
+        paged_attention(q, self.k[layer], self.v[layer], self.page_table, lengths,
+                        weights=self.weights[layer])
+
     def gather(self, layer: int, b: int):
         """(K, V) ``[H_kv, length, D]`` of sequence b, copied out of its pages."""
         n = self.host_lengths[b]

@@ -63,3 +63,44 @@ def test_f16_weights_far_below_the_largest(D, G, nats):
     # the denominators: fp32 sums of n terms, whatever their order
     lse_tol = (n + 64) * 2 * ref.EPS + 64 * ref.EPS * nats
     assert (lse.double() - (nats + math.log(total))).abs().max() <= lse_tol
+
+
+def _model(layers=2):
+    from dcr_b200.models.llama.model import DCRLlamaDecoder, LlamaDecodeConfig
+    cfg = LlamaDecodeConfig(vocab=512, hidden=256, intermediate=512, layers=layers, heads=4, kv_heads=2)
+    return DCRLlamaDecoder(cfg, attention="dense", dtype=torch.float32, device=DEV, seed=0)
+
+
+@pytest.mark.parametrize("slack", [1, 5])
+def test_a_prompt_over_the_budget_keeps_what_its_last_token_attended_to(slack):
+    from dcr_b200.models.llama.paged import PagedLlamaDecoder
+    paged = PagedLlamaDecoder(_model(), max_positions=128)
+    cache = paged.new_cache(3, 40, 128, page_size=8, budget=24, sinks=2, recent=4, slack=slack)
+    g = torch.Generator().manual_seed(7)
+    lengths = [60, 27, 10]
+    plain, turned = cache.append, []
+    cache.append = lambda *a, **kw: turned.append(plain(*a, **kw)) or turned[-1]
+    paged.prefill([torch.randint(0, 512, (n,), generator=g).tolist() for n in lengths], cache)
+    last = torch.tensor([59, 86, 96], device=DEV)
+    W, tol = [], []
+    for i in range(2):  # the definition, over what the pages hold; the third is not over the budget
+        r = ref.attend(turned[i][last], cache.k[i], cache.v[i], cache.page_table, [60, 27, 0])
+        W.append(r[2]), tol.append(r[5])
+        assert ((cache.weights[i].double() - r[2]).abs() <= r[5]).all()
+    paged.step(torch.tensor([1, 2, 3], device=DEV), cache)
+    assert cache.host_lengths == [25, 25, 11]
+    by_index = True
+    for i in range(2):
+        for b in range(2):
+            n = lengths[b]
+            for h in range(2):
+                kept = set(cache.pos[i][b, h, :24].tolist())
+                sure = set(range(2)) | set(range(n - 4, n))
+                assert len(kept) == 24 and sure <= kept
+                dropped = sorted(set(range(n)) - kept)
+                least = min(float(W[i][b, h, p]) for p in kept - sure)
+                most = max(float(W[i][b, h, p]) for p in dropped)
+                assert least >= most - 2 * float(tol[i][b, h, :n].max())
+                by_index &= kept == set(range(20)) | sure
+    assert not by_index
+    assert _status() == 0
