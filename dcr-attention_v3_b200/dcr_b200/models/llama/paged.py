@@ -44,14 +44,20 @@ class PagedLlamaDecoder(torch.nn.Module):
         return PagedKVCache(len(self.model.layers), batch, self.model.cfg.kv_heads, pages, max_slots,
                             dtype=self.model.dtype, device=self.model.device, **kw)
 
+    def _check_positions(self, cache: PagedKVCache, new_tokens: Sequence[int]) -> None:
+        """Refuses, before the cache changes, tokens past the position table."""
+        require(len(new_tokens) == cache.batch, f"{cache.batch} sequences expected")
+        for b, n in enumerate(new_tokens):
+            require(n == 0 or cache.host_seen[b] + n <= self.cos.shape[0],
+                    f"sequence {b} would reach position {cache.host_seen[b] + n} of a table of "
+                    f"{self.cos.shape[0]}")
+
     def _layers(self, tokens: torch.Tensor, cache: PagedKVCache,
                 attend: Callable[[int, torch.Tensor], torch.Tensor]) -> torch.Tensor:
         """The normed hidden states [T, hidden] of T reserved tokens."""
         cfg = self.model.cfg
         nq, nk = cfg.heads * HEAD_DIM, cfg.kv_heads * HEAD_DIM
         T = tokens.shape[0]
-        require(max(cache.host_seen) <= self.cos.shape[0],
-                f"positions past the table of {self.cos.shape[0]}")
         h, delta = self.model.embed_tokens(tokens), None
         for i, layer in enumerate(self.model.layers):
             eps = layer.input_layernorm.eps
@@ -79,6 +85,7 @@ class PagedLlamaDecoder(torch.nn.Module):
         require(not any(cache.host_lengths), "prefill expects an empty cache")
         lengths = [len(p) for p in prompts]
         require(sum(lengths) > 0, "at least one prompt must hold a token")
+        self._check_positions(cache, lengths)
         cache.reserve(lengths)
         flat = torch.tensor([t for p in prompts for t in p], dtype=torch.int64).to(self.model.device)
         begins = [sum(lengths[:b]) for b in range(len(lengths))]
@@ -115,9 +122,10 @@ class PagedLlamaDecoder(torch.nn.Module):
         """One decode step: appends ``tokens`` [batch] (int64, on the device) and returns the logits
         [batch, vocab]. Sequences that are not ``active`` neither grow nor attend (their rows mean
         nothing). Evicts first where the cache is over its budget."""
+        live = [True] * cache.batch if active is None else [bool(a) for a in active]
+        self._check_positions(cache, [int(a) for a in live])
         if cache.over_budget():
             cache.evict()
-        live = [True] * cache.batch if active is None else list(active)
         T = cache.reserve([int(a) for a in live])
         if T == cache.batch:
             x = self._layers(tokens, cache, lambda i, q: cache.attend(i, q))

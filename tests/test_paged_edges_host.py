@@ -1,0 +1,45 @@
+"""Refusals and page handling of the paged cache and decoder that need no GPU: what is refused
+changes nothing, and what a sequence holds is followed everywhere."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+
+def _decoder(rows):
+    from dcr_b200.models.llama.model import DCRLlamaDecoder, LlamaDecodeConfig
+    from dcr_b200.models.llama.paged import PagedLlamaDecoder
+    cfg = LlamaDecodeConfig(vocab=50, hidden=128, intermediate=128, layers=1, heads=2, kv_heads=1)
+    model = DCRLlamaDecoder(cfg, attention="dense", dtype=torch.float32, device="cpu", seed=0)
+    return PagedLlamaDecoder(model, max_positions=rows)
+
+
+def _state(c):
+    return (list(c.host_lengths), list(c.host_seen), [list(p) for p in c.host_pages],
+            list(c.free_pages), c.lengths.tolist(), c.seen.tolist(), c.queried.tolist(),
+            c.page_table.tolist(), c._tokens)
+
+
+def _refused(c, call, *args):
+    before = _state(c)
+    with pytest.raises(AssertionError):
+        call(*args)
+    assert _state(c) == before
+
+
+def test_positions_past_the_table_are_refused_before_anything_changes():
+    paged = _decoder(4)
+    cache = paged.new_cache(3, 10, 40, page_size=8)
+    _refused(cache, paged.prefill, [[1, 2, 3, 4, 5], [1], []], cache)
+    cache.reserve([4, 2, 0])
+    _refused(cache, paged.step, torch.tensor([1, 2, 3]), cache)
+    _refused(cache, paged.step, torch.tensor([1, 2, 3]), cache, [True, False, False])
+
+
+def test_a_refused_step_does_not_evict():
+    paged = _decoder(4)
+    cache = paged.new_cache(2, 10, 40, page_size=8, budget=3, sinks=0, recent=1)
+    cache.reserve([4, 1])
+    cache.evict = lambda: pytest.fail("evicted")
+    _refused(cache, paged.step, torch.tensor([1, 2]), cache)
+    _refused(cache, paged.step, torch.tensor([1, 2]), cache, [True])
