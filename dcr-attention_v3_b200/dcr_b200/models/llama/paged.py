@@ -119,9 +119,12 @@ class PagedLlamaDecoder(torch.nn.Module):
     @torch.no_grad()
     def step(self, tokens: torch.Tensor, cache: PagedKVCache,
              active: Optional[Sequence[bool]] = None) -> torch.Tensor:
-        """One decode step: appends ``tokens`` [batch] (int64, on the device) and returns the logits
+        """One decode step: appends ``tokens`` [batch] (ids on the device) and returns the logits
         [batch, vocab]. Sequences that are not ``active`` neither grow nor attend (their rows mean
         nothing). Evicts first where the cache is over its budget."""
+        require(tokens.shape == (cache.batch,) and tokens.dtype in (torch.int64, torch.int32) and
+                tokens.device == self.cos.device,
+                f"tokens must be {cache.batch} ids on {self.cos.device}")
         live = [True] * cache.batch if active is None else [bool(a) for a in active]
         self._check_positions(cache, [int(a) for a in live])
         if cache.over_budget():
@@ -155,6 +158,7 @@ class PagedLlamaDecoder(torch.nn.Module):
         :func:`~dcr_b200.kernel.cuda.logits.process_logits`; ``allowed(generated)`` returns a step's
         mask (or None). A sequence ends at the token ``stop`` (kept), or where its mask allows
         none; its pages are freed then."""
+        require(len(prompts) == cache.batch, f"{cache.batch} prompts expected")
         require(max_new > 0 and all(len(p) > 0 for p in prompts), "prompts must hold a token each")
         B, dev = cache.batch, self.model.device
         width = max(len(p) for p in prompts) + max_new

@@ -43,3 +43,20 @@ def test_a_refused_step_does_not_evict():
     cache.evict = lambda: pytest.fail("evicted")
     _refused(cache, paged.step, torch.tensor([1, 2]), cache)
     _refused(cache, paged.step, torch.tensor([1, 2]), cache, [True])
+
+
+@pytest.mark.parametrize("tokens", [torch.tensor([1, 2]), torch.tensor([[1], [2], [3]]),
+                                    torch.tensor([1.0, 2.0, 3.0])])
+def test_tokens_that_are_not_one_id_a_sequence_are_refused(tokens):
+    paged = _decoder(64)
+    cache = paged.new_cache(3, 10, 40, page_size=8)
+    cache.reserve([4, 2, 1])
+    _refused(cache, paged.step, tokens, cache)
+    _refused(cache, paged.step, tokens, cache, [True, False, True])
+
+
+def test_generate_wants_a_prompt_for_every_sequence():
+    paged = _decoder(64)
+    cache = paged.new_cache(2, 10, 40, page_size=8)
+    for prompts in ([[1]], [[1], [2], [3]]):
+        _refused(cache, paged.generate, prompts, cache, 3)
