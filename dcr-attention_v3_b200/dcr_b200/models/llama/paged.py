@@ -85,6 +85,8 @@ class PagedLlamaDecoder(torch.nn.Module):
         require(not any(cache.host_lengths), "prefill expects an empty cache")
         lengths = [len(p) for p in prompts]
         require(sum(lengths) > 0, "at least one prompt must hold a token")
+        vocab = self.model.cfg.vocab
+        require(all(0 <= t < vocab for p in prompts for t in p), f"prompt ids must be in [0, {vocab})")
         self._check_positions(cache, lengths)
         cache.reserve(lengths)
         flat = torch.tensor([t for p in prompts for t in p], dtype=torch.int64).to(self.model.device)

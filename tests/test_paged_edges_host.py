@@ -60,3 +60,11 @@ def test_generate_wants_a_prompt_for_every_sequence():
     cache = paged.new_cache(2, 10, 40, page_size=8)
     for prompts in ([[1]], [[1], [2], [3]]):
         _refused(cache, paged.generate, prompts, cache, 3)
+
+
+@pytest.mark.parametrize("prompt", [[50], [3, -1], [1, 2, 1 << 40]])
+def test_prompt_ids_outside_the_vocabulary_are_refused(prompt):
+    paged = _decoder(64)
+    cache = paged.new_cache(2, 10, 40, page_size=8)
+    _refused(cache, paged.prefill, [[1], prompt], cache)
+    _refused(cache, paged.generate, [[1], prompt], cache, 3)
