@@ -65,13 +65,13 @@ class PagedKVCache:
         self.free_pages = list(range(pages - 1, -1, -1))
         self.host_lengths = [0] * batch
         self.host_seen = [0] * batch
+        self._grew = [False] * batch                 # the sequences that reserved a token last
         self.host_pages: List[List[int]] = [[] for _ in range(batch)]
         self._tokens = None  # (seq, slots, positions) of the tokens reserved last
 
     # ------------------------------------------------------------------------------- host side
-    def _publish(self, rows: Sequence[int], grew: Optional[Sequence[int]] = None) -> None:
-        """Copies the host's lengths and the page table's given rows to the device; ``grew``: the
-        tokens that each sequence got just now."""
+    def _publish(self, rows: Sequence[int]) -> None:
+        """Copies the host's lengths and the page table's given rows to the device."""
         pinned = self.device.type == "cuda"
 
         def to_device(dst, values):
@@ -79,8 +79,7 @@ class PagedKVCache:
             dst.copy_(src.pin_memory() if pinned else src, non_blocking=pinned)
         to_device(self.lengths, self.host_lengths)
         to_device(self.seen, self.host_seen)
-        if grew is not None:
-            to_device(self.queried, [n if g else 0 for n, g in zip(self.host_lengths, grew)])
+        to_device(self.queried, [n if g else 0 for n, g in zip(self.host_lengths, self._grew)])
         for b in rows:
             held = self.host_pages[b]
             to_device(self.page_table[b], held + [-1] * (self.max_pages - len(held)))
@@ -114,7 +113,8 @@ class PagedKVCache:
         positions = [self.host_seen[b] + i for b, n in enumerate(new_tokens) for i in range(n)]
         changed = [b for b, n in enumerate(want) if self._resize(b, n)]
         self.host_seen = [s + n for s, n in zip(self.host_seen, new_tokens)]
-        self._publish(changed, new_tokens)
+        self._grew = [n > 0 for n in new_tokens]
+        self._publish(changed)
         i32 = dict(dtype=torch.int32)
         self._tokens = tuple(torch.tensor(x, **i32).to(self.device) for x in (seq, slots, positions))
         return len(seq)
@@ -122,7 +122,7 @@ class PagedKVCache:
     def release(self, b: int) -> None:
         """Ends sequence b: its pages go back to the pool."""
         self._resize(b, 0)
-        self.host_seen[b] = 0
+        self.host_seen[b], self._grew[b] = 0, False
         self._publish([b])
 
     def over_budget(self) -> bool:

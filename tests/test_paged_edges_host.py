@@ -68,3 +68,21 @@ def test_prompt_ids_outside_the_vocabulary_are_refused(prompt):
     cache = paged.new_cache(2, 10, 40, page_size=8)
     _refused(cache, paged.prefill, [[1], prompt], cache)
     _refused(cache, paged.generate, [[1], prompt], cache, 3)
+
+
+def test_eviction_and_release_reach_what_is_attended_to(monkeypatch):
+    from dcr_b200 import paged_cache
+    monkeypatch.setattr(paged_cache, "paged_evict", lambda *a, **kw: None)
+    cache = paged_cache.PagedKVCache(2, 3, 2, 20, 40, page_size=8, dtype=torch.bfloat16, device="cpu",
+                                     budget=10, sinks=1, recent=2)
+    cache.reserve([30, 9, 12])
+    assert cache.queried.tolist() == [30, 9, 12]
+    cache.evict()
+    assert cache.queried.tolist() == cache.lengths.tolist() == [10, 9, 10]
+    cache.reserve([1, 0, 1])
+    assert cache.queried.tolist() == [11, 0, 11]
+    cache.evict()
+    assert cache.queried.tolist() == [10, 0, 10]  # the second has asked for nothing since
+    cache.reserve([1, 1, 1])
+    cache.release(0)
+    assert cache.queried.tolist() == [0, 10, 11] and cache.lengths.tolist() == [0, 10, 11]
