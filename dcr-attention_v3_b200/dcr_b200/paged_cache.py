@@ -164,7 +164,8 @@ class PagedKVCache:
         return tuple(x[pages].transpose(0, 1).flatten(1, 2)[:, :n] for x in (self.k[layer], self.v[layer]))
 
     def evict(self) -> None:
-        """Brings every sequence down to the budget, in all layers, and frees the pages past it."""
+        """Brings every sequence down to the budget, in all layers, and frees the pages past it.
+        Tokens reserved before it that are not appended yet have no slots any more."""
         require(self.budget is not None, "this cache has no budget")
         for i in range(len(self.k)):
             paged_evict(self.k[i], self.v[i], self.page_table, self.lengths, self.weights[i],
@@ -172,6 +173,8 @@ class PagedKVCache:
                         weights_out=self._spare_weights, pos_out=self._spare_pos)
             self.weights[i], self._spare_weights = self._spare_weights, self.weights[i]
             self.pos[i], self._spare_pos = self._spare_pos, self.pos[i]
+        if max(self.host_lengths) > self.budget:
+            self._tokens = None
         changed = [b for b, n in enumerate(self.host_lengths)
                    if n > self.budget and self._resize(b, self.budget)]
         self._publish(changed)

@@ -86,3 +86,20 @@ def test_eviction_and_release_reach_what_is_attended_to(monkeypatch):
     cache.reserve([1, 1, 1])
     cache.release(0)
     assert cache.queried.tolist() == [0, 10, 11] and cache.lengths.tolist() == [0, 10, 11]
+
+
+def test_tokens_reserved_before_an_eviction_are_not_appended_after_it(monkeypatch):
+    from dcr_b200 import paged_cache
+    monkeypatch.setattr(paged_cache, "paged_evict", lambda *a, **kw: None)
+    monkeypatch.setattr(paged_cache, "paged_append", lambda *a, **kw: a[0])
+    cache = paged_cache.PagedKVCache(1, 2, 2, 20, 40, page_size=8, dtype=torch.bfloat16, device="cpu",
+                                     budget=10, sinks=1, recent=2)
+    cache.reserve([9, 3])
+    cache.evict()                      # nothing is over the budget
+    cache.append(0, 1, 2, 3, 4, 5)
+    cache.reserve([4, 1])
+    cache.evict()                      # slots 9 to 12 are gone
+    with pytest.raises(AssertionError):
+        cache.append(0, 1, 2, 3, 4, 5)
+    cache.reserve([1, 1])
+    cache.append(0, 1, 2, 3, 4, 5)
