@@ -46,15 +46,18 @@ struct PagePool {
   FastDiv page;           // page.d slots a page
 };
 
-// The page that holds `slot` of sequence b, or -1 (unmapped, or out of range: raises the
-// status). slot must be below max_pages * page_size.
-__device__ __forceinline__ int page_of(const PagePool& c, int b, uint32_t page_index) {
-  const int pg = c.table[b * c.tstride + page_index];
+// A table's entry as a page, or -1 (unmapped, or out of range: raises the status).
+__device__ __forceinline__ int checked_page(const PagePool& c, int pg) {
   if (pg >= c.num_pages) {
     raise_status(DCR_ERR_DEVICE_INDEX);
     return -1;
   }
   return pg < 0 ? -1 : pg;
+}
+
+// Page page_index (below max_pages) of sequence b, or -1 as above.
+__device__ __forceinline__ int page_of(const PagePool& c, int b, uint32_t page_index) {
+  return checked_page(c, c.table[b * c.tstride + page_index]);
 }
 
 // A sequence's length, held to [0, max_pages * page_size] (beyond it: raises the status).

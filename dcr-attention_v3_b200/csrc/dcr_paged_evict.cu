@@ -366,9 +366,10 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_select_kernel(const Pa
 
 // The i-th mover of a row goes to its i-th hole, kUnroll pairs per lane group at a time. The
 // sequence's page table is read into shared memory before the first kernel is done (where it
-// fits), and a round's pairs while the round before is on its way, so that a round waits for one
-// read of the rows (with three dependent reads a round and three waves of CTAs, the call for
-// 134,000 pairs of 128-byte rows took 34.0 us instead of 31.9).
+// fits; an entry is checked where a move uses it, the others may hold anything), and a round's
+// pairs while the round before is on its way, so that a round waits for one read of the rows (with
+// three dependent reads a round and three waves of CTAs, the call for 134,000 pairs of 128-byte
+// rows took 34.0 us instead of 31.9).
 constexpr int kEvPages = 4096;
 
 template <int RowBytes>
@@ -381,7 +382,7 @@ __global__ void __launch_bounds__(256) paged_evict_move_kernel(const PagedEvictP
   const int b = static_cast<int>(row / p.H_kv), h = static_cast<int>(row - static_cast<int64_t>(b) * p.H_kv);
   const bool local = p.c.max_pages <= kEvPages;
   if (local)
-    for (int i = threadIdx.x; i < p.c.max_pages; i += 256) pages[i] = page_of(p.c, b, i);
+    for (int i = threadIdx.x; i < p.c.max_pages; i += 256) pages[i] = p.c.table[b * p.c.tstride + i];
   __syncthreads();
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int n = p.n_moves[row];
@@ -417,7 +418,8 @@ __global__ void __launch_bounds__(256) paged_evict_move_kernel(const PagedEvictP
       moves[i] = false;
       if (to[i] < 0) continue;
       const uint32_t fi = p.c.page.div(from[i]), ti = p.c.page.div(to[i]);
-      const int fp = local ? pages[fi] : page_of(p.c, b, fi), tp = local ? pages[ti] : page_of(p.c, b, ti);
+      const int fp = local ? checked_page(p.c, pages[fi]) : page_of(p.c, b, fi);
+      const int tp = local ? checked_page(p.c, pages[ti]) : page_of(p.c, b, ti);
       if (ch == 0) {
         wx[i] = w[from[i]];
         px[i] = ps[from[i]];

@@ -65,6 +65,39 @@ def test_f16_weights_far_below_the_largest(D, G, nats):
     assert (lse.double() - (nats + math.log(total))).abs().max() <= lse_tol
 
 
+def _evicted(lengths, budget, spoil, width=None, page=16):
+    """(k, v before; k, v after; table, weights, pos, results) of one eviction; `spoil` changes the
+    page table after the pool is filled."""
+    from dcr_b200.kernel.cuda.paged import paged_evict
+    g = _gen(budget)
+    k, v, table = ref.make_pool(lengths, 2, page, 64, torch.bfloat16, DEV, g, width=width, garbage=0.0)
+    cap = table.shape[1] * page
+    w = torch.rand(len(lengths), 2, cap, generator=g, device=DEV)
+    pos = torch.arange(cap, dtype=torch.int32, device=DEV).expand(len(lengths), 2, cap).contiguous()
+    spoil(table, k.shape[0])
+    k0, v0 = k.clone(), v.clone()
+    assert _status() == 0
+    out = paged_evict(k, v, table, _i32(lengths), w, pos, _i32([cap] * len(lengths)), budget)
+    return k0, v0, k, v, table, w, pos, out
+
+
+def _plan(w, lengths, budget, b, h):
+    n = lengths[b]
+    return ref.evict(w[b, h, :n].tolist(), list(range(n)), n, 1 << 20, budget, 0, 0)
+
+
+@pytest.mark.parametrize("lengths", [[100, 20, 0], [42, 41, 40], [40, 3, 0]])
+def test_evict_does_not_look_at_entries_past_the_length(lengths):
+    def spoil(table, pages):
+        for b, n in enumerate(lengths):
+            table[b, -(-n // 16):] = pages + 5 + b
+    k0, v0, k, v, table, w, pos, (src, wo, po, no) = _evicted(lengths, 40, spoil, width=9)
+    assert _status() == 0
+    for b in range(3):
+        for h in range(2):
+            assert src[b, h].tolist() == _plan(w, lengths, 40, b, h)
+
+
 def _model(layers=2):
     from dcr_b200.models.llama.model import DCRLlamaDecoder, LlamaDecodeConfig
     cfg = LlamaDecodeConfig(vocab=512, hidden=256, intermediate=512, layers=layers, heads=4, kv_heads=2)
