@@ -243,14 +243,15 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_select_kernel(const Pa
       if (stays && movers++ == warp) mover = slot;
     }
     if (hole < 0 || mover < 0) return;  // holes and movers are as many
-    if (lane == 0) {
-      src[hole] = mover;
-      wo[hole] = w[mover];
-      po[hole] = ps[mover];
-    }
     const uint32_t fi = p.c.page.div(mover), ti = p.c.page.div(hole);
     const int fp = page_of(p.c, b, fi), tp = page_of(p.c, b, ti);
-    if (fp < 0 || tp < 0) {
+    const bool moves = fp >= 0 && tp >= 0;
+    if (lane == 0) {
+      src[hole] = moves ? mover : -1;
+      wo[hole] = moves ? w[mover] : 0.0f;
+      po[hole] = moves ? ps[mover] : -1;
+    }
+    if (!moves) {  // a row without a mapped page on either side
       raise_status(DCR_ERR_DEVICE_INDEX);
       return;
     }
@@ -426,6 +427,8 @@ __global__ void __launch_bounds__(256) paged_evict_move_kernel(const PagedEvictP
       }
       if (fp < 0 || tp < 0) {  // a row without a mapped page on either side
         raise_status(DCR_ERR_DEVICE_INDEX);
+        from[i] = px[i] = -1;
+        wx[i] = 0.0f;
         continue;
       }
       moves[i] = true;

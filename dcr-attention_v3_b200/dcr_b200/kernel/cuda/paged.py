@@ -89,7 +89,9 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.
     go by the lower slot, NaN ranks highest. Kept rows at or past the budget move, in place and in
     slot order, into the evicted slots before it. ``src [B, H_kv, budget]`` int32 is the slot each
     kept row came from (-1 past the new length); ``weights_out`` and ``pos_out`` (new tensors
-    ``[B, H_kv, budget]`` unless given; not the inputs) hold the kept slots' entries."""
+    ``[B, H_kv, budget]`` unless given; not the inputs) hold the kept slots' entries. Every page
+    below a length must be mapped: a row that would come from or go to one that is not stays where
+    it is, its new slot is -1 in ``src`` and the device status is set."""
     r = _lib.torch_ops().evict(k_pages, v_pages, page_table, lengths, weights, pos, seen, budget,
                                sinks, recent, weights_out, pos_out, workspace_buf)
     if type(r) is int:

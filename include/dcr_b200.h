@@ -488,7 +488,9 @@ size_t dcr_paged_evict_workspace_bytes(int B, int H_kv, int budget);
  * -1 past the new length). weights_out and pos_out (first `budget` slots; other tensors than
  * weights and pos) receive the kept slots' entries, 0 and -1 past the new length; lengths_out
  * [B] = min(lengths, budget) (another tensor than lengths). The sequences' pages must not be
- * shared with one another: a shared row would be moved for each of them. */
+ * shared with one another: a shared row would be moved for each of them. Every page below a
+ * length must be mapped: a kept row whose old or new slot has no page is not moved, its new slot
+ * gets src -1, weight 0 and position -1, and the device status is set. */
 int dcr_paged_evict(void* k_pages, void* v_pages, int dtype, int64_t k_stride_p,
                     int64_t k_stride_h, int64_t k_stride_s, int64_t v_stride_p,
                     int64_t v_stride_h, int64_t v_stride_s, int num_pages, int page_size,

@@ -98,6 +98,36 @@ def test_evict_does_not_look_at_entries_past_the_length(lengths):
             assert src[b, h].tolist() == _plan(w, lengths, 40, b, h)
 
 
+@pytest.mark.parametrize("n", [42, 100])  # few evictions, and many
+@pytest.mark.parametrize("gone", [0, -1])  # a page of holes, a page of movers
+def test_evict_reports_rows_without_a_page(n, gone):
+    """A kept row that cannot be moved is not passed off as moved: src -1, weight 0, position -1."""
+    from dcr_b200 import _lib
+    budget, page = 40, 16
+
+    def spoil(table, pages):
+        table[0, gone] = -1
+    k0, v0, k, v, table, w, pos, (src, wo, po, no) = _evicted([n, n], budget, spoil)
+    lost = 0
+    for b in range(2):
+        for h in range(2):
+            want = _plan(w, [n, n], budget, b, h)
+            ek, ev = k0.clone(), v0.clone()
+            for i, s in enumerate(want):
+                fp, tp = int(table[b, s // page]), int(table[b, i // page])
+                if s != i and (fp < 0 or tp < 0):
+                    lost += 1
+                    assert (int(src[b, h, i]), float(wo[b, h, i]), int(po[b, h, i])) == (-1, 0.0, -1)
+                    continue
+                assert int(src[b, h, i]) == s and float(wo[b, h, i]) == float(w[b, h, s])
+                assert int(po[b, h, i]) == s
+                if s != i:
+                    ek[tp, h, i % page], ev[tp, h, i % page] = k0[fp, h, s % page], v0[fp, h, s % page]
+            held = [int(x) for x in table[b] if x >= 0]
+            assert torch.equal(k[held, h], ek[held, h]) and torch.equal(v[held, h], ev[held, h])
+    assert _status() == (_lib.DCR_ERR_DEVICE_INDEX if lost else 0)
+
+
 def _model(layers=2):
     from dcr_b200.models.llama.model import DCRLlamaDecoder, LlamaDecodeConfig
     cfg = LlamaDecodeConfig(vocab=512, hidden=256, intermediate=512, layers=layers, heads=4, kv_heads=2)
