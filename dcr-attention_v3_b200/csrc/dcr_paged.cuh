@@ -10,6 +10,7 @@
 #pragma once
 
 #include "dcr_common.cuh"
+#include "dcr_tables.h"
 
 namespace dcr {
 

@@ -287,8 +287,11 @@ extern "C" int dcr_paged_append(
                          reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin) |
                          reinterpret_cast<uintptr_t>(q_weight) | reinterpret_cast<uintptr_t>(k_weight);
   if (ptrs & 15u) return DCR_ERR_ALIGN;
-  if ((weights != nullptr && (w_stride_b < 0 || w_stride_h < 0)) ||
-      (pos != nullptr && (p_stride_b < 0 || p_stride_h < 0)))
+  const int64_t max_slots = static_cast<int64_t>(max_pages) * page_size;
+  if ((weights != nullptr && (w_stride_b < 0 || w_stride_h < 0 ||
+                              !rows_apart(n_seq, H_kv, max_slots, w_stride_b, w_stride_h))) ||
+      (pos != nullptr && (p_stride_b < 0 || p_stride_h < 0 ||
+                          !rows_apart(n_seq, H_kv, max_slots, p_stride_b, p_stride_h))))
     return DCR_ERR_SHAPE;
   PagedAppendParams p;
   p.c = make_pool(k_pages, v_pages, kp_stride_p, kp_stride_h, kp_stride_s, vp_stride_p,

@@ -1083,7 +1083,9 @@ int dcr_paged_attend(const void* q, int64_t q_stride_b, int64_t q_stride_h, cons
     return DCR_ERR_ALIGN;
   if (q_stride_b < 0 || q_stride_h < 0) return DCR_ERR_SHAPE;
   const int max_slots = max_pages * page_size;
-  if (weights != nullptr && (w_stride_h < 0 || w_stride_b < 0)) return DCR_ERR_SHAPE;
+  if (weights != nullptr && (w_stride_h < 0 || w_stride_b < 0 ||
+                             !rows_apart(B, H_kv, max_slots, w_stride_b, w_stride_h)))
+    return DCR_ERR_SHAPE;
   const int G = H / H_kv;
   const PagedAttendLayout w = pa_layout(B, H, G, D, max_slots, weights != nullptr);
   if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15u) ||

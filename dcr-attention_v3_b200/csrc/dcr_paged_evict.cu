@@ -526,6 +526,9 @@ int dcr_paged_evict(void* k_pages, void* v_pages, int dtype, int64_t k_stride_p,
                               wo_stride_b, wo_stride_h, po_stride_b, po_stride_h};
   for (int i = 0; i < 8; ++i)
     if (strides[i] < 0) return DCR_ERR_SHAPE;
+  if (!rows_apart(B, H_kv, budget, wo_stride_b, wo_stride_h) ||
+      !rows_apart(B, H_kv, budget, po_stride_b, po_stride_h))
+    return DCR_ERR_SHAPE;
   if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15u) ||
       workspace_bytes < dcr_paged_evict_workspace_bytes(B, H_kv, budget))
     return DCR_ERR_WORKSPACE;

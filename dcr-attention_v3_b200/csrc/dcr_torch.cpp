@@ -22,6 +22,7 @@
 #include <string>
 
 #include "dcr_b200.h"
+#include "dcr_tables.h"
 
 namespace {
 
@@ -127,8 +128,10 @@ struct Table {
   int64_t sb = 0, sh = 0;
 };
 
-// A per-slot table [B, H_kv, >= slots] with contiguous rows, or None.
-Table slot_table(PyObject* o, const char* name, at::ScalarType type, const Pool& p, int64_t slots) {
+// A per-slot table [B, H_kv, >= slots] with contiguous rows, or None; one that is written has no
+// two rows that share elements (an expanded tensor, say).
+Table slot_table(PyObject* o, const char* name, at::ScalarType type, const Pool& p, int64_t slots,
+                 bool written = true) {
   Table r;
   if (o == Py_None) return r;
   const at::Tensor& t = cuda_tensor(o, name);
@@ -140,6 +143,8 @@ Table slot_table(PyObject* o, const char* name, at::ScalarType type, const Pool&
   r.data = t.data_ptr();
   r.sb = t.stride(0);
   r.sh = t.stride(1);
+  if (written && !dcr::rows_apart(p.sequences, p.H_kv, slots, r.sb, r.sh))
+    refuse(std::string(name) + " must not have rows that share elements");
   return r;
 }
 
@@ -317,8 +322,8 @@ PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const void* lengths = vector_of(a[3], "lengths", at::kInt, B, p.device);
     cuda_tensor(a[4], "weights");
     cuda_tensor(a[5], "pos");
-    const Table w = slot_table(a[4], "weights", at::kFloat, p, p.slots);
-    const Table pos = slot_table(a[5], "pos", at::kInt, p, p.slots);
+    const Table w = slot_table(a[4], "weights", at::kFloat, p, p.slots, false);
+    const Table pos = slot_table(a[5], "pos", at::kInt, p, p.slots, false);
     const void* seen = vector_of(a[6], "seen", at::kInt, B, p.device);
     const int64_t budget = integer(a[7], "budget");
     const int64_t sinks = integer(a[8], "sinks"), recent = integer(a[9], "recent");

@@ -53,7 +53,7 @@ def up_to_date() -> bool:
 
 def build_torch(force: bool = False, verbose: bool = False) -> str:
     """Compile the torch binding (host code only) if a source is newer than it."""
-    sources = [TORCH_SOURCE, os.path.join(INCLUDE, "dcr_b200.h")]
+    sources = [TORCH_SOURCE, os.path.join(CSRC, "dcr_tables.h"), os.path.join(INCLUDE, "dcr_b200.h")]
     if not force and os.path.exists(TORCH_PATH) and all(
             os.path.getmtime(s) <= os.path.getmtime(TORCH_PATH) for s in sources):
         return TORCH_PATH

@@ -434,7 +434,9 @@ int dcr_silu_mul_packed(const void* gate_up, int dtype, int rows, int inter, voi
  * DCR_ERR_DEVICE_INDEX in the device status (a length beyond max_pages * page_size is taken as
  * that, a negative one as 0).
  * Attended slots must be finite for finite results: slots past the length, before the window
- * or in unmapped pages may hold anything. */
+ * or in unmapped pages may hold anything.
+ * The rows of a per-slot table that is written (weights, pos, weights_out, pos_out) must not share
+ * elements: one of its two strides spans all rows of the other dimension (else DCR_ERR_SHAPE). */
 
 /* Bytes of workspace dcr_paged_attend needs; it need not be initialised. 0: invalid shape. */
 size_t dcr_paged_workspace_bytes(int B, int H, int H_kv, int D, int max_slots, int with_weights);

@@ -1,0 +1,45 @@
+"""More refusals of the paged serving operators at the C ABI (CPU only): memory that two writers, or
+a reader and a writer, would share. As in test_capi_paged.py no pointer is followed."""
+from __future__ import annotations
+
+import pytest
+from test_capi_paged import (APPEND, ATTEND, B, EVICT, H_KV, MAX_PAGES, P, PAGE, SHAPE, _names,
+                             lib)  # noqa: F401
+
+SLOTS = MAX_PAGES * PAGE  # 64 a row
+
+# one row for both heads, for both sequences, rows that begin inside one another, sequences inside heads
+SHARED = [dict(b=H_KV * SLOTS, h=0), dict(b=0, h=SLOTS), dict(b=H_KV * SLOTS, h=SLOTS - 1),
+          dict(b=H_KV * SLOTS - 1, h=SLOTS), dict(b=SLOTS, h=SLOTS), dict(b=SLOTS, h=2 * SLOTS - 1)]
+APART = [dict(b=H_KV * SLOTS, h=SLOTS), dict(b=SLOTS, h=B * SLOTS), dict(b=1 << 40, h=SLOTS + 3)]
+
+
+def _call(lib, func, base, **change):  # noqa: F811
+    args = dict(base, **change)
+    return getattr(lib, func)(*[args[n] for n in _names(func)])
+
+
+def _writes(s, slots):
+    """Every operator that writes a per-slot table, given one of these strides (scaled to `slots`)."""
+    yield "dcr_paged_attend", ATTEND, dict(weights=P, w_stride_b=s["b"], w_stride_h=s["h"])
+    yield "dcr_paged_append", APPEND, dict(weights=P, w_stride_b=s["b"], w_stride_h=s["h"])
+    yield "dcr_paged_append", APPEND, dict(pos=P, p_stride_b=s["b"], p_stride_h=s["h"])
+    yield "dcr_paged_evict", dict(EVICT, budget=slots), dict(wo_stride_b=s["b"], wo_stride_h=s["h"])
+    yield "dcr_paged_evict", dict(EVICT, budget=slots), dict(po_stride_b=s["b"], po_stride_h=s["h"])
+
+
+@pytest.mark.parametrize("s", SHARED, ids=str)
+def test_tables_whose_rows_share_elements(lib, s):  # noqa: F811
+    for func, base, change in _writes(s, SLOTS):
+        assert _call(lib, func, base, **change) == SHAPE, (func, change)
+
+
+@pytest.mark.parametrize("s", APART, ids=str)
+def test_tables_whose_rows_lie_apart_pass_the_checks(lib, s):  # noqa: F811
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("the addresses here are not to be followed")
+    for func, base, change in _writes(s, SLOTS):
+        if func == "dcr_paged_evict":
+            change = dict(change, pos_out=P + (1 << 50))
+        assert _call(lib, func, base, **change) != SHAPE, (func, change)

@@ -128,6 +128,46 @@ def test_evict_reports_rows_without_a_page(n, gone):
     assert _status() == (_lib.DCR_ERR_DEVICE_INDEX if lost else 0)
 
 
+def _shared_rows(dtype=torch.float32, slots=48):
+    """Per-slot tables [2, 2, slots] whose rows share elements: expanded over heads, over sequences,
+    rows that begin inside one another."""
+    yield torch.zeros(2, 1, slots, dtype=dtype, device=DEV).expand(2, 2, slots)
+    yield torch.zeros(1, 2, slots, dtype=dtype, device=DEV).expand(2, 2, slots)
+    yield torch.zeros(4 * slots, dtype=dtype, device=DEV).as_strided((2, 2, slots), (2 * slots, slots // 2, 1))
+
+
+def _small(seed=2):
+    k, v, table = ref.make_pool([40, 40], 2, 16, 64, torch.bfloat16, DEV, _gen(seed), garbage=0.0)
+    q = torch.randn(2, 4, 64, generator=_gen(seed + 1), device=DEV).to(torch.bfloat16)
+    return k, v, table, q, _i32([40, 40])
+
+
+def test_written_tables_must_not_share_elements():
+    from dcr_b200.kernel.cuda.paged import paged_append, paged_attention, paged_evict
+    k, v, table, q, n = _small()
+    cos = torch.ones(64, 64, dtype=torch.bfloat16, device=DEV)
+    good, ids = torch.zeros(2, 2, 48, device=DEV), torch.zeros(2, 2, 48, dtype=torch.int32, device=DEV)
+    append = lambda **kw: paged_append(q, q[:, :2], q[:, 2:], cos, cos, _i32([1, 1]), k, v, table,  # noqa: E731
+                                       _i32([7, 7]), **kw)
+    for w, pos in zip(_shared_rows(), _shared_rows(torch.int32)):
+        for call in (lambda: paged_attention(q, k, v, table, n, weights=w), lambda: append(weights=w),
+                     lambda: append(pos=pos),
+                     lambda: paged_evict(k, v, table, n, good, ids, n, 30, weights_out=w),
+                     lambda: paged_evict(k, v, table, n, good, ids, n, 30, pos_out=pos)):
+            with pytest.raises(AssertionError, match="share"):
+                call()
+        # what is only read may be shared
+        src, wo, po, _ = paged_evict(k.clone(), v.clone(), table, n, w, pos, n, 30)
+        assert (src == torch.arange(30, device=DEV)).all() and (wo == 0).all() and (po == 0).all()
+    plain = torch.zeros(2, 2, 48, device=DEV)
+    paged_attention(q, k, v, table, n, weights=plain)
+    for apart in (torch.zeros(2, 2, 48, device=DEV).transpose(0, 1), torch.zeros(2, 4, 50, device=DEV)[:, ::2, 1:49],
+                  torch.zeros(2, 3, 2, 48, device=DEV)[:, 1]):
+        paged_attention(q, k, v, table, n, weights=apart)
+        assert torch.equal(apart, plain)
+    assert _status() == 0
+
+
 def _model(layers=2):
     from dcr_b200.models.llama.model import DCRLlamaDecoder, LlamaDecodeConfig
     cfg = LlamaDecodeConfig(vocab=512, hidden=256, intermediate=512, layers=layers, heads=4, kv_heads=2)
