@@ -532,6 +532,15 @@ int dcr_paged_evict(void* k_pages, void* v_pages, int dtype, int64_t k_stride_p,
   if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15u) ||
       workspace_bytes < dcr_paged_evict_workspace_bytes(B, H_kv, budget))
     return DCR_ERR_WORKSPACE;
+  const int64_t cap = static_cast<int64_t>(max_pages) * page_size;
+  const TableSpan w_in(weights, B, H_kv, cap, w_stride_b, w_stride_h);
+  const TableSpan p_in(pos, B, H_kv, cap, p_stride_b, p_stride_h);
+  const TableSpan w_to(weights_out, B, H_kv, budget, wo_stride_b, wo_stride_h);
+  const TableSpan p_to(pos_out, B, H_kv, budget, po_stride_b, po_stride_h);
+  if (tables_meet(w_in, w_to) || tables_meet(p_in, w_to) || tables_meet(w_in, p_to) ||
+      tables_meet(p_in, p_to) || tables_meet(w_to, p_to) ||
+      tables_meet(TableSpan(lengths, 1, 1, B, 0, 0), TableSpan(lengths_out, 1, 1, B, 0, 0)))
+    return DCR_ERR_SHAPE;
   const int64_t per16 = dtype == DCR_DTYPE_F32 ? 4 : 8;
   PagedEvictParams p;
   p.c = make_pool(k_pages, v_pages, k_stride_p / per16, k_stride_h / per16, k_stride_s / per16,

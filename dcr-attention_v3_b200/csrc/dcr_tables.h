@@ -17,4 +17,46 @@ inline bool rows_apart(int64_t n_b, int64_t n_h, int64_t slots, int64_t sb, int6
          (sb >= slots && sh >= slots && (sh - slots) / (n_b - 1) >= sb);
 }
 
+// A table as bytes.
+struct TableSpan {
+  const char* data;
+  int64_t n_b, n_h, bytes, sb, sh;  // rows, a row's bytes, strides in bytes
+
+  TableSpan(const void* table, int64_t nb, int64_t nh, int64_t slots, int64_t stride_b, int64_t stride_h)
+      : data(static_cast<const char*>(table)), n_b(nb), n_h(nh), bytes(4 * slots),
+        sb(nb > 1 ? 4 * stride_b : 0), sh(nh > 1 ? 4 * stride_h : 0) {}
+  int64_t size() const { return (n_b - 1) * sb + (n_h - 1) * sh + bytes; }
+};
+
+// Whether a row of `a` shares a byte with a row of `b`, whose own rows are apart. Tables that lie
+// one after the other, the usual case, need two comparisons; rows that lie between one another's
+// are compared by division, a few of `b` for each of `a`.
+inline bool tables_meet(const TableSpan& a, const TableSpan& b) {
+  const int64_t off = static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.data) -
+                                           reinterpret_cast<uintptr_t>(b.data));
+  if (off >= b.size() || -off >= a.size()) return false;
+  const bool b_outer = b.n_h <= 1 || (b.n_b > 1 && b.sb >= b.sh);
+  const int64_t n_out = b_outer ? b.n_b : b.n_h, n_in = b_outer ? b.n_h : b.n_b;
+  const int64_t s_out = b_outer ? b.sb : b.sh, s_in = b_outer ? b.sh : b.sb;
+  const int64_t block = (n_in - 1) * s_in + b.bytes;  // an outer index's rows
+  // the indexes whose [i * stride, i * stride + size) may meet [x, x + a.bytes)
+  auto first = [](int64_t x, int64_t size, int64_t stride) {
+    return x < size || stride == 0 ? 0 : (x - size) / stride + 1;
+  };
+  auto last = [&](int64_t x, int64_t stride, int64_t n) {
+    const int64_t end = x + a.bytes - 1;
+    if (end < 0) return static_cast<int64_t>(-1);
+    return stride == 0 || end / stride >= n ? n - 1 : end / stride;
+  };
+  for (int64_t i = 0; i < a.n_b; ++i)
+    for (int64_t j = 0; j < a.n_h; ++j) {
+      const int64_t x = off + i * a.sb + j * a.sh;
+      for (int64_t o = first(x, block, s_out); o <= last(x, s_out, n_out); ++o) {
+        const int64_t y = x - o * s_out;
+        if (first(y, b.bytes, s_in) <= last(y, s_in, n_in)) return true;
+      }
+    }
+  return false;
+}
+
 }  // namespace dcr

@@ -352,8 +352,15 @@ PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor src = at::empty({B, p.H_kv, budget}, i32);
     const at::Tensor lengths_out = at::empty({B}, i32);
     if (B > 0) {
-      if (two.data == w.data || tpo.data == pos.data)
-        refuse("weights_out and pos_out must be other tensors than weights and pos");
+      auto span = [&](const Table& t, int64_t slots) {
+        return dcr::TableSpan(t.data, B, p.H_kv, slots, t.sb, t.sh);
+      };
+      const dcr::TableSpan from[2] = {span(w, p.slots), span(pos, p.slots)};
+      const dcr::TableSpan to[2] = {span(two, budget), span(tpo, budget)};
+      if (dcr::tables_meet(from[0], to[0]) || dcr::tables_meet(from[1], to[0]) ||
+          dcr::tables_meet(from[0], to[1]) || dcr::tables_meet(from[1], to[1]) ||
+          dcr::tables_meet(to[0], to[1]))
+        refuse("weights_out and pos_out must share no memory with weights, pos or one another");
       const size_t bytes = dcr_paged_evict_workspace_bytes(
           static_cast<int>(B), static_cast<int>(p.H_kv), static_cast<int>(budget));
       const at::Tensor ws = scratch(a[12], bytes, p.device);

@@ -487,9 +487,9 @@ size_t dcr_paged_evict_workspace_bytes(int B, int H_kv, int budget);
  * the lower slot (-0 equals +0, NaN ranks highest). Kept slots at or past the budget move, in
  * slot order, into the evicted slots before it, K and V rows included, in place. src_out
  * [B, H_kv, budget] int32: the slot each one's row came from (its own for a row that stayed,
- * -1 past the new length). weights_out and pos_out (first `budget` slots; other tensors than
- * weights and pos) receive the kept slots' entries, 0 and -1 past the new length; lengths_out
- * [B] = min(lengths, budget) (another tensor than lengths). The sequences' pages must not be
+ * -1 past the new length). weights_out and pos_out (first `budget` slots; no memory in common with
+ * weights, pos or one another) receive the kept slots' entries, 0 and -1 past the new length;
+ * lengths_out [B] = min(lengths, budget) (none in common with lengths). The sequences' pages must not be
  * shared with one another: a shared row would be moved for each of them. Every page below a
  * length must be mapped: a kept row whose old or new slot has no page is not moved, its new slot
  * gets src -1, weight 0 and position -1, and the device status is set. */

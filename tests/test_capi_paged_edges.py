@@ -43,3 +43,32 @@ def test_tables_whose_rows_lie_apart_pass_the_checks(lib, s):  # noqa: F811
         if func == "dcr_paged_evict":
             change = dict(change, pos_out=P + (1 << 50))
         assert _call(lib, func, base, **change) != SHAPE, (func, change)
+
+
+DENSE_OUT = dict(wo_stride_b=H_KV * SLOTS, wo_stride_h=SLOTS, po_stride_b=H_KV * SLOTS, po_stride_h=SLOTS)
+TABLE = 4 * B * H_KV * SLOTS  # bytes of a dense table
+
+
+@pytest.mark.parametrize("change", [
+    dict(weights_out=P + TABLE - 4 * SLOTS), dict(weights_out=P - TABLE + 4 * SLOTS),
+    dict(pos_out=P + 4), dict(pos_out=P - 4),
+    dict(weights=5 * P, pos=P, weights_out=P + 8),             # into the positions
+    dict(weights=P, pos=5 * P, pos_out=P + 8),                 # into the weights
+    dict(weights_out=3 * P, pos_out=3 * P + TABLE // 2),       # into one another
+    dict(lengths=9 * P, lengths_out=9 * P + 4 * (B - 1))], ids=str)
+def test_evict_outputs_that_reach_into_inputs(lib, change):  # noqa: F811
+    base = dict(EVICT, **DENSE_OUT, pos_out=3 * P)
+    base.update(w_stride_b=H_KV * SLOTS, w_stride_h=SLOTS, p_stride_b=H_KV * SLOTS, p_stride_h=SLOTS)
+    assert _call(lib, "dcr_paged_evict", base, **change) == SHAPE
+
+
+def test_evict_outputs_between_the_rows_of_inputs_pass(lib):  # noqa: F811
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("the addresses here are not to be followed")
+    wide = dict(w_stride_b=2 * H_KV * SLOTS, w_stride_h=2 * SLOTS, wo_stride_b=2 * H_KV * SLOTS,
+                wo_stride_h=2 * SLOTS, pos=5 * P, pos_out=3 * P)
+    for budget, at, fits in ((SLOTS, SLOTS, True), (32, SLOTS + 32, True), (33, SLOTS + 32, False),
+                             (SLOTS, SLOTS - 1, False), (32, -32, True), (32, -31, False)):
+        got = _call(lib, "dcr_paged_evict", EVICT, **wide, budget=budget, weights_out=P + 4 * at)
+        assert (got != SHAPE) == fits, (budget, at)

@@ -168,6 +168,27 @@ def test_written_tables_must_not_share_elements():
     assert _status() == 0
 
 
+def test_evict_outputs_must_not_reach_into_inputs():
+    from dcr_b200.kernel.cuda.paged import paged_evict
+    k, v, table, _, n = _small()
+    both = torch.rand(2, 2, 2, 48, generator=_gen(4), device=DEV)
+    ids = torch.arange(48, dtype=torch.int32, device=DEV).expand(2, 2, 48).contiguous()
+    flat = both.view(-1)
+    evict = lambda w, pos, **kw: paged_evict(k, v, table, n, w, pos, n, 20, **kw)  # noqa: E731
+    for w, pos, kw in ((both[0], ids, dict(weights_out=flat[96:288].view(2, 2, 48))),
+                       (both[:, 0], ids, dict(weights_out=both[:, 0, :, 8:])),
+                       (both[0], ids, dict(weights_out=ids.view(torch.float32))),
+                       (both[0], ids, dict(pos_out=both[0].view(torch.int32))),
+                       (both[0], ids, dict(weights_out=both[1], pos_out=both[1].view(torch.int32)))):
+        with pytest.raises(AssertionError, match="memory"):
+            evict(w, pos, **kw)
+    # between the rows of the inputs there is room
+    want = paged_evict(k.clone(), v.clone(), table, n, both[:, 0].clone(), ids, n, 20)
+    got = evict(both[:, 0], ids, weights_out=both[:, 1])
+    assert torch.equal(got[1][:, :, :20], want[1]) and torch.equal(got[0], want[0])
+    assert torch.equal(got[2], want[2]) and _status() == 0
+
+
 def _model(layers=2):
     from dcr_b200.models.llama.model import DCRLlamaDecoder, LlamaDecodeConfig
     cfg = LlamaDecodeConfig(vocab=512, hidden=256, intermediate=512, layers=layers, heads=4, kv_heads=2)
