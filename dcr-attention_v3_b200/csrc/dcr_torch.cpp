@@ -232,7 +232,9 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t window = integer(a[6], "window");
     if (window < 0 || window > INT32_MAX) refuse("window must be >= 0");
     const Table w = slot_table(a[7], "weights", at::kFloat, p, p.slots);
-    const bool want_lse = a[8] == Py_True;
+    const int truth = PyObject_IsTrue(a[8]);
+    if (truth < 0) throw Refused{};
+    const bool want_lse = truth != 0;
     const c10::cuda::OptionalCUDAGuard guard(p.k->device());
     const at::Tensor o = output(a[9], {B, H, p.D}, p.k->options());
     at::Tensor lse;

@@ -65,6 +65,17 @@ def test_f16_weights_far_below_the_largest(D, G, nats):
     assert (lse.double() - (nats + math.log(total))).abs().max() <= lse_tol
 
 
+def test_return_lse_takes_any_truth_value():
+    from dcr_b200.kernel.cuda.paged import paged_attention
+    k, v, table = ref.make_pool([40], 2, 16, 64, torch.bfloat16, DEV, _gen(2))
+    q = torch.randn(1, 4, 64, generator=_gen(3), device=DEV).to(torch.bfloat16)
+    o, lse = paged_attention(q, k, v, table, _i32([40]), return_lse=True)
+    got = paged_attention(q, k, v, table, _i32([40]), return_lse=1)
+    assert isinstance(got, tuple) and torch.equal(got[0], o) and torch.equal(got[1], lse)
+    for no in (0, False, None):
+        assert torch.equal(paged_attention(q, k, v, table, _i32([40]), return_lse=no), o)
+
+
 def _evicted(lengths, budget, spoil, width=None, page=16):
     """(k, v before; k, v after; table, weights, pos, results) of one eviction; `spoil` changes the
     page table after the pool is filled."""
