@@ -7,11 +7,13 @@ It links the CUDA runtime statically and reaches the driver's tensor-map encoder
 ``cudaGetDriverEntryPoint``, so it needs neither ``-lcuda`` nor a matching libcudart at
 run time.
 
-Usage: ``python -m dcr_b200.build [--force]`` (with ``dcr-attention_v3_b200`` on sys.path).
+Usage: ``python -m dcr_b200.build [--force] [--no-binding]`` (with ``dcr-attention_v3_b200`` on
+sys.path). The binding is built where torch is installed; ``--no-binding`` leaves it out.
 """
 from __future__ import annotations
 
 import glob
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -26,6 +28,7 @@ LIB_DIR = os.path.join(PKG_DIR, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libdcr_b200.so")
 TORCH_PATH = os.path.join(LIB_DIR, "dcr_b200_torch.so")
 TORCH_SOURCE = os.path.join(CSRC, "dcr_torch.cpp")
+TORCH_STAMP = os.path.join(LIB_DIR, "dcr_b200_torch.stamp")  # what the binding was built for
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-shared",
@@ -52,14 +55,16 @@ def up_to_date() -> bool:
 
 
 def build_torch(force: bool = False, verbose: bool = False) -> str:
-    """Compile the torch binding (host code only) if a source is newer than it."""
+    """Compile the torch binding (host code only) if a source is newer than it, or if it was built
+    for another torch or Python."""
+    import torch
+    stamp = f"{torch.__version__} {sys.implementation.cache_tag}"
     sources = [TORCH_SOURCE, os.path.join(CSRC, "dcr_tables.h"), os.path.join(INCLUDE, "dcr_b200.h")]
-    if not force and os.path.exists(TORCH_PATH) and all(
+    if not force and os.path.exists(TORCH_PATH) and _stamp() == stamp and all(
             os.path.getmtime(s) <= os.path.getmtime(TORCH_PATH) for s in sources):
         return TORCH_PATH
     import sysconfig
 
-    import torch
     from torch.utils.cpp_extension import include_paths, library_paths
     cuda_include = os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include")
     includes = [INCLUDE, *include_paths(), cuda_include, sysconfig.get_path("include")]
@@ -76,14 +81,26 @@ def build_torch(force: bool = False, verbose: bool = False) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"the torch binding failed to build ({r.returncode}):\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, TORCH_PATH)
+    with open(TORCH_STAMP, "w") as f:
+        f.write(stamp)
     return TORCH_PATH
 
 
-def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile the libraries if any of their sources is newer; return libdcr_b200.so's path."""
+def _stamp() -> str:
+    try:
+        with open(TORCH_STAMP) as f:
+            return f.read()
+    except OSError:
+        return ""
+
+
+def build(force: bool = False, verbose: bool = False, binding: bool = True) -> str:
+    """Compile the libraries if any of their sources is newer; return libdcr_b200.so's path. The
+    torch binding is left out without ``binding`` or where torch is not installed."""
     if force or not up_to_date():
         _build_library(verbose)
-    build_torch(force, verbose)
+    if binding and importlib.util.find_spec("torch") is not None:
+        build_torch(force, verbose)
     return LIB_PATH
 
 
@@ -103,4 +120,4 @@ def _build_library(verbose: bool) -> None:
 
 
 if __name__ == "__main__":
-    print(build(force="--force" in sys.argv, verbose=True))
+    print(build(force="--force" in sys.argv, verbose=True, binding="--no-binding" not in sys.argv))
