@@ -141,7 +141,7 @@ const char* dcr_status_string(int status) {
     case DCR_ERR_SHAPE: return "unsupported shape or stride (D must be 64, H/H_kv in {1,2,4,8})";
     case DCR_ERR_K_RANGE: return "k_eff must be in (0, N); caller must dispatch to SDPA";
     case DCR_ERR_DTYPE: return "unknown dtype code";
-    case DCR_ERR_ALIGN: return "pointer or stride is not 16-byte aligned";
+    case DCR_ERR_ALIGN: return "pointer or stride is not aligned (to 16 bytes, or to its elements)";
     case DCR_ERR_WORKSPACE: return "workspace is NULL or smaller than dcr_workspace_bytes()";
     case DCR_ERR_CUDA: return "a CUDA runtime call failed";
     case DCR_ERR_DEVICE_TIMEOUT: return "device: a bounded wait expired";

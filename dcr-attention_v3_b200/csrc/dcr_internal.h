@@ -32,6 +32,12 @@ inline int record_mark(void* event, cudaStream_t s) {
 // Sets the dynamic shared-memory limit of a kernel once per (kernel, device).
 cudaError_t ensure_smem_attr(const void* func, int bytes);
 
+// Whether a pointer is off a boundary of n bytes, a power of two (null is on every one).
+template <typename... Pointers>
+bool misaligned(size_t n, Pointers... pointers) {
+  return ((reinterpret_cast<uintptr_t>(pointers) | ...) & (n - 1)) != 0;
+}
+
 // Launches a kernel as a grid of 1-D thread-block clusters of `cluster` CTAs.
 template <typename Kernel, typename... Args>
 cudaError_t launch_cluster(Kernel kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t st,

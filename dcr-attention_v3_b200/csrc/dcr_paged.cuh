@@ -10,6 +10,7 @@
 #pragma once
 
 #include "dcr_common.cuh"
+#include "dcr_internal.h"
 #include "dcr_tables.h"
 
 namespace dcr {
@@ -97,7 +98,7 @@ inline int check_pool(const void* k, const void* v, int dtype, int64_t ksp, int6
   if (page_size > 1 && (ksr < D || vsr < D)) return DCR_ERR_SHAPE;
   if (H_kv > 1 && (ksh < D || vsh < D)) return DCR_ERR_SHAPE;
   if (num_pages > 1 && (ksp < D || vsp < D)) return DCR_ERR_SHAPE;
-  if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) return DCR_ERR_ALIGN;
+  if (misaligned(16, k, v) || misaligned(4, table)) return DCR_ERR_ALIGN;
   return DCR_OK;
 }
 

@@ -282,11 +282,9 @@ extern "C" int dcr_paged_append(
     if (strides[i] < 0) return DCR_ERR_SHAPE;
     if (strides[i] % per16 != 0) return DCR_ERR_ALIGN;
   }
-  const uintptr_t ptrs = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
-                         reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(q_out) |
-                         reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin) |
-                         reinterpret_cast<uintptr_t>(q_weight) | reinterpret_cast<uintptr_t>(k_weight);
-  if (ptrs & 15u) return DCR_ERR_ALIGN;
+  if (misaligned(16, q, k, v, q_out, cos, sin, q_weight, k_weight) ||
+      misaligned(4, positions, seq, slots, weights, pos))
+    return DCR_ERR_ALIGN;
   const int64_t max_slots = static_cast<int64_t>(max_pages) * page_size;
   if ((weights != nullptr && (w_stride_b < 0 || w_stride_h < 0 ||
                               !rows_apart(n_seq, H_kv, max_slots, w_stride_b, w_stride_h))) ||

@@ -1078,8 +1078,8 @@ int dcr_paged_attend(const void* q, int64_t q_stride_b, int64_t q_stride_h, cons
                             table_stride, max_pages, H_kv, D);
   if (st != DCR_OK) return st;
   const int64_t per16 = dtype == DCR_DTYPE_F32 ? 4 : 8;
-  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(o)) & 15u) ||
-      q_stride_b % per16 || q_stride_h % per16)
+  if (misaligned(16, q, o) || misaligned(4, lengths, lse, weights) || q_stride_b % per16 ||
+      q_stride_h % per16)
     return DCR_ERR_ALIGN;
   if (q_stride_b < 0 || q_stride_h < 0) return DCR_ERR_SHAPE;
   const int max_slots = max_pages * page_size;

@@ -520,6 +520,8 @@ int dcr_paged_evict(void* k_pages, void* v_pages, int dtype, int64_t k_stride_p,
                             table_stride, max_pages, H_kv, D);
   if (st != DCR_OK) return st;
   if (budget > max_pages * page_size) return DCR_ERR_SHAPE;
+  if (misaligned(4, lengths, weights, pos, seen, src_out, weights_out, pos_out, lengths_out))
+    return DCR_ERR_ALIGN;
   // the tables are gathered, not updated in place
   if (weights_out == weights || pos_out == pos || lengths_out == lengths) return DCR_ERR_SHAPE;
   const int64_t strides[8] = {w_stride_b,  w_stride_h,  p_stride_b,  p_stride_h,

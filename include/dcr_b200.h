@@ -61,7 +61,8 @@ typedef enum dcr_status {
   DCR_ERR_SHAPE = 2,            /* B, H, H_kv, N, D or a stride out of range          */
   DCR_ERR_K_RANGE = 3,          /* k_eff not in (0, N): caller must dispatch to SDPA  */
   DCR_ERR_DTYPE = 4,            /* unknown dtype code                                 */
-  DCR_ERR_ALIGN = 5,            /* pointer or stride not 16-byte aligned              */
+  DCR_ERR_ALIGN = 5,            /* pointer or stride not 16-byte aligned, or a pointer
+                                   off its own elements' boundary                     */
   DCR_ERR_WORKSPACE = 6,        /* workspace pointer NULL or smaller than required    */
   DCR_ERR_CUDA = 7,             /* a CUDA runtime call failed                         */
   DCR_ERR_DEVICE_TIMEOUT = 8,   /* device status: a bounded wait expired              */

@@ -1,10 +1,11 @@
 """More refusals of the paged serving operators at the C ABI (CPU only): memory that two writers, or
-a reader and a writer, would share. As in test_capi_paged.py no pointer is followed."""
+a reader and a writer, would share, and pointers off their elements' boundary. As in
+test_capi_paged.py no pointer is followed."""
 from __future__ import annotations
 
 import pytest
-from test_capi_paged import (APPEND, ATTEND, B, EVICT, H_KV, MAX_PAGES, P, PAGE, SHAPE, _names,
-                             lib)  # noqa: F401
+from test_capi_paged import (ALIGN, APPEND, ATTEND, B, BF16, EVICT, H_KV, LOGITS, MAX_PAGES, P, PAGE,
+                             SHAPE, _names, lib)  # noqa: F401
 
 SLOTS = MAX_PAGES * PAGE  # 64 a row
 
@@ -72,3 +73,24 @@ def test_evict_outputs_between_the_rows_of_inputs_pass(lib):  # noqa: F811
                              (SLOTS, SLOTS - 1, False), (32, -32, True), (32, -31, False)):
         got = _call(lib, "dcr_paged_evict", EVICT, **wide, budget=budget, weights_out=P + 4 * at)
         assert (got != SHAPE) == fits, (budget, at)
+
+
+def _off(func, base, names, by, **kw):
+    return [(func, base, dict(kw, **{n: 8 * P + by})) for n in names]
+
+
+@pytest.mark.parametrize("func,base,change", (
+    _off("dcr_paged_attend", ATTEND, ("lengths", "page_table", "lse"), 2)
+    + _off("dcr_paged_attend", ATTEND, ("weights",), 2, w_stride_b=H_KV * SLOTS, w_stride_h=SLOTS)
+    + _off("dcr_paged_append", APPEND, ("positions", "seq", "slots", "page_table"), 1)
+    + _off("dcr_paged_append", APPEND, ("weights",), 2, w_stride_b=H_KV * SLOTS, w_stride_h=SLOTS)
+    + _off("dcr_paged_append", APPEND, ("pos",), 3, p_stride_b=H_KV * SLOTS, p_stride_h=SLOTS)
+    + _off("dcr_paged_evict", dict(EVICT, pos_out=3 * P), (
+        "lengths", "weights", "pos", "seen", "src_out", "weights_out", "pos_out", "lengths_out"), 2)
+    + _off("dcr_process_logits", LOGITS, ("logits", "out", "tokens", "token_lengths", "prompt_lengths",
+                                          "repetition", "presence", "frequency", "bias", "allowed"), 2)
+    + _off("dcr_process_logits", dict(LOGITS, dtype=BF16), ("logits", "out"), 1)
+    + _off("dcr_process_logits", LOGITS, ("tokens",), 4, tokens_are_int64=1)
+    + _off("dcr_process_logits", LOGITS, ("next_token",), 4)), ids=lambda x: str(x) if isinstance(x, str) else None)
+def test_pointers_off_their_elements_boundary(lib, func, base, change):  # noqa: F811
+    assert _call(lib, func, base, **change) == ALIGN, change
