@@ -39,6 +39,7 @@
 
 #include "dcr_common.cuh"
 #include "dcr_internal.h"
+#include "dcr_tables.h"
 
 namespace dcr {
 
@@ -541,6 +542,8 @@ int dcr_process_logits(const void* logits, int64_t l_stride_b, int dtype, int B,
   if (L > 0 && tokens == nullptr) return DCR_ERR_NULL;
   if (l_stride_b < 0 || t_stride_b < 0 || bias_stride_b < 0 || a_stride_b < 0) return DCR_ERR_SHAPE;
   if (B > 1 && o_stride_b < V) return DCR_ERR_SHAPE;
+  if (logits_meet(logits, l_stride_b, out, o_stride_b, B, V, dtype == DCR_DTYPE_F32 ? 4 : 2))
+    return DCR_ERR_SHAPE;
   if (misaligned(dtype == DCR_DTYPE_F32 ? 4 : 2, logits, out) || misaligned(8, next_token) ||
       misaligned(tokens_are_int64 ? 8 : 4, tokens) ||
       misaligned(4, token_lengths, prompt_lengths, repetition, presence, frequency, bias, allowed))

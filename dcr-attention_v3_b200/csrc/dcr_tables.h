@@ -1,6 +1,7 @@
-// dcr_tables.h — whether per-slot tables share memory (host only; no CUDA, no torch).
+// dcr_tables.h — whether tables of strided rows share memory (host only; no CUDA, no torch).
 //
-// A table's row (b, h) is `slots` neighbouring 4-byte elements at b * sb + h * sh.
+// A table's row (b, h) is `slots` neighbouring elements at b * sb + h * sh: a slot's entries of 4
+// bytes, or the logits of a row.
 #pragma once
 
 #include <stdint.h>
@@ -22,9 +23,10 @@ struct TableSpan {
   const char* data;
   int64_t n_b, n_h, bytes, sb, sh;  // rows, a row's bytes, strides in bytes
 
-  TableSpan(const void* table, int64_t nb, int64_t nh, int64_t slots, int64_t stride_b, int64_t stride_h)
-      : data(static_cast<const char*>(table)), n_b(nb), n_h(nh), bytes(4 * slots),
-        sb(nb > 1 ? 4 * stride_b : 0), sh(nh > 1 ? 4 * stride_h : 0) {}
+  TableSpan(const void* table, int64_t nb, int64_t nh, int64_t slots, int64_t stride_b,
+            int64_t stride_h, int64_t element = 4)
+      : data(static_cast<const char*>(table)), n_b(nb), n_h(nh), bytes(element * slots),
+        sb(nb > 1 ? element * stride_b : 0), sh(nh > 1 ? element * stride_h : 0) {}
   int64_t size() const { return (n_b - 1) * sb + (n_h - 1) * sh + bytes; }
 };
 
@@ -57,6 +59,15 @@ inline bool tables_meet(const TableSpan& a, const TableSpan& b) {
       }
     }
   return false;
+}
+
+// Whether rows [B, V] processed into rows of other strides or another address would be read after
+// they are written. In place, row for row, is fine.
+inline bool logits_meet(const void* from, int64_t from_stride, const void* to, int64_t to_stride,
+                        int64_t B, int64_t V, int64_t element) {
+  if (from == to && (B <= 1 || from_stride == to_stride)) return false;
+  return tables_meet(TableSpan(from, B, 1, V, from_stride, 0, element),
+                     TableSpan(to, B, 1, V, to_stride, 0, element));
 }
 
 }  // namespace dcr

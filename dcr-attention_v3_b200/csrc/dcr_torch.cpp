@@ -455,6 +455,10 @@ PyObject* process_logits(PyObject*, PyObject* const* a, Py_ssize_t n) {
         refuse("out must match logits, with contiguous rows");
       if (out.data_ptr() == x.data_ptr() && out.strides() != x.strides())
         refuse("logits processed in place must keep their strides");
+      if ((B <= 1 || out.stride(0) >= V) &&  // else refused below
+          dcr::logits_meet(x.data_ptr(), x.stride(0), out.data_ptr(), out.stride(0), B, V,
+                           x.element_size()))
+        refuse("out must be the logits themselves or share no memory with them");
     }
     const at::Tensor token = at::empty({B}, x.options().dtype(at::kLong));
     if (B > 0) {

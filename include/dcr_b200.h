@@ -516,7 +516,7 @@ int dcr_paged_evict(void* k_pages, void* v_pages, int dtype, int64_t k_stride_p,
  * padding; >= V: skipped, device status), of which a row's first token_lengths[b] count (NULL:
  * L) and of these the first prompt_lengths[b] are its prompt (NULL: 0). repetition, presence,
  * frequency [B], bias (row stride 0: one for all rows) and allowed may be NULL. out may be
- * logits itself (same strides). */
+ * logits itself (same strides), else it shares no memory with them. */
 int dcr_process_logits(const void* logits, int64_t l_stride_b, int dtype, int B, int V,
                        const void* tokens, int tokens_are_int64, int64_t t_stride_b, int L,
                        const int32_t* token_lengths, const int32_t* prompt_lengths,

@@ -94,3 +94,23 @@ def _off(func, base, names, by, **kw):
     + _off("dcr_process_logits", LOGITS, ("next_token",), 4)), ids=lambda x: str(x) if isinstance(x, str) else None)
 def test_pointers_off_their_elements_boundary(lib, func, base, change):  # noqa: F811
     assert _call(lib, func, base, **change) == ALIGN, change
+
+
+@pytest.mark.parametrize("change", [
+    dict(out=P + 4 * 50), dict(out=P - 4 * 50), dict(out=P + 4),       # reaches into other rows
+    dict(out=P, o_stride_b=101),                                       # in place, other rows
+    dict(out=P, l_stride_b=0), dict(out=P + 4 * 150, l_stride_b=200),
+    dict(dtype=BF16, out=P + 2 * 199)], ids=str)
+def test_processed_logits_that_reach_into_the_logits(lib, change):  # noqa: F811
+    assert _call(lib, "dcr_process_logits", LOGITS, **change) == SHAPE
+
+
+@pytest.mark.parametrize("change", [
+    dict(), dict(out=P + 4 * 200), dict(dtype=BF16, out=P + 2 * 200), dict(out=P - 4 * 200),
+    dict(out=P, l_stride_b=200, o_stride_b=200), dict(out=P + 4 * 100, l_stride_b=200, o_stride_b=200),
+    dict(B=1, out=P, o_stride_b=7)], ids=str)
+def test_processed_logits_in_place_and_between_the_rows_pass(lib, change):  # noqa: F811
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("the addresses here are not to be followed")
+    assert _call(lib, "dcr_process_logits", dict(LOGITS, next_token=64 * P), **change) not in (SHAPE, ALIGN)

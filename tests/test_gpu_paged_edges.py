@@ -200,6 +200,24 @@ def test_evict_outputs_must_not_reach_into_inputs():
     assert torch.equal(got[2], want[2]) and _status() == 0
 
 
+def test_processed_logits_must_not_reach_into_the_logits():
+    from dcr_b200.kernel.cuda.logits import process_logits
+    flat = torch.randn(1000, generator=_gen(1), device=DEV)
+    x = flat[:400].view(4, 100)
+    for out in (flat[50:450].view(4, 100), flat[1:401].view(4, 100), flat[:800].view(4, 200)[:, :100]):
+        with pytest.raises(AssertionError):
+            process_logits(x, out=out)
+    with pytest.raises(AssertionError):
+        process_logits(flat[:100].expand(4, 100), out=x)
+    want, token = process_logits(x.clone())
+    wide = torch.zeros(4, 200, device=DEV)
+    wide[:, 100:] = x
+    got, t = process_logits(wide[:, 100:], out=wide[:, :100])
+    assert torch.equal(got, want) and torch.equal(t, token)
+    got, t = process_logits(x, out=x)
+    assert torch.equal(got, want) and torch.equal(t, token) and _status() == 0
+
+
 def _model(layers=2):
     from dcr_b200.models.llama.model import DCRLlamaDecoder, LlamaDecodeConfig
     cfg = LlamaDecodeConfig(vocab=512, hidden=256, intermediate=512, layers=layers, heads=4, kv_heads=2)
