@@ -291,6 +291,7 @@ extern "C" int dcr_paged_append(
       (pos != nullptr && (p_stride_b < 0 || p_stride_h < 0 ||
                           !rows_apart(n_seq, H_kv, max_slots, p_stride_b, p_stride_h))))
     return DCR_ERR_SHAPE;
+  if (rows_meet(q, q_stride_t, q_stride_h, q_out, T, H, D, 16 / per16)) return DCR_ERR_SHAPE;
   PagedAppendParams p;
   p.c = make_pool(k_pages, v_pages, kp_stride_p, kp_stride_h, kp_stride_s, vp_stride_p,
                   vp_stride_h, vp_stride_s, num_pages, page_size, page_table, table_stride,

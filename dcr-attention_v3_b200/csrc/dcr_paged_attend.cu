@@ -1091,6 +1091,7 @@ int dcr_paged_attend(const void* q, int64_t q_stride_b, int64_t q_stride_h, cons
   if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15u) ||
       workspace_bytes < w.total)
     return DCR_ERR_WORKSPACE;
+  if (rows_meet(q, q_stride_b, q_stride_h, o, B, H, D, 16 / per16)) return DCR_ERR_SHAPE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const int HB = pa_head_block(G, D, dtype);
   PagedAttendParams p;

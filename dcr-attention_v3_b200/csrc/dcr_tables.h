@@ -61,6 +61,15 @@ inline bool tables_meet(const TableSpan& a, const TableSpan& b) {
   return false;
 }
 
+// Whether contiguous output rows [n, heads, D] reach into the strided rows that they are computed
+// from. In place, row for row, is fine: a row is written after all reads of it.
+inline bool rows_meet(const void* from, int64_t stride_n, int64_t stride_h, const void* to, int64_t n,
+                      int64_t heads, int64_t D, int64_t element) {
+  if (from == to && (n <= 1 || stride_n == heads * D) && (heads <= 1 || stride_h == D)) return false;
+  return tables_meet(TableSpan(from, n, heads, D, stride_n, stride_h, element),
+                     TableSpan(to, n, heads, D, heads * D, D, element));
+}
+
 // Whether rows [B, V] processed into rows of other strides or another address would be read after
 // they are written. In place, row for row, is fine.
 inline bool logits_meet(const void* from, int64_t from_stride, const void* to, int64_t to_stride,

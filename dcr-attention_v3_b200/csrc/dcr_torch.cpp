@@ -182,6 +182,13 @@ at::Tensor output(PyObject* o, at::IntArrayRef shape, const at::TensorOptions& o
   return t;
 }
 
+// Refuses an output that reaches into the rows [tokens, heads, D] it is computed from.
+void check_apart(PyObject* out, const at::Tensor& o, const Rows& q, const Pool& p, int64_t tokens, int64_t heads) {
+  if (out != Py_None &&
+      dcr::rows_meet(q.data, q.st, q.sh, o.data_ptr(), tokens, heads, p.D, o.element_size()))
+    refuse("out must be q itself (contiguous) or share no memory with it");
+}
+
 // The caller's workspace (checked) or a fresh one from torch's allocator.
 at::Tensor scratch(PyObject* o, size_t bytes, int device) {
   if (o == Py_None)
@@ -237,6 +244,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const bool want_lse = truth != 0;
     const c10::cuda::OptionalCUDAGuard guard(p.k->device());
     const at::Tensor o = output(a[9], {B, H, p.D}, p.k->options());
+    check_apart(a[9], o, q, p, B, H);
     at::Tensor lse;
     if (want_lse) lse = at::empty({B, H}, p.k->options().dtype(at::kFloat));
     if (B > 0) {
@@ -295,6 +303,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Table pos = slot_table(a[15], "pos", at::kInt, p, p.slots);
     const c10::cuda::OptionalCUDAGuard guard(p.k->device());
     const at::Tensor o = output(a[16], {T, H, p.D}, p.k->options());
+    check_apart(a[16], o, q, p, T, H);
     if (T > 0) {
       const int st = dcr_paged_append(
           q.data, q.st, q.sh, k.data, k.st, k.sh, v.data, v.st, v.sh, qw, kw,

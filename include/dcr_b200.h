@@ -448,7 +448,8 @@ size_t dcr_paged_workspace_bytes(int B, int H, int H_kv, int D, int max_slots, i
  * log of the softmax denominators. weights (or NULL; fp32, weights[b * w_stride_b +
  * h_kv * w_stride_h + slot], max_pages * page_size slots) is increased by every slot's
  * softmax weight, summed over the KV head's query heads in a fixed order. A row with no valid
- * slot gets O = 0 and lse = -inf; a score of -inf counts as a masked slot. */
+ * slot gets O = 0 and lse = -inf; a score of -inf counts as a masked slot. O may be q itself
+ * where q is contiguous, else it shares no memory with it; so q_out of dcr_paged_append. */
 int dcr_paged_attend(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k_pages,
                      const void* v_pages, int dtype, int64_t k_stride_p, int64_t k_stride_h,
                      int64_t k_stride_s, int64_t v_stride_p, int64_t v_stride_h,

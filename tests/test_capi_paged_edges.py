@@ -4,8 +4,8 @@ test_capi_paged.py no pointer is followed."""
 from __future__ import annotations
 
 import pytest
-from test_capi_paged import (ALIGN, APPEND, ATTEND, B, BF16, EVICT, H_KV, LOGITS, MAX_PAGES, P, PAGE,
-                             SHAPE, _names, lib)  # noqa: F401
+from test_capi_paged import (ALIGN, APPEND, ATTEND, B, BF16, D, EVICT, H, H_KV, LOGITS, MAX_PAGES, P,
+                             PAGE, SHAPE, _names, lib)  # noqa: F401
 
 SLOTS = MAX_PAGES * PAGE  # 64 a row
 
@@ -114,3 +114,27 @@ def test_processed_logits_in_place_and_between_the_rows_pass(lib, change):  # no
     if torch.cuda.is_available():
         pytest.skip("the addresses here are not to be followed")
     assert _call(lib, "dcr_process_logits", dict(LOGITS, next_token=64 * P), **change) not in (SHAPE, ALIGN)
+
+
+ROWS = 2 * B * H * D  # bytes of a call's bf16 queries
+QKV = dict(q_stride_t=(H + 2 * H_KV) * D, k_stride_t=(H + 2 * H_KV) * D, v_stride_t=(H + 2 * H_KV) * D,
+           q=8 * P, k=8 * P + 2 * H * D, v=8 * P + 2 * (H + H_KV) * D)  # slices of packed rows
+
+
+@pytest.mark.parametrize("func,base,change,fits", [
+    ("dcr_paged_attend", ATTEND, dict(q=8 * P, o=8 * P), True),
+    ("dcr_paged_attend", ATTEND, dict(q=8 * P, o=8 * P + ROWS), True),
+    ("dcr_paged_attend", ATTEND, dict(q=8 * P, o=8 * P + 2 * D), False),
+    ("dcr_paged_attend", ATTEND, dict(q=8 * P, o=8 * P - 2 * D), False),
+    ("dcr_paged_attend", ATTEND, dict(q=8 * P, o=8 * P, q_stride_b=2 * H * D), False),
+    ("dcr_paged_attend", ATTEND, dict(q=8 * P, o=8 * P, q_stride_b=0), False),
+    ("dcr_paged_append", APPEND, dict(q=8 * P, q_out=8 * P, k=16 * P, v=32 * P), True),
+    ("dcr_paged_append", APPEND, dict(QKV, q_out=64 * P), True),
+    ("dcr_paged_append", APPEND, dict(QKV, q_out=8 * P), False),
+    ("dcr_paged_append", dict(APPEND, T=1), dict(QKV, q_out=8 * P), True)],
+    ids=lambda x: str(x) if isinstance(x, (str, bool)) else None)
+def test_outputs_that_reach_into_queries(lib, func, base, change, fits):  # noqa: F811
+    import torch
+    if fits and torch.cuda.is_available():
+        pytest.skip("the addresses here are not to be followed")
+    assert (_call(lib, func, base, **change) != SHAPE) == fits

@@ -218,6 +218,30 @@ def test_processed_logits_must_not_reach_into_the_logits():
     assert torch.equal(got, want) and torch.equal(t, token) and _status() == 0
 
 
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_attention_and_append_in_place_or_apart(dt):
+    from dcr_b200.kernel.cuda.paged import paged_append, paged_attention
+    lengths = [3000, 0, 17, 900]
+    k, v, table = ref.make_pool(lengths, 2, 16, 64, dt, DEV, _gen(5), garbage=0.0)
+    packed = torch.randn(4, 24, 64, generator=_gen(6), device=DEV).to(dt)
+    q = packed[:, :20].contiguous()
+    x = q.clone()
+    want = paged_attention(q, k, v, table, _i32(lengths))
+    assert paged_attention(x, k, v, table, _i32(lengths), out=x) is x and torch.equal(x, want)
+    cos = torch.rand(64, 64, generator=_gen(7), device=DEV).to(dt)
+    append = lambda x, **kw: paged_append(x, packed[:, 20:22], packed[:, 22:], cos, cos, _i32([1, 2, 3, 4]),  # noqa: E731
+                                          k, v, table, _i32([7, -1, 7, 7]), q_weight=cos[0], **kw)
+    turned = append(q)
+    into = packed.view(-1)[:4 * 20 * 64].view(4, 20, 64)  # contiguous, over the packed rows
+    for call in (lambda: paged_attention(packed[:, :20], k, v, table, _i32(lengths), out=into),
+                 lambda: append(packed[:, :20], out=into)):
+        with pytest.raises(AssertionError, match="memory"):
+            call()
+    x = q.clone()
+    assert append(x, out=x) is x and torch.equal(x, turned)
+    assert _status() == 0
+
+
 def _model(layers=2):
     from dcr_b200.models.llama.model import DCRLlamaDecoder, LlamaDecodeConfig
     cfg = LlamaDecodeConfig(vocab=512, hidden=256, intermediate=512, layers=layers, heads=4, kv_heads=2)
