@@ -22,8 +22,7 @@
 // size that registers cannot hold is read again at every level. Kernel 2 (a programmatic
 // dependent) pairs the i-th hole with the i-th mover and copies the rows, 16 bytes a lane. Up to
 // kEvFew evictions a row, a decode step's steady state, are found one by one as the smallest claim
-// left and moved by the first kernel itself (64 rows of 4917 slots, one to go: 7.9 instead of 11.4
-// us). Measured: 32 rows of 32768 slots to 4916, 134,000 rows of 128 bytes moved in K and in V: 29.6
+// left and moved by the first kernel itself. Measured: 32 rows of 32768 slots to 4916, 134,000 rows of 128 bytes moved in K and in V: 29.6
 // us a call, 2.7 TB/s of the 79 MB it cannot do without.
 #include <cooperative_groups.h>
 
@@ -37,7 +36,10 @@ namespace cg = cooperative_groups;
 constexpr int kEvThreads = 1024;
 constexpr int kEvWarps = kEvThreads / 32;
 constexpr int kEvBins = 4096;
-constexpr int kEvFew = 4;  // evictions that are taken one by one
+// Evictions that are taken one by one. One by one / by the histograms, for 1, 2, 3 and 4 of them: 64
+// rows of 4917 slots 7.4 / 10.8, 9.2 / 10.8, 11.2 / 11.0, 12.8 / 11.2 us; 256 rows of 1025 8.2 / 11.4,
+// 10.2 / 11.5, 12.5 / 11.5, 14.3 / 11.5; 32 rows of 20001 8.8 / 13.3, 11.7 / 13.8, 14.2 / 13.8, 16.3 / 13.8.
+constexpr int kEvFew = 2;
 constexpr int kEvAllBins = kEvBins + 2048;  // of the three levels
 
 struct PagedEvictParams {
