@@ -59,11 +59,16 @@ cudaError_t launch_cluster(Kernel kernel, dim3 grid, dim3 block, size_t smem, cu
 
 // Launches a kernel as a programmatic dependent of the one before it on the stream (with
 // cluster > 1, as clusters of that many CTAs): its CTAs may be placed while that kernel drains.
-// Every such kernel begins with griddepcontrol.wait in all its threads, before it reads or
-// writes anything a kernel before it may touch; so kernels of a stream still follow one another,
-// whatever came before, and only the launch itself overlaps. They read what others may have
-// written by plain loads: a read-only (non-coherent) load promises that nothing writes the data
-// while the kernel exists, and it exists before its predecessor is done.
+// The first kernel of a call waits (griddepcontrol.wait) in all its threads before it reads or
+// writes anything a kernel before it may touch, and lets its dependents start
+// (griddepcontrol.launch_dependents) only after that; so calls of a stream follow one another,
+// whatever came before, and only the launch itself overlaps. A later kernel of the call may read
+// ahead of its own wait what no kernel of the call writes (lengths, page tables, the weights that
+// it will add to): it starts when the first one has passed its wait, so all that came before the
+// call is complete. At least one of its CTAs waits for the kernel before it, so that it does not
+// end earlier. What others may have written is read by plain loads: a read-only (non-coherent)
+// load promises that nothing writes the data while the kernel exists, and it exists before its
+// predecessor is done.
 template <typename... Args>
 cudaError_t launch_dependent(void (*kernel)(Args...), dim3 grid, dim3 block, size_t smem,
                              cudaStream_t st, int cluster, Args... args) {

@@ -719,6 +719,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const Paged
   __shared__ PaPiece pieces[2 * kPaWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  // not before the wait: the call's other kernels read lengths and weights ahead of their own
   asm volatile("griddepcontrol.launch_dependents;");
   uint8_t* ring = pa_smem + warp * (S::NH * S::kHalf);
   uint8_t* own = pa_smem + kPaWarps * (S::NH * S::kHalf) + warp * (S::kPiece + S::kQ + S::kP + 64);

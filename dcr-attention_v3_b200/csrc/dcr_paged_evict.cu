@@ -119,6 +119,7 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_select_kernel(const Pa
   const int rank = static_cast<int>(cluster.block_rank());
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  // not before the wait: the second kernel reads the page table ahead of its own
   asm volatile("griddepcontrol.launch_dependents;");
   const int64_t row = blockIdx.x / C;
   const int b = static_cast<int>(row / p.H_kv), h = static_cast<int>(row - static_cast<int64_t>(b) * p.H_kv);
