@@ -26,12 +26,16 @@
 // A vector is looked at for the best token only if its maximum reaches the CTA's so far; the
 // CTAs' best tokens meet in CTA 0.
 //
-// Measured (calls back to back): 128 rows of 128256 fp32 logits, 131 MB: 24.7 us with 16 tokens of
-// history (5.3 TB/s), 31.4 us with 6144 on average, 39.3 us with a bias and a mask too (3.5 TB/s);
-// one bf16 row with 1000 tokens of history 9.3 us, of which 3 us are the history's phases and 3 us
-// the launch and the cluster's barriers. Counts of all tokens in shared memory (a slice of 16032
-// tokens a CTA) took 78 us for the first case with bias, mask and history; finishing the marked
-// tokens by all warps before the stream 50.9 us.
+// Measured (calls back to back on three sets of logits and two outputs in turn): 128 rows of 128256
+// fp32 logits, 131 MB: 27.8 us with 16 tokens of history (4.7 TB/s), 39.5 us with 6144 on average;
+// a bias adds 3.4 to 4.0 us, a mask 0.4 to 0.8, both with that history 43.1 us (3.2 TB/s). In bf16,
+// 66 MB: 20.5 us, 28.7 us with the history, 31.8 with the bias, 42.9 with history, bias and mask:
+// there the bias, of twice the logits' bytes, costs 11 to 13 us (0.58 instructions a scheduler's
+// cycle, two vectors of 48 bytes in flight a thread). One bf16 row with 1000 tokens of history 8.9
+// us, of which 3 us are the history's phases and 3 us the launch and the cluster's barriers. Counts
+// of all tokens in shared memory (a slice of 16032 tokens a CTA) took 78 us for the first case with
+// bias, mask and history, finishing the marked tokens by all warps before the stream 50.9 us, both
+// with one output used again and again (part of it stays in L2), where the kept form takes 39.0.
 #include <cooperative_groups.h>
 #include <math.h>
 

@@ -19,8 +19,8 @@
 // key, value): the token's table rows times the norm weights are folded into two factors once,
 // x' = rs * (x * (w c) + x_far * (w_far s)), and all its rows are in flight before the first is
 // used. Rows are read and written once, as streaming accesses (77.3 us without the hint on both
-// sides, 70.0 with it). Measured: 16381 tokens of 32 + 2 x 8 heads of 128 in f16, 404 MB, in 70.0
-// us, 5.77 TB/s, 88% of the measured copy bandwidth; a warp that took a whole token, the next rows
+// sides, 70.0 with it). Measured: 16381 tokens of 32 + 2 x 8 heads of 128 in f16, 404 MB, in 69 to 73
+// us by run, 5.5 to 5.9 TB/s, 84 to 90% of the measured copy bandwidth; a warp that took a whole token, the next rows
 // on their way meanwhile, needed 126 registers and 83 us.
 #include <type_traits>
 

@@ -40,7 +40,7 @@
 // the stream at 7 TB/s, 4 us its beginning (lengths, page table, first rows) and 5 us the folds; 48
 // sequences of 0 to 16000 slots, f16 (747 MB): 120 us, 6.2 TB/s; 16 x 8 heads of 128 in a window of
 // 8191, bf16 (537 MB): 92 us, 5.8 TB/s; 3 x 16 heads over 8195 slots in fp32 (201 MB): 38 us, 5.3
-// TB/s; 8 x 8 heads over 16385 slots with weights (277 MB): 58.7 us; one sequence of 1000: 7.8 us.
+// TB/s; 8 x 8 heads over 16385 slots with weights (277 MB): 58.7 us; one sequence of 1000: 7.6 us.
 // Tiles of 2 KB instead of 4 needed 453 instead of 261 instructions per 16 slots (66.8 instead of
 // 51.7 us for the first case at that step).
 #include <math.h>
@@ -244,8 +244,10 @@ __device__ __forceinline__ PaCursor pa_seek(const PagedAttendParams& p, const Pa
 
 // The copies of one tile: K's rows, then V's. Where pages hold whole groups of 16 slots (or R,
 // if that is less) a page is looked up per group and its rows are a fixed stride apart;
-// otherwise every row is looked up. Slots that are not valid are filled with zeros: a copy of
-// no bytes reads nothing, whatever its address.
+// otherwise every row is looked up by itself, one after the other, which makes the first case
+// above 128 us with pages of 8 and 125 with pages of 24 (47 with 16 or 64), the fp32 case 90 with
+// pages of 4, 8 or 12 (38). Slots that are not valid are filled with zeros: a copy of no bytes
+// reads nothing, whatever its address.
 template <typename T, int D, int HB>
 struct PaLoader {
   using S = PaShape<T, D, HB>;

@@ -22,8 +22,9 @@
 // size that registers cannot hold is read again at every level. Kernel 2 (a programmatic
 // dependent) pairs the i-th hole with the i-th mover and copies the rows, 16 bytes a lane. Up to
 // kEvFew evictions a row, a decode step's steady state, are found one by one as the smallest claim
-// left and moved by the first kernel itself. Measured: 32 rows of 32768 slots to 4916, 134,000 rows of 128 bytes moved in K and in V: 29.6
-// us a call, 2.7 TB/s of the 79 MB it cannot do without.
+// left and moved by the first kernel itself. Measured: 32 rows of 32768 slots to 4916, 134,000 rows
+// of 128 bytes moved in K and in V: 30.0 us a call, 2.6 TB/s of the 79 MB it cannot do without; 64 rows
+// of 4917 slots, one to go: 7.7 us.
 #include <cooperative_groups.h>
 
 #include "dcr_internal.h"
