@@ -66,15 +66,16 @@ struct PagedAttendParams {
   const void* q;
   int64_t qsb, qsh;
   const int32_t* lengths;
+  const int32_t* prefix;  // Own: sequence b's first prefix[b] slots are attended elsewhere
   int B, H, H_kv, G;
   int units;      // per sequence: H_kv * blocks of query heads
   int hblocks;    // blocks of query heads per KV head
   float scale2;   // scale * log2(e)
   int window;
   int page16;     // page_size is a multiple of a group: a group lies in one page
-  void* o;        // [B][H][D]
+  void* o;        // [B][H][D] (Own: fp32)
   float* lse;     // [B][H] natural log, or null
-  float2* stats;  // [B][H] (base of the exponents, 1 / sum), with scores
+  float2* stats;  // [B][H] (base of the exponents, 1 / sum), with scores and with Own
   float* part;    // [CTAs][2][HB][D + 2]: o, m, l of the open units
   float* scores;  // [B][H][s_stride] base-2 scores, or null
   int64_t s_stride;
@@ -140,12 +141,18 @@ __device__ __forceinline__ void pa_store2(T* dst, float a, float b) {
     *reinterpret_cast<__nv_bfloat162*>(dst) = __floats2bfloat162_rn(a, b);
 }
 
-// Tiles of sequence b: its length, first valid slot and tile range.
-template <int R>
+// fp32 output pairs, for the part that is joined with others before it is rounded.
+__device__ __forceinline__ void pa_store2(float* dst, float a, float b) {
+  *reinterpret_cast<float2*>(dst) = make_float2(a, b);
+}
+
+// Tiles of sequence b: its length, first valid slot and tile range. Own: without the prefix.
+template <int R, bool Own>
 __device__ __forceinline__ void pa_sequence(const PagedAttendParams& p, int b, int& len, int& lo,
                                             int& t_lo, int& t_hi) {
   len = checked_length(p.c, p.lengths[b]);
   lo = p.window > 0 && len > p.window ? len - p.window : 0;
+  if constexpr (Own) lo = max(lo, min(p.prefix[b], len));
   t_lo = lo / R;
   t_hi = (len + R - 1) / R;
 }
@@ -155,14 +162,14 @@ struct PaCursor {
   int b, u, t, t_lo, t_hi, len, lo;
 };
 
-template <int R>
+template <int R, bool Own>
 __device__ __forceinline__ void pa_next(const PagedAttendParams& p, PaCursor& c) {
   if (++c.t < c.t_hi) return;
   if (++c.u == p.units) {
     c.u = 0;
     do {
       if (++c.b >= p.B) return;  // past the end: the caller's count stops here
-      pa_sequence<R>(p, c.b, c.len, c.lo, c.t_lo, c.t_hi);
+      pa_sequence<R, Own>(p, c.b, c.len, c.lo, c.t_lo, c.t_hi);
     } while (c.t_lo >= c.t_hi);
   }
   c.t = c.t_lo;
@@ -188,7 +195,7 @@ struct PaLine {
   }
 };
 
-template <int R>
+template <int R, bool Own>
 __device__ __forceinline__ PaLine pa_line(const PagedAttendParams& p, int ctas) {
   const int lane = threadIdx.x & 31;
   PaLine a;
@@ -199,7 +206,7 @@ __device__ __forceinline__ PaLine pa_line(const PagedAttendParams& p, int ctas) 
     const int b = lane * a.per + j;
     if (b < p.B) {
       int len, lo, t_lo, t_hi;
-      pa_sequence<R>(p, b, len, lo, t_lo, t_hi);
+      pa_sequence<R, Own>(p, b, len, lo, t_lo, t_hi);
       a.upto += t_hi - t_lo;
     }
   }
@@ -217,7 +224,7 @@ __device__ __forceinline__ PaLine pa_line(const PagedAttendParams& p, int ctas) 
 }
 
 // The cursor at place s (< total) of the line.
-template <int R>
+template <int R, bool Own>
 __device__ __forceinline__ PaCursor pa_seek(const PagedAttendParams& p, const PaLine& line,
                                             int64_t s) {
   const unsigned hit = __ballot_sync(0xffffffffu, s < line.upto * p.units);
@@ -226,14 +233,14 @@ __device__ __forceinline__ PaCursor pa_seek(const PagedAttendParams& p, const Pa
   before = l > 0 ? before * p.units : 0;
   PaCursor c;
   c.b = l * line.per;
-  pa_sequence<R>(p, c.b, c.len, c.lo, c.t_lo, c.t_hi);
+  pa_sequence<R, Own>(p, c.b, c.len, c.lo, c.t_lo, c.t_hi);
 #pragma unroll 1
   while (c.b + 1 < p.B) {
     const int64_t tiles = static_cast<int64_t>(c.t_hi - c.t_lo) * p.units;
     if (s < before + tiles) break;
     before += tiles;
     ++c.b;
-    pa_sequence<R>(p, c.b, c.len, c.lo, c.t_lo, c.t_hi);
+    pa_sequence<R, Own>(p, c.b, c.len, c.lo, c.t_lo, c.t_hi);
   }
   const int nt = c.t_hi - c.t_lo;
   const int64_t off = s - before;
@@ -508,6 +515,7 @@ struct PaState16 {
     }
   }
 
+  template <typename TO>
   __device__ __forceinline__ void write(const PagedAttendParams& p, const PaCursor& c) const {
     const int lane = threadIdx.x & 31;
     const int hk = c.u / p.hblocks;
@@ -517,7 +525,7 @@ struct PaState16 {
       if (g >= p.G) continue;
       const int64_t row = static_cast<int64_t>(c.b) * p.H + hk * p.G + g;
       const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
-      T* out = static_cast<T*>(p.o) + row * D + 2 * (lane & 3);
+      TO* out = static_cast<TO*>(p.o) + row * D + 2 * (lane & 3);
 #pragma unroll
       for (int j = 0; j < D / 8; ++j)
         pa_store2(out + 8 * j, o[j][2 * i] * inv, o[j][2 * i + 1] * inv);
@@ -678,6 +686,7 @@ struct PaState32 {
       for (int off = 16; off >= 1; off >>= 1) l[g] += __shfl_xor_sync(0xffffffffu, l[g], off);
   }
 
+  template <typename TO>
   __device__ __forceinline__ void write(const PagedAttendParams& p, const PaCursor& c) const {
     const int lane = threadIdx.x & 31;
     const int hk = c.u / p.hblocks;
@@ -713,9 +722,12 @@ struct PaPiece {
   int before, after;
 };
 
-template <typename T, int D, int HB>
+// Own: only the slots past each sequence's prefix, into fp32 rows and their statistics, which
+// are joined with the prefix's afterwards.
+template <typename T, int D, int HB, bool Own>
 __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const PagedAttendParams p) {
   using S = PaShape<T, D, HB>;
+  using TO = typename std::conditional<Own, float, T>::type;
   using State = typename std::conditional<S::k16, PaState16<T, D, HB>, PaState32<T, D, HB>>::type;
   extern __shared__ __align__(128) uint8_t pa_smem[];
   __shared__ PaPiece pieces[2 * kPaWarps];
@@ -729,7 +741,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const Paged
   uint8_t* extra = own + S::kPiece;                       // fp32: queries and weights
   uint32_t* masks = reinterpret_cast<uint32_t*>(own + S::kPiece + S::kQ + S::kP);  // [16]
 
-  const PaLine line = pa_line<S::R>(p, gridDim.x);
+  const PaLine line = pa_line<S::R, Own>(p, gridDim.x);
   const bool works = static_cast<int>(blockIdx.x) < line.ctas;
   const int64_t c0 = line.begin(blockIdx.x);
   const int n_cta = works ? static_cast<int>(line.each) + (static_cast<int>(blockIdx.x) < line.more) : 0;
@@ -739,7 +751,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const Paged
   if (lane == 0) pieces[2 * warp].u = pieces[2 * warp + 1].u = -1;
 
   if (n > 0) {
-    PaCursor in = pa_seek<S::R>(p, line, s0);  // where loads are
+    PaCursor in = pa_seek<S::R, Own>(p, line, s0);  // where loads are
     PaCursor at = in;                          // where the arithmetic is
     PaLoader<T, D, HB> load;
     State st;
@@ -769,7 +781,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const Paged
       }
       if (j < n) {
         load.values(p, ring + hs_in * S::kHalf);
-        if (j + 1 < n) pa_next<S::R>(p, in);
+        if (j + 1 < n) pa_next<S::R, Own>(p, in);
       }
       cp_async_commit();
       hs_in = hs_in + 1 == S::NH ? 0 : hs_in + 1;
@@ -781,7 +793,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const Paged
         st.close();
         const bool before = first > at.t_lo;
         if (!before && ends) {
-          st.write(p, at);
+          st.template write<TO>(p, at);
         } else {
           // before: the only piece that can be followed by others, so it has its own place;
           // a piece that goes on after the share is the last, and the ring is free then
@@ -801,7 +813,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const Paged
           }
         }
         if (i + 1 < n) {
-          pa_next<S::R>(p, at);
+          pa_next<S::R, Own>(p, at);
           first = at.t;
           st.begin(p, at, extra);
         }
@@ -862,7 +874,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const Paged
         const float inv = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
         for (int e = 0; e < D / 32; ++e)
-          ElemTraits<T>::store(static_cast<T*>(p.o) + row * D, lane + 32 * e, acc[e] * inv);
+          ElemTraits<TO>::store(static_cast<TO*>(p.o) + row * D, lane + 32 * e, acc[e] * inv);
         if (lane == 0) pa_store_stats(p, row, M, L);
       } else {
         float* dst = p.part + ((2 * static_cast<int64_t>(blockIdx.x) + (before ? 0 : 1)) * HB + g) * (D + 2);
@@ -881,11 +893,11 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const Paged
 #pragma unroll 1
   for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
     int len, lo, t_lo, t_hi;
-    pa_sequence<S::R>(p, b, len, lo, t_lo, t_hi);
+    pa_sequence<S::R, Own>(p, b, len, lo, t_lo, t_hi);
     if (t_lo < t_hi) continue;
     const int64_t row0 = static_cast<int64_t>(b) * p.H;
     for (int i = threadIdx.x; i < p.H * D; i += kPaThreads)
-      ElemTraits<T>::store(static_cast<T*>(p.o) + row0 * D, i, 0.0f);
+      ElemTraits<TO>::store(static_cast<TO*>(p.o) + row0 * D, i, 0.0f);
     for (int i = threadIdx.x; i < p.H; i += kPaThreads) pa_store_stats(p, row0 + i, 0.0f, 0.0f);
   }
 }
@@ -898,20 +910,21 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attend_kernel(const Paged
 // the first: the kernel must not end before the one it waits for.)
 constexpr int kFoldThreads = 128, kFoldParts = 32;
 
-template <typename T, int D, int HB>
+template <typename T, int D, int HB, bool Own>
 __global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const PagedAttendParams p) {
   using S = PaShape<T, D, HB>;
+  using TO = typename std::conditional<Own, float, T>::type;
   constexpr int W = D + 2;              // o, m, l
   __shared__ __align__(8) float part[kFoldParts * W];
   asm volatile("griddepcontrol.launch_dependents;");
-  const PaLine line = pa_line<S::R>(p, gridDim.x);
+  const PaLine line = pa_line<S::R, Own>(p, gridDim.x);
   const int c0 = blockIdx.x;
   const int64_t end_cta = line.begin(c0 + 1);
   bool open = c0 + 1 < line.ctas;
   PaCursor c;
   int last = 0, hk = 0, h = 0;
   if (open) {
-    c = pa_seek<S::R>(p, line, end_cta - 1);
+    c = pa_seek<S::R, Own>(p, line, end_cta - 1);
     const int64_t begin = end_cta - 1 - (c.t - c.t_lo), end = begin + (c.t_hi - c.t_lo);
     hk = c.u / p.hblocks;
     h = (c.u - hk * p.hblocks) * HB + blockIdx.y;
@@ -957,7 +970,7 @@ __global__ void __launch_bounds__(kFoldThreads) paged_fold_kernel(const PagedAtt
   }
   if (d >= D) return;
   const int64_t row = static_cast<int64_t>(c.b) * p.H + hk * p.G + h;
-  ElemTraits<T>::store(static_cast<T*>(p.o) + row * D, d, L == 0.0f ? 0.0f : acc / L);
+  ElemTraits<TO>::store(static_cast<TO*>(p.o) + row * D, d, L == 0.0f ? 0.0f : acc / L);
   if (d == 0) pa_store_stats(p, row, M, L);
 }
 
@@ -1029,28 +1042,37 @@ static PagedAttendLayout pa_layout(int B, int H, int G, int D, int max_slots, bo
   return w;
 }
 
-template <typename T, int D, int HB>
+template <typename T, int D, int HB, bool Own>
 static int pa_launch(const PagedAttendParams& p, int ctas, cudaStream_t s) {
   using S = PaShape<T, D, HB>;
-  auto kernel = paged_attend_kernel<T, D, HB>;
+  auto kernel = paged_attend_kernel<T, D, HB, Own>;
   if (ensure_smem_attr(reinterpret_cast<const void*>(kernel), S::kSmem) != cudaSuccess)
     return DCR_ERR_CUDA;
   PagedAttendParams q = p;
   q.page16 = p.c.page.d % S::kGroup == 0;
   const int rows = p.G < HB ? p.G : HB;
   if (launch_dependent(kernel, dim3(ctas), dim3(kPaThreads), S::kSmem, s, 1, q) != cudaSuccess ||
-      launch_dependent(paged_fold_kernel<T, D, HB>, dim3(ctas, rows), dim3(kFoldThreads), 0, s, 1, q) != cudaSuccess)
+      launch_dependent(paged_fold_kernel<T, D, HB, Own>, dim3(ctas, rows), dim3(kFoldThreads), 0, s, 1, q) != cudaSuccess)
     return DCR_ERR_CUDA;
   return DCR_OK;
 }
 
-template <typename T>
+template <typename T, bool Own>
 static int pa_launch_t(const PagedAttendParams& p, int D, int HB, int ctas, cudaStream_t s) {
-  if (D == 64) return HB == 8 ? pa_launch<T, 64, 8>(p, ctas, s) : pa_launch<T, 64, 16>(p, ctas, s);
+  if (D == 64) return HB == 8 ? pa_launch<T, 64, 8, Own>(p, ctas, s) : pa_launch<T, 64, 16, Own>(p, ctas, s);
   if constexpr (sizeof(T) == 2) {
-    if (HB == 16) return pa_launch<T, 128, 16>(p, ctas, s);
+    if (HB == 16) return pa_launch<T, 128, 16, Own>(p, ctas, s);
   }
-  return pa_launch<T, 128, 8>(p, ctas, s);
+  return pa_launch<T, 128, 8, Own>(p, ctas, s);
+}
+
+template <bool Own>
+static int pa_launch_any(const PagedAttendParams& p, int dtype, int D, int HB, int ctas, cudaStream_t s) {
+  switch (dtype) {
+    case DCR_DTYPE_BF16: return pa_launch_t<__nv_bfloat16, Own>(p, D, HB, ctas, s);
+    case DCR_DTYPE_F16: return pa_launch_t<__half, Own>(p, D, HB, ctas, s);
+    default: return pa_launch_t<float, Own>(p, D, HB, ctas, s);
+  }
 }
 
 }  // namespace dcr
@@ -1104,6 +1126,7 @@ int dcr_paged_attend(const void* q, int64_t q_stride_b, int64_t q_stride_h, cons
   p.qsb = q_stride_b;
   p.qsh = q_stride_h;
   p.lengths = lengths;
+  p.prefix = nullptr;
   p.B = B;
   p.H = H;
   p.H_kv = H_kv;
@@ -1120,12 +1143,7 @@ int dcr_paged_attend(const void* q, int64_t q_stride_b, int64_t q_stride_h, cons
   p.scores = weights != nullptr ? reinterpret_cast<float*>(ws + w.scores) : nullptr;
   p.s_stride = w.s_stride;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int rc;
-  switch (dtype) {
-    case DCR_DTYPE_BF16: rc = pa_launch_t<__nv_bfloat16>(p, D, HB, w.ctas, s); break;
-    case DCR_DTYPE_F16: rc = pa_launch_t<__half>(p, D, HB, w.ctas, s); break;
-    default: rc = pa_launch_t<float>(p, D, HB, w.ctas, s); break;
-  }
+  const int rc = pa_launch_any<false>(p, dtype, D, HB, w.ctas, s);
   if (rc != DCR_OK || weights == nullptr) return rc;
   const int chunk = kWeightThreads * kWeightSlots;
   const dim3 grid((max_slots + chunk - 1) / chunk, H_kv, B < 65535 ? B : 65535);

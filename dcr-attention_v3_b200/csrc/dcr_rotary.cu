@@ -1,0 +1,515 @@
+// dcr_rotary.cu — position rotation of query and key heads from frequencies, in place or into other
+// rows, or with the append of keys and values into a paged cache (sm_100a).
+//
+// For token t at position x_t and frequency i < r / 2 (r rotated elements a row, the first ones):
+//   a = x_t * inv_freq[i],  c = factor * cos a,  s = factor * sin a
+//   (u, w) -> (u c - w s, w c + u s)   for the elements (i, i + r/2), or (2i, 2i + 1) interleaved
+// and elements r.. stay as they are. Scaling for long contexts is in the frequencies and the
+// factor. With norm weights (the paged form) every row is first x * rsqrt(mean(x^2) + eps) * weight.
+// All in fp32 from the stored inputs, rounded once. The angle is taken in turns in 64 bits, x_t *
+// (inv_freq / 2 pi) less its nearest integer, so a position of 2^31 loses 2^-22 of a turn at most and
+// one of a million 2^-33; an fp32 product would be off by a hundredth of a turn there. The
+// reference's step is HF apply_rotary_pos_emb from tables (dcr_attention/models/llama/attention.py:395);
+// layouts, parts of a head, pages and norms have no counterpart there.
+//
+// Bound: the rows, read and written once. A CTA takes a few tokens: their angles, once for all heads,
+// go to shared memory while the first rows are on their way. A lane takes two 16-byte chunks that
+// hold whole pairs: chunks r/2 elements apart, or neighbours. Where r is not a multiple of two chunks
+// a warp takes a row element by element.
+#include <type_traits>
+
+#include "dcr_internal.h"
+#include "dcr_paged.cuh"
+
+namespace dcr {
+
+struct RotaryParams {
+  const void* q;
+  const void* k;
+  const void* v;             // paged
+  int64_t qst, qsh, kst, ksh, vst, vsh;
+  void* q_out;
+  void* k_out;               // not paged
+  int64_t qost, qosh, kost, kosh;
+  const float* inv_freq;     // [rot / 2]
+  const void* positions;     // [T] int32 or int64
+  int wide;                  // positions are int64
+  int interleaved;
+  int T, H, H_kv, D, rot;
+  int parts;                 // items (two chunks) of a row: all of it, or its rotated part in place
+  int per_cta;               // tokens a CTA
+  float factor;
+  // paged
+  PagePool c;
+  void* k_pages;
+  void* v_pages;
+  const int32_t* seq;
+  const int32_t* slots;
+  int n_seq;
+  const void* qw;
+  const void* kw;
+  float eps;
+  float* weights;
+  int64_t wsb, wsh;
+  int32_t* pos;
+  int64_t psb, psh;
+};
+
+constexpr int kRoThreads = 128;
+constexpr int kRoSteps = 3;        // items a thread has in flight
+constexpr int kRoMaxTokens = 16;   // tokens a CTA at most
+constexpr int kRoMaxDim = 512;
+
+// Where a token's key and value go.
+struct RotaryPlace {
+  int64_t k, v;   // element offsets of head 0's row
+  int b, slot;    // slot < 0: nowhere
+  int64_t position;
+};
+
+template <typename T>
+__device__ __forceinline__ uint4 ro_round(const float (&f)[ElemTraits<T>::kPerChunk]) {
+  float2 x[ElemTraits<T>::kPerChunk / 2];
+#pragma unroll
+  for (int e = 0; e < ElemTraits<T>::kPerChunk / 2; ++e) x[e] = make_float2(f[2 * e], f[2 * e + 1]);
+  return ap_round<T>(x);
+}
+
+template <bool Paged>
+__device__ __forceinline__ RotaryPlace ro_place(const RotaryParams& p, int t) {
+  RotaryPlace r;
+  r.position = p.wide ? static_cast<const int64_t*>(p.positions)[t]
+                      : static_cast<const int32_t*>(p.positions)[t];
+  r.k = r.v = 0;
+  r.b = 0;
+  r.slot = -1;
+  if constexpr (Paged) {
+    const int slot = p.slots[t];
+    if (slot < 0) return r;
+    const int b = p.seq != nullptr ? p.seq[t] : t;
+    int pg = -1;
+    uint32_t pi = 0;
+    if (b >= 0 && b < p.n_seq && slot < p.c.max_pages * static_cast<int>(p.c.page.d)) {
+      pi = p.c.page.div(slot);
+      pg = page_of(p.c, b, pi);
+    }
+    if (pg < 0) {  // no such place, or not mapped: the row would be lost
+      raise_status(DCR_ERR_DEVICE_INDEX);
+      return r;
+    }
+    const int64_t in = slot - static_cast<int>(pi * p.c.page.d);
+    r.k = pg * p.c.ksp + in * p.c.ksr;
+    r.v = pg * p.c.vsp + in * p.c.vsr;
+    r.b = b;
+    r.slot = slot;
+  }
+  return r;
+}
+
+// cos and sin of every token of the CTA, times the factor.
+__device__ __forceinline__ void ro_angles(const RotaryParams& p, const RotaryPlace* place, int tokens,
+                                          float2* turn) {
+  const int half = p.rot / 2;
+  for (int i = threadIdx.x; i < tokens * half; i += kRoThreads) {
+    const int t = i / half, f = i - t * half;
+    const double turns = static_cast<double>(place[t].position) *
+                         (static_cast<double>(p.inv_freq[f]) * 0.15915494309189533577);
+    float s, c;
+    sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
+    turn[i] = make_float2(c * p.factor, s * p.factor);
+  }
+}
+
+// A row's source and destination.
+template <typename T, bool Paged>
+__device__ __forceinline__ const T* ro_source(const RotaryParams& p, int t, int row) {
+  if (row < p.H) return static_cast<const T*>(p.q) + t * p.qst + row * p.qsh;
+  if (!Paged || row < p.H + p.H_kv) return static_cast<const T*>(p.k) + t * p.kst + (row - p.H) * p.ksh;
+  return static_cast<const T*>(p.v) + t * p.vst + (row - p.H - p.H_kv) * p.vsh;
+}
+
+template <typename T, bool Paged>
+__device__ __forceinline__ T* ro_target(const RotaryParams& p, const RotaryPlace& at, int t, int row) {
+  if (row < p.H) return static_cast<T*>(p.q_out) + t * p.qost + row * p.qosh;
+  if constexpr (Paged) {
+    if (at.slot < 0) return nullptr;
+    return row < p.H + p.H_kv ? static_cast<T*>(p.k_pages) + at.k + (row - p.H) * p.c.ksh
+                              : static_cast<T*>(p.v_pages) + at.v + (row - p.H - p.H_kv) * p.c.vsh;
+  } else {
+    return static_cast<T*>(p.k_out) + t * p.kost + (row - p.H) * p.kosh;
+  }
+}
+
+// The two chunks of item i of a row.
+__device__ __forceinline__ int2 ro_chunks(const RotaryParams& p, int i, int n) {
+  const int turned = p.rot / (2 * n);
+  if (i < turned && !p.interleaved) return make_int2(i, i + turned);
+  return make_int2(2 * i, 2 * i + 1);
+}
+
+template <typename T, bool Paged>
+__global__ void __launch_bounds__(kRoThreads) rotary_kernel(const RotaryParams p) {
+  constexpr int N = ElemTraits<T>::kPerChunk;
+  extern __shared__ __align__(16) float2 ro_turn[];
+  __shared__ RotaryPlace place[kRoMaxTokens];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int t0 = blockIdx.x * p.per_cta;
+  const int tokens = min(p.per_cta, p.T - t0);
+  const int rows = p.H + (Paged ? 2 : 1) * p.H_kv;
+  const int total = tokens * rows * p.parts;
+  uint4 x[kRoSteps][2];
+  auto load = [&](int first) {
+#pragma unroll
+    for (int i = 0; i < kRoSteps; ++i) {
+      const int item = first + i * kRoThreads;
+      if (item < total) {
+        const int part = item % p.parts, row = item / p.parts % rows, t = item / (p.parts * rows);
+        const uint4* src = reinterpret_cast<const uint4*>(ro_source<T, Paged>(p, t0 + t, row));
+        const int2 ch = ro_chunks(p, part, N);
+        x[i][0] = __ldcs(src + ch.x);
+        x[i][1] = __ldcs(src + ch.y);
+      } else {
+        x[i][0] = x[i][1] = make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+  };
+  load(threadIdx.x);
+  if (threadIdx.x < tokens) place[threadIdx.x] = ro_place<Paged>(p, t0 + threadIdx.x);
+  __syncthreads();
+  ro_angles(p, place, tokens, ro_turn);
+  __syncthreads();
+#pragma unroll 1
+  for (int first = threadIdx.x; first - static_cast<int>(threadIdx.x) < total;
+       first += kRoSteps * kRoThreads) {
+    if (first != static_cast<int>(threadIdx.x)) load(first);
+#pragma unroll
+    for (int i = 0; i < kRoSteps; ++i) {
+      const int item = first + i * kRoThreads;
+      const bool in = item < total;
+      const int part = item % p.parts, row = in ? item / p.parts % rows : 0;
+      const int t = in ? item / (p.parts * rows) : 0;
+      const int2 ch = ro_chunks(p, part, N);
+      const bool value = Paged && row >= p.H + p.H_kv;
+      float f[2][N];
+      ElemTraits<T>::widen(x[i][0], f[0]);
+      ElemTraits<T>::widen(x[i][1], f[1]);
+      const void* w = Paged && !value ? (row < p.H ? p.qw : p.kw) : nullptr;
+      if (Paged && (p.qw != nullptr || p.kw != nullptr)) {  // all lanes of a row take part
+        float ss = 0.0f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) ss = fmaf(f[0][e], f[0][e], fmaf(f[1][e], f[1][e], ss));
+        for (int o = p.parts / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (w != nullptr) {
+          const float rs = rsqrtf(ss / p.D + p.eps);
+          float g[2][N];
+          ap_load<T, N>(w, ch.x * N, g[0]);
+          ap_load<T, N>(w, ch.y * N, g[1]);
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            f[0][e] *= rs * g[0][e];
+            f[1][e] *= rs * g[1][e];
+          }
+        }
+      }
+      if (!in) continue;
+      if (!value && part < p.rot / (2 * N)) {
+        const float2* turn = ro_turn + t * (p.rot / 2) + part * N;
+        if (p.interleaved) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < N; e += 2) {
+              const float2 cs = turn[(h * N + e) / 2];
+              const float a = f[h][e], b = f[h][e + 1];
+              f[h][e] = a * cs.x - b * cs.y;
+              f[h][e + 1] = b * cs.x + a * cs.y;
+            }
+        } else {
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const float2 cs = turn[e];
+            const float a = f[0][e], b = f[1][e];
+            f[0][e] = a * cs.x - b * cs.y;
+            f[1][e] = b * cs.x + a * cs.y;
+          }
+        }
+      }
+      T* dst = ro_target<T, Paged>(p, place[t], t0 + t, row);
+      if (dst == nullptr) continue;
+      // what no arithmetic touched is stored as it was read
+      const bool same = value || (w == nullptr && part >= p.rot / (2 * N));
+      __stcs(reinterpret_cast<uint4*>(dst) + ch.x, same ? x[i][0] : ro_round<T>(f[0]));
+      __stcs(reinterpret_cast<uint4*>(dst) + ch.y, same ? x[i][1] : ro_round<T>(f[1]));
+      if (Paged && part == 0 && row >= p.H && !value) {
+        const int h = row - p.H;
+        if (p.weights != nullptr) p.weights[place[t].b * p.wsb + h * p.wsh + place[t].slot] = 0.0f;
+        if (p.pos != nullptr)
+          p.pos[place[t].b * p.psb + h * p.psh + place[t].slot] = static_cast<int32_t>(place[t].position);
+      }
+    }
+  }
+}
+
+// Element by element, a warp a row: any even number of rotated elements.
+template <typename T, bool Paged>
+__global__ void __launch_bounds__(kRoThreads) rotary_any_kernel(const RotaryParams p) {
+  extern __shared__ __align__(16) float2 ro_turn[];
+  __shared__ RotaryPlace place[kRoMaxTokens];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int t0 = blockIdx.x * p.per_cta;
+  const int tokens = min(p.per_cta, p.T - t0);
+  const int rows = p.H + (Paged ? 2 : 1) * p.H_kv;
+  const int lane = threadIdx.x & 31, half = p.rot / 2;
+  if (threadIdx.x < tokens) place[threadIdx.x] = ro_place<Paged>(p, t0 + threadIdx.x);
+  __syncthreads();
+  ro_angles(p, place, tokens, ro_turn);
+  __syncthreads();
+  auto value_of = [](const T* row, int i) {
+    if constexpr (sizeof(T) == 4) return row[i];
+    else return ElemTraits<T>::widen1(reinterpret_cast<const uint16_t*>(row)[i]);
+  };
+#pragma unroll 1
+  for (int item = threadIdx.x >> 5; item < tokens * rows; item += kRoThreads / 32) {
+    const int t = item / rows, row = item - t * rows;
+    const T* src = ro_source<T, Paged>(p, t0 + t, row);
+    T* dst = ro_target<T, Paged>(p, place[t], t0 + t, row);
+    const bool value = Paged && row >= p.H + p.H_kv;
+    const T* w = Paged && !value ? static_cast<const T*>(row < p.H ? p.qw : p.kw) : nullptr;
+    float rs = 1.0f;
+    if (w != nullptr) {
+      float ss = 0.0f;
+      for (int e = lane; e < p.D; e += 32) ss = fmaf(value_of(src, e), value_of(src, e), ss);
+#pragma unroll
+      for (int o = 16; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      rs = rsqrtf(ss / p.D + p.eps);
+    }
+    if (dst == nullptr) continue;
+    auto normed = [&](int e) {
+      return w != nullptr ? value_of(src, e) * (rs * value_of(w, e)) : value_of(src, e);
+    };
+    if (!value)
+      for (int f = lane; f < half; f += 32) {
+        const int i = p.interleaved ? 2 * f : f, j = p.interleaved ? 2 * f + 1 : f + half;
+        const float2 cs = ro_turn[t * half + f];
+        const float a = normed(i), b = normed(j);
+        ElemTraits<T>::store(dst, i, a * cs.x - b * cs.y);
+        ElemTraits<T>::store(dst, j, b * cs.x + a * cs.y);
+      }
+    if (dst != src || w != nullptr)
+      for (int e = (value ? 0 : p.rot) + lane; e < p.D; e += 32) {
+        if (w == nullptr) dst[e] = src[e];
+        else ElemTraits<T>::store(dst, e, normed(e));
+      }
+    if (Paged && lane == 0 && row >= p.H && !value) {
+      const int h = row - p.H;
+      if (p.weights != nullptr) p.weights[place[t].b * p.wsb + h * p.wsh + place[t].slot] = 0.0f;
+      if (p.pos != nullptr)
+        p.pos[place[t].b * p.psb + h * p.psh + place[t].slot] = static_cast<int32_t>(place[t].position);
+    }
+  }
+}
+
+template <typename T, bool Paged>
+static int ro_launch(RotaryParams p, bool in_place, cudaStream_t s) {
+  constexpr int N = ElemTraits<T>::kPerChunk;
+  const bool whole = p.D % (2 * N) == 0 && p.rot % (2 * N) == 0;
+  p.parts = (in_place ? p.rot : p.D) / (2 * N);
+  const int rows = p.H + (Paged ? 2 : 1) * p.H_kv;
+  // enough tokens for every thread to have kRoSteps items, few enough to fill the SMs
+  int per = whole ? kRoSteps * kRoThreads / (rows * p.parts) : 4;
+  const int spread = p.T / (4 * device_sm_count());
+  if (per > spread) per = spread;
+  if (per > kRoMaxTokens) per = kRoMaxTokens;
+  if (per < 1) per = 1;
+  p.per_cta = per;
+  const size_t smem = static_cast<size_t>(per) * (p.rot / 2) * sizeof(float2);
+  const dim3 grid((p.T + per - 1) / per);
+  const cudaError_t e = launch_dependent(whole ? rotary_kernel<T, Paged> : rotary_any_kernel<T, Paged>,
+                                         grid, dim3(kRoThreads), smem, s, 1, p);
+  return e == cudaSuccess ? DCR_OK : DCR_ERR_CUDA;
+}
+
+template <bool Paged>
+static int ro_launch_t(const RotaryParams& p, int dtype, bool in_place, cudaStream_t s) {
+  switch (dtype) {
+    case DCR_DTYPE_BF16: return ro_launch<__nv_bfloat16, Paged>(p, in_place, s);
+    case DCR_DTYPE_F16: return ro_launch<__half, Paged>(p, in_place, s);
+    default: return ro_launch<float, Paged>(p, in_place, s);
+  }
+}
+
+// Shapes that both forms share.
+static int ro_check(int T, int H, int H_kv, int D, int rot) {
+  if (T <= 0 || H <= 0 || H_kv <= 0 || rot <= 0 || rot % 2 != 0 || rot > D) return DCR_ERR_SHAPE;
+  if (static_cast<int64_t>(T) * (H + 2 * static_cast<int64_t>(H_kv)) > 0x7fffff00ll) return DCR_ERR_SHAPE;
+  if (static_cast<int64_t>(H) + 2 * static_cast<int64_t>(H_kv) > 0x10000) return DCR_ERR_SHAPE;
+  return DCR_OK;
+}
+
+// Whether rows [T, heads, D] of one tensor share bytes with those of another. Slices of one packed
+// row per token, the usual case, are told apart by their places in the row.
+static bool ro_meet(const void* a, int64_t ast, int64_t ash, int64_t a_heads, const void* b, int64_t bst,
+                    int64_t bsh, int64_t b_heads, int64_t T, int64_t D, int64_t element) {
+  if (T > 1 && ast == bst && ast > 0) {
+    const int64_t period = ast * element, ea = ((a_heads - 1) * (a_heads > 1 ? ash : 0) + D) * element;
+    const int64_t eb = ((b_heads - 1) * (b_heads > 1 ? bsh : 0) + D) * element;
+    int64_t d = static_cast<int64_t>(reinterpret_cast<uintptr_t>(a) - reinterpret_cast<uintptr_t>(b)) % period;
+    if (d < 0) d += period;
+    if (d >= eb && d + ea <= period) return false;
+  }
+  return tables_meet(TableSpan(a, T, a_heads, D, ast, ash, element),
+                     TableSpan(b, T, b_heads, D, bst, bsh, element));
+}
+
+}  // namespace dcr
+
+using namespace dcr;
+
+extern "C" {
+
+int dcr_rotary(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+               int64_t k_stride_t, int64_t k_stride_h, const float* inv_freq, int rotated,
+               const void* positions, int positions_are_int64, int interleaved, float factor,
+               int dtype, int T, int H, int H_kv, int D, void* q_out, int64_t qo_stride_t,
+               int64_t qo_stride_h, void* k_out, int64_t ko_stride_t, int64_t ko_stride_h,
+               void* stream) {
+  if (q == nullptr || k == nullptr || inv_freq == nullptr || positions == nullptr || q_out == nullptr ||
+      k_out == nullptr)
+    return DCR_ERR_NULL;
+  if (dtype != DCR_DTYPE_BF16 && dtype != DCR_DTYPE_F16 && dtype != DCR_DTYPE_F32) return DCR_ERR_DTYPE;
+  const int64_t per16 = dtype == DCR_DTYPE_F32 ? 4 : 8, element = 16 / per16;
+  if (D <= 0 || D > kRoMaxDim || D % per16 != 0) return DCR_ERR_SHAPE;
+  const int st = ro_check(T, H, H_kv, D, rotated);
+  if (st != DCR_OK) return st;
+  const int64_t strides[8] = {q_stride_t, q_stride_h, k_stride_t, k_stride_h,
+                              qo_stride_t, qo_stride_h, ko_stride_t, ko_stride_h};
+  for (int64_t x : strides) {
+    if (x < 0) return DCR_ERR_SHAPE;
+    if (x % per16 != 0) return DCR_ERR_ALIGN;
+  }
+  if (misaligned(16, q, k, q_out, k_out) || misaligned(4, inv_freq, positions) ||
+      (positions_are_int64 && misaligned(8, positions)))
+    return DCR_ERR_ALIGN;
+  if (!rows_apart(T, H, D, qo_stride_t, qo_stride_h) || !rows_apart(T, H_kv, D, ko_stride_t, ko_stride_h))
+    return DCR_ERR_SHAPE;
+  auto same = [](const void* a, int64_t at, int64_t ah, const void* b, int64_t bt, int64_t bh, int T_, int h) {
+    return a == b && (T_ <= 1 || at == bt) && (h <= 1 || ah == bh);
+  };
+  const bool q_in = same(q, q_stride_t, q_stride_h, q_out, qo_stride_t, qo_stride_h, T, H);
+  const bool k_in = same(k, k_stride_t, k_stride_h, k_out, ko_stride_t, ko_stride_h, T, H_kv);
+  // no output reaches into an input that is not itself, nor into the other output
+  if ((!q_in && ro_meet(q, q_stride_t, q_stride_h, H, q_out, qo_stride_t, qo_stride_h, H, T, D, element)) ||
+      (!k_in && ro_meet(k, k_stride_t, k_stride_h, H_kv, k_out, ko_stride_t, ko_stride_h, H_kv, T, D, element)) ||
+      ro_meet(k, k_stride_t, k_stride_h, H_kv, q_out, qo_stride_t, qo_stride_h, H, T, D, element) ||
+      ro_meet(q, q_stride_t, q_stride_h, H, k_out, ko_stride_t, ko_stride_h, H_kv, T, D, element) ||
+      ro_meet(q_out, qo_stride_t, qo_stride_h, H, k_out, ko_stride_t, ko_stride_h, H_kv, T, D, element))
+    return DCR_ERR_SHAPE;
+  RotaryParams p = {};
+  p.q = q;
+  p.k = k;
+  p.qst = q_stride_t;
+  p.qsh = q_stride_h;
+  p.kst = k_stride_t;
+  p.ksh = k_stride_h;
+  p.q_out = q_out;
+  p.k_out = k_out;
+  p.qost = qo_stride_t;
+  p.qosh = qo_stride_h;
+  p.kost = ko_stride_t;
+  p.kosh = ko_stride_h;
+  p.inv_freq = inv_freq;
+  p.positions = positions;
+  p.wide = positions_are_int64 != 0;
+  p.interleaved = interleaved != 0;
+  p.T = T;
+  p.H = H;
+  p.H_kv = H_kv;
+  p.D = D;
+  p.rot = rotated;
+  p.factor = factor;
+  return ro_launch_t<false>(p, dtype, q_in && k_in, static_cast<cudaStream_t>(stream));
+}
+
+int dcr_paged_rotary_append(
+    const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
+    int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h,
+    const void* q_weight, const void* k_weight, float eps, const float* inv_freq, int rotated,
+    int interleaved, float factor, const int32_t* positions, const int32_t* seq,
+    const int32_t* slots, int dtype, int T, int H, int H_kv, int D, void* q_out, void* k_pages,
+    void* v_pages, int64_t kp_stride_p, int64_t kp_stride_h, int64_t kp_stride_s,
+    int64_t vp_stride_p, int64_t vp_stride_h, int64_t vp_stride_s, int num_pages, int page_size,
+    const int32_t* page_table, int64_t table_stride, int n_seq, int max_pages, float* weights,
+    int64_t w_stride_b, int64_t w_stride_h, int32_t* pos, int64_t p_stride_b, int64_t p_stride_h,
+    void* stream) {
+  if (q == nullptr || k == nullptr || v == nullptr || inv_freq == nullptr || positions == nullptr ||
+      slots == nullptr || q_out == nullptr)
+    return DCR_ERR_NULL;
+  int st = ro_check(T, H, H_kv, D, rotated);
+  if (st != DCR_OK) return st;
+  if (n_seq <= 0 || (seq == nullptr && T > n_seq)) return DCR_ERR_SHAPE;
+  st = check_pool(k_pages, v_pages, dtype, kp_stride_p, kp_stride_h, kp_stride_s, vp_stride_p,
+                  vp_stride_h, vp_stride_s, num_pages, page_size, page_table, table_stride,
+                  max_pages, H_kv, D);
+  if (st != DCR_OK) return st;
+  if (H % H_kv != 0) return DCR_ERR_SHAPE;
+  const int64_t per16 = dtype == DCR_DTYPE_F32 ? 4 : 8;
+  const int64_t strides[6] = {q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h};
+  for (int64_t x : strides) {
+    if (x < 0) return DCR_ERR_SHAPE;
+    if (x % per16 != 0) return DCR_ERR_ALIGN;
+  }
+  if (misaligned(16, q, k, v, q_out, q_weight, k_weight) ||
+      misaligned(4, inv_freq, positions, seq, slots, weights, pos))
+    return DCR_ERR_ALIGN;
+  const int64_t max_slots = static_cast<int64_t>(max_pages) * page_size;
+  if ((weights != nullptr && (w_stride_b < 0 || w_stride_h < 0 ||
+                              !rows_apart(n_seq, H_kv, max_slots, w_stride_b, w_stride_h))) ||
+      (pos != nullptr && (p_stride_b < 0 || p_stride_h < 0 ||
+                          !rows_apart(n_seq, H_kv, max_slots, p_stride_b, p_stride_h))))
+    return DCR_ERR_SHAPE;
+  if (rows_meet(q, q_stride_t, q_stride_h, q_out, T, H, D, 16 / per16)) return DCR_ERR_SHAPE;
+  RotaryParams p = {};
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.qst = q_stride_t;
+  p.qsh = q_stride_h;
+  p.kst = k_stride_t;
+  p.ksh = k_stride_h;
+  p.vst = v_stride_t;
+  p.vsh = v_stride_h;
+  p.q_out = q_out;
+  p.qost = static_cast<int64_t>(H) * D;
+  p.qosh = D;
+  p.inv_freq = inv_freq;
+  p.positions = positions;
+  p.interleaved = interleaved != 0;
+  p.T = T;
+  p.H = H;
+  p.H_kv = H_kv;
+  p.D = D;
+  p.rot = rotated;
+  p.factor = factor;
+  p.c = make_pool(k_pages, v_pages, kp_stride_p, kp_stride_h, kp_stride_s, vp_stride_p,
+                  vp_stride_h, vp_stride_s, num_pages, page_size, page_table, table_stride,
+                  max_pages);
+  p.k_pages = k_pages;
+  p.v_pages = v_pages;
+  p.seq = seq;
+  p.slots = slots;
+  p.n_seq = n_seq;
+  p.qw = q_weight;
+  p.kw = k_weight;
+  p.eps = eps;
+  p.weights = weights;
+  p.wsb = w_stride_b;
+  p.wsh = w_stride_h;
+  p.pos = pos;
+  p.psb = p_stride_b;
+  p.psh = p_stride_h;
+  return ro_launch_t<true>(p, dtype, false, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

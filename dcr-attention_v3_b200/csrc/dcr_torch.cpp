@@ -19,6 +19,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -62,6 +63,18 @@ int64_t integer(PyObject* o, const char* name) {
     refuse(std::string(name) + " must be an integer");
   }
   return v;
+}
+
+double number(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw Refused{};
+  return v;
+}
+
+bool truth_of(PyObject* o) {
+  const int truth = PyObject_IsTrue(o);
+  if (truth < 0) throw Refused{};
+  return truth != 0;
 }
 
 int dtype_code(const at::Tensor& t, const char* name) {
@@ -224,6 +237,26 @@ PyObject* guarded(PyObject* const* a, Py_ssize_t n, Py_ssize_t want, F&& f) {
   }
 }
 
+// The scale of the scores: the given one, or 1 / sqrt(D).
+double scale_of(PyObject* o, const Pool& p) {
+  if (o == Py_None) return 1.0 / std::sqrt(static_cast<double>(p.D));
+  return number(o);
+}
+
+int64_t window_of(PyObject* o) {
+  const int64_t window = integer(o, "window");
+  if (window < 0 || window > INT32_MAX) refuse("window must be >= 0");
+  return window;
+}
+
+PyObject* pair_of(const at::Tensor& x, const at::Tensor& y) {
+  PyObject* r = PyTuple_New(2);
+  if (r == nullptr) return nullptr;
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(x));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(y));
+  return r;
+}
+
 // (q, k_pages, v_pages, page_table, lengths, scale, window, weights, return_lse, out, workspace)
 PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded(a, n, 11, [&]() -> PyObject* {
@@ -232,17 +265,10 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Rows q = rows_of(a[0], "q", p, B, H);
     if (p.sequences != B) refuse("page_table must have " + std::to_string(B) + " rows");
     const void* lengths = vector_of(a[4], "lengths", at::kInt, B, p.device);
-    double scale = 1.0 / std::sqrt(static_cast<double>(p.D));
-    if (a[5] != Py_None) {
-      scale = PyFloat_AsDouble(a[5]);
-      if (scale == -1.0 && PyErr_Occurred()) throw Refused{};
-    }
-    const int64_t window = integer(a[6], "window");
-    if (window < 0 || window > INT32_MAX) refuse("window must be >= 0");
+    const double scale = scale_of(a[5], p);
+    const int64_t window = window_of(a[6]);
     const Table w = slot_table(a[7], "weights", at::kFloat, p, p.slots);
-    const int truth = PyObject_IsTrue(a[8]);
-    if (truth < 0) throw Refused{};
-    const bool want_lse = truth != 0;
+    const bool want_lse = truth_of(a[8]);
     const c10::cuda::OptionalCUDAGuard guard(p.k->device());
     const at::Tensor o = output(a[9], {B, H, p.D}, p.k->options());
     check_apart(a[9], o, q, p, B, H);
@@ -265,12 +291,92 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
           w.sb, w.sh, ws.data_ptr(), static_cast<size_t>(ws.numel()), stream_of(p.device));
       if (st != DCR_OK) return PyLong_FromLong(st);
     }
-    if (!want_lse) return THPVariable_Wrap(o);
-    PyObject* r = PyTuple_New(2);
-    if (r == nullptr) return nullptr;
-    PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(o));
-    PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(lse));
-    return r;
+    return want_lse ? pair_of(o, lse) : THPVariable_Wrap(o);
+  });
+}
+
+// (q, k_pages, v_pages, page_table, lengths, starts, scale, window, causal, return_lse, out,
+//  workspace)
+PyObject* prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(a, n, 12, [&]() -> PyObject* {
+    const Pool p = pool_of(a[1], a[2], a[3]);
+    const auto [T, H] = query_shape(a[0], p);
+    const Rows q = rows_of(a[0], "q", p, T, H);
+    const int64_t B = p.sequences;
+    const void* lengths = vector_of(a[4], "lengths", at::kInt, B, p.device);
+    const void* starts = vector_of(a[5], "starts", at::kInt, B + 1, p.device);
+    const double scale = scale_of(a[6], p);
+    const int64_t window = window_of(a[7]);
+    const bool causal = truth_of(a[8]), want_lse = truth_of(a[9]);
+    if (window > 0 && !causal) refuse("a window needs causal attention");
+    const c10::cuda::OptionalCUDAGuard guard(p.k->device());
+    const at::Tensor o = output(a[10], {T, H, p.D}, p.k->options());
+    check_apart(a[10], o, q, p, T, H);
+    at::Tensor lse;
+    if (want_lse) lse = at::empty({T, H}, p.k->options().dtype(at::kFloat));
+    if (T > 0 && B > 0) {
+      const size_t bytes = dcr_paged_prefill_workspace_bytes(
+          static_cast<int>(T), static_cast<int>(B), static_cast<int>(H), static_cast<int>(p.H_kv),
+          static_cast<int>(p.D), static_cast<int>(p.slots), static_cast<int>(window));
+      const at::Tensor ws = scratch(a[11], bytes, p.device);
+      const int st = dcr_paged_prefill(
+          q.data, q.st, q.sh, p.k->data_ptr(), p.v->data_ptr(), p.dtype, p.k->stride(0),
+          p.k->stride(1), p.k->stride(2), p.v->stride(0), p.v->stride(1), p.v->stride(2),
+          static_cast<int>(p.pages), static_cast<int>(p.page_size),
+          static_cast<const int32_t*>(p.table->data_ptr()), p.table_stride,
+          static_cast<int>(p.max_pages), static_cast<const int32_t*>(lengths),
+          static_cast<const int32_t*>(starts), static_cast<int>(T), static_cast<int>(B),
+          static_cast<int>(H), static_cast<int>(p.H_kv), static_cast<int>(p.D),
+          static_cast<float>(scale), static_cast<int>(window), causal, o.data_ptr(),
+          want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr, ws.data_ptr(),
+          static_cast<size_t>(ws.numel()), stream_of(p.device));
+      if (st != DCR_OK) return PyLong_FromLong(st);
+    }
+    return want_lse ? pair_of(o, lse) : THPVariable_Wrap(o);
+  });
+}
+
+// (q, k_pages, v_pages, page_table, lengths, groups, prefix, scale, window, return_lse, out, workspace)
+PyObject* shared(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(a, n, 12, [&]() -> PyObject* {
+    const Pool p = pool_of(a[1], a[2], a[3]);
+    const auto [B, H] = query_shape(a[0], p);
+    const Rows q = rows_of(a[0], "q", p, B, H);
+    if (p.sequences != B) refuse("page_table must have " + std::to_string(B) + " rows");
+    const void* lengths = vector_of(a[4], "lengths", at::kInt, B, p.device);
+    const at::Tensor& g = cuda_tensor(a[5], "groups");
+    if (!(g.dim() == 1 && g.size(0) >= 2 && g.size(0) - 1 <= std::max<int64_t>(B, 1)))
+      refuse("groups must be int32 [groups + 1] of 1 to " + std::to_string(B) + " groups");
+    const void* groups = vector_of(a[5], "groups", at::kInt, g.size(0), p.device);
+    const void* prefix = vector_of(a[6], "prefix", at::kInt, B, p.device);
+    const double scale = scale_of(a[7], p);
+    const int64_t window = window_of(a[8]);
+    const bool want_lse = truth_of(a[9]);
+    const c10::cuda::OptionalCUDAGuard guard(p.k->device());
+    const at::Tensor o = output(a[10], {B, H, p.D}, p.k->options());
+    check_apart(a[10], o, q, p, B, H);
+    at::Tensor lse;
+    if (want_lse) lse = at::empty({B, H}, p.k->options().dtype(at::kFloat));
+    if (B > 0) {
+      const int n_groups = static_cast<int>(g.size(0) - 1);
+      const size_t bytes = dcr_paged_shared_workspace_bytes(
+          static_cast<int>(B), n_groups, static_cast<int>(H), static_cast<int>(p.H_kv),
+          static_cast<int>(p.D), static_cast<int>(p.slots));
+      const at::Tensor ws = scratch(a[11], bytes, p.device);
+      const int st = dcr_paged_shared_attend(
+          q.data, q.st, q.sh, p.k->data_ptr(), p.v->data_ptr(), p.dtype, p.k->stride(0),
+          p.k->stride(1), p.k->stride(2), p.v->stride(0), p.v->stride(1), p.v->stride(2),
+          static_cast<int>(p.pages), static_cast<int>(p.page_size),
+          static_cast<const int32_t*>(p.table->data_ptr()), p.table_stride,
+          static_cast<int>(p.max_pages), static_cast<const int32_t*>(lengths),
+          static_cast<const int32_t*>(groups), n_groups, static_cast<const int32_t*>(prefix),
+          static_cast<int>(B), static_cast<int>(H), static_cast<int>(p.H_kv),
+          static_cast<int>(p.D), static_cast<float>(scale), static_cast<int>(window), o.data_ptr(),
+          want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr, ws.data_ptr(),
+          static_cast<size_t>(ws.numel()), stream_of(p.device));
+      if (st != DCR_OK) return PyLong_FromLong(st);
+    }
+    return want_lse ? pair_of(o, lse) : THPVariable_Wrap(o);
   });
 }
 
@@ -298,8 +404,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       refuse(std::to_string(T) + " tokens without seq need as many sequences, got " + std::to_string(p.sequences));
     const void* qw = optional_vector(a[11], "q_weight", type, p.D, p.device);
     const void* kw = optional_vector(a[12], "k_weight", type, p.D, p.device);
-    const double eps = PyFloat_AsDouble(a[13]);
-    if (eps == -1.0 && PyErr_Occurred()) throw Refused{};
+    const double eps = number(a[13]);
     const Table w = slot_table(a[14], "weights", at::kFloat, p, p.slots);
     const Table pos = slot_table(a[15], "pos", at::kInt, p, p.slots);
     const c10::cuda::OptionalCUDAGuard guard(p.k->device());
@@ -310,6 +415,110 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
           q.data, q.st, q.sh, k.data, k.st, k.sh, v.data, v.st, v.sh, qw, kw,
           static_cast<float>(eps), cos.data_ptr(), sin.data_ptr(), dtype_code(cos, "cos"),
           static_cast<int>(cos.size(0)), static_cast<const int32_t*>(positions),
+          static_cast<const int32_t*>(seq), static_cast<const int32_t*>(slots), p.dtype,
+          static_cast<int>(T), static_cast<int>(H), static_cast<int>(p.H_kv),
+          static_cast<int>(p.D), o.data_ptr(), p.k->data_ptr(), p.v->data_ptr(), p.k->stride(0),
+          p.k->stride(1), p.k->stride(2), p.v->stride(0), p.v->stride(1), p.v->stride(2),
+          static_cast<int>(p.pages), static_cast<int>(p.page_size),
+          static_cast<const int32_t*>(p.table->data_ptr()), p.table_stride,
+          static_cast<int>(p.sequences), static_cast<int>(p.max_pages),
+          static_cast<float*>(w.data), w.sb, w.sh, static_cast<int32_t*>(pos.data), pos.sb, pos.sh,
+          stream_of(p.device));
+      if (st != DCR_OK) return PyLong_FromLong(st);
+    }
+    return THPVariable_Wrap(o);
+  });
+}
+
+// Frequencies: (data, rotated elements a row).
+std::pair<const float*, int64_t> frequencies_of(PyObject* o, int64_t D, int device) {
+  const at::Tensor& t = cuda_tensor(o, "inv_freq");
+  if (!(t.dim() == 1 && t.size(0) > 0 && 2 * t.size(0) <= D && t.scalar_type() == at::kFloat &&
+        t.get_device() == device && t.is_contiguous()))
+    refuse("inv_freq must be a contiguous Float [1 to " + std::to_string(D / 2) + "] on cuda:" +
+           std::to_string(device));
+  return {static_cast<const float*>(t.data_ptr()), 2 * t.size(0)};
+}
+
+// (q, k, inv_freq, positions, interleaved, factor, q_out, k_out)
+PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(a, n, 8, [&]() -> PyObject* {
+    const at::Tensor &q = cuda_tensor(a[0], "q"), &k = cuda_tensor(a[1], "k");
+    const int dtype = dtype_code(q, "q"), device = q.get_device();
+    if (!(q.dim() == 3 && k.dim() == 3 && k.size(0) == q.size(0) && k.size(2) == q.size(2) &&
+          q.size(1) > 0 && k.size(1) > 0 && k.scalar_type() == q.scalar_type() && k.get_device() == device))
+      refuse("q and k must be [T, H, D] and [T, H_kv, D] of one dtype and device");
+    const int64_t T = q.size(0), H = q.size(1), H_kv = k.size(1), D = q.size(2);
+    if (T > INT32_MAX || H > INT32_MAX || H_kv > INT32_MAX) refuse("q and k are too large");
+    if (D <= 0 || D > 512 || D % (16 / q.element_size()) != 0)
+      refuse("head dim must be a multiple of 16 bytes, at most 512, got " + std::to_string(D));
+    const auto [inv_freq, rotated] = frequencies_of(a[2], D, device);
+    const at::Tensor& pos = cuda_tensor(a[3], "positions");
+    if (!(pos.dim() == 1 && pos.size(0) == T && pos.get_device() == device && pos.is_contiguous() &&
+          (pos.scalar_type() == at::kInt || pos.scalar_type() == at::kLong)))
+      refuse("positions must be a contiguous int32 or int64 [" + std::to_string(T) + "] on cuda:" +
+             std::to_string(device));
+    const bool interleaved = truth_of(a[4]);
+    const double factor = number(a[5]);
+    const c10::cuda::OptionalCUDAGuard guard(q.device());
+    auto to = [&](PyObject* o, const at::Tensor& x, const char* name) {
+      if (o == Py_None) return at::empty(x.sizes(), x.options());
+      const at::Tensor& t = cuda_tensor(o, name);
+      if (!(t.sizes() == x.sizes() && t.scalar_type() == x.scalar_type() && t.get_device() == device &&
+            t.stride(2) == 1))
+        refuse(std::string(name) + " must be " + dims(x.sizes()) + " of the input's dtype and device, with contiguous rows");
+      return t;
+    };
+    if (q.stride(2) != 1 || k.stride(2) != 1) refuse("q and k must have contiguous rows");
+    const at::Tensor qo = to(a[6], q, "q_out"), ko = to(a[7], k, "k_out");
+    if (T > 0) {
+      auto st = [](const at::Tensor& t, int d) { return t.size(d) > 1 ? t.stride(d) : 0; };
+      const int rc = dcr_rotary(
+          q.data_ptr(), st(q, 0), st(q, 1), k.data_ptr(), st(k, 0), st(k, 1), inv_freq,
+          static_cast<int>(rotated), pos.data_ptr(), pos.scalar_type() == at::kLong, interleaved,
+          static_cast<float>(factor), dtype, static_cast<int>(T), static_cast<int>(H),
+          static_cast<int>(H_kv), static_cast<int>(D), qo.data_ptr(), st(qo, 0), st(qo, 1),
+          ko.data_ptr(), st(ko, 0), st(ko, 1), stream_of(device));
+      if (rc == DCR_ERR_SHAPE)
+        refuse("q_out and k_out must be q and k themselves or share no memory with them, one another "
+               "or among their rows");
+      if (rc != DCR_OK) return PyLong_FromLong(rc);
+    }
+    return pair_of(qo, ko);
+  });
+}
+
+// (q, k, v, inv_freq, positions, k_pages, v_pages, page_table, slots, seq, interleaved, factor,
+//  q_weight, k_weight, eps, weights, pos, out)
+PyObject* rotary_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(a, n, 18, [&]() -> PyObject* {
+    const Pool p = pool_of(a[5], a[6], a[7]);
+    const auto [T, H] = query_shape(a[0], p);
+    const Rows q = rows_of(a[0], "q", p, T, H);
+    const Rows k = rows_of(a[1], "k", p, T, p.H_kv);
+    const Rows v = rows_of(a[2], "v", p, T, p.H_kv);
+    const auto [inv_freq, rotated] = frequencies_of(a[3], p.D, p.device);
+    const at::ScalarType type = p.k->scalar_type();
+    const void* positions = vector_of(a[4], "positions", at::kInt, T, p.device);
+    const void* slots = vector_of(a[8], "slots", at::kInt, T, p.device);
+    const void* seq = optional_vector(a[9], "seq", at::kInt, T, p.device);
+    if (seq == nullptr && T > p.sequences)
+      refuse(std::to_string(T) + " tokens without seq need as many sequences, got " + std::to_string(p.sequences));
+    const bool interleaved = truth_of(a[10]);
+    const double factor = number(a[11]);
+    const void* qw = optional_vector(a[12], "q_weight", type, p.D, p.device);
+    const void* kw = optional_vector(a[13], "k_weight", type, p.D, p.device);
+    const double eps = number(a[14]);
+    const Table w = slot_table(a[15], "weights", at::kFloat, p, p.slots);
+    const Table pos = slot_table(a[16], "pos", at::kInt, p, p.slots);
+    const c10::cuda::OptionalCUDAGuard guard(p.k->device());
+    const at::Tensor o = output(a[17], {T, H, p.D}, p.k->options());
+    check_apart(a[17], o, q, p, T, H);
+    if (T > 0) {
+      const int st = dcr_paged_rotary_append(
+          q.data, q.st, q.sh, k.data, k.st, k.sh, v.data, v.st, v.sh, qw, kw,
+          static_cast<float>(eps), inv_freq, static_cast<int>(rotated), interleaved,
+          static_cast<float>(factor), static_cast<const int32_t*>(positions),
           static_cast<const int32_t*>(seq), static_cast<const int32_t*>(slots), p.dtype,
           static_cast<int>(T), static_cast<int>(H), static_cast<int>(p.H_kv),
           static_cast<int>(p.D), o.data_ptr(), p.k->data_ptr(), p.v->data_ptr(), p.k->stride(0),
@@ -491,6 +700,11 @@ PyObject* process_logits(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 PyMethodDef kMethods[] = {
     {"attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attend)), METH_FASTCALL, nullptr},
+    {"prefill", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(prefill)), METH_FASTCALL, nullptr},
+    {"shared", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(shared)), METH_FASTCALL, nullptr},
+    {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rotary)), METH_FASTCALL, nullptr},
+    {"rotary_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rotary_append)), METH_FASTCALL,
+     nullptr},
     {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(append)), METH_FASTCALL, nullptr},
     {"evict", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(evict)), METH_FASTCALL, nullptr},
     {"process_logits", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(process_logits)),

@@ -6,7 +6,11 @@ view) and ``page_table [B, max_pages]`` int32 names the pages of each sequence; 
 is not mapped. ``page_size`` is any number >= 1, D is 64 or 128, H any multiple of H_kv.
 
 * :func:`paged_append`    - query/key norms, position rotation, append (csrc/dcr_paged_append.cu)
+* :func:`paged_rotary_append` - the same, rotated by frequencies in any layout (csrc/dcr_rotary.cu)
 * :func:`paged_attention` - attention of one new token (csrc/dcr_paged_attend.cu)
+* :func:`paged_prefill`   - attention of many new tokens (csrc/dcr_paged_rows.cu)
+* :func:`paged_shared_attention` - attention of one new token where sequences share their first
+  pages (csrc/dcr_paged_rows.cu)
 * :func:`paged_evict`     - eviction by accumulated weight (csrc/dcr_paged_evict.cu)
 
 All take device lengths, so a captured CUDA graph can be replayed while they grow. Arguments are
@@ -53,6 +57,61 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     return r
 
 
+def paged_prefill_workspace_bytes(T: int, B: int, H: int, H_kv: int, D: int, max_slots: int,
+                                  window: int = 0) -> int:
+    """Bytes :func:`paged_prefill` needs for T tokens of B sequences (max_slots = max_pages *
+    page_size)."""
+    return int(_lib.load().dcr_paged_prefill_workspace_bytes(T, B, H, H_kv, D, max_slots, window))
+
+
+def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                  page_table: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor, *,
+                  scale: Optional[float] = None, window: int = 0, causal: bool = True,
+                  return_lse: bool = False, out: Optional[torch.Tensor] = None,
+                  workspace_buf: Optional[torch.Tensor] = None):
+    """Attention of many new tokens per sequence over its cached slots, their own among them.
+
+    q ``[T, H, D]`` (any token and head strides); tokens ``starts[b]`` to ``starts[b + 1] - 1``
+    (``starts [B + 1]`` int32 on the device, ascending) are the last of sequence b's ``lengths[b]``
+    slots, whose keys and values are in the pages already: a whole prompt, a chunk of one behind
+    its history, or drafted tokens to verify. A token sees the slots up to its own (``causal=False``:
+    all of the sequence's) and with ``window > 0`` the last ``window`` of these. Returns O ``[T, H,
+    D]`` in q's dtype, or (O, lse ``[T, H]`` fp32) with ``return_lse``. Rows of q that belong to no
+    sequence are not written: give ``out`` where theirs matter. Statistics and sums are fp32, the
+    weights of 16-bit caches enter the second product in 16 bits, O is rounded once."""
+    r = _lib.torch_ops().prefill(q, k_pages, v_pages, page_table, lengths, starts, scale, window,
+                                 causal, return_lse, out, workspace_buf)
+    if type(r) is int:
+        _lib.check(r, "dcr_paged_prefill")
+    return r
+
+
+def paged_shared_workspace_bytes(B: int, groups: int, H: int, H_kv: int, D: int,
+                                 max_slots: int) -> int:
+    """Bytes :func:`paged_shared_attention` needs (max_slots = max_pages * page_size)."""
+    return int(_lib.load().dcr_paged_shared_workspace_bytes(B, groups, H, H_kv, D, max_slots))
+
+
+def paged_shared_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                           page_table: torch.Tensor, lengths: torch.Tensor, groups: torch.Tensor,
+                           prefix: torch.Tensor, *, scale: Optional[float] = None, window: int = 0,
+                           return_lse: bool = False, out: Optional[torch.Tensor] = None,
+                           workspace_buf: Optional[torch.Tensor] = None):
+    """:func:`paged_attention` where groups of sequences hold the same pages in their first slots,
+    which are read once for a group.
+
+    Sequences ``groups[p]`` to ``groups[p + 1] - 1`` (``groups [P + 1]`` int32 on the device, from 0
+    to B) share the first ``prefix[b]`` slots (``prefix [B]`` int32 on the device) with the group's
+    first sequence, whose row of ``page_table`` names the pages; the other slots are looked up in
+    the sequence's own row. A group may be one sequence and a prefix 0. Other arguments and the
+    result are :func:`paged_attention`'s."""
+    r = _lib.torch_ops().shared(q, k_pages, v_pages, page_table, lengths, groups, prefix, scale, window,
+                                return_lse, out, workspace_buf)
+    if type(r) is int:
+        _lib.check(r, "dcr_paged_shared_attend")
+    return r
+
+
 def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor,
                  sin: torch.Tensor, positions: torch.Tensor, k_pages: torch.Tensor,
                  v_pages: torch.Tensor, page_table: torch.Tensor, slots: torch.Tensor, *,
@@ -73,6 +132,26 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.T
                                 seq, q_weight, k_weight, eps, weights, pos, out)
     if type(r) is int:
         _lib.check(r, "dcr_paged_append")
+    return r
+
+
+def paged_rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, inv_freq: torch.Tensor,
+                        positions: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                        page_table: torch.Tensor, slots: torch.Tensor, *,
+                        seq: Optional[torch.Tensor] = None, interleaved: bool = False,
+                        factor: float = 1.0, q_weight: Optional[torch.Tensor] = None,
+                        k_weight: Optional[torch.Tensor] = None, eps: float = 1e-5,
+                        weights: Optional[torch.Tensor] = None, pos: Optional[torch.Tensor] = None,
+                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`paged_append` with the rotation of :func:`~dcr_b200.kernel.cuda.rotary.rotary`: angles
+    from ``inv_freq`` ``[r / 2]`` fp32 instead of tables (any position), the first r elements of a
+    head, neighbours paired with ``interleaved``, scaled by ``factor``. Returns the rotated
+    queries."""
+    r = _lib.torch_ops().rotary_append(q, k, v, inv_freq, positions, k_pages, v_pages, page_table, slots,
+                                       seq, interleaved, factor, q_weight, k_weight, eps, weights, pos,
+                                       out)
+    if type(r) is int:
+        _lib.check(r, "dcr_paged_rotary_append")
     return r
 
 

@@ -421,7 +421,8 @@ int dcr_silu_mul(const void* gate, const void* up, int dtype, int64_t n, void* o
 int dcr_silu_mul_packed(const void* gate_up, int dtype, int rows, int inter, void* out,
                         void* stream);
 
-/* ---- paged serving (dcr_paged_attend.cu, dcr_paged_append.cu, dcr_paged_evict.cu) ---------
+/* ---- paged serving (dcr_paged_attend.cu, dcr_paged_rows.cu, dcr_paged_append.cu,
+ * dcr_paged_evict.cu) ----------------------------------------------------------------------
  * A decode step over a paged key-value cache. No counterpart in the reference, whose cache is
  * one contiguous tensor per layer (dcr_attention/models/llama/compat.py:208-254).
  *
@@ -458,6 +459,48 @@ int dcr_paged_attend(const void* q, int64_t q_stride_b, int64_t q_stride_h, cons
                      int H_kv, int D, float scale, int window, void* o, float* lse,
                      float* weights, int64_t w_stride_b, int64_t w_stride_h, void* workspace,
                      size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace dcr_paged_prefill needs for T tokens of B sequences (max_slots = max_pages *
+ * page_size); it need not be initialised. 0: invalid shape. */
+size_t dcr_paged_prefill_workspace_bytes(int T, int B, int H, int H_kv, int D, int max_slots, int window);
+
+/* Attention of many new tokens per sequence: tokens starts[b] .. starts[b + 1] - 1 (starts [B + 1],
+ * ascending within [0, T]) of q [T, H, D] are the last of sequence b's lengths[b] slots, whose keys
+ * and values are in the pages already. Token i of n sees the slots up to its own position x =
+ * lengths[b] - n + i (causal != 0; else all lengths[b]) and, with window > 0 (causal only), of these
+ * the last `window`. O [T, H, D] and lse [T, H] (or NULL) as dcr_paged_attend, with fp32 statistics
+ * and sums; in bf16 and f16 the weights enter the second product rounded to 16 bits. Rows of q that
+ * belong to no sequence are not touched in O and lse; a token before the sequence's first slot (n >
+ * lengths[b]) sees nothing and gets 0 and -inf. A value that is not finite spoils all elements of the
+ * rows that see it, and no others. O may be q itself where q is contiguous, else it shares no memory
+ * with it. */
+int dcr_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_pages,
+                      const void* v_pages, int dtype, int64_t k_stride_p, int64_t k_stride_h,
+                      int64_t k_stride_s, int64_t v_stride_p, int64_t v_stride_h,
+                      int64_t v_stride_s, int num_pages, int page_size, const int32_t* page_table,
+                      int64_t table_stride, int max_pages, const int32_t* lengths,
+                      const int32_t* starts, int T, int B, int H, int H_kv, int D, float scale,
+                      int window, int causal, void* o, float* lse, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace dcr_paged_shared_attend needs; it need not be initialised. 0: invalid shape. */
+size_t dcr_paged_shared_workspace_bytes(int B, int groups, int H, int H_kv, int D, int max_slots);
+
+/* dcr_paged_attend (without weights) where sequences hold the same pages in their first slots, which
+ * are then read once for all of them: sequences groups[p] .. groups[p + 1] - 1 (groups [n_groups + 1],
+ * ascending, from 0 to B) share the first prefix[b] slots of the group's first sequence, whose row of
+ * page_table names their pages (a sequence's own row is read from slot prefix[b] on). prefix[b] may
+ * be 0, differ between the sequences of a group, and end inside a page. A sequence that no group
+ * holds is attended without its prefix and sets the device status. */
+int dcr_paged_shared_attend(const void* q, int64_t q_stride_b, int64_t q_stride_h,
+                            const void* k_pages, const void* v_pages, int dtype, int64_t k_stride_p,
+                            int64_t k_stride_h, int64_t k_stride_s, int64_t v_stride_p,
+                            int64_t v_stride_h, int64_t v_stride_s, int num_pages, int page_size,
+                            const int32_t* page_table, int64_t table_stride, int max_pages,
+                            const int32_t* lengths, const int32_t* groups, int n_groups,
+                            const int32_t* prefix, int B, int H, int H_kv, int D, float scale,
+                            int window, void* o, float* lse, void* workspace,
+                            size_t workspace_bytes, void* stream);
 
 /* For T tokens: q_out [T, H, D] and the pages' new key rows get rotate(norm(x)), with norm(x) =
  * x * rsqrt(mean(x^2) + eps) * weight (a NULL weight: x itself) and rotate as HF
@@ -506,6 +549,34 @@ int dcr_paged_evict(void* k_pages, void* v_pages, int dtype, int64_t k_stride_p,
                     int64_t wo_stride_b, int64_t wo_stride_h, int32_t* pos_out,
                     int64_t po_stride_b, int64_t po_stride_h, int32_t* lengths_out,
                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- position rotation from frequencies (dcr_rotary.cu) --------------------------------
+ * The first `rotated` elements (even, at most D) of every query and key row, in pairs (i, i +
+ * rotated / 2), or (2i, 2i + 1) with interleaved != 0, are turned by the angle positions[t] *
+ * inv_freq[i] and scaled by factor; the others are copied. In fp32 from angles reduced in 64 bits,
+ * rounded once. q [T, H, D], k [T, H_kv, D] and the outputs have token and head strides (multiples
+ * of 16 bytes); D is a multiple of 16 bytes of elements, at most 512. positions [T] are int32 or
+ * int64, of any sign. An output may be its input itself (same strides); apart from that outputs
+ * share no memory with the inputs or one another. */
+int dcr_rotary(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+               int64_t k_stride_t, int64_t k_stride_h, const float* inv_freq, int rotated,
+               const void* positions, int positions_are_int64, int interleaved, float factor,
+               int dtype, int T, int H, int H_kv, int D, void* q_out, int64_t qo_stride_t,
+               int64_t qo_stride_h, void* k_out, int64_t ko_stride_t, int64_t ko_stride_h,
+               void* stream);
+
+/* dcr_paged_append with that rotation in place of the tables' (any position is valid). */
+int dcr_paged_rotary_append(
+    const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
+    int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h,
+    const void* q_weight, const void* k_weight, float eps, const float* inv_freq, int rotated,
+    int interleaved, float factor, const int32_t* positions, const int32_t* seq,
+    const int32_t* slots, int dtype, int T, int H, int H_kv, int D, void* q_out, void* k_pages,
+    void* v_pages, int64_t kp_stride_p, int64_t kp_stride_h, int64_t kp_stride_s,
+    int64_t vp_stride_p, int64_t vp_stride_h, int64_t vp_stride_s, int num_pages, int page_size,
+    const int32_t* page_table, int64_t table_stride, int n_seq, int max_pages, float* weights,
+    int64_t w_stride_b, int64_t w_stride_h, int32_t* pos, int64_t p_stride_b, int64_t p_stride_h,
+    void* stream);
 
 /* ---- logits of a decode step (dcr_logits.cu) ------------------------------------------ */
 /* Per row of logits [B, V], in fp32 and in this order, rounded once to dtype: x > 0 ?
