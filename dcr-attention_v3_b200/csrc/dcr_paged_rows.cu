@@ -26,6 +26,7 @@
 
 #include "dcr_internal.h"
 #include "dcr_paged.cuh"
+#include "dcr_tc.cuh"
 
 namespace dcr {
 
@@ -383,6 +384,428 @@ __global__ void __launch_bounds__(kRfThreads) rows_fma_kernel(const RowsParams p
   }
 }
 
+// ---------------------------------------------------------------------------------------
+// 16-bit rows: NSUB blocks of 128 query rows against tiles of 128 slots on the tensor cores.
+//
+// Warps: four per block of rows for the softmax, a row a thread; four that bring K and V in, a
+// slot's address a thread; one that issues the products. Per tile and block S = Q K^T goes to tensor
+// memory, the softmax warps read their rows, keep the running base and sum (m, l) and write the
+// weights P back over S, and O += P V accumulates in tensor memory with P as its A operand. K and V
+// tiles take turns in a ring that the loaders fill by 16-byte cp.async: any page size and stride, slots
+// that are not valid filled with zeros and never read. With two blocks the tensor cores and the loaders
+// serve one while the softmax warps of the other compute.
+//
+// The base is raised only when a row's score is 8 above the largest it was set by, so O is rescaled
+// for few tiles, and never while a product on it runs: S of a tile is only seen complete after the
+// products before it. In f16 the base stays 7 below the maximum, so that small weights keep their
+// bits (2^-24 of 2^7). A weight enters the second product rounded to 16 bits, half a step of
+// which is off by as much as the output's own rounding, and averages out over the slots; with Parts =
+// 2 its remainder goes in as well, in a second product.
+// ---------------------------------------------------------------------------------------
+constexpr int kTcSlots = 128;
+
+template <int D, int NSUB>
+struct RowsTc {
+  static constexpr int kPanel = 128 * 128;           // bytes of 128 rows of 64 elements
+  static constexpr int kTile = D / 64 * kPanel;
+  static constexpr int kStages = D == 64 ? (NSUB == 2 ? 8 : 5) : (NSUB == 2 ? 4 : 5);
+  // Tiles that may be on their way before the oldest is announced: two fewer than the ring has, since
+  // a V tile is only released after the K tile behind it was used.
+  static constexpr int kLag = kStages - 2;
+  static constexpr int kSmem = 1024 + NSUB * kTile + kStages * kTile;
+  static constexpr int kColumns = NSUB * (128 + D) > 256 ? 512 : 256;
+  static constexpr int kLoad0 = NSUB * 128;          // first loader thread
+  static constexpr int kMma = kLoad0 + 128;          // the issuing warp's first thread
+  static constexpr int kThreads = kMma + 32;
+};
+
+struct RowsTcShared {
+  RowsUnit u;
+  uint64_t q_full, s_full[2], p_full[2], o_full[2], drained;
+  uint64_t full[8], empty[8];
+  uint32_t tmem;
+  uint32_t mask[8][4];          // mapped slots of the tiles in flight
+  int64_t koff[2][kTcSlots], voff[2][kTcSlots];
+  int2 limits[256];
+  uint8_t spoilt[256];          // rows that see a value that is not finite, in a tile not seen whole
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t rows_pack(float a, float b, float& ra, float& rb) {
+  uint32_t hi;
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    ra = a - f.x;
+    rb = b - f.y;
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    ra = a - __uint_as_float(hi << 16);
+    rb = b - __uint_as_float(hi & 0xffff0000u);
+  }
+  return hi;
+}
+
+// Bits [from, to) of a word that begins at 0.
+__device__ __forceinline__ uint32_t rows_bits(int from, int to) {
+  from = max(0, min(32, from));
+  to = max(0, min(32, to));
+  const uint32_t below = to == 32 ? 0xffffffffu : (1u << to) - 1u;
+  return from == 32 ? 0u : below & (0xffffffffu << from);
+}
+
+template <int N>
+__device__ __forceinline__ void rows_hide(uint32_t (&s)[N], const uint32_t* words) {
+#pragma unroll
+  for (int c = 0; c < N; ++c)
+    if (!((words[c / 32] >> (c % 32)) & 1u)) s[c] = 0xff800000u;  // -inf
+}
+
+// The loader warps: tiles [tiles.x, tiles.y), K then V, into the ring.
+template <typename T, int D, int NSUB>
+__device__ __forceinline__ void rows_tc_load(const RowsParams& p, RowsTcShared& sh, uint8_t* ring, int2 tiles) {
+  using S = RowsTc<D, NSUB>;
+  constexpr int C = D / 8, RP = 128 / C;  // chunks of a row, rows a step
+  const RowsUnit& u = sh.u;
+  const int lt = threadIdx.x - S::kLoad0, lane = threadIdx.x & 31;
+  const int ch = lt % C, r0 = lt / C;
+  const uint32_t column = (ch >> 3) * S::kPanel;
+  int issued = 0, announced = 0;
+  bool fine = true;  // after a wait that ran out a thread only keeps the others company at the barrier
+  auto stage = [&](int e) { return ring + (e % S::kStages) * S::kTile; };
+  // the oldest tile that is not announced yet has landed
+  auto announce = [&]() {
+    const int e = announced++, t = tiles.x + e / 2;
+    if (e & 1) {
+      const int j0 = t * kTcSlots;
+      if (j0 < u.lo_max || j0 + kTcSlots > u.hi_min) {  // not seen whole by every row
+#pragma unroll 1
+        for (int i = 0; i < kTcSlots / RP; ++i) {
+          const int r = r0 + i * RP;
+          uint4* at = reinterpret_cast<uint4*>(stage(e) + column + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
+          float f[8];
+          ElemTraits<T>::widen(*at, f);
+          bool finite = true;
+#pragma unroll
+          for (int x = 0; x < 8; ++x) finite = finite && rows_finite(f[x]);
+          if (finite) continue;
+          uint16_t* e16 = reinterpret_cast<uint16_t*>(at);
+          for (int x = 0; x < 8; ++x)
+            if (!rows_finite(ElemTraits<T>::widen1(e16[x]))) e16[x] = 0;
+          for (int x = 0; x < u.rows; ++x)
+            if (j0 + r >= sh.limits[x].x && j0 + r < sh.limits[x].y) sh.spoilt[x] = 1;
+        }
+      }
+    }
+    fence_proxy_async_smem();
+    mbar_arrive(&sh.full[e % S::kStages]);
+  };
+#pragma unroll 1
+  for (int t = tiles.x; t < tiles.y; ++t) {
+    int64_t k, v;
+    const bool ok = rows_slot(p, u, t * kTcSlots + lt, k, v);
+    const unsigned held = __ballot_sync(0xffffffffu, ok);
+    const int b = t & 1;
+    sh.koff[b][lt] = ok ? k : -1;
+    sh.voff[b][lt] = ok ? v : -1;
+    if (lane == 0) sh.mask[(t - tiles.x) & 7][lt >> 5] = held;
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+#pragma unroll 1
+    for (int half = 0; fine && half < 2; ++half) {
+      if (issued >= S::kStages)
+        fine = mbar_wait_bounded(&sh.empty[issued % S::kStages], (issued / S::kStages - 1) & 1);
+      if (!fine) break;
+      const T* base = static_cast<const T*>(half == 0 ? p.c.k : p.c.v) + ch * 8;
+      const int64_t* off = half == 0 ? sh.koff[b] : sh.voff[b];
+      uint8_t* dst = stage(issued) + column;
+#pragma unroll
+      for (int i = 0; i < kTcSlots / RP; ++i) {
+        const int r = r0 + i * RP;
+        const int64_t o = off[r];
+        cp_async_16(dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4), base + (o < 0 ? 0 : o), o < 0 ? 0u : 16u);
+      }
+      cp_async_commit();
+      if (++issued > S::kLag) {
+        cp_async_wait<S::kLag>();
+        announce();
+      }
+    }
+  }
+  cp_async_wait<0>();
+  while (fine && announced < issued) announce();
+}
+
+// The issuing thread.
+template <typename T, int D, int NSUB, int Parts>
+__device__ __forceinline__ void rows_tc_issue(RowsTcShared& sh, uint32_t q, uint32_t ring, int n, int blocks) {
+  using S = RowsTc<D, NSUB>;
+  constexpr uint32_t kS = tc_instruction<T>(kTcSlots, false), kO = tc_instruction<T>(D, true);
+  const uint32_t tmem = sh.tmem;
+  auto full = [&](int e) { return mbar_wait_bounded(&sh.full[e % S::kStages], (e / S::kStages) & 1); };
+  auto scores = [&](int x, int t) {
+    const uint32_t a = q + x * S::kTile, b = ring + (2 * t % S::kStages) * S::kTile;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      const uint32_t at = (k / 4) * S::kPanel + (k % 4) * 32;
+      tc_mma(tmem + x * 128, tc_descriptor(a + at, 16), tc_descriptor(b + at, 16), kS, k > 0);
+    }
+    tc_commit(&sh.s_full[x]);
+  };
+  bool fine = mbar_wait_bounded(&sh.q_full, 0) && full(0);
+  if (fine) {
+    tc_fence_after();
+    for (int x = 0; x < blocks; ++x) scores(x, 0);
+    tc_commit(&sh.empty[0]);
+  }
+#pragma unroll 1
+  for (int t = 0; fine && t < n; ++t) {
+    const int ev = 2 * t + 1;
+    fine = full(ev) && (t + 1 >= n || full(ev + 1));
+    if (!fine) break;
+    const uint32_t v = ring + (ev % S::kStages) * S::kTile;
+    for (int x = 0; x < blocks; ++x) {
+      fine = mbar_wait_bounded(&sh.p_full[x], t & 1);
+      if (!fine) break;
+      tc_fence_after();
+#pragma unroll
+      for (int part = 0; part < Parts; ++part)
+#pragma unroll
+        for (int k = 0; k < kTcSlots / 16; ++k)
+          tc_mma_ts(tmem + NSUB * 128 + x * D, tmem + x * 128 + part * 64 + k * 8,
+                    tc_descriptor(v + k * 2048, S::kPanel), kO, t > 0 || part > 0 || k > 0);
+      if (t + 1 < n) scores(x, t + 1);
+      else tc_commit(&sh.o_full[x]);
+    }
+    if (!fine) break;
+    tc_commit(&sh.empty[ev % S::kStages]);
+    if (t + 1 < n) tc_commit(&sh.empty[(ev + 1) % S::kStages]);
+  }
+  // nothing is left in flight when the tensor memory is freed
+  tc_commit(&sh.drained);
+  mbar_wait_bounded(&sh.drained, 0);
+}
+
+// A softmax thread: row `r` of the CTA.
+template <typename T, int D, int NSUB, int Parts>
+__device__ __forceinline__ void rows_tc_softmax(const RowsParams& p, RowsTcShared& sh, int2 tiles, float scale2) {
+  constexpr float kBelow = std::is_same<T, __half>::value ? 7.0f : 0.0f;
+  const RowsUnit& u = sh.u;
+  const int r = threadIdx.x, x = r / 128;
+  const uint32_t lane0 = static_cast<uint32_t>((r % 128) / 32 * 32) << 16;
+  const uint32_t s_at = sh.tmem + lane0 + x * 128, o_at = sh.tmem + lane0 + NSUB * 128 + x * D;
+  const int2 lim = sh.limits[r];
+  const bool idle = (r & ~31) >= u.rows;  // no row of this warp is one
+  float m = -INFINITY, l = 0.0f;
+  bool fine = true;
+#pragma unroll 1
+  for (int t = tiles.x; t < tiles.y; ++t) {
+    const int i = t - tiles.x, j0 = t * kTcSlots;
+    fine = __all_sync(0xffffffffu, mbar_wait_bounded(&sh.s_full[x], i & 1));
+    if (!fine) break;
+    if (!idle) {
+      tc_fence_after();
+      uint32_t words[4];
+      bool whole = j0 >= u.lo_max && j0 + kTcSlots <= u.hi_min;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        words[w] = *reinterpret_cast<volatile uint32_t*>(&sh.mask[i & 7][w]);
+        whole = whole && words[w] == 0xffffffffu;
+      }
+      if (!whole) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) words[w] &= rows_bits(lim.x - j0 - 32 * w, lim.y - j0 - 32 * w);
+      }
+      uint32_t a[64];
+      tc_load(s_at, a);
+      if (!whole) rows_hide(a, words);
+      float top = __uint_as_float(a[0]);
+#pragma unroll
+      for (int c = 1; c < 64; ++c) top = fmaxf(top, __uint_as_float(a[c]));
+#pragma unroll
+      for (int c0 = 64; c0 < 128; c0 += 32) {
+        uint32_t b[32];
+        tc_load(s_at + c0, b);
+        if (!whole) rows_hide(b, words + c0 / 32);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) top = fmaxf(top, __uint_as_float(b[c]));
+      }
+      top *= scale2;
+      if (__any_sync(0xffffffffu, top > m + (8.0f + kBelow))) {
+        const float mn = fmaxf(m, top - kBelow);
+        const float f = m == -INFINITY ? 0.0f : rows_exp2(m - mn);
+        m = mn;
+        l *= f;
+        if (i > 0) {
+#pragma unroll 1
+          for (int c0 = 0; c0 < D; c0 += 32) {
+            uint32_t o[32];
+            tc_load(o_at + c0, o);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
+            tc_store(o_at + c0, o);
+          }
+        }
+      }
+      const float base = m == -INFINITY ? 0.0f : -m;
+      // 64 weights in 16 bits, 2 a word; with Parts = 2 the remainders too
+      float2 sum = make_float2(0.0f, 0.0f);
+      uint32_t hi[32], lo[32];
+      auto weigh = [&](const uint32_t (&s)[64]) {
+#pragma unroll
+        for (int c = 0; c < 64; c += 2) {
+          const float2 z = ffma2(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])),
+                                 make_float2(scale2, scale2), make_float2(base, base));
+          const float2 w = make_float2(rows_exp2(z.x), rows_exp2(z.y));
+          sum = make_float2(sum.x + w.x, sum.y + w.y);
+          float ra, rb;
+          hi[c / 2] = rows_pack<T>(w.x, w.y, ra, rb);
+          if constexpr (Parts == 2) {
+            float na, nb;
+            lo[c / 2] = rows_pack<T>(ra, rb, na, nb);
+          }
+        }
+      };
+      weigh(a);
+      uint32_t b[64];
+      tc_load(s_at + 64, b);  // before the remainders are stored there
+      if (!whole) rows_hide(b, words + 2);
+      tc_store(s_at, hi);
+      if constexpr (Parts == 2) tc_store(s_at + 64, lo);
+      weigh(b);
+      tc_store(s_at + 32, hi);
+      if constexpr (Parts == 2) tc_store(s_at + 96, lo);
+      l += sum.x + sum.y;
+      tc_wait_stores();
+      tc_fence_before();
+    }
+    mbar_arrive(&sh.p_full[x]);
+  }
+  if (fine) fine = __all_sync(0xffffffffu, mbar_wait_bounded(&sh.o_full[x], 0));
+  if (!fine || idle) return;
+  tc_fence_after();
+  const bool in = r < u.rows;
+  const int rr = in ? u.row0 + r : 0;
+  const int t = rr / p.G, g = rr - t * p.G;
+  const int64_t row = static_cast<int64_t>(u.tok0 + t) * p.H + u.hk * p.G + g;
+  const float nan = __int_as_float(0x7fffffff);
+  const float spoil = in && sh.spoilt[r] ? nan : 1.0f;
+  const int64_t part = u.split * (static_cast<int64_t>(p.T) * p.H) + row;
+  const float inv = p.part_o != nullptr ? spoil : l == 0.0f ? 0.0f : spoil / l;
+#pragma unroll 1
+  for (int c0 = 0; c0 < D; c0 += 32) {
+    uint32_t o[32];
+    __syncwarp();
+    tc_load(o_at + c0, o);
+    float f[32];
+#pragma unroll
+    for (int c = 0; c < 32; ++c) f[c] = l == 0.0f ? 0.0f : __uint_as_float(o[c]) * inv;
+    if (in && p.part_o != nullptr) {
+      float4* dst = reinterpret_cast<float4*>(p.part_o + part * D + c0);
+#pragma unroll
+      for (int c = 0; c < 32; c += 4) dst[c / 4] = make_float4(f[c], f[c + 1], f[c + 2], f[c + 3]);
+    } else if (in) {
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.o) + row * D + c0);
+#pragma unroll
+      for (int c = 0; c < 32; c += 8) {
+        float ra, rb;
+        uint32_t h[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] = rows_pack<T>(f[c + 2 * e], f[c + 2 * e + 1], ra, rb);
+        dst[c / 8] = make_uint4(h[0], h[1], h[2], h[3]);
+      }
+    }
+  }
+  if (!in) return;
+  if (p.part_o != nullptr) p.part_ml[part] = make_float2(m, l);
+  else if (p.lse != nullptr) p.lse[row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+template <typename T, int D, int NSUB, int Parts>
+__global__ void __launch_bounds__(RowsTc<D, NSUB>::kThreads, NSUB == 1 && D == 64 ? 2 : 1)
+    rows_tc_kernel(const RowsParams p) {
+  using S = RowsTc<D, NSUB>;
+  extern __shared__ uint8_t rt_raw[];
+  __shared__ RowsTcShared sh;
+  uint8_t* q = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(rt_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = q + NSUB * S::kTile;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (!rows_begin<NSUB * 128>(p, sh.u, sh.limits)) return;
+  const RowsUnit& u = sh.u;
+  const int2 tiles = rows_tiles<kTcSlots>(p, u);
+  const int tid = threadIdx.x, n = tiles.y - tiles.x;
+  if (n <= 0) {  // no row of this part sees a slot
+    for (int r = tid; r < u.rows; r += S::kThreads) {
+      const int t = (u.row0 + r) / p.G, g = u.row0 + r - t * p.G;
+      const int64_t row = static_cast<int64_t>(u.tok0 + t) * p.H + u.hk * p.G + g;
+      if (p.part_o != nullptr) {
+        p.part_ml[u.split * (static_cast<int64_t>(p.T) * p.H) + row] = make_float2(-INFINITY, 0.0f);
+        continue;
+      }
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.o) + row * D);
+      for (int c = 0; c < D / 8; ++c) dst[c] = make_uint4(0u, 0u, 0u, 0u);
+      if (p.lse != nullptr) p.lse[row] = -INFINITY;
+    }
+    return;
+  }
+  const int blocks = NSUB == 2 && u.rows > 128 ? 2 : 1;
+  if (tid == S::kMma) {
+    mbar_init(&sh.q_full, blocks * 128);
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&sh.s_full[x], 1);
+      mbar_init(&sh.p_full[x], 128);
+      mbar_init(&sh.o_full[x], 1);
+    }
+    mbar_init(&sh.drained, 1);
+    for (int e = 0; e < S::kStages; ++e) {
+      mbar_init(&sh.full[e], 128);
+      mbar_init(&sh.empty[e], 1);
+    }
+    fence_mbar_init();
+  }
+  if (tid < 256) sh.spoilt[tid] = 0;
+  __syncwarp();
+  if (tid >= S::kMma) tc_alloc(&sh.tmem, S::kColumns);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // scores are scaled by |scale|: its sign goes into q, and for a scale of 0 q is 0
+  const float scale2 = p.scale2 == 0.0f ? 1.0f : fabsf(p.scale2);
+  if (tid < S::kLoad0) {
+    if (tid / 128 < blocks) {
+      constexpr int C = D / 8;
+      const uint32_t flip = p.scale2 < 0.0f ? 0x80008000u : 0u;
+      uint8_t* block = q + tid / 128 * S::kTile;
+#pragma unroll 4
+      for (int i = tid % 128; i < 128 * C; i += 128) {
+        const int r = i / C, ch = i - r * C, rr = u.row0 + tid / 128 * 128 + r;
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        if (tid / 128 * 128 + r < u.rows && p.scale2 != 0.0f) {
+          const int t = rr / p.G, g = rr - t * p.G;
+          w = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (u.tok0 + t) * p.qst +
+                                             (u.hk * p.G + g) * p.qsh)[ch];
+          w = make_uint4(w.x ^ flip, w.y ^ flip, w.z ^ flip, w.w ^ flip);
+        }
+        *reinterpret_cast<uint4*>(block + (ch >> 3) * S::kPanel + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = w;
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&sh.q_full);
+      rows_tc_softmax<T, D, NSUB, Parts>(p, sh, tiles, scale2);
+    }
+  } else if (tid < S::kMma) {
+    rows_tc_load<T, D, NSUB>(p, sh, ring, tiles);
+  } else {
+    if (tid == S::kMma) rows_tc_issue<T, D, NSUB, Parts>(sh, smem_u32(q), smem_u32(ring), n, blocks);
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (tid >= S::kMma) tc_free(sh.tmem, S::kColumns);
+}
+
 // Joins a row's parts: those of its splits, and with `own` (fp32 rows and (m, 1 / l)) that of its own
 // slots. A warp takes a row; parts without a slot (l = 0) have no o.
 constexpr int kRowsMaxSplits = 64;
@@ -452,26 +875,30 @@ __global__ void __launch_bounds__(kRjWarps * 32) rows_join_kernel(const RowsPara
   if (lane == 0 && p.lse != nullptr) p.lse[row] = L == 0.0f ? -INFINITY : (M + log2f(L)) * kLn2;
 }
 
-// How a call is cut: rows a CTA, parts a segment's slots are cut into, CTAs.
+// How a call is cut: query rows a CTA, parts a segment's slots are cut into, CTAs.
 struct RowsPlan {
   int bm, splits;
   int64_t ctas;
 };
 
-static RowsPlan rows_plan(int T, int nseg, int H_kv, int G, int max_slots, int window) {
+static RowsPlan rows_plan(int dtype, int T, int nseg, int H_kv, int G, int D, int max_slots, int window) {
   RowsPlan r;
-  r.bm = kRfRows;
   const int64_t rows = static_cast<int64_t>(T) * G;
-  // every segment adds one tile at most that is not full
+  const bool tc = dtype != DCR_DTYPE_F32;
+  // two blocks of rows where segments have more than one on average
+  r.bm = !tc ? kRfRows : rows > 128ll * nseg ? 256 : 128;
+  // every segment adds one tile of rows at most that is not full
   const int64_t tiles = rows / r.bm + (nseg < rows ? nseg : rows);
+  const int64_t units = tiles * H_kv;
   int64_t slots = max_slots;
   if (window > 0 && static_cast<int64_t>(window) + T < slots) slots = static_cast<int64_t>(window) + T;
-  const int64_t most = slots / (4 * kRfSlots) > 1 ? slots / (4 * kRfSlots) : 1;
-  int64_t want = (4ll * device_sm_count() + tiles * H_kv - 1) / (tiles * H_kv);
+  const int64_t most = slots / (4 * (tc ? kTcSlots : kRfSlots));
+  const int per_sm = !tc ? 4 : r.bm == 128 && D == 64 ? 2 : 1;
+  int64_t want = static_cast<int64_t>(per_sm) * device_sm_count() / units;
   if (want > most) want = most;
   if (want > kRowsMaxSplits) want = kRowsMaxSplits;
-  r.splits = static_cast<int>(want);
-  r.ctas = tiles * H_kv * r.splits;
+  r.splits = want > 1 ? static_cast<int>(want) : 1;
+  r.ctas = units * r.splits;
   return r;
 }
 
@@ -499,15 +926,24 @@ static RowsLayout rows_layout(const RowsPlan& r, int T, int H, int D, size_t att
   return w;
 }
 
-template <typename T, int D>
-static int rows_launch(const RowsParams& p, const RowsPlan& plan, cudaStream_t s) {
-  auto kernel = rows_fma_kernel<T, D>;
-  if (ensure_smem_attr(reinterpret_cast<const void*>(kernel), RowsFma<D>::kSmem) != cudaSuccess)
-    return DCR_ERR_CUDA;
-  return launch_dependent(kernel, dim3(static_cast<unsigned>(plan.ctas)), dim3(kRfThreads),
-                          RowsFma<D>::kSmem, s, 1, p) == cudaSuccess
+template <typename Kernel>
+static int rows_launch_as(Kernel kernel, int threads, int smem, const RowsParams& p, const RowsPlan& plan,
+                          cudaStream_t s) {
+  if (ensure_smem_attr(reinterpret_cast<const void*>(kernel), smem) != cudaSuccess) return DCR_ERR_CUDA;
+  return launch_dependent(kernel, dim3(static_cast<unsigned>(plan.ctas)), dim3(threads), smem, s, 1, p) ==
+                 cudaSuccess
              ? DCR_OK
              : DCR_ERR_CUDA;
+}
+
+template <typename T, int D, int Parts>
+static int rows_launch(const RowsParams& p, const RowsPlan& plan, cudaStream_t s) {
+  if constexpr (sizeof(T) == 4)
+    return rows_launch_as(rows_fma_kernel<T, D>, kRfThreads, RowsFma<D>::kSmem, p, plan, s);
+  else if (plan.bm == 256)
+    return rows_launch_as(rows_tc_kernel<T, D, 2, Parts>, RowsTc<D, 2>::kThreads, RowsTc<D, 2>::kSmem, p, plan, s);
+  else
+    return rows_launch_as(rows_tc_kernel<T, D, 1, Parts>, RowsTc<D, 1>::kThreads, RowsTc<D, 1>::kSmem, p, plan, s);
 }
 
 template <typename T, int D>
@@ -553,10 +989,11 @@ using namespace dcr;
 
 extern "C" {
 
-size_t dcr_paged_prefill_workspace_bytes(int T, int B, int H, int H_kv, int D, int max_slots, int window) {
+size_t dcr_paged_prefill_workspace_bytes(int dtype, int T, int B, int H, int H_kv, int D, int max_slots,
+                                         int window) {
   if (B <= 0 || max_slots <= 0 || (D != 64 && D != 128) || rows_check(T, H, H_kv, window) != DCR_OK)
     return 0;
-  return rows_layout(rows_plan(T, B, H_kv, H / H_kv, max_slots, window), T, H, D, 0, false).total;
+  return rows_layout(rows_plan(dtype, T, B, H_kv, H / H_kv, D, max_slots, window), T, H, D, 0, false).total;
 }
 
 int dcr_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_pages,
@@ -577,7 +1014,7 @@ int dcr_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, con
   if (st != DCR_OK) return st;
   st = rows_check_rows(q, q_stride_t, q_stride_h, o, lse, lengths, starts, nullptr, dtype, T, H, D);
   if (st != DCR_OK) return st;
-  const RowsPlan plan = rows_plan(T, B, H_kv, H / H_kv, max_pages * page_size, window);
+  const RowsPlan plan = rows_plan(dtype, T, B, H_kv, H / H_kv, D, max_pages * page_size, window);
   if (plan.ctas > INT32_MAX) return DCR_ERR_SHAPE;
   const RowsLayout w = rows_layout(plan, T, H, D, 0, false);
   if (workspace == nullptr || misaligned(16, workspace) || workspace_bytes < w.total)
@@ -609,15 +1046,15 @@ int dcr_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, con
   return rows_dispatch(dtype, D, [&](auto type, auto dims) {
     using Ty = decltype(type);
     constexpr int kDim = decltype(dims)::value;
-    const int rc = rows_launch<Ty, kDim>(p, plan, s);
+    const int rc = rows_launch<Ty, kDim, 1>(p, plan, s);
     return rc != DCR_OK || plan.splits == 1 ? rc : rows_join<Ty, kDim>(p, nullptr, nullptr, s);
   });
 }
 
-size_t dcr_paged_shared_workspace_bytes(int B, int groups, int H, int H_kv, int D, int max_slots) {
+size_t dcr_paged_shared_workspace_bytes(int dtype, int B, int groups, int H, int H_kv, int D, int max_slots) {
   if (groups <= 0 || max_slots <= 0 || (D != 64 && D != 128) || rows_check(B, H, H_kv, 0) != DCR_OK)
     return 0;
-  return rows_layout(rows_plan(B, groups, H_kv, H / H_kv, max_slots, 0), B, H, D,
+  return rows_layout(rows_plan(dtype, B, groups, H_kv, H / H_kv, D, max_slots, 0), B, H, D,
                      pa_layout(B, H, H / H_kv, D, max_slots, false).total, true).total;
 }
 
@@ -642,7 +1079,7 @@ int dcr_paged_shared_attend(const void* q, int64_t q_stride_b, int64_t q_stride_
   st = rows_check_rows(q, q_stride_b, q_stride_h, o, lse, lengths, groups, prefix, dtype, B, H, D);
   if (st != DCR_OK) return st;
   const int G = H / H_kv, max_slots = max_pages * page_size;
-  const RowsPlan plan = rows_plan(B, n_groups, H_kv, G, max_slots, 0);
+  const RowsPlan plan = rows_plan(dtype, B, n_groups, H_kv, G, D, max_slots, 0);
   if (plan.ctas > INT32_MAX) return DCR_ERR_SHAPE;
   const PagedAttendLayout a = pa_layout(B, H, G, D, max_slots, false);
   const RowsLayout w = rows_layout(plan, B, H, D, a.total, true);
@@ -700,7 +1137,7 @@ int dcr_paged_shared_attend(const void* q, int64_t q_stride_b, int64_t q_stride_
   return rows_dispatch(dtype, D, [&](auto type, auto dims) {
     using Ty = decltype(type);
     constexpr int kDim = decltype(dims)::value;
-    const int r = rows_launch<Ty, kDim>(p, plan, s);
+    const int r = rows_launch<Ty, kDim, 2>(p, plan, s);
     return r != DCR_OK ? r
                        : rows_join<Ty, kDim>(p, reinterpret_cast<const float*>(ws + w.own_o),
                                              reinterpret_cast<const float2*>(ws + w.own_ml), s);

@@ -316,7 +316,7 @@ PyObject* prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (want_lse) lse = at::empty({T, H}, p.k->options().dtype(at::kFloat));
     if (T > 0 && B > 0) {
       const size_t bytes = dcr_paged_prefill_workspace_bytes(
-          static_cast<int>(T), static_cast<int>(B), static_cast<int>(H), static_cast<int>(p.H_kv),
+          p.dtype, static_cast<int>(T), static_cast<int>(B), static_cast<int>(H), static_cast<int>(p.H_kv),
           static_cast<int>(p.D), static_cast<int>(p.slots), static_cast<int>(window));
       const at::Tensor ws = scratch(a[11], bytes, p.device);
       const int st = dcr_paged_prefill(
@@ -360,7 +360,7 @@ PyObject* shared(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (B > 0) {
       const int n_groups = static_cast<int>(g.size(0) - 1);
       const size_t bytes = dcr_paged_shared_workspace_bytes(
-          static_cast<int>(B), n_groups, static_cast<int>(H), static_cast<int>(p.H_kv),
+          p.dtype, static_cast<int>(B), n_groups, static_cast<int>(H), static_cast<int>(p.H_kv),
           static_cast<int>(p.D), static_cast<int>(p.slots));
       const at::Tensor ws = scratch(a[11], bytes, p.device);
       const int st = dcr_paged_shared_attend(

@@ -58,10 +58,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
 
 def paged_prefill_workspace_bytes(T: int, B: int, H: int, H_kv: int, D: int, max_slots: int,
-                                  window: int = 0) -> int:
+                                  window: int = 0, dtype: torch.dtype = torch.bfloat16) -> int:
     """Bytes :func:`paged_prefill` needs for T tokens of B sequences (max_slots = max_pages *
     page_size)."""
-    return int(_lib.load().dcr_paged_prefill_workspace_bytes(T, B, H, H_kv, D, max_slots, window))
+    return int(_lib.load().dcr_paged_prefill_workspace_bytes(_lib.DTYPE_CODES[dtype], T, B, H, H_kv, D,
+                                                             max_slots, window))
 
 
 def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -87,9 +88,10 @@ def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
 
 
 def paged_shared_workspace_bytes(B: int, groups: int, H: int, H_kv: int, D: int,
-                                 max_slots: int) -> int:
+                                 max_slots: int, dtype: torch.dtype = torch.bfloat16) -> int:
     """Bytes :func:`paged_shared_attention` needs (max_slots = max_pages * page_size)."""
-    return int(_lib.load().dcr_paged_shared_workspace_bytes(B, groups, H, H_kv, D, max_slots))
+    return int(_lib.load().dcr_paged_shared_workspace_bytes(_lib.DTYPE_CODES[dtype], B, groups, H,
+                                                            H_kv, D, max_slots))
 
 
 def paged_shared_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,

@@ -64,11 +64,11 @@ def test_refused(lib, func, base, change, status):  # noqa: F811
 
 def test_workspace_sizes(lib):  # noqa: F811
     slots = MAX_PAGES * PAGE
-    assert lib.dcr_paged_prefill_workspace_bytes(T, B, H, H_KV, D, slots, 0) > 0
-    assert lib.dcr_paged_prefill_workspace_bytes(T, B, 7, H_KV, D, slots, 0) == 0
-    assert lib.dcr_paged_prefill_workspace_bytes(T, B, H, H_KV, 96, slots, 0) == 0
-    assert lib.dcr_paged_shared_workspace_bytes(B, 1, H, H_KV, D, slots) > 0
-    assert lib.dcr_paged_shared_workspace_bytes(B, 0, H, H_KV, D, slots) == 0
+    assert lib.dcr_paged_prefill_workspace_bytes(0, T, B, H, H_KV, D, slots, 0) > 0
+    assert lib.dcr_paged_prefill_workspace_bytes(0, T, B, 7, H_KV, D, slots, 0) == 0
+    assert lib.dcr_paged_prefill_workspace_bytes(0, T, B, H, H_KV, 96, slots, 0) == 0
+    assert lib.dcr_paged_shared_workspace_bytes(0, B, 1, H, H_KV, D, slots) > 0
+    assert lib.dcr_paged_shared_workspace_bytes(0, B, 0, H, H_KV, D, slots) == 0
 
 
 def test_frequencies():
