@@ -409,19 +409,25 @@ struct RowsTc {
   static constexpr int kPanel = 128 * 128;           // bytes of 128 rows of 64 elements
   static constexpr int kTile = D / 64 * kPanel;
   static constexpr int kStages = D == 64 ? (NSUB == 2 ? 8 : 5) : (NSUB == 2 ? 4 : 5);
-  // Tiles that may be on their way before the oldest is announced: two fewer than the ring has, since
-  // a V tile is only released after the K tile behind it was used.
-  static constexpr int kLag = kStages - 2;
+  // Half tiles issued before the oldest is announced. It is announced when the one kLag behind it has
+  // found its place released, so with a lag near the ring's size the products wait for releases
+  // instead of for memory (6 of 8 and 2 of 4: 400 us for a case that takes XX with this).
+  static constexpr int kLag = kStages == 8 ? 4 : kStages == 5 ? 2 : 1;
   static constexpr int kSmem = 1024 + NSUB * kTile + kStages * kTile;
   static constexpr int kColumns = NSUB * (128 + D) > 256 ? 512 : 256;
   static constexpr int kLoad0 = NSUB * 128;          // first loader thread
   static constexpr int kMma = kLoad0 + 128;          // the issuing warp's first thread
-  static constexpr int kThreads = kMma + 32;
+  static constexpr int kThreads = kMma + 128;
+  // Registers a thread: at launch, of the softmax warps and of the others.
+  static constexpr int kAtLaunch = NSUB == 2 ? 128 : 168;
+  static constexpr int kOthers = 56;
+  static constexpr int kSoftmax = NSUB == 2 ? 200 : 240;
+  static_assert(kLoad0 * kSoftmax + 256 * kOthers <= kThreads * kAtLaunch, "shares of the launch's registers");
 };
 
 struct RowsTcShared {
   RowsUnit u;
-  uint64_t q_full, s_full[2], p_full[2], o_full[2], drained;
+  uint64_t q_full, s_full[2], p_full[2][2], o_full[2], drained;
   uint64_t full[8], empty[8];
   uint32_t tmem;
   uint32_t mask[8][4];          // mapped slots of the tiles in flight
@@ -537,54 +543,95 @@ __device__ __forceinline__ void rows_tc_load(const RowsParams& p, RowsTcShared& 
   while (fine && announced < issued) announce();
 }
 
-// The issuing thread.
+// The issuing warp: one of its lanes issues.
 template <typename T, int D, int NSUB, int Parts>
 __device__ __forceinline__ void rows_tc_issue(RowsTcShared& sh, uint32_t q, uint32_t ring, int n, int blocks) {
   using S = RowsTc<D, NSUB>;
   constexpr uint32_t kS = tc_instruction<T>(kTcSlots, false), kO = tc_instruction<T>(D, true);
-  const uint32_t tmem = sh.tmem;
-  auto full = [&](int e) { return mbar_wait_bounded(&sh.full[e % S::kStages], (e / S::kStages) & 1); };
-  auto scores = [&](int x, int t) {
-    const uint32_t a = q + x * S::kTile, b = ring + (2 * t % S::kStages) * S::kTile;
-#pragma unroll
-    for (int k = 0; k < D / 16; ++k) {
-      const uint32_t at = (k / 4) * S::kPanel + (k % 4) * 32;
-      tc_mma(tmem + x * 128, tc_descriptor(a + at, 16), tc_descriptor(b + at, 16), kS, k > 0);
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
+  const uint64_t q_desc = tc_descriptor(q, 16), k_desc = tc_descriptor(ring, 16),
+                 v_desc = tc_descriptor(ring, S::kPanel);
+  int k_stage = 0, v_stage = 1;                 // places of the next K and V
+  uint32_t k_phase = 0, v_phase = 0;
+  auto next = [](int& stage, uint32_t& phase) {
+    stage += 2;
+    if (stage >= S::kStages) {
+      stage -= S::kStages;
+      phase ^= 1;
     }
-    tc_commit(&sh.s_full[x]);
   };
-  bool fine = mbar_wait_bounded(&sh.q_full, 0) && full(0);
+  auto wait = [](uint64_t* bar, uint32_t phase) {
+    return __all_sync(0xffffffffu, mbar_wait_bounded(bar, phase));
+  };
+  auto scores = [&](int x) {
+    const uint64_t a = q_desc + x * (S::kTile / 16), b = k_desc + k_stage * (S::kTile / 16);
+    if (tc_elected()) {
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        constexpr int kStep = S::kPanel / 16;
+        tc_mma(tmem + x * 128, a + (k / 4) * kStep + (k % 4) * 2, b + (k / 4) * kStep + (k % 4) * 2, kS, k > 0);
+      }
+      tc_commit(&sh.s_full[x]);
+    }
+  };
+  bool fine = wait(&sh.q_full, 0) && wait(&sh.full[0], 0);
   if (fine) {
     tc_fence_after();
-    for (int x = 0; x < blocks; ++x) scores(x, 0);
-    tc_commit(&sh.empty[0]);
+    for (int x = 0; x < blocks; ++x) scores(x);
+    if (tc_elected()) tc_commit(&sh.empty[0]);
   }
+  next(k_stage, k_phase);
 #pragma unroll 1
   for (int t = 0; fine && t < n; ++t) {
-    const int ev = 2 * t + 1;
-    fine = full(ev) && (t + 1 >= n || full(ev + 1));
-    if (!fine) break;
-    const uint32_t v = ring + (ev % S::kStages) * S::kTile;
-    for (int x = 0; x < blocks; ++x) {
-      fine = mbar_wait_bounded(&sh.p_full[x], t & 1);
+    const bool last = t + 1 >= n;
+    fine = wait(&sh.full[v_stage], v_phase);
+    const uint64_t v = v_desc + v_stage * (S::kTile / 16);
+#pragma unroll 1
+    for (int x = 0; fine && x < blocks; ++x) {
+      // the first half of the tile's slots while the weights of the second are computed
+#pragma unroll
+      for (int half = 0; fine && half < 2; ++half) {
+        fine = wait(&sh.p_full[x][half], t & 1);
+        if (!fine) break;
+        tc_fence_after();
+        if (tc_elected()) {
+#pragma unroll
+          for (int part = 0; part < Parts; ++part)
+#pragma unroll
+            for (int k = 4 * half; k < 4 * half + 4; ++k)
+              tc_mma_ts(tmem + NSUB * 128 + x * D, tmem + x * 128 + part * 64 + k * 8, v + k * 128, kO,
+                        t > 0 || part > 0 || k > 0);
+          if (half == 1 && last) tc_commit(&sh.o_full[x]);
+        }
+      }
       if (!fine) break;
-      tc_fence_after();
-#pragma unroll
-      for (int part = 0; part < Parts; ++part)
-#pragma unroll
-        for (int k = 0; k < kTcSlots / 16; ++k)
-          tc_mma_ts(tmem + NSUB * 128 + x * D, tmem + x * 128 + part * 64 + k * 8,
-                    tc_descriptor(v + k * 2048, S::kPanel), kO, t > 0 || part > 0 || k > 0);
-      if (t + 1 < n) scores(x, t + 1);
-      else tc_commit(&sh.o_full[x]);
+      if (last) continue;
+      if (x == 0) fine = wait(&sh.full[k_stage], k_phase);
+      if (fine) scores(x);
     }
-    if (!fine) break;
-    tc_commit(&sh.empty[ev % S::kStages]);
-    if (t + 1 < n) tc_commit(&sh.empty[(ev + 1) % S::kStages]);
+    if (fine && tc_elected()) {
+      tc_commit(&sh.empty[v_stage]);
+      if (!last) tc_commit(&sh.empty[k_stage]);
+    }
+    next(v_stage, v_phase);
+    next(k_stage, k_phase);
   }
   // nothing is left in flight when the tensor memory is freed
-  tc_commit(&sh.drained);
-  mbar_wait_bounded(&sh.drained, 0);
+  if (tc_elected()) tc_commit(&sh.drained);
+  wait(&sh.drained, 0);
+}
+
+// The largest of 64 scores, by chains that do not wait for one another.
+__device__ __forceinline__ float rows_max(const uint32_t (&s)[64]) {
+  float m[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m[i] = __uint_as_float(s[i]);
+#pragma unroll
+  for (int c = 4; c < 64; c += 8)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      m[i] = fmaxf(fmaxf(m[i], __uint_as_float(s[c + i])), c + 4 + i < 64 ? __uint_as_float(s[c + 4 + i]) : -INFINITY);
+  return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
 
 // A softmax thread: row `r` of the CTA.
@@ -617,21 +664,15 @@ __device__ __forceinline__ void rows_tc_softmax(const RowsParams& p, RowsTcShare
 #pragma unroll
         for (int w = 0; w < 4; ++w) words[w] &= rows_bits(lim.x - j0 - 32 * w, lim.y - j0 - 32 * w);
       }
-      uint32_t a[64];
-      tc_load(s_at, a);
+      uint32_t a[64], b[64];
+      tc_load_start(s_at, a);
+      tc_load_wait(a);
+      tc_load_start(s_at + 64, b);
       if (!whole) rows_hide(a, words);
-      float top = __uint_as_float(a[0]);
-#pragma unroll
-      for (int c = 1; c < 64; ++c) top = fmaxf(top, __uint_as_float(a[c]));
-#pragma unroll
-      for (int c0 = 64; c0 < 128; c0 += 32) {
-        uint32_t b[32];
-        tc_load(s_at + c0, b);
-        if (!whole) rows_hide(b, words + c0 / 32);
-#pragma unroll
-        for (int c = 0; c < 32; ++c) top = fmaxf(top, __uint_as_float(b[c]));
-      }
-      top *= scale2;
+      float top = rows_max(a);
+      tc_load_wait(b);
+      if (!whole) rows_hide(b, words + 2);
+      top = fmaxf(top, rows_max(b)) * scale2;
       if (__any_sync(0xffffffffu, top > m + (8.0f + kBelow))) {
         const float mn = fmaxf(m, top - kBelow);
         const float f = m == -INFINITY ? 0.0f : rows_exp2(m - mn);
@@ -668,19 +709,21 @@ __device__ __forceinline__ void rows_tc_softmax(const RowsParams& p, RowsTcShare
         }
       };
       weigh(a);
-      uint32_t b[64];
-      tc_load(s_at + 64, b);  // before the remainders are stored there
-      if (!whole) rows_hide(b, words + 2);
       tc_store(s_at, hi);
       if constexpr (Parts == 2) tc_store(s_at + 64, lo);
+      tc_wait_stores();
+      tc_fence_before();
+      mbar_arrive(&sh.p_full[x][0]);
       weigh(b);
       tc_store(s_at + 32, hi);
       if constexpr (Parts == 2) tc_store(s_at + 96, lo);
       l += sum.x + sum.y;
       tc_wait_stores();
       tc_fence_before();
+    } else {
+      mbar_arrive(&sh.p_full[x][0]);
     }
-    mbar_arrive(&sh.p_full[x]);
+    mbar_arrive(&sh.p_full[x][1]);
   }
   if (fine) fine = __all_sync(0xffffffffu, mbar_wait_bounded(&sh.o_full[x], 0));
   if (!fine || idle) return;
@@ -723,8 +766,7 @@ __device__ __forceinline__ void rows_tc_softmax(const RowsParams& p, RowsTcShare
 }
 
 template <typename T, int D, int NSUB, int Parts>
-__global__ void __launch_bounds__(RowsTc<D, NSUB>::kThreads, NSUB == 1 && D == 64 ? 2 : 1)
-    rows_tc_kernel(const RowsParams p) {
+__global__ void __launch_bounds__(RowsTc<D, NSUB>::kThreads, 1) rows_tc_kernel(const RowsParams p) {
   using S = RowsTc<D, NSUB>;
   extern __shared__ uint8_t rt_raw[];
   __shared__ RowsTcShared sh;
@@ -755,7 +797,8 @@ __global__ void __launch_bounds__(RowsTc<D, NSUB>::kThreads, NSUB == 1 && D == 6
     mbar_init(&sh.q_full, blocks * 128);
     for (int x = 0; x < 2; ++x) {
       mbar_init(&sh.s_full[x], 1);
-      mbar_init(&sh.p_full[x], 128);
+      mbar_init(&sh.p_full[x][0], 128);
+      mbar_init(&sh.p_full[x][1], 128);
       mbar_init(&sh.o_full[x], 1);
     }
     mbar_init(&sh.drained, 1);
@@ -767,13 +810,14 @@ __global__ void __launch_bounds__(RowsTc<D, NSUB>::kThreads, NSUB == 1 && D == 6
   }
   if (tid < 256) sh.spoilt[tid] = 0;
   __syncwarp();
-  if (tid >= S::kMma) tc_alloc(&sh.tmem, S::kColumns);
+  if (tid / 32 == S::kMma / 32) tc_alloc(&sh.tmem, S::kColumns);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   // scores are scaled by |scale|: its sign goes into q, and for a scale of 0 q is 0
   const float scale2 = p.scale2 == 0.0f ? 1.0f : fabsf(p.scale2);
   if (tid < S::kLoad0) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSoftmax));
     if (tid / 128 < blocks) {
       constexpr int C = D / 8;
       const uint32_t flip = p.scale2 < 0.0f ? 0x80008000u : 0u;
@@ -795,15 +839,16 @@ __global__ void __launch_bounds__(RowsTc<D, NSUB>::kThreads, NSUB == 1 && D == 6
       rows_tc_softmax<T, D, NSUB, Parts>(p, sh, tiles, scale2);
     }
   } else if (tid < S::kMma) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kOthers));
     rows_tc_load<T, D, NSUB>(p, sh, ring, tiles);
   } else {
-    if (tid == S::kMma) rows_tc_issue<T, D, NSUB, Parts>(sh, smem_u32(q), smem_u32(ring), n, blocks);
-    __syncwarp();
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kOthers));
+    if (tid < S::kMma + 32) rows_tc_issue<T, D, NSUB, Parts>(sh, smem_u32(q), smem_u32(ring), n, blocks);
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (tid >= S::kMma) tc_free(sh.tmem, S::kColumns);
+  if (tid / 32 == S::kMma / 32) tc_free(sh.tmem, S::kColumns);
 }
 
 // Joins a row's parts: those of its splits, and with `own` (fp32 rows and (m, 1 / l)) that of its own
@@ -893,7 +938,7 @@ static RowsPlan rows_plan(int dtype, int T, int nseg, int H_kv, int G, int D, in
   int64_t slots = max_slots;
   if (window > 0 && static_cast<int64_t>(window) + T < slots) slots = static_cast<int64_t>(window) + T;
   const int64_t most = slots / (4 * (tc ? kTcSlots : kRfSlots));
-  const int per_sm = !tc ? 4 : r.bm == 128 && D == 64 ? 2 : 1;
+  const int per_sm = tc ? 1 : 4;
   int64_t want = static_cast<int64_t>(per_sm) * device_sm_count() / units;
   if (want > most) want = most;
   if (want > kRowsMaxSplits) want = kRowsMaxSplits;
