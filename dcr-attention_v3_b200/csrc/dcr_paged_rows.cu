@@ -20,6 +20,7 @@
 // Shared: the prefix is read once for a group instead of once for each of its sequences. Each
 // sequence's own slots go through dcr_paged_attend.cu's kernels into fp32 rows; the parts' (m, l, o)
 // are joined by rows_join_kernel, as are those of a run that is split over several CTAs.
+#include <cuda.h>
 #include <math.h>
 
 #include <type_traits>
@@ -45,6 +46,12 @@ struct RowsParams {
   float* lse;              // [T][H] natural log, or null
   float* part_o;           // [splits][T][H][D], or null: o and lse are written at once
   float2* part_ml;         // [splits][T][H] base of the exponents and sum
+  int box;                 // neighbouring slots that a tensor-map copy brings in (0: no such copies)
+};
+
+// Tensor maps of the pool, for tiles that are whole: boxes of `box` slots of one page.
+struct RowsMaps {
+  CUtensorMap k, v;
 };
 
 // A CTA's rows: BM of a segment's, for one KV head.
@@ -412,7 +419,7 @@ struct RowsTc {
   // Half tiles issued before the oldest is announced. It is announced when the one kLag behind it has
   // found its place released, so with a lag near the ring's size the products wait for releases
   // instead of for memory (6 of 8 and 2 of 4: 400 us for a case that takes XX with this).
-  static constexpr int kLag = kStages == 8 ? 4 : kStages == 5 ? 2 : 1;
+    static constexpr int kLag = kStages == 8 ? 4 : kStages == 5 ? 2 : 1;
   static constexpr int kSmem = 1024 + NSUB * kTile + kStages * kTile;
   static constexpr int kColumns = NSUB * (128 + D) > 256 ? 512 : 256;
   static constexpr int kLoad0 = NSUB * 128;          // first loader thread
@@ -427,7 +434,7 @@ struct RowsTc {
 
 struct RowsTcShared {
   RowsUnit u;
-  uint64_t q_full, s_full[2], p_full[2][2], o_full[2], drained;
+  uint64_t q_full, s_full[2][2], p_full[2][2], o_done[2][2], drained[2];  // [block][half]
   uint64_t full[8], empty[8];
   uint32_t tmem;
   uint32_t mask[8][4];          // mapped slots of the tiles in flight
@@ -454,12 +461,32 @@ __device__ __forceinline__ uint32_t rows_pack(float a, float b, float& ra, float
   return hi;
 }
 
+__device__ __forceinline__ float2 fadd2(float2 a, float2 b) { return ffma2(a, make_float2(1.0f, 1.0f), b); }
+
 // Bits [from, to) of a word that begins at 0.
 __device__ __forceinline__ uint32_t rows_bits(int from, int to) {
   from = max(0, min(32, from));
   to = max(0, min(32, to));
   const uint32_t below = to == 32 ? 0xffffffffu : (1u << to) - 1u;
   return from == 32 ? 0u : below & (0xffffffffu << from);
+}
+
+// Chunk ch of slot row r of a V tile at slot j0: elements that are not finite become 0, and rows that
+// see the slot are noted.
+template <typename T>
+__device__ __forceinline__ void rows_tc_clean(RowsTcShared& sh, uint8_t* column, int j0, int r, int ch) {
+  uint16_t* at = reinterpret_cast<uint16_t*>(column + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
+  const uint4 w = *reinterpret_cast<const uint4*>(at);
+  float f[8];
+  ElemTraits<T>::widen(w, f);
+  bool finite = true;
+#pragma unroll
+  for (int x = 0; x < 8; ++x) finite = finite && rows_finite(f[x]);
+  if (finite) return;
+  for (int x = 0; x < 8; ++x)
+    if (!rows_finite(ElemTraits<T>::widen1(at[x]))) at[x] = 0;
+  for (int x = 0; x < sh.u.rows; ++x)
+    if (j0 + r >= sh.limits[x].x && j0 + r < sh.limits[x].y) sh.spoilt[x] = 1;
 }
 
 template <int N>
@@ -469,68 +496,91 @@ __device__ __forceinline__ void rows_hide(uint32_t (&s)[N], const uint32_t* word
     if (!((words[c / 32] >> (c % 32)) & 1u)) s[c] = 0xff800000u;  // -inf
 }
 
-// The loader warps: tiles [tiles.x, tiles.y), K then V, into the ring.
+// The loader warps: tiles [tiles.x, tiles.y), K then V, into the ring. Thread r looks up slot r of a
+// tile, one tile ahead. A tile whose slots are all there comes by tensor-map copies of up to a page
+// each, which announce themselves; the others (the ends, pages that are not mapped, pages of no
+// multiple of 8 slots) by 16-byte cp.async, zeros for what is not there, announced when they have
+// landed: kLag half tiles later.
 template <typename T, int D, int NSUB>
-__device__ __forceinline__ void rows_tc_load(const RowsParams& p, RowsTcShared& sh, uint8_t* ring, int2 tiles) {
+__device__ __forceinline__ void rows_tc_load(const RowsParams& p, const RowsMaps& maps, RowsTcShared& sh,
+                                             uint8_t* ring, int2 tiles) {
   using S = RowsTc<D, NSUB>;
   constexpr int C = D / 8, RP = 128 / C;  // chunks of a row, rows a step
   const RowsUnit& u = sh.u;
   const int lt = threadIdx.x - S::kLoad0, lane = threadIdx.x & 31;
   const int ch = lt % C, r0 = lt / C;
   const uint32_t column = (ch >> 3) * S::kPanel;
+  const int32_t* table = p.c.table + rows_table(p, u) * p.c.tstride;
   int issued = 0, announced = 0;
-  bool fine = true;  // after a wait that ran out a thread only keeps the others company at the barrier
+  uint32_t by_map = 0;  // of the last 32 half tiles: brought by the tensor map
+  bool fine = true;     // after a wait that ran out a thread only keeps the others company at the barrier
   auto stage = [&](int e) { return ring + (e % S::kStages) * S::kTile; };
-  // the oldest tile that is not announced yet has landed
+  // the oldest half tile that is not announced yet has landed
   auto announce = [&]() {
     const int e = announced++, t = tiles.x + e / 2;
+    if ((by_map >> (e & 31)) & 1u) return;
     if (e & 1) {
       const int j0 = t * kTcSlots;
       if (j0 < u.lo_max || j0 + kTcSlots > u.hi_min) {  // not seen whole by every row
 #pragma unroll 1
-        for (int i = 0; i < kTcSlots / RP; ++i) {
-          const int r = r0 + i * RP;
-          uint4* at = reinterpret_cast<uint4*>(stage(e) + column + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
-          float f[8];
-          ElemTraits<T>::widen(*at, f);
-          bool finite = true;
-#pragma unroll
-          for (int x = 0; x < 8; ++x) finite = finite && rows_finite(f[x]);
-          if (finite) continue;
-          uint16_t* e16 = reinterpret_cast<uint16_t*>(at);
-          for (int x = 0; x < 8; ++x)
-            if (!rows_finite(ElemTraits<T>::widen1(e16[x]))) e16[x] = 0;
-          for (int x = 0; x < u.rows; ++x)
-            if (j0 + r >= sh.limits[x].x && j0 + r < sh.limits[x].y) sh.spoilt[x] = 1;
-        }
+        for (int i = 0; i < kTcSlots / RP; ++i) rows_tc_clean<T>(sh, stage(e) + column, j0, r0 + i * RP, ch);
       }
     }
     fence_proxy_async_smem();
     mbar_arrive(&sh.full[e % S::kStages]);
   };
+  // the table's entry for slot j (below 0: none that any row sees)
+  auto entry = [&](int j, uint32_t& in) {
+    const uint32_t pi = p.c.page.div(j);
+    in = j - pi * p.c.page.d;
+    return j >= u.lo_min && j < u.hi_max ? table[pi] : -1;
+  };
+  uint32_t in;
+  int pg = entry(tiles.x * kTcSlots + lt, in);
 #pragma unroll 1
   for (int t = tiles.x; t < tiles.y; ++t) {
-    int64_t k, v;
-    const bool ok = rows_slot(p, u, t * kTcSlots + lt, k, v);
-    const unsigned held = __ballot_sync(0xffffffffu, ok);
+    const int page = checked_page(p.c, pg), slot = in;
+    if (t + 1 < tiles.y) pg = entry((t + 1) * kTcSlots + lt, in);
+    const unsigned held = __ballot_sync(0xffffffffu, page >= 0);
     const int b = t & 1;
-    sh.koff[b][lt] = ok ? k : -1;
-    sh.voff[b][lt] = ok ? v : -1;
+    sh.koff[b][lt] = page < 0 ? -1 : page * p.c.ksp + u.hk * p.c.ksh + slot * p.c.ksr;
+    sh.voff[b][lt] = page < 0 ? -1 : page * p.c.vsp + u.hk * p.c.vsh + slot * p.c.vsr;
     if (lane == 0) sh.mask[(t - tiles.x) & 7][lt >> 5] = held;
-    asm volatile("bar.sync 1, 128;" ::: "memory");
+    const bool seen = t * kTcSlots >= u.lo_max && (t + 1) * kTcSlots <= u.hi_min;
+    uint32_t whole;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+        "bar.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(whole)
+        : "r"(static_cast<uint32_t>(seen && page >= 0 && p.box > 0))
+        : "memory");
 #pragma unroll 1
     for (int half = 0; fine && half < 2; ++half) {
       if (issued >= S::kStages)
-        fine = mbar_wait_bounded(&sh.empty[issued % S::kStages], (issued / S::kStages - 1) & 1);
+        fine = mbar_wait_short(&sh.empty[issued % S::kStages], (issued / S::kStages - 1) & 1);
       if (!fine) break;
-      const T* base = static_cast<const T*>(half == 0 ? p.c.k : p.c.v) + ch * 8;
-      const int64_t* off = half == 0 ? sh.koff[b] : sh.voff[b];
-      uint8_t* dst = stage(issued) + column;
+      uint64_t* full = &sh.full[issued % S::kStages];
+      by_map = (by_map & ~(1u << (issued & 31))) | (whole << (issued & 31));
+      if (whole != 0) {
+        if ((lt & (p.box - 1)) == 0) {
+          mbar_arrive_expect_tx(full, static_cast<uint32_t>(p.box) * D * 2);
 #pragma unroll
-      for (int i = 0; i < kTcSlots / RP; ++i) {
-        const int r = r0 + i * RP;
-        const int64_t o = off[r];
-        cp_async_16(dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4), base + (o < 0 ? 0 : o), o < 0 ? 0u : 16u);
+          for (int x = 0; x < D / 64; ++x)
+            tma_load_4d_tile(stage(issued) + x * S::kPanel + lt * 128, half == 0 ? &maps.k : &maps.v, full,
+                             64 * x, slot, u.hk, page);
+        } else {
+          mbar_arrive(full);
+        }
+      } else {
+        const T* base = static_cast<const T*>(half == 0 ? p.c.k : p.c.v) + ch * 8;
+        const int64_t* off = half == 0 ? sh.koff[b] : sh.voff[b];
+        uint8_t* dst = stage(issued) + column;
+#pragma unroll
+        for (int i = 0; i < kTcSlots / RP; ++i) {
+          const int r = r0 + i * RP;
+          const int64_t o = off[r];
+          cp_async_16(dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4), base + (o < 0 ? 0 : o), o < 0 ? 0u : 16u);
+        }
       }
       cp_async_commit();
       if (++issued > S::kLag) {
@@ -541,15 +591,18 @@ __device__ __forceinline__ void rows_tc_load(const RowsParams& p, RowsTcShared& 
   }
   cp_async_wait<0>();
   while (fine && announced < issued) announce();
+  // nothing is left on its way into shared memory
+  for (int e = fine ? issued : max(0, issued - S::kStages); e < issued; ++e)
+    if ((by_map >> (e & 31)) & 1u) mbar_wait_bounded(&sh.full[e % S::kStages], (e / S::kStages) & 1);
 }
 
-// The issuing warp: one of its lanes issues.
+// The issuing warp of block x: one of its lanes issues.
 template <typename T, int D, int NSUB, int Parts>
-__device__ __forceinline__ void rows_tc_issue(RowsTcShared& sh, uint32_t q, uint32_t ring, int n, int blocks) {
+__device__ __forceinline__ void rows_tc_issue(RowsTcShared& sh, uint32_t q, uint32_t ring, int n, int x) {
   using S = RowsTc<D, NSUB>;
-  constexpr uint32_t kS = tc_instruction<T>(kTcSlots, false), kO = tc_instruction<T>(D, true);
+  constexpr uint32_t kS = tc_instruction<T>(kTcSlots / 2, false), kO = tc_instruction<T>(D, true);
   const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
-  const uint64_t q_desc = tc_descriptor(q, 16), k_desc = tc_descriptor(ring, 16),
+  const uint64_t q_desc = tc_descriptor(q + x * S::kTile, 16), k_desc = tc_descriptor(ring, 16),
                  v_desc = tc_descriptor(ring, S::kPanel);
   int k_stage = 0, v_stage = 1;                 // places of the next K and V
   uint32_t k_phase = 0, v_phase = 0;
@@ -561,23 +614,24 @@ __device__ __forceinline__ void rows_tc_issue(RowsTcShared& sh, uint32_t q, uint
     }
   };
   auto wait = [](uint64_t* bar, uint32_t phase) {
-    return __all_sync(0xffffffffu, mbar_wait_bounded(bar, phase));
+    return __all_sync(0xffffffffu, mbar_wait_short(bar, phase));
   };
-  auto scores = [&](int x) {
-    const uint64_t a = q_desc + x * (S::kTile / 16), b = k_desc + k_stage * (S::kTile / 16);
+  // S of half h of the tile in k_stage
+  auto scores = [&](int h) {
+    const uint64_t b = k_desc + k_stage * (S::kTile / 16) + h * 512;
     if (tc_elected()) {
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
         constexpr int kStep = S::kPanel / 16;
-        tc_mma(tmem + x * 128, a + (k / 4) * kStep + (k % 4) * 2, b + (k / 4) * kStep + (k % 4) * 2, kS, k > 0);
+        tc_mma(tmem + x * 128 + h * 64, q_desc + (k / 4) * kStep + (k % 4) * 2, b + (k / 4) * kStep + (k % 4) * 2, kS, k > 0);
       }
-      tc_commit(&sh.s_full[x]);
+      tc_commit(&sh.s_full[x][h]);
     }
   };
   bool fine = wait(&sh.q_full, 0) && wait(&sh.full[0], 0);
   if (fine) {
     tc_fence_after();
-    for (int x = 0; x < blocks; ++x) scores(x);
+    for (int h = 0; h < 2; ++h) scores(h);
     if (tc_elected()) tc_commit(&sh.empty[0]);
   }
   next(k_stage, k_phase);
@@ -586,28 +640,23 @@ __device__ __forceinline__ void rows_tc_issue(RowsTcShared& sh, uint32_t q, uint
     const bool last = t + 1 >= n;
     fine = wait(&sh.full[v_stage], v_phase);
     const uint64_t v = v_desc + v_stage * (S::kTile / 16);
-#pragma unroll 1
-    for (int x = 0; fine && x < blocks; ++x) {
-      // the first half of the tile's slots while the weights of the second are computed
 #pragma unroll
-      for (int half = 0; fine && half < 2; ++half) {
-        fine = wait(&sh.p_full[x][half], t & 1);
-        if (!fine) break;
-        tc_fence_after();
-        if (tc_elected()) {
-#pragma unroll
-          for (int part = 0; part < Parts; ++part)
-#pragma unroll
-            for (int k = 4 * half; k < 4 * half + 4; ++k)
-              tc_mma_ts(tmem + NSUB * 128 + x * D, tmem + x * 128 + part * 64 + k * 8, v + k * 128, kO,
-                        t > 0 || part > 0 || k > 0);
-          if (half == 1 && last) tc_commit(&sh.o_full[x]);
-        }
-      }
+    for (int h = 0; fine && h < 2; ++h) {
+      fine = wait(&sh.p_full[x][h], t & 1);
       if (!fine) break;
+      tc_fence_after();
+      if (tc_elected()) {
+#pragma unroll
+        for (int part = 0; part < Parts; ++part)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tc_mma_ts(tmem + NSUB * 128 + x * D, tmem + x * 128 + h * 64 + part * 32 + k * 8,
+                      v + h * 512 + k * 128, kO, t > 0 || h > 0 || part > 0 || k > 0);
+        tc_commit(&sh.o_done[x][h]);
+      }
       if (last) continue;
-      if (x == 0) fine = wait(&sh.full[k_stage], k_phase);
-      if (fine) scores(x);
+      if (h == 0) fine = wait(&sh.full[k_stage], k_phase);
+      if (fine) scores(h);
     }
     if (fine && tc_elected()) {
       tc_commit(&sh.empty[v_stage]);
@@ -617,8 +666,8 @@ __device__ __forceinline__ void rows_tc_issue(RowsTcShared& sh, uint32_t q, uint
     next(k_stage, k_phase);
   }
   // nothing is left in flight when the tensor memory is freed
-  if (tc_elected()) tc_commit(&sh.drained);
-  wait(&sh.drained, 0);
+  if (tc_elected()) tc_commit(&sh.drained[x]);
+  wait(&sh.drained[x], 0);
 }
 
 // The largest of 64 scores, by chains that do not wait for one another.
@@ -646,39 +695,45 @@ __device__ __forceinline__ void rows_tc_softmax(const RowsParams& p, RowsTcShare
   const bool idle = (r & ~31) >= u.rows;  // no row of this warp is one
   float m = -INFINITY, l = 0.0f;
   bool fine = true;
+  const int halves = 2 * (tiles.y - tiles.x);
+  auto wait_scores = [&](int i) {
+    fine = __all_sync(0xffffffffu, mbar_wait_short(&sh.s_full[x][i & 1], (i >> 1) & 1));
+    tc_fence_after();
+  };
+  // The product of half i is done. Its barrier is at that phase or the one before: the half after the
+  // next one has not begun.
+  auto wait_output = [&](int i) {
+    fine = __all_sync(0xffffffffu, mbar_wait_short(&sh.o_done[x][i & 1], (i >> 1) & 1));
+    tc_fence_after();
+  };
 #pragma unroll 1
-  for (int t = tiles.x; t < tiles.y; ++t) {
-    const int i = t - tiles.x, j0 = t * kTcSlots;
-    fine = __all_sync(0xffffffffu, mbar_wait_bounded(&sh.s_full[x], i & 1));
+  for (int i = 0; i < halves; ++i) {
+    const int h = i & 1, j0 = tiles.x * kTcSlots + i * 64;
+    wait_scores(i);
     if (!fine) break;
     if (!idle) {
-      tc_fence_after();
-      uint32_t words[4];
-      bool whole = j0 >= u.lo_max && j0 + kTcSlots <= u.hi_min;
+      uint32_t s[64], words[2];
+      tc_load_start(s_at + h * 64, s);
+      bool whole = j0 >= u.lo_max && j0 + 64 <= u.hi_min;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        words[w] = *reinterpret_cast<volatile uint32_t*>(&sh.mask[i & 7][w]);
+      for (int w = 0; w < 2; ++w) {
+        words[w] = *reinterpret_cast<volatile uint32_t*>(&sh.mask[(i >> 1) & 7][2 * h + w]);
         whole = whole && words[w] == 0xffffffffu;
       }
+      tc_load_wait(s);
       if (!whole) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) words[w] &= rows_bits(lim.x - j0 - 32 * w, lim.y - j0 - 32 * w);
+        for (int w = 0; w < 2; ++w) words[w] &= rows_bits(lim.x - j0 - 32 * w, lim.y - j0 - 32 * w);
+        rows_hide(s, words);
       }
-      uint32_t a[64], b[64];
-      tc_load_start(s_at, a);
-      tc_load_wait(a);
-      tc_load_start(s_at + 64, b);
-      if (!whole) rows_hide(a, words);
-      float top = rows_max(a);
-      tc_load_wait(b);
-      if (!whole) rows_hide(b, words + 2);
-      top = fmaxf(top, rows_max(b)) * scale2;
+      const float top = rows_max(s) * scale2;
       if (__any_sync(0xffffffffu, top > m + (8.0f + kBelow))) {
         const float mn = fmaxf(m, top - kBelow);
         const float f = m == -INFINITY ? 0.0f : rows_exp2(m - mn);
         m = mn;
         l *= f;
         if (i > 0) {
+          wait_output(i - 1);
 #pragma unroll 1
           for (int c0 = 0; c0 < D; c0 += 32) {
             uint32_t o[32];
@@ -693,39 +748,28 @@ __device__ __forceinline__ void rows_tc_softmax(const RowsParams& p, RowsTcShare
       // 64 weights in 16 bits, 2 a word; with Parts = 2 the remainders too
       float2 sum = make_float2(0.0f, 0.0f);
       uint32_t hi[32], lo[32];
-      auto weigh = [&](const uint32_t (&s)[64]) {
 #pragma unroll
-        for (int c = 0; c < 64; c += 2) {
-          const float2 z = ffma2(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])),
-                                 make_float2(scale2, scale2), make_float2(base, base));
-          const float2 w = make_float2(rows_exp2(z.x), rows_exp2(z.y));
-          sum = make_float2(sum.x + w.x, sum.y + w.y);
-          float ra, rb;
-          hi[c / 2] = rows_pack<T>(w.x, w.y, ra, rb);
-          if constexpr (Parts == 2) {
-            float na, nb;
-            lo[c / 2] = rows_pack<T>(ra, rb, na, nb);
-          }
+      for (int c = 0; c < 64; c += 2) {
+        const float2 z = ffma2(make_float2(__uint_as_float(s[c]), __uint_as_float(s[c + 1])),
+                               make_float2(scale2, scale2), make_float2(base, base));
+        const float2 w = make_float2(rows_exp2(z.x), rows_exp2(z.y));
+        sum = fadd2(sum, w);
+        float ra, rb;
+        hi[c / 2] = rows_pack<T>(w.x, w.y, ra, rb);
+        if constexpr (Parts == 2) {
+          float na, nb;
+          lo[c / 2] = rows_pack<T>(ra, rb, na, nb);
         }
-      };
-      weigh(a);
-      tc_store(s_at, hi);
-      if constexpr (Parts == 2) tc_store(s_at + 64, lo);
-      tc_wait_stores();
-      tc_fence_before();
-      mbar_arrive(&sh.p_full[x][0]);
-      weigh(b);
-      tc_store(s_at + 32, hi);
-      if constexpr (Parts == 2) tc_store(s_at + 96, lo);
+      }
+      tc_store(s_at + h * 64, hi);
+      if constexpr (Parts == 2) tc_store(s_at + h * 64 + 32, lo);
       l += sum.x + sum.y;
       tc_wait_stores();
       tc_fence_before();
-    } else {
-      mbar_arrive(&sh.p_full[x][0]);
     }
-    mbar_arrive(&sh.p_full[x][1]);
+    mbar_arrive(&sh.p_full[x][h]);
   }
-  if (fine) fine = __all_sync(0xffffffffu, mbar_wait_bounded(&sh.o_full[x], 0));
+  if (fine) wait_output(halves - 1);
   if (!fine || idle) return;
   tc_fence_after();
   const bool in = r < u.rows;
@@ -766,7 +810,7 @@ __device__ __forceinline__ void rows_tc_softmax(const RowsParams& p, RowsTcShare
 }
 
 template <typename T, int D, int NSUB, int Parts>
-__global__ void __launch_bounds__(RowsTc<D, NSUB>::kThreads, 1) rows_tc_kernel(const RowsParams p) {
+__global__ void __launch_bounds__(RowsTc<D, NSUB>::kThreads, 1) rows_tc_kernel(const RowsParams p, const __grid_constant__ RowsMaps maps) {
   using S = RowsTc<D, NSUB>;
   extern __shared__ uint8_t rt_raw[];
   __shared__ RowsTcShared sh;
@@ -796,15 +840,16 @@ __global__ void __launch_bounds__(RowsTc<D, NSUB>::kThreads, 1) rows_tc_kernel(c
   if (tid == S::kMma) {
     mbar_init(&sh.q_full, blocks * 128);
     for (int x = 0; x < 2; ++x) {
-      mbar_init(&sh.s_full[x], 1);
-      mbar_init(&sh.p_full[x][0], 128);
-      mbar_init(&sh.p_full[x][1], 128);
-      mbar_init(&sh.o_full[x], 1);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&sh.s_full[x][h], 1);
+        mbar_init(&sh.p_full[x][h], 128);
+        mbar_init(&sh.o_done[x][h], 1);
+      }
+      mbar_init(&sh.drained[x], 1);
     }
-    mbar_init(&sh.drained, 1);
     for (int e = 0; e < S::kStages; ++e) {
       mbar_init(&sh.full[e], 128);
-      mbar_init(&sh.empty[e], 1);
+      mbar_init(&sh.empty[e], blocks);
     }
     fence_mbar_init();
   }
@@ -840,10 +885,11 @@ __global__ void __launch_bounds__(RowsTc<D, NSUB>::kThreads, 1) rows_tc_kernel(c
     }
   } else if (tid < S::kMma) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kOthers));
-    rows_tc_load<T, D, NSUB>(p, sh, ring, tiles);
+    rows_tc_load<T, D, NSUB>(p, maps, sh, ring, tiles);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kOthers));
-    if (tid < S::kMma + 32) rows_tc_issue<T, D, NSUB, Parts>(sh, smem_u32(q), smem_u32(ring), n, blocks);
+    const int x = __shfl_sync(0xffffffffu, (tid - S::kMma) / 32, 0);
+    if (x < blocks) rows_tc_issue<T, D, NSUB, Parts>(sh, smem_u32(q), smem_u32(ring), n, x);
   }
   tc_fence_before();
   __syncthreads();
@@ -971,24 +1017,54 @@ static RowsLayout rows_layout(const RowsPlan& r, int T, int H, int D, size_t att
   return w;
 }
 
-template <typename Kernel>
-static int rows_launch_as(Kernel kernel, int threads, int smem, const RowsParams& p, const RowsPlan& plan,
-                          cudaStream_t s) {
+template <typename Kernel, typename... Args>
+static int rows_launch_as(Kernel kernel, int threads, int smem, const RowsPlan& plan, cudaStream_t s,
+                          const Args&... args) {
   if (ensure_smem_attr(reinterpret_cast<const void*>(kernel), smem) != cudaSuccess) return DCR_ERR_CUDA;
-  return launch_dependent(kernel, dim3(static_cast<unsigned>(plan.ctas)), dim3(threads), smem, s, 1, p) ==
+  return launch_dependent(kernel, dim3(static_cast<unsigned>(plan.ctas)), dim3(threads), smem, s, 1, args...) ==
                  cudaSuccess
              ? DCR_OK
              : DCR_ERR_CUDA;
 }
 
+// The pool as tensor maps of boxes of `box` slots; false where its strides are none that a map takes.
+template <typename T>
+static bool rows_map(CUtensorMap* map, const PagePool& c, const void* base, int64_t sp, int64_t sh,
+                     int64_t sr, int H_kv, int D, int box) {
+  EncodeTiledFn encode = get_encode_fn();
+  if (!encode) return false;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), c.page.d, static_cast<cuuint64_t>(H_kv),
+                              static_cast<cuuint64_t>(c.num_pages)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(sr) * 2, static_cast<cuuint64_t>(sh) * 2,
+                                 static_cast<cuuint64_t>(sp) * 2};
+  const cuuint32_t size[4] = {64u, static_cast<cuuint32_t>(box), 1u, 1u}, step[4] = {1u, 1u, 1u, 1u};
+  return encode(map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                4, const_cast<void*>(base), dims, strides, size, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int D, int Parts>
-static int rows_launch(const RowsParams& p, const RowsPlan& plan, cudaStream_t s) {
-  if constexpr (sizeof(T) == 4)
-    return rows_launch_as(rows_fma_kernel<T, D>, kRfThreads, RowsFma<D>::kSmem, p, plan, s);
-  else if (plan.bm == 256)
-    return rows_launch_as(rows_tc_kernel<T, D, 2, Parts>, RowsTc<D, 2>::kThreads, RowsTc<D, 2>::kSmem, p, plan, s);
-  else
-    return rows_launch_as(rows_tc_kernel<T, D, 1, Parts>, RowsTc<D, 1>::kThreads, RowsTc<D, 1>::kSmem, p, plan, s);
+static int rows_launch(const RowsParams& params, const RowsPlan& plan, cudaStream_t s) {
+  if constexpr (sizeof(T) == 4) {
+    return rows_launch_as(rows_fma_kernel<T, D>, kRfThreads, RowsFma<D>::kSmem, plan, s, params);
+  } else {
+    RowsParams p = params;
+    RowsMaps maps = {};
+    // the largest power of two that divides a page, at most a tile; 8 slots are a swizzle's period
+    int box = static_cast<int>(p.c.page.d & (~p.c.page.d + 1));
+    if (box > kTcSlots) box = kTcSlots;
+    p.box = box >= 8 && rows_map<T>(&maps.k, p.c, p.c.k, p.c.ksp, p.c.ksh, p.c.ksr, p.H_kv, D, box) &&
+                    rows_map<T>(&maps.v, p.c, p.c.v, p.c.vsp, p.c.vsh, p.c.vsr, p.H_kv, D, box)
+                ? box
+                : 0;
+    if (plan.bm == 256)
+      return rows_launch_as(rows_tc_kernel<T, D, 2, Parts>, RowsTc<D, 2>::kThreads, RowsTc<D, 2>::kSmem, plan, s,
+                            p, maps);
+    return rows_launch_as(rows_tc_kernel<T, D, 1, Parts>, RowsTc<D, 1>::kThreads, RowsTc<D, 1>::kSmem, plan, s,
+                          p, maps);
+  }
 }
 
 template <typename T, int D>
@@ -1087,6 +1163,7 @@ int dcr_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, con
   p.lse = lse;
   p.part_o = plan.splits > 1 ? reinterpret_cast<float*>(ws + w.o) : nullptr;
   p.part_ml = plan.splits > 1 ? reinterpret_cast<float2*>(ws + w.ml) : nullptr;
+  p.box = 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return rows_dispatch(dtype, D, [&](auto type, auto dims) {
     using Ty = decltype(type);
@@ -1176,6 +1253,7 @@ int dcr_paged_shared_attend(const void* q, int64_t q_stride_b, int64_t q_stride_
   p.lse = lse;
   p.part_o = reinterpret_cast<float*>(ws + w.o);
   p.part_ml = reinterpret_cast<float2*>(ws + w.ml);
+  p.box = 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int rc = pa_launch_any<true>(own, dtype, D, HB, a.ctas, s);
   if (rc != DCR_OK) return rc;

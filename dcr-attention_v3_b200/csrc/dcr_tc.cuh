@@ -78,6 +78,34 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// 4-D tiled TMA load (no multicast) completing on an mbarrier.
+__device__ __forceinline__ void tma_load_4d_tile(void* smem_dst, const void* tmap, uint64_t* bar, int x, int y,
+                                                 int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+// mbar_wait_bounded for waits that are short as a rule: a try suspends the thread for up to 1 ms, so
+// that waiting warps take no issue slots, and the clock is looked at after 2000 of them only.
+__device__ __forceinline__ bool mbar_wait_short(uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+  for (int i = 0; i < 2000; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+        : "memory");
+    if (done != 0) return true;
+  }
+  return mbar_wait_bounded(bar, parity);
+}
+
 // Columns of this thread's lane (each warp reaches the 32 lanes of its place in its warpgroup): started,
 // and waited for by a statement that every register goes through, so that nothing uses one before it
 // is there. The wait is for all loads of the thread.
