@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(kRfThreads) rows_fma_kernel(const RowsParams p
 }
 
 // ---------------------------------------------------------------------------------------
-// 16-bit rows: NSUB blocks of 128 query rows against tiles of 128 slots on the tensor cores.
+// 16-bit rows: two blocks of 128 query rows against tiles of 128 slots on the tensor cores.
 //
 // Warps: four per block of rows for the softmax, a row a thread; four that bring K and V in, a
 // slot's address a thread; one that issues the products. Per tile and block S = Q K^T goes to tensor
@@ -411,35 +411,36 @@ __global__ void __launch_bounds__(kRfThreads) rows_fma_kernel(const RowsParams p
 // ---------------------------------------------------------------------------------------
 constexpr int kTcSlots = 128;
 
-template <int D, int NSUB>
+template <int D, bool Twin>
 struct RowsTc {
+  static constexpr int kRows = Twin ? 128 : 256;     // query rows a CTA
   static constexpr int kPanel = 128 * 128;           // bytes of 128 rows of 64 elements
   static constexpr int kTile = D / 64 * kPanel;
-  static constexpr int kStages = D == 64 ? (NSUB == 2 ? 8 : 5) : (NSUB == 2 ? 4 : 5);
-  // Half tiles issued before the oldest is announced. It is announced when the one kLag behind it has
-  // found its place released, so with a lag near the ring's size the products wait for releases
-  // instead of for memory (6 of 8 and 2 of 4: 400 us for a case that takes XX with this).
-    static constexpr int kLag = kStages == 8 ? 4 : kStages == 5 ? 2 : 1;
-  static constexpr int kSmem = 1024 + NSUB * kTile + kStages * kTile;
-  static constexpr int kColumns = NSUB * (128 + D) > 256 ? 512 : 256;
-  static constexpr int kLoad0 = NSUB * 128;          // first loader thread
-  static constexpr int kMma = kLoad0 + 128;          // the issuing warp's first thread
+  static constexpr int kQ = kRows / 128 * kTile;
+  static constexpr int kStages = Twin ? (D == 64 ? 12 : 5) : (D == 64 ? 8 : 4);
+  // Half tiles issued before the oldest that cp.async brings is announced. It is announced when the one
+  // kLag behind it has found its place released, so with a lag near the ring's size the products
+  // wait for releases instead of for memory.
+  static constexpr int kLag = kStages / 2 - 1;
+  static constexpr int kSmem = 1024 + kQ + kStages * kTile;
+  static constexpr int kColumns = 512;
+  static constexpr int kLoad0 = 256;                 // first loader thread
+  static constexpr int kMma = kLoad0 + 128;          // the issuing warps' first thread
   static constexpr int kThreads = kMma + 128;
   // Registers a thread: at launch, of the softmax warps and of the others.
-  static constexpr int kAtLaunch = NSUB == 2 ? 128 : 168;
-  static constexpr int kOthers = 56;
-  static constexpr int kSoftmax = NSUB == 2 ? 200 : 240;
+  static constexpr int kAtLaunch = 128, kOthers = 56, kSoftmax = 200;
   static_assert(kLoad0 * kSoftmax + 256 * kOthers <= kThreads * kAtLaunch, "shares of the launch's registers");
 };
 
 struct RowsTcShared {
   RowsUnit u;
   uint64_t q_full, s_full[2][2], p_full[2][2], o_done[2][2], drained[2];  // [block][half]
-  uint64_t full[8], empty[8];
+  uint64_t full[12], empty[12];
   uint32_t tmem;
   uint32_t mask[8][4];          // mapped slots of the tiles in flight
   int64_t koff[2][kTcSlots], voff[2][kTcSlots];
   int2 limits[256];
+  float2 part[128];             // Twin: the second block's bases and sums
   uint8_t spoilt[256];          // rows that see a value that is not finite, in a tile not seen whole
 };
 
@@ -501,10 +502,10 @@ __device__ __forceinline__ void rows_hide(uint32_t (&s)[N], const uint32_t* word
 // each, which announce themselves; the others (the ends, pages that are not mapped, pages of no
 // multiple of 8 slots) by 16-byte cp.async, zeros for what is not there, announced when they have
 // landed: kLag half tiles later.
-template <typename T, int D, int NSUB>
+template <typename T, int D, bool Twin>
 __device__ __forceinline__ void rows_tc_load(const RowsParams& p, const RowsMaps& maps, RowsTcShared& sh,
                                              uint8_t* ring, int2 tiles) {
-  using S = RowsTc<D, NSUB>;
+  using S = RowsTc<D, Twin>;
   constexpr int C = D / 8, RP = 128 / C;  // chunks of a row, rows a step
   const RowsUnit& u = sh.u;
   const int lt = threadIdx.x - S::kLoad0, lane = threadIdx.x & 31;
@@ -597,14 +598,14 @@ __device__ __forceinline__ void rows_tc_load(const RowsParams& p, const RowsMaps
 }
 
 // The issuing warp of block x: one of its lanes issues.
-template <typename T, int D, int NSUB, int Parts>
+template <typename T, int D, bool Twin, int Parts>
 __device__ __forceinline__ void rows_tc_issue(RowsTcShared& sh, uint32_t q, uint32_t ring, int n, int x) {
-  using S = RowsTc<D, NSUB>;
+  using S = RowsTc<D, Twin>;
   constexpr uint32_t kS = tc_instruction<T>(kTcSlots / 2, false), kO = tc_instruction<T>(D, true);
   const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
-  const uint64_t q_desc = tc_descriptor(q + x * S::kTile, 16), k_desc = tc_descriptor(ring, 16),
+  const uint64_t q_desc = tc_descriptor(q + (Twin ? 0 : x * S::kTile), 16), k_desc = tc_descriptor(ring, 16),
                  v_desc = tc_descriptor(ring, S::kPanel);
-  int k_stage = 0, v_stage = 1;                 // places of the next K and V
+  int k_stage = 0, v_stage = 1;                 // places of the K and V in use
   uint32_t k_phase = 0, v_phase = 0;
   auto next = [](int& stage, uint32_t& phase) {
     stage += 2;
@@ -616,54 +617,53 @@ __device__ __forceinline__ void rows_tc_issue(RowsTcShared& sh, uint32_t q, uint
   auto wait = [](uint64_t* bar, uint32_t phase) {
     return __all_sync(0xffffffffu, mbar_wait_short(bar, phase));
   };
-  // S of half h of the tile in k_stage
-  auto scores = [&](int h) {
-    const uint64_t b = k_desc + k_stage * (S::kTile / 16) + h * 512;
+  bool fine = wait(&sh.q_full, 0);
+  tc_fence_after();
+  // S of a step, buffer b: with Twin this block's half of the next K tile, else half b of it
+  auto scores = [&](int b) {
+    const int h = Twin ? x : b;
+    if (Twin || b == 0) fine = fine && wait(&sh.full[k_stage], k_phase);
+    if (!fine) return;
+    const uint64_t k0 = k_desc + k_stage * (S::kTile / 16) + h * 512;
     if (tc_elected()) {
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
         constexpr int kStep = S::kPanel / 16;
-        tc_mma(tmem + x * 128 + h * 64, q_desc + (k / 4) * kStep + (k % 4) * 2, b + (k / 4) * kStep + (k % 4) * 2, kS, k > 0);
+        tc_mma(tmem + x * 128 + b * 64, q_desc + (k / 4) * kStep + (k % 4) * 2, k0 + (k / 4) * kStep + (k % 4) * 2,
+               kS, k > 0);
       }
-      tc_commit(&sh.s_full[x][h]);
+      tc_commit(&sh.s_full[x][b]);
+      if (Twin || b == 1) tc_commit(&sh.empty[k_stage]);
     }
+    if (Twin || b == 1) next(k_stage, k_phase);
   };
-  bool fine = wait(&sh.q_full, 0) && wait(&sh.full[0], 0);
-  if (fine) {
-    tc_fence_after();
-    for (int h = 0; h < 2; ++h) scores(h);
-    if (tc_elected()) tc_commit(&sh.empty[0]);
-  }
-  next(k_stage, k_phase);
+  const int steps = Twin ? n : 2 * n;
+  scores(0);
+  if (steps > 1) scores(1);
 #pragma unroll 1
-  for (int t = 0; fine && t < n; ++t) {
-    const bool last = t + 1 >= n;
-    fine = wait(&sh.full[v_stage], v_phase);
-    const uint64_t v = v_desc + v_stage * (S::kTile / 16);
+  for (int i = 0; fine && i < steps; i += 2) {
 #pragma unroll
-    for (int h = 0; fine && h < 2; ++h) {
-      fine = wait(&sh.p_full[x][h], t & 1);
+    for (int b = 0; b < 2; ++b) {
+      if (i + b >= steps) break;
+      const int h = Twin ? x : b;
+      if (Twin || b == 0) fine = wait(&sh.full[v_stage], v_phase);
+      fine = fine && wait(&sh.p_full[x][b], (i >> 1) & 1);
       if (!fine) break;
       tc_fence_after();
+      const uint64_t v = v_desc + v_stage * (S::kTile / 16) + h * 512;
       if (tc_elected()) {
 #pragma unroll
         for (int part = 0; part < Parts; ++part)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            tc_mma_ts(tmem + NSUB * 128 + x * D, tmem + x * 128 + h * 64 + part * 32 + k * 8,
-                      v + h * 512 + k * 128, kO, t > 0 || h > 0 || part > 0 || k > 0);
-        tc_commit(&sh.o_done[x][h]);
+            tc_mma_ts(tmem + 256 + x * D, tmem + x * 128 + b * 64 + part * 32 + k * 8, v + k * 128, kO,
+                      i > 0 || b > 0 || part > 0 || k > 0);
+        tc_commit(&sh.o_done[x][b]);
+        if (Twin || b == 1) tc_commit(&sh.empty[v_stage]);
       }
-      if (last) continue;
-      if (h == 0) fine = wait(&sh.full[k_stage], k_phase);
-      if (fine) scores(h);
+      if (Twin || b == 1) next(v_stage, v_phase);
+      if (i + b + 2 < steps) scores(b);
     }
-    if (fine && tc_elected()) {
-      tc_commit(&sh.empty[v_stage]);
-      if (!last) tc_commit(&sh.empty[k_stage]);
-    }
-    next(v_stage, v_phase);
-    next(k_stage, k_phase);
   }
   // nothing is left in flight when the tensor memory is freed
   if (tc_elected()) tc_commit(&sh.drained[x]);
@@ -683,19 +683,22 @@ __device__ __forceinline__ float rows_max(const uint32_t (&s)[64]) {
   return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
 
-// A softmax thread: row `r` of the CTA.
-template <typename T, int D, int NSUB, int Parts>
-__device__ __forceinline__ void rows_tc_softmax(const RowsParams& p, RowsTcShared& sh, int2 tiles, float scale2) {
+// A softmax thread: row `r` of the CTA, of which it leaves base and sum in `state`. False: a wait ran
+// out.
+template <typename T, int D, bool Twin, int Parts>
+__device__ __forceinline__ bool rows_tc_softmax(const RowsParams& p, RowsTcShared& sh, int2 tiles, float scale2,
+                                                float2& state) {
   constexpr float kBelow = std::is_same<T, __half>::value ? 7.0f : 0.0f;
   const RowsUnit& u = sh.u;
-  const int r = threadIdx.x, x = r / 128;
-  const uint32_t lane0 = static_cast<uint32_t>((r % 128) / 32 * 32) << 16;
-  const uint32_t s_at = sh.tmem + lane0 + x * 128, o_at = sh.tmem + lane0 + NSUB * 128 + x * D;
+  const int x = threadIdx.x / 128, r = threadIdx.x % 128 + (Twin ? 0 : x * 128);
+  const uint32_t lane0 = static_cast<uint32_t>((threadIdx.x % 128) / 32 * 32) << 16;
+  const uint32_t s_at = sh.tmem + lane0 + x * 128, o_at = sh.tmem + lane0 + 256 + x * D;
   const int2 lim = sh.limits[r];
   const bool idle = (r & ~31) >= u.rows;  // no row of this warp is one
-  float m = -INFINITY, l = 0.0f;
+  float& m = state.x;
+  float& l = state.y;
   bool fine = true;
-  const int halves = 2 * (tiles.y - tiles.x);
+  const int steps = (Twin ? 1 : 2) * (tiles.y - tiles.x);
   auto wait_scores = [&](int i) {
     fine = __all_sync(0xffffffffu, mbar_wait_short(&sh.s_full[x][i & 1], (i >> 1) & 1));
     tc_fence_after();
@@ -707,17 +710,18 @@ __device__ __forceinline__ void rows_tc_softmax(const RowsParams& p, RowsTcShare
     tc_fence_after();
   };
 #pragma unroll 1
-  for (int i = 0; i < halves; ++i) {
-    const int h = i & 1, j0 = tiles.x * kTcSlots + i * 64;
+  for (int i = 0; i < steps; ++i) {
+    const int b = i & 1, tile = Twin ? i : i >> 1, h = Twin ? x : b;  // buffer; half of the tile
+    const int j0 = (tiles.x + tile) * kTcSlots + h * 64;
     wait_scores(i);
     if (!fine) break;
     if (!idle) {
       uint32_t s[64], words[2];
-      tc_load_start(s_at + h * 64, s);
+      tc_load_start(s_at + b * 64, s);
       bool whole = j0 >= u.lo_max && j0 + 64 <= u.hi_min;
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
-        words[w] = *reinterpret_cast<volatile uint32_t*>(&sh.mask[(i >> 1) & 7][2 * h + w]);
+        words[w] = *reinterpret_cast<volatile uint32_t*>(&sh.mask[tile & 7][2 * h + w]);
         whole = whole && words[w] == 0xffffffffu;
       }
       tc_load_wait(s);
@@ -761,17 +765,52 @@ __device__ __forceinline__ void rows_tc_softmax(const RowsParams& p, RowsTcShare
           lo[c / 2] = rows_pack<T>(ra, rb, na, nb);
         }
       }
-      tc_store(s_at + h * 64, hi);
-      if constexpr (Parts == 2) tc_store(s_at + h * 64 + 32, lo);
+      tc_store(s_at + b * 64, hi);
+      if constexpr (Parts == 2) tc_store(s_at + b * 64 + 32, lo);
       l += sum.x + sum.y;
       tc_wait_stores();
       tc_fence_before();
     }
-    mbar_arrive(&sh.p_full[x][h]);
+    mbar_arrive(&sh.p_full[x][b]);
   }
-  if (fine) wait_output(halves - 1);
-  if (!fine || idle) return;
-  tc_fence_after();
+  if (fine) wait_output(steps - 1);
+  return fine;
+}
+
+// Writes the rows. With Twin the blocks hold two parts of the same rows: the second lays its part out in
+// shared memory, element by element of all rows, and the first joins them.
+template <typename T, int D, bool Twin>
+__device__ __forceinline__ void rows_tc_write(const RowsParams& p, RowsTcShared& sh, float* other, float2 state,
+                                              bool fine) {
+  const RowsUnit& u = sh.u;
+  const int x = threadIdx.x / 128, lr = threadIdx.x % 128, r = lr + (Twin ? 0 : x * 128);
+  const uint32_t o_at = sh.tmem + (static_cast<uint32_t>(lr / 32 * 32) << 16) + 256 + x * D;
+  const bool works = fine && (r & ~31) < u.rows;  // alike for a warp
+  float m = state.x, l = state.y, own = 1.0f, theirs = 0.0f;
+  if constexpr (Twin) {
+    asm volatile("bar.sync 2, 256;" ::: "memory");  // both blocks' products are done: the ring is free
+    if (works && x == 1) {
+      sh.part[lr] = state;
+#pragma unroll 1
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t o[32];
+        tc_load(o_at + c0, o);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) other[(c0 + c) * 128 + lr] = __uint_as_float(o[c]);
+      }
+    }
+    asm volatile("bar.sync 2, 256;" ::: "memory");
+    if (!works || x == 1) return;
+    const float2 b = sh.part[lr];
+    const float M = fmaxf(m, b.x);
+    own = m == -INFINITY ? 0.0f : rows_exp2(m - M);
+    theirs = b.x == -INFINITY ? 0.0f : rows_exp2(b.x - M);
+    // a part without a slot (sum 0) counts for nothing; what else is there is finite, or NaN by right
+    l = (l == 0.0f ? 0.0f : own * l) + (b.y == 0.0f ? 0.0f : theirs * b.y);
+    m = M;
+  } else if (!works) {
+    return;
+  }
   const bool in = r < u.rows;
   const int rr = in ? u.row0 + r : 0;
   const int t = rr / p.G, g = rr - t * p.G;
@@ -787,7 +826,11 @@ __device__ __forceinline__ void rows_tc_softmax(const RowsParams& p, RowsTcShare
     tc_load(o_at + c0, o);
     float f[32];
 #pragma unroll
-    for (int c = 0; c < 32; ++c) f[c] = l == 0.0f ? 0.0f : __uint_as_float(o[c]) * inv;
+    for (int c = 0; c < 32; ++c) {
+      f[c] = __uint_as_float(o[c]);
+      if constexpr (Twin) f[c] = fmaf(theirs, other[(c0 + c) * 128 + lr], own * f[c]);
+      f[c] = l == 0.0f ? 0.0f : f[c] * inv;
+    }
     if (in && p.part_o != nullptr) {
       float4* dst = reinterpret_cast<float4*>(p.part_o + part * D + c0);
 #pragma unroll
@@ -809,16 +852,16 @@ __device__ __forceinline__ void rows_tc_softmax(const RowsParams& p, RowsTcShare
   else if (p.lse != nullptr) p.lse[row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
-template <typename T, int D, int NSUB, int Parts>
-__global__ void __launch_bounds__(RowsTc<D, NSUB>::kThreads, 1) rows_tc_kernel(const RowsParams p, const __grid_constant__ RowsMaps maps) {
-  using S = RowsTc<D, NSUB>;
+template <typename T, int D, bool Twin, int Parts>
+__global__ void __launch_bounds__(RowsTc<D, Twin>::kThreads, 1) rows_tc_kernel(const RowsParams p, const __grid_constant__ RowsMaps maps) {
+  using S = RowsTc<D, Twin>;
   extern __shared__ uint8_t rt_raw[];
   __shared__ RowsTcShared sh;
   uint8_t* q = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(rt_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* ring = q + NSUB * S::kTile;
+  uint8_t* ring = q + S::kQ;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
-  if (!rows_begin<NSUB * 128>(p, sh.u, sh.limits)) return;
+  if (!rows_begin<S::kRows>(p, sh.u, sh.limits)) return;
   const RowsUnit& u = sh.u;
   const int2 tiles = rows_tiles<kTcSlots>(p, u);
   const int tid = threadIdx.x, n = tiles.y - tiles.x;
@@ -836,7 +879,7 @@ __global__ void __launch_bounds__(RowsTc<D, NSUB>::kThreads, 1) rows_tc_kernel(c
     }
     return;
   }
-  const int blocks = NSUB == 2 && u.rows > 128 ? 2 : 1;
+  const int blocks = Twin || u.rows > 128 ? 2 : 1;
   if (tid == S::kMma) {
     mbar_init(&sh.q_full, blocks * 128);
     for (int x = 0; x < 2; ++x) {
@@ -864,32 +907,36 @@ __global__ void __launch_bounds__(RowsTc<D, NSUB>::kThreads, 1) rows_tc_kernel(c
   if (tid < S::kLoad0) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSoftmax));
     if (tid / 128 < blocks) {
-      constexpr int C = D / 8;
+      // the block's rows of q; with Twin each block brings in half of them
+      constexpr int C = D / 8, kRowsHere = Twin ? 64 : 128;
+      const int r0 = tid / 128 * kRowsHere;
       const uint32_t flip = p.scale2 < 0.0f ? 0x80008000u : 0u;
-      uint8_t* block = q + tid / 128 * S::kTile;
 #pragma unroll 4
-      for (int i = tid % 128; i < 128 * C; i += 128) {
-        const int r = i / C, ch = i - r * C, rr = u.row0 + tid / 128 * 128 + r;
+      for (int i = tid % 128; i < kRowsHere * C; i += 128) {
+        const int r = r0 + i / C, ch = i % C, rr = u.row0 + r;
         uint4 w = make_uint4(0u, 0u, 0u, 0u);
-        if (tid / 128 * 128 + r < u.rows && p.scale2 != 0.0f) {
+        if (r < u.rows && p.scale2 != 0.0f) {
           const int t = rr / p.G, g = rr - t * p.G;
           w = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (u.tok0 + t) * p.qst +
                                              (u.hk * p.G + g) * p.qsh)[ch];
           w = make_uint4(w.x ^ flip, w.y ^ flip, w.z ^ flip, w.w ^ flip);
         }
-        *reinterpret_cast<uint4*>(block + (ch >> 3) * S::kPanel + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = w;
+        *reinterpret_cast<uint4*>(q + r / 128 * S::kTile + (ch >> 3) * S::kPanel + r % 128 * 128 +
+                                  (((ch & 7) ^ (r & 7)) << 4)) = w;
       }
       fence_proxy_async_smem();
       mbar_arrive(&sh.q_full);
-      rows_tc_softmax<T, D, NSUB, Parts>(p, sh, tiles, scale2);
+      float2 state = make_float2(-INFINITY, 0.0f);
+      const bool fine = rows_tc_softmax<T, D, Twin, Parts>(p, sh, tiles, scale2, state);
+      rows_tc_write<T, D, Twin>(p, sh, reinterpret_cast<float*>(ring), state, fine);
     }
   } else if (tid < S::kMma) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kOthers));
-    rows_tc_load<T, D, NSUB>(p, maps, sh, ring, tiles);
+    rows_tc_load<T, D, Twin>(p, maps, sh, ring, tiles);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kOthers));
     const int x = __shfl_sync(0xffffffffu, (tid - S::kMma) / 32, 0);
-    if (x < blocks) rows_tc_issue<T, D, NSUB, Parts>(sh, smem_u32(q), smem_u32(ring), n, x);
+    if (x < blocks) rows_tc_issue<T, D, Twin, Parts>(sh, smem_u32(q), smem_u32(ring), n, x);
   }
   tc_fence_before();
   __syncthreads();
@@ -1060,10 +1107,10 @@ static int rows_launch(const RowsParams& params, const RowsPlan& plan, cudaStrea
                 ? box
                 : 0;
     if (plan.bm == 256)
-      return rows_launch_as(rows_tc_kernel<T, D, 2, Parts>, RowsTc<D, 2>::kThreads, RowsTc<D, 2>::kSmem, plan, s,
-                            p, maps);
-    return rows_launch_as(rows_tc_kernel<T, D, 1, Parts>, RowsTc<D, 1>::kThreads, RowsTc<D, 1>::kSmem, plan, s,
-                          p, maps);
+      return rows_launch_as(rows_tc_kernel<T, D, false, Parts>, RowsTc<D, false>::kThreads,
+                            RowsTc<D, false>::kSmem, plan, s, p, maps);
+    return rows_launch_as(rows_tc_kernel<T, D, true, Parts>, RowsTc<D, true>::kThreads, RowsTc<D, true>::kSmem,
+                          plan, s, p, maps);
   }
 }
 
