@@ -417,11 +417,11 @@ struct RowsTc {
   static constexpr int kPanel = 128 * 128;           // bytes of 128 rows of 64 elements
   static constexpr int kTile = D / 64 * kPanel;
   static constexpr int kQ = kRows / 128 * kTile;
-  static constexpr int kStages = Twin ? (D == 64 ? 12 : 5) : (D == 64 ? 8 : 4);
-  // Half tiles issued before the oldest that cp.async brings is announced. It is announced when the one
-  // kLag behind it has found its place released, so with a lag near the ring's size the products
-  // wait for releases instead of for memory.
-  static constexpr int kLag = kStages / 2 - 1;
+  // Places of K and V in turn: an even number, so that each of the two loader groups has its own. (A
+  // thread that used another's could find the phase before the last one's parity, and take a place
+  // that is still in use for released.)
+  static constexpr int kStages = Twin ? (D == 64 ? 12 : 4) : (D == 64 ? 8 : 4);
+  static_assert(kStages % 2 == 0, "places of K and V in turn");
   static constexpr int kSmem = 1024 + kQ + kStages * kTile;
   static constexpr int kColumns = 512;
   static constexpr int kLoad0 = 256;                 // first loader thread
@@ -437,8 +437,8 @@ struct RowsTcShared {
   uint64_t q_full, s_full[2][2], p_full[2][2], o_done[2][2], drained[2];  // [block][half]
   uint64_t full[12], empty[12];
   uint32_t tmem;
-  uint32_t mask[8][4];          // mapped slots of the tiles in flight
-  int64_t koff[2][kTcSlots], voff[2][kTcSlots];
+  uint32_t mask[16][4];         // mapped slots of the tiles in flight
+  int64_t off[2][kTcSlots];     // element offsets of a loader group's slots
   int2 limits[256];
   float2 part[128];             // Twin: the second block's bases and sums
   uint8_t spoilt[256];          // rows that see a value that is not finite, in a tile not seen whole
@@ -497,104 +497,112 @@ __device__ __forceinline__ void rows_hide(uint32_t (&s)[N], const uint32_t* word
     if (!((words[c / 32] >> (c % 32)) & 1u)) s[c] = 0xff800000u;  // -inf
 }
 
-// The loader warps: tiles [tiles.x, tiles.y), K then V, into the ring. Thread r looks up slot r of a
-// tile, one tile ahead. A tile whose slots are all there comes by tensor-map copies of up to a page
-// each, which announce themselves; the others (the ends, pages that are not mapped, pages of no
-// multiple of 8 slots) by 16-byte cp.async, zeros for what is not there, announced when they have
-// landed: kLag half tiles later.
+// A group of two loader warps: the K or the V tiles of [tiles.x, tiles.y), into every other place of the
+// ring. A thread looks up two slots, for the next tile ahead of this one's wait. A tile whose slots are
+// all there comes by tensor-map copies of up to a page each, which announce themselves; the others (the
+// ends, pages that are not mapped, pages of no multiple of 8 slots) by 16-byte cp.async, zeros for what
+// is not there. (One group of four warps for K and V took 1800 cycles a tile of 16-slot pages.)
 template <typename T, int D, bool Twin>
 __device__ __forceinline__ void rows_tc_load(const RowsParams& p, const RowsMaps& maps, RowsTcShared& sh,
                                              uint8_t* ring, int2 tiles) {
   using S = RowsTc<D, Twin>;
-  constexpr int C = D / 8, RP = 128 / C;  // chunks of a row, rows a step
+  constexpr int C = D / 8, RP = 64 / C;  // chunks of a row, rows a step
   const RowsUnit& u = sh.u;
-  const int lt = threadIdx.x - S::kLoad0, lane = threadIdx.x & 31;
-  const int ch = lt % C, r0 = lt / C;
-  const uint32_t column = (ch >> 3) * S::kPanel;
+  const int kind = (threadIdx.x - S::kLoad0) / 64, gt = threadIdx.x % 64, lane = threadIdx.x & 31;  // 0: K, 1: V
   const int32_t* table = p.c.table + rows_table(p, u) * p.c.tstride;
-  int issued = 0, announced = 0;
-  uint32_t by_map = 0;  // of the last 32 half tiles: brought by the tensor map
-  bool fine = true;     // after a wait that ran out a thread only keeps the others company at the barrier
-  auto stage = [&](int e) { return ring + (e % S::kStages) * S::kTile; };
-  // the oldest half tile that is not announced yet has landed
-  auto announce = [&]() {
-    const int e = announced++, t = tiles.x + e / 2;
-    if ((by_map >> (e & 31)) & 1u) return;
-    if (e & 1) {
-      const int j0 = t * kTcSlots;
-      if (j0 < u.lo_max || j0 + kTcSlots > u.hi_min) {  // not seen whole by every row
-#pragma unroll 1
-        for (int i = 0; i < kTcSlots / RP; ++i) rows_tc_clean<T>(sh, stage(e) + column, j0, r0 + i * RP, ch);
-      }
+  const void* map = kind ? &maps.v : &maps.k;
+  const int64_t sp = kind ? p.c.vsp : p.c.ksp, sr = kind ? p.c.vsr : p.c.ksr;
+  const T* base = static_cast<const T*>(kind ? p.c.v : p.c.k) + u.hk * (kind ? p.c.vsh : p.c.ksh) + gt % C * 8;
+  const uint32_t column = (gt % C >> 3) * S::kPanel;
+  int64_t* off = sh.off[kind];
+  const int n = tiles.y - tiles.x;
+  int pg[2];
+  // the table's entries for the thread's slots of tile t (below 0: none that any row sees)
+  auto look_up = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int j = (tiles.x + t) * kTcSlots + gt + 64 * i;
+      pg[i] = t < n && j >= u.lo_min && j < u.hi_max ? table[p.c.page.div(j)] : -1;
     }
-    fence_proxy_async_smem();
-    mbar_arrive(&sh.full[e % S::kStages]);
   };
-  // the table's entry for slot j (below 0: none that any row sees)
-  auto entry = [&](int j, uint32_t& in) {
-    const uint32_t pi = p.c.page.div(j);
-    in = j - pi * p.c.page.d;
-    return j >= u.lo_min && j < u.hi_max ? table[pi] : -1;
-  };
-  uint32_t in;
-  int pg = entry(tiles.x * kTcSlots + lt, in);
+  look_up(0);
+  int st = kind;
+  uint32_t phase = 1;  // of the release before this use of a place: the first use waits for none
+  int issued = 0;
+  bool fine = true;    // after a wait that ran out a thread only keeps the others company at the barrier
 #pragma unroll 1
-  for (int t = tiles.x; t < tiles.y; ++t) {
-    const int page = checked_page(p.c, pg), slot = in;
-    if (t + 1 < tiles.y) pg = entry((t + 1) * kTcSlots + lt, in);
-    const unsigned held = __ballot_sync(0xffffffffu, page >= 0);
-    const int b = t & 1;
-    sh.koff[b][lt] = page < 0 ? -1 : page * p.c.ksp + u.hk * p.c.ksh + slot * p.c.ksr;
-    sh.voff[b][lt] = page < 0 ? -1 : page * p.c.vsp + u.hk * p.c.vsh + slot * p.c.vsr;
-    if (lane == 0) sh.mask[(t - tiles.x) & 7][lt >> 5] = held;
-    const bool seen = t * kTcSlots >= u.lo_max && (t + 1) * kTcSlots <= u.hi_min;
+  for (int t = 0; t < n; ++t) {
+    const int j0 = (tiles.x + t) * kTcSlots;
+    const bool seen = j0 >= u.lo_max && j0 + kTcSlots <= u.hi_min;  // whole, by every row
+    int page[2], in[2];
+    unsigned held[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      page[i] = checked_page(p.c, pg[i]);
+      held[i] = __ballot_sync(0xffffffffu, page[i] >= 0);
+      in[i] = j0 + gt + 64 * i - static_cast<int>(p.c.page.div(j0 + gt + 64 * i) * p.c.page.d);
+    }
+    look_up(t + 1);
     uint32_t whole;
     asm volatile(
         "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
-        "bar.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        "bar.red.and.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
         : "=r"(whole)
-        : "r"(static_cast<uint32_t>(seen && page >= 0 && p.box > 0))
+        : "r"(static_cast<uint32_t>(seen && p.box > 0 && (held[0] & held[1]) == 0xffffffffu)), "r"(2 + kind)
         : "memory");
-#pragma unroll 1
-    for (int half = 0; fine && half < 2; ++half) {
-      if (issued >= S::kStages)
-        fine = mbar_wait_short(&sh.empty[issued % S::kStages], (issued / S::kStages - 1) & 1);
-      if (!fine) break;
-      uint64_t* full = &sh.full[issued % S::kStages];
-      by_map = (by_map & ~(1u << (issued & 31))) | (whole << (issued & 31));
-      if (whole != 0) {
-        if ((lt & (p.box - 1)) == 0) {
-          mbar_arrive_expect_tx(full, static_cast<uint32_t>(p.box) * D * 2);
+    if (fine && 2 * t >= S::kStages) fine = __all_sync(0xffffffffu, mbar_wait_short(&sh.empty[st], phase));
+    // A tile's mask is read by steps that lag its S by two at most, and S of the tile kStages / 2 before
+    // this one is done: 16 places are enough.
+    if (kind == 0 && lane < 2) sh.mask[t & 15][gt / 32 + 2 * lane] = held[lane];
+    __syncwarp();
+    uint8_t* tile = ring + st * S::kTile;
+    if (whole != 0) {
+      if (fine) {
+        // a warp announces half the bytes, whoever copies them
+        if (lane == 0) mbar_arrive_expect_tx(&sh.full[st], S::kTile / 2);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = gt + 64 * i;
+          if ((r & (p.box - 1)) != 0) continue;
 #pragma unroll
           for (int x = 0; x < D / 64; ++x)
-            tma_load_4d_tile(stage(issued) + x * S::kPanel + lt * 128, half == 0 ? &maps.k : &maps.v, full,
-                             64 * x, slot, u.hk, page);
-        } else {
-          mbar_arrive(full);
-        }
-      } else {
-        const T* base = static_cast<const T*>(half == 0 ? p.c.k : p.c.v) + ch * 8;
-        const int64_t* off = half == 0 ? sh.koff[b] : sh.voff[b];
-        uint8_t* dst = stage(issued) + column;
-#pragma unroll
-        for (int i = 0; i < kTcSlots / RP; ++i) {
-          const int r = r0 + i * RP;
-          const int64_t o = off[r];
-          cp_async_16(dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4), base + (o < 0 ? 0 : o), o < 0 ? 0u : 16u);
+            tma_load_4d_tile(tile + x * S::kPanel + r * 128, map, &sh.full[st], 64 * x, in[i], u.hk, page[i]);
         }
       }
-      cp_async_commit();
-      if (++issued > S::kLag) {
-        cp_async_wait<S::kLag>();
-        announce();
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) off[gt + 64 * i] = page[i] < 0 ? -1 : page[i] * sp + in[i] * sr;
+      asm volatile("bar.sync %0, 64;" ::"r"(2 + kind) : "memory");
+      if (fine) {
+#pragma unroll 8
+        for (int i = 0; i < kTcSlots / RP; ++i) {
+          const int r = gt / C + i * RP;
+          const int64_t o = off[r];
+          cp_async_16(tile + column + r * 128 + (((gt % C & 7) ^ (r & 7)) << 4), base + (o < 0 ? 0 : o),
+                      o < 0 ? 0u : 16u);
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        if (kind == 1 && !seen) {
+#pragma unroll 1
+          for (int i = 0; i < kTcSlots / RP; ++i)
+            rows_tc_clean<T>(sh, tile + column, j0, gt / C + i * RP, gt % C);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.full[st]);
       }
     }
+    issued += fine;
+    st += 2;
+    if (st >= S::kStages) {
+      st -= S::kStages;
+      phase ^= 1;
+    }
   }
-  cp_async_wait<0>();
-  while (fine && announced < issued) announce();
-  // nothing is left on its way into shared memory
-  for (int e = fine ? issued : max(0, issued - S::kStages); e < issued; ++e)
-    if ((by_map >> (e & 31)) & 1u) mbar_wait_bounded(&sh.full[e % S::kStages], (e / S::kStages) & 1);
+  // after a wait that ran out: what was issued before it must not be left on its way into shared memory
+  for (int t = max(0, issued - S::kStages / 2); !fine && t < issued; ++t)
+    mbar_wait_bounded(&sh.full[kind + 2 * (t % (S::kStages / 2))], (t / (S::kStages / 2)) & 1);
 }
 
 // The issuing warp of block x: one of its lanes issues.
@@ -721,7 +729,7 @@ __device__ __forceinline__ bool rows_tc_softmax(const RowsParams& p, RowsTcShare
       bool whole = j0 >= u.lo_max && j0 + 64 <= u.hi_min;
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
-        words[w] = *reinterpret_cast<volatile uint32_t*>(&sh.mask[tile & 7][2 * h + w]);
+        words[w] = *reinterpret_cast<volatile uint32_t*>(&sh.mask[tile & 15][2 * h + w]);
         whole = whole && words[w] == 0xffffffffu;
       }
       tc_load_wait(s);
@@ -788,7 +796,7 @@ __device__ __forceinline__ void rows_tc_write(const RowsParams& p, RowsTcShared&
   const bool works = fine && (r & ~31) < u.rows;  // alike for a warp
   float m = state.x, l = state.y, own = 1.0f, theirs = 0.0f;
   if constexpr (Twin) {
-    asm volatile("bar.sync 2, 256;" ::: "memory");  // both blocks' products are done: the ring is free
+    asm volatile("bar.sync 1, 256;" ::: "memory");  // both blocks' products are done: the ring is free
     if (works && x == 1) {
       sh.part[lr] = state;
 #pragma unroll 1
@@ -799,7 +807,7 @@ __device__ __forceinline__ void rows_tc_write(const RowsParams& p, RowsTcShared&
         for (int c = 0; c < 32; ++c) other[(c0 + c) * 128 + lr] = __uint_as_float(o[c]);
       }
     }
-    asm volatile("bar.sync 2, 256;" ::: "memory");
+    asm volatile("bar.sync 1, 256;" ::: "memory");
     if (!works || x == 1) return;
     const float2 b = sh.part[lr];
     const float M = fmaxf(m, b.x);
@@ -891,7 +899,7 @@ __global__ void __launch_bounds__(RowsTc<D, Twin>::kThreads, 1) rows_tc_kernel(c
       mbar_init(&sh.drained[x], 1);
     }
     for (int e = 0; e < S::kStages; ++e) {
-      mbar_init(&sh.full[e], 128);
+      mbar_init(&sh.full[e], 2);
       mbar_init(&sh.empty[e], blocks);
     }
     fence_mbar_init();
