@@ -39,13 +39,15 @@ struct RowsParams {
   const int32_t* starts;   // [nseg + 1] tokens of each segment
   const int32_t* prefix;   // shared: [T]; prefill: null
   int T, nseg, H, H_kv, G;
-  int splits;              // parts that a segment's slots are cut into
+  int pieces;              // CTAs that units are cut up for (0: a unit is one CTA's)
   int window, causal;
   float scale2;            // scale * log2(e)
   void* o;                 // [T][H][D]
   float* lse;              // [T][H] natural log, or null
-  float* part_o;           // [splits][T][H][D], or null: o and lse are written at once
-  float2* part_ml;         // [splits][T][H] base of the exponents and sum
+  float* part_o;           // [places][D], or null: o and lse are written at once
+  float2* part_ml;         // [places] base of the exponents and sum
+  int64_t places;
+  int2* part_of;           // [T][H] a row's first place (the next ones are a CTA's rows on) and their number
   int box;                 // neighbouring slots that a tensor-map copy brings in (0: no such copies)
 };
 
@@ -57,7 +59,7 @@ struct RowsMaps {
 // A CTA's rows: BM of a segment's, for one KV head.
 struct RowsUnit {
   int seg, tok0, ntok, len;  // the segment, its tokens; prefill: its sequence's length
-  int hk, split;
+  int hk, split, parts;      // this CTA's part of the slots
   int row0, rows;            // first row in the segment and their number (0: nothing to do)
   int lo_min, lo_max, hi_min, hi_max;  // over the rows
 };
@@ -85,23 +87,73 @@ __device__ __forceinline__ int2 rows_limits(const RowsParams& p, const RowsUnit&
   return make_int2(p.window > 0 ? max(0, x + 1 - p.window) : 0, p.causal ? x + 1 : u.len);
 }
 
-// Finds this CTA's rows (blockIdx.x = (tile * H_kv + head) * splits + split, tiles from the last to
-// the first, since a causal segment's last rows see most) and their limits. False: none.
+// Tiles of 128 slots that a segment's rows may see, by its first token: how units are cut up goes by
+// them, not what they see.
+__device__ __forceinline__ int rows_weight(const RowsParams& p, int s, int tok0, int ntok) {
+  if (ntok == 0) return 0;
+  int hi, lo = 0;
+  if (p.prefix != nullptr) {
+    const int len = checked_length(p.c, p.lengths[tok0]);
+    hi = min(len, p.prefix[tok0]);
+    if (p.window > 0) lo = len - p.window;
+  } else {
+    hi = checked_length(p.c, p.lengths[s]);
+    if (p.window > 0) lo = hi - ntok + 1 - p.window;
+  }
+  return max(1, (hi - max(lo, 0) + 127) / 128);
+}
+
+constexpr int kRowsMaxParts = 64;
+constexpr int kRowsMinPart = 4;  // tiles of 128 slots: smaller parts gain nothing, larger ones idle SMs
+
+// Finds this CTA's rows and their limits. A unit is a KV head's tile of BM rows of a segment. Where
+// units are many (pieces = 0) blockIdx.x is one, tiles from the last to the first, since a causal
+// segment's last rows see most. Else units are cut into parts of at most a number of slots, the least
+// for which all parts are no more than the grid. False: nothing to do.
 template <int BM>
 __device__ __forceinline__ bool rows_begin(const RowsParams& p, RowsUnit& u, int2* limits) {
   const int lane = threadIdx.x & 31;
   if (threadIdx.x < 32) {
-    const int rest = blockIdx.x / p.splits;
-    const int tile = rest / p.H_kv;
     const int per = (p.nseg + 31) >> 5;
+    auto tiles_of = [&](int ntok) { return (ntok * p.G + BM - 1) / BM * p.H_kv; };  // units of a segment
+    int chunk = 0;
+    if (p.pieces > 0) {
+      int most = 0;
+      for (int j = 0; j < per; ++j) {
+        const int s = lane * per + j;
+        int tok0, ntok;
+        if (s >= p.nseg) break;
+        rows_segment(p, s, tok0, ntok);
+        most = max(most, rows_weight(p, s, tok0, ntok));
+      }
+      most = __reduce_max_sync(0xffffffffu, most);
+      int least = min(most, max(kRowsMinPart, (most + kRowsMaxParts - 1) / kRowsMaxParts));
+      while (least < most) {  // parts are no more for a larger chunk
+        const int mid = (least + most) >> 1;
+        int n = 0;
+        for (int j = 0; j < per; ++j) {
+          const int s = lane * per + j;
+          int tok0, ntok;
+          if (s >= p.nseg) break;
+          rows_segment(p, s, tok0, ntok);
+          n += tiles_of(ntok) * ((rows_weight(p, s, tok0, ntok) + mid - 1) / mid);
+        }
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (n > p.pieces) least = mid + 1;
+        else most = mid;
+      }
+      chunk = max(1, most);
+    }
+    auto parts_of = [&](int s, int tok0, int ntok) {
+      return p.pieces > 0 ? (rows_weight(p, s, tok0, ntok) + chunk - 1) / chunk : 1;
+    };
     int mine = 0;
     for (int j = 0; j < per; ++j) {
       const int s = lane * per + j;
       int tok0, ntok;
-      if (s < p.nseg) {
-        rows_segment(p, s, tok0, ntok);
-        mine += (ntok * p.G + BM - 1) / BM;
-      }
+      if (s >= p.nseg) break;
+      rows_segment(p, s, tok0, ntok);
+      mine += tiles_of(ntok) * parts_of(s, tok0, ntok);
     }
     int upto = mine;
 #pragma unroll
@@ -109,7 +161,11 @@ __device__ __forceinline__ bool rows_begin(const RowsParams& p, RowsUnit& u, int
       const int y = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += y;
     }
-    const int want = __shfl_sync(0xffffffffu, upto, 31) - 1 - tile;
+    int want = blockIdx.x;
+    if (p.pieces == 0) {  // the order of tiles reversed, heads of a tile side by side
+      const int tile = want / p.H_kv;
+      want = __shfl_sync(0xffffffffu, upto, 31) - (tile + 1) * p.H_kv + (want - tile * p.H_kv);
+    }
     if (lane == 0) u.rows = 0;
     __syncwarp();
     int before = upto - mine;
@@ -117,18 +173,20 @@ __device__ __forceinline__ bool rows_begin(const RowsParams& p, RowsUnit& u, int
       for (int s = lane * per;; ++s) {
         int tok0, ntok;
         rows_segment(p, s, tok0, ntok);
-        const int n = (ntok * p.G + BM - 1) / BM;
+        const int parts = parts_of(s, tok0, ntok), n = tiles_of(ntok) * parts;
         if (want >= before + n) {
           before += n;
           continue;
         }
+        const int unit = (want - before) / parts, tile = unit / p.H_kv;
         u.seg = s;
         u.tok0 = tok0;
         u.ntok = ntok;
         u.len = p.prefix == nullptr ? checked_length(p.c, p.lengths[s]) : 0;
-        u.hk = rest - tile * p.H_kv;
-        u.split = blockIdx.x - rest * p.splits;
-        u.row0 = (want - before) * BM;
+        u.hk = unit - tile * p.H_kv;
+        u.split = want - before - unit * parts;
+        u.parts = parts;
+        u.row0 = tile * BM;
         u.rows = min(BM, ntok * p.G - u.row0);
         u.lo_min = u.hi_min = INT32_MAX;
         u.lo_max = u.hi_max = 0;
@@ -164,8 +222,22 @@ template <int BN>
 __device__ __forceinline__ int2 rows_tiles(const RowsParams& p, const RowsUnit& u) {
   if (u.lo_min >= u.hi_max) return make_int2(0, 0);
   const int a = u.lo_min / BN, n = (u.hi_max + BN - 1) / BN - a;
-  return make_int2(a + static_cast<int>(static_cast<int64_t>(n) * u.split / p.splits),
-                   a + static_cast<int>(static_cast<int64_t>(n) * (u.split + 1) / p.splits));
+  return make_int2(a + static_cast<int>(static_cast<int64_t>(n) * u.split / u.parts),
+                   a + static_cast<int>(static_cast<int64_t>(n) * (u.split + 1) / u.parts));
+}
+
+// Whether the CTA's rows are joined with others' before they are rounded; a whole unit of a prefill is
+// written at once, and noted as no parts.
+__device__ __forceinline__ bool rows_in_parts(const RowsParams& p, const RowsUnit& u) {
+  return p.part_o != nullptr && (p.prefix != nullptr || u.parts > 1);
+}
+
+// Where row r of the CTA (output row `row`) leaves its part; the unit's first CTA notes where they are.
+template <int BM>
+__device__ __forceinline__ int64_t rows_place(const RowsParams& p, const RowsUnit& u, int r, int64_t row) {
+  const int64_t at = p.pieces > 0 ? static_cast<int64_t>(blockIdx.x) * BM + r : row;
+  if (u.split == 0) p.part_of[row] = make_int2(static_cast<int>(at), u.parts);
+  return at;
 }
 
 // The page table's row of a segment: its sequence, or its first token's.
@@ -365,8 +437,8 @@ __global__ void __launch_bounds__(kRfThreads) rows_fma_kernel(const RowsParams p
     const int t = (u.row0 + r) / p.G, g = u.row0 + r - t * p.G;
     const int64_t row = static_cast<int64_t>(u.tok0 + t) * p.H + u.hk * p.G + g;
     const float nan = __int_as_float(0x7fffffff);
-    if (p.part_o != nullptr) {
-      const int64_t at = u.split * (static_cast<int64_t>(p.T) * p.H) + row;
+    if (rows_in_parts(p, u)) {
+      const int64_t at = rows_place<kRfRows>(p, u, r, row);
       if (tx == 0) p.part_ml[at] = make_float2(m[i], l[i]);
       if (l[i] == 0.0f) continue;  // not read
 #pragma unroll
@@ -376,6 +448,7 @@ __global__ void __launch_bounds__(kRfThreads) rows_fma_kernel(const RowsParams p
                    : make_float4(o[i][2 * x].x, o[i][2 * x].y, o[i][2 * x + 1].x, o[i][2 * x + 1].y);
       continue;
     }
+    if (p.part_of != nullptr && tx == 0) p.part_of[row] = make_int2(0, 0);
     const float inv = l[i] == 0.0f ? 0.0f : spoilt ? nan : 1.0f / l[i];
     T* dst = static_cast<T*>(p.o) + row * D;
 #pragma unroll
@@ -825,8 +898,10 @@ __device__ __forceinline__ void rows_tc_write(const RowsParams& p, RowsTcShared&
   const int64_t row = static_cast<int64_t>(u.tok0 + t) * p.H + u.hk * p.G + g;
   const float nan = __int_as_float(0x7fffffff);
   const float spoil = in && sh.spoilt[r] ? nan : 1.0f;
-  const int64_t part = u.split * (static_cast<int64_t>(p.T) * p.H) + row;
-  const float inv = p.part_o != nullptr ? spoil : l == 0.0f ? 0.0f : spoil / l;
+  const bool parts = rows_in_parts(p, u);
+  const int64_t part = in && parts ? rows_place<RowsTc<D, Twin>::kRows>(p, u, r, row) : 0;
+  if (in && !parts && p.part_of != nullptr) p.part_of[row] = make_int2(0, 0);
+  const float inv = parts ? spoil : l == 0.0f ? 0.0f : spoil / l;
 #pragma unroll 1
   for (int c0 = 0; c0 < D; c0 += 32) {
     uint32_t o[32];
@@ -839,7 +914,7 @@ __device__ __forceinline__ void rows_tc_write(const RowsParams& p, RowsTcShared&
       if constexpr (Twin) f[c] = fmaf(theirs, other[(c0 + c) * 128 + lr], own * f[c]);
       f[c] = l == 0.0f ? 0.0f : f[c] * inv;
     }
-    if (in && p.part_o != nullptr) {
+    if (in && parts) {
       float4* dst = reinterpret_cast<float4*>(p.part_o + part * D + c0);
 #pragma unroll
       for (int c = 0; c < 32; c += 4) dst[c / 4] = make_float4(f[c], f[c + 1], f[c + 2], f[c + 3]);
@@ -856,7 +931,7 @@ __device__ __forceinline__ void rows_tc_write(const RowsParams& p, RowsTcShared&
     }
   }
   if (!in) return;
-  if (p.part_o != nullptr) p.part_ml[part] = make_float2(m, l);
+  if (parts) p.part_ml[part] = make_float2(m, l);
   else if (p.lse != nullptr) p.lse[row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
@@ -867,9 +942,18 @@ __global__ void __launch_bounds__(RowsTc<D, Twin>::kThreads, 1) rows_tc_kernel(c
   __shared__ RowsTcShared sh;
   uint8_t* q = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(rt_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring = q + S::kQ;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // A shared prefix's kernel is the third of its call and reads nothing that the first two write, so it
+  // waits for them last of all (in every CTA: it must not end before them).
+  const bool early = p.prefix != nullptr;
+  if (!early) asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
-  if (!rows_begin<S::kRows>(p, sh.u, sh.limits)) return;
+  auto wait_late = [&]() {
+    if (early) asm volatile("griddepcontrol.wait;" ::: "memory");
+  };
+  if (!rows_begin<S::kRows>(p, sh.u, sh.limits)) {
+    wait_late();
+    return;
+  }
   const RowsUnit& u = sh.u;
   const int2 tiles = rows_tiles<kTcSlots>(p, u);
   const int tid = threadIdx.x, n = tiles.y - tiles.x;
@@ -877,14 +961,16 @@ __global__ void __launch_bounds__(RowsTc<D, Twin>::kThreads, 1) rows_tc_kernel(c
     for (int r = tid; r < u.rows; r += S::kThreads) {
       const int t = (u.row0 + r) / p.G, g = u.row0 + r - t * p.G;
       const int64_t row = static_cast<int64_t>(u.tok0 + t) * p.H + u.hk * p.G + g;
-      if (p.part_o != nullptr) {
-        p.part_ml[u.split * (static_cast<int64_t>(p.T) * p.H) + row] = make_float2(-INFINITY, 0.0f);
+      if (rows_in_parts(p, u)) {
+        p.part_ml[rows_place<S::kRows>(p, u, r, row)] = make_float2(-INFINITY, 0.0f);
         continue;
       }
+      if (p.part_of != nullptr) p.part_of[row] = make_int2(0, 0);
       uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.o) + row * D);
       for (int c = 0; c < D / 8; ++c) dst[c] = make_uint4(0u, 0u, 0u, 0u);
       if (p.lse != nullptr) p.lse[row] = -INFINITY;
     }
+    wait_late();
     return;
   }
   const int blocks = Twin || u.rows > 128 ? 2 : 1;
@@ -950,16 +1036,16 @@ __global__ void __launch_bounds__(RowsTc<D, Twin>::kThreads, 1) rows_tc_kernel(c
   __syncthreads();
   tc_fence_after();
   if (tid / 32 == S::kMma / 32) tc_free(sh.tmem, S::kColumns);
+  wait_late();
 }
 
-// Joins a row's parts: those of its splits, and with `own` (fp32 rows and (m, 1 / l)) that of its own
-// slots. A warp takes a row; parts without a slot (l = 0) have no o.
-constexpr int kRowsMaxSplits = 64;
+// Joins a row's parts: those of its CTAs, and with `own` (fp32 rows and (m, 1 / l)) that of its own slots.
+// A warp takes a row; parts without a slot (l = 0) have no o.
 constexpr int kRjWarps = 4;
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kRjWarps * 32) rows_join_kernel(const RowsParams p, const float* own_o,
-                                                                  const float2* own_ml) {
+__global__ void __launch_bounds__(kRjWarps * 32) rows_join_kernel(const RowsParams p, int stride,
+                                                                  const float* own_o, const float2* own_ml) {
   constexpr int E = D / 32;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
@@ -974,11 +1060,15 @@ __global__ void __launch_bounds__(kRjWarps * 32) rows_join_kernel(const RowsPara
     if (lane == 0) raise_status(DCR_ERR_DEVICE_INDEX);
   }
   // lane x holds parts x and x + 32, then the own part's
+  int2 of = held ? p.part_of[row] : make_int2(0, 0);
+  if (of.x < 0 || of.y < 0 || of.y > kRowsMaxParts || of.x + (of.y - 1) * static_cast<int64_t>(stride) >= p.places)
+    of.y = 0;  // starts out of order: a row that no CTA took
+  if (of.y == 0 && p.prefix == nullptr) return;  // written already
   float2 ml[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int s = lane + 32 * i;
-    ml[i] = held && s < p.splits ? p.part_ml[s * rows + row] : make_float2(-INFINITY, 0.0f);
+    ml[i] = s < of.y ? p.part_ml[of.x + static_cast<int64_t>(s) * stride] : make_float2(-INFINITY, 0.0f);
   }
   float2 own = make_float2(-INFINITY, 0.0f);
   if (own_ml != nullptr) {
@@ -1010,7 +1100,7 @@ __global__ void __launch_bounds__(kRjWarps * 32) rows_join_kernel(const RowsPara
       const int s = __ffs(left) - 1;
       left &= left - 1;
       const float a = __shfl_sync(0xffffffffu, w[i], s);
-      const float* src = p.part_o + ((s + 32 * i) * rows + row) * D;
+      const float* src = p.part_o + (of.x + static_cast<int64_t>(s + 32 * i) * stride) * D;
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] = fmaf(a, src[lane + 32 * e], acc[e]);
     }
@@ -1021,36 +1111,32 @@ __global__ void __launch_bounds__(kRjWarps * 32) rows_join_kernel(const RowsPara
   if (lane == 0 && p.lse != nullptr) p.lse[row] = L == 0.0f ? -INFINITY : (M + log2f(L)) * kLn2;
 }
 
-// How a call is cut: query rows a CTA, parts a segment's slots are cut into, CTAs.
+// How a call is cut: query rows a CTA, CTAs that units are cut up for (0: a CTA a unit), CTAs.
 struct RowsPlan {
-  int bm, splits;
-  int64_t ctas;
+  int bm, pieces;
+  int64_t units, ctas;
 };
 
-static RowsPlan rows_plan(int dtype, int T, int nseg, int H_kv, int G, int D, int max_slots, int window) {
+static RowsPlan rows_plan(int dtype, int T, int nseg, int H_kv, int G, bool shared) {
   RowsPlan r;
   const int64_t rows = static_cast<int64_t>(T) * G;
   const bool tc = dtype != DCR_DTYPE_F32;
   // two blocks of rows where segments have more than one on average
   r.bm = !tc ? kRfRows : rows > 128ll * nseg ? 256 : 128;
   // every segment adds one tile of rows at most that is not full
-  const int64_t tiles = rows / r.bm + (nseg < rows ? nseg : rows);
-  const int64_t units = tiles * H_kv;
-  int64_t slots = max_slots;
-  if (window > 0 && static_cast<int64_t>(window) + T < slots) slots = static_cast<int64_t>(window) + T;
-  const int64_t most = slots / (4 * (tc ? kTcSlots : kRfSlots));
-  const int per_sm = tc ? 1 : 4;
-  int64_t want = static_cast<int64_t>(per_sm) * device_sm_count() / units;
-  if (want > most) want = most;
-  if (want > kRowsMaxSplits) want = kRowsMaxSplits;
-  r.splits = want > 1 ? static_cast<int>(want) : 1;
-  r.ctas = units * r.splits;
+  const int64_t units = (rows / r.bm + (nseg < rows ? nseg : rows)) * H_kv;
+  // units are cut up where the grid has more than one CTA for each
+  const int64_t slots = static_cast<int64_t>(tc ? 1 : 4) * device_sm_count();
+  r.pieces = units <= slots && (shared || 2 * units <= slots) ? static_cast<int>(slots) : 0;
+  r.units = units;
+  r.ctas = r.pieces > 0 ? r.pieces : units;
   return r;
 }
 
 // Workspace sections.
 struct RowsLayout {
-  size_t o, ml, own_o, own_ml, attend, total;
+  size_t o, ml, of, own_o, own_ml, attend, total;
+  int64_t places;
 };
 
 static RowsLayout rows_layout(const RowsPlan& r, int T, int H, int D, size_t attend, bool shared) {
@@ -1062,14 +1148,26 @@ static RowsLayout rows_layout(const RowsPlan& r, int T, int H, int D, size_t att
     return at;
   };
   const size_t rows = static_cast<size_t>(T) * H;
-  const size_t parts = shared || r.splits > 1 ? r.splits : 0;
-  w.o = take(parts * rows * D * sizeof(float));
-  w.ml = take(parts * rows * sizeof(float2));
+  w.places = r.pieces > 0 ? static_cast<int64_t>(r.pieces) * r.bm : shared ? static_cast<int64_t>(rows) : 0;
+  w.o = take(w.places * D * sizeof(float));
+  w.ml = take(w.places * sizeof(float2));
+  w.of = take(w.places > 0 ? rows * sizeof(int2) : 0);
   w.own_o = take(shared ? rows * D * sizeof(float) : 0);
   w.own_ml = take(shared ? rows * sizeof(float2) : 0);
   w.attend = take(attend);
   w.total = off > 256 ? off : 256;
   return w;
+}
+
+// The parts' fields of the parameters.
+static void rows_set_parts(RowsParams& p, const RowsPlan& plan, const RowsLayout& w, uint8_t* ws) {
+  const bool parts = w.places > 0;
+  p.pieces = plan.pieces;
+  p.places = w.places;
+  p.part_o = parts ? reinterpret_cast<float*>(ws + w.o) : nullptr;
+  p.part_ml = parts ? reinterpret_cast<float2*>(ws + w.ml) : nullptr;
+  p.part_of = parts ? reinterpret_cast<int2*>(ws + w.of) : nullptr;
+  p.box = 0;
 }
 
 template <typename Kernel, typename... Args>
@@ -1123,10 +1221,10 @@ static int rows_launch(const RowsParams& params, const RowsPlan& plan, cudaStrea
 }
 
 template <typename T, int D>
-static int rows_join(const RowsParams& p, const float* own_o, const float2* own_ml, cudaStream_t s) {
+static int rows_join(const RowsParams& p, const RowsPlan& plan, const float* own_o, const float2* own_ml, cudaStream_t s) {
   const int64_t rows = static_cast<int64_t>(p.T) * p.H;
   return launch_dependent(rows_join_kernel<T, D>, dim3(static_cast<unsigned>((rows + kRjWarps - 1) / kRjWarps)),
-                          dim3(kRjWarps * 32), 0, s, 1, p, own_o, own_ml) == cudaSuccess
+                          dim3(kRjWarps * 32), 0, s, 1, p, plan.bm, own_o, own_ml) == cudaSuccess
              ? DCR_OK
              : DCR_ERR_CUDA;
 }
@@ -1165,11 +1263,10 @@ using namespace dcr;
 
 extern "C" {
 
-size_t dcr_paged_prefill_workspace_bytes(int dtype, int T, int B, int H, int H_kv, int D, int max_slots,
-                                         int window) {
-  if (B <= 0 || max_slots <= 0 || (D != 64 && D != 128) || rows_check(T, H, H_kv, window) != DCR_OK)
+size_t dcr_paged_prefill_workspace_bytes(int dtype, int T, int B, int H, int H_kv, int D) {
+  if (B <= 0 || (D != 64 && D != 128) || rows_check(T, H, H_kv, 0) != DCR_OK)
     return 0;
-  return rows_layout(rows_plan(dtype, T, B, H_kv, H / H_kv, D, max_slots, window), T, H, D, 0, false).total;
+  return rows_layout(rows_plan(dtype, T, B, H_kv, H / H_kv, false), T, H, D, 0, false).total;
 }
 
 int dcr_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_pages,
@@ -1190,7 +1287,11 @@ int dcr_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, con
   if (st != DCR_OK) return st;
   st = rows_check_rows(q, q_stride_t, q_stride_h, o, lse, lengths, starts, nullptr, dtype, T, H, D);
   if (st != DCR_OK) return st;
-  const RowsPlan plan = rows_plan(dtype, T, B, H_kv, H / H_kv, D, max_pages * page_size, window);
+  RowsPlan plan = rows_plan(dtype, T, B, H_kv, H / H_kv, false);
+  if (max_pages * page_size <= 128 * kRowsMinPart) {  // nothing to cut up
+    plan.pieces = 0;
+    plan.ctas = plan.units;
+  }
   if (plan.ctas > INT32_MAX) return DCR_ERR_SHAPE;
   const RowsLayout w = rows_layout(plan, T, H, D, 0, false);
   if (workspace == nullptr || misaligned(16, workspace) || workspace_bytes < w.total)
@@ -1210,29 +1311,26 @@ int dcr_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, con
   p.H = H;
   p.H_kv = H_kv;
   p.G = H / H_kv;
-  p.splits = plan.splits;
   p.window = window;
   p.causal = causal != 0;
   p.scale2 = scale * kLog2e;
   p.o = o;
   p.lse = lse;
-  p.part_o = plan.splits > 1 ? reinterpret_cast<float*>(ws + w.o) : nullptr;
-  p.part_ml = plan.splits > 1 ? reinterpret_cast<float2*>(ws + w.ml) : nullptr;
-  p.box = 0;
+  rows_set_parts(p, plan, w, ws);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return rows_dispatch(dtype, D, [&](auto type, auto dims) {
     using Ty = decltype(type);
     constexpr int kDim = decltype(dims)::value;
     const int rc = rows_launch<Ty, kDim, 1>(p, plan, s);
-    return rc != DCR_OK || plan.splits == 1 ? rc : rows_join<Ty, kDim>(p, nullptr, nullptr, s);
+    return rc != DCR_OK || plan.pieces == 0 ? rc : rows_join<Ty, kDim>(p, plan, nullptr, nullptr, s);
   });
 }
 
-size_t dcr_paged_shared_workspace_bytes(int dtype, int B, int groups, int H, int H_kv, int D, int max_slots) {
-  if (groups <= 0 || max_slots <= 0 || (D != 64 && D != 128) || rows_check(B, H, H_kv, 0) != DCR_OK)
+size_t dcr_paged_shared_workspace_bytes(int dtype, int B, int groups, int H, int H_kv, int D) {
+  if (groups <= 0 || (D != 64 && D != 128) || rows_check(B, H, H_kv, 0) != DCR_OK)
     return 0;
-  return rows_layout(rows_plan(dtype, B, groups, H_kv, H / H_kv, D, max_slots, 0), B, H, D,
-                     pa_layout(B, H, H / H_kv, D, max_slots, false).total, true).total;
+  return rows_layout(rows_plan(dtype, B, groups, H_kv, H / H_kv, true), B, H, D,
+                     pa_layout(B, H, H / H_kv, D, 1, false).total, true).total;
 }
 
 int dcr_paged_shared_attend(const void* q, int64_t q_stride_b, int64_t q_stride_h,
@@ -1255,10 +1353,10 @@ int dcr_paged_shared_attend(const void* q, int64_t q_stride_b, int64_t q_stride_
   if (st != DCR_OK) return st;
   st = rows_check_rows(q, q_stride_b, q_stride_h, o, lse, lengths, groups, prefix, dtype, B, H, D);
   if (st != DCR_OK) return st;
-  const int G = H / H_kv, max_slots = max_pages * page_size;
-  const RowsPlan plan = rows_plan(dtype, B, n_groups, H_kv, G, D, max_slots, 0);
+  const int G = H / H_kv;
+  const RowsPlan plan = rows_plan(dtype, B, n_groups, H_kv, G, true);
   if (plan.ctas > INT32_MAX) return DCR_ERR_SHAPE;
-  const PagedAttendLayout a = pa_layout(B, H, G, D, max_slots, false);
+  const PagedAttendLayout a = pa_layout(B, H, G, D, 1, false);
   const RowsLayout w = rows_layout(plan, B, H, D, a.total, true);
   if (workspace == nullptr || misaligned(16, workspace) || workspace_bytes < w.total)
     return DCR_ERR_WORKSPACE;
@@ -1300,15 +1398,12 @@ int dcr_paged_shared_attend(const void* q, int64_t q_stride_b, int64_t q_stride_
   p.H = H;
   p.H_kv = H_kv;
   p.G = G;
-  p.splits = plan.splits;
   p.window = window;
   p.causal = 0;
   p.scale2 = own.scale2;
   p.o = o;
   p.lse = lse;
-  p.part_o = reinterpret_cast<float*>(ws + w.o);
-  p.part_ml = reinterpret_cast<float2*>(ws + w.ml);
-  p.box = 0;
+  rows_set_parts(p, plan, w, ws);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int rc = pa_launch_any<true>(own, dtype, D, HB, a.ctas, s);
   if (rc != DCR_OK) return rc;
@@ -1317,7 +1412,7 @@ int dcr_paged_shared_attend(const void* q, int64_t q_stride_b, int64_t q_stride_
     constexpr int kDim = decltype(dims)::value;
     const int r = rows_launch<Ty, kDim, 2>(p, plan, s);
     return r != DCR_OK ? r
-                       : rows_join<Ty, kDim>(p, reinterpret_cast<const float*>(ws + w.own_o),
+                       : rows_join<Ty, kDim>(p, plan, reinterpret_cast<const float*>(ws + w.own_o),
                                              reinterpret_cast<const float2*>(ws + w.own_ml), s);
   });
 }

@@ -317,7 +317,7 @@ PyObject* prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (T > 0 && B > 0) {
       const size_t bytes = dcr_paged_prefill_workspace_bytes(
           p.dtype, static_cast<int>(T), static_cast<int>(B), static_cast<int>(H), static_cast<int>(p.H_kv),
-          static_cast<int>(p.D), static_cast<int>(p.slots), static_cast<int>(window));
+          static_cast<int>(p.D));
       const at::Tensor ws = scratch(a[11], bytes, p.device);
       const int st = dcr_paged_prefill(
           q.data, q.st, q.sh, p.k->data_ptr(), p.v->data_ptr(), p.dtype, p.k->stride(0),
@@ -361,7 +361,7 @@ PyObject* shared(PyObject*, PyObject* const* a, Py_ssize_t n) {
       const int n_groups = static_cast<int>(g.size(0) - 1);
       const size_t bytes = dcr_paged_shared_workspace_bytes(
           p.dtype, static_cast<int>(B), n_groups, static_cast<int>(H), static_cast<int>(p.H_kv),
-          static_cast<int>(p.D), static_cast<int>(p.slots));
+          static_cast<int>(p.D));
       const at::Tensor ws = scratch(a[11], bytes, p.device);
       const int st = dcr_paged_shared_attend(
           q.data, q.st, q.sh, p.k->data_ptr(), p.v->data_ptr(), p.dtype, p.k->stride(0),

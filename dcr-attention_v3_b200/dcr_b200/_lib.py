@@ -118,11 +118,11 @@ SIGNATURES = {
                                                         _vp, _vp, _i32, _i32, _i32, _i32, _i32,
                                                         _vp, _vp, _vp] + [_i64] * 6 + [
         _i32, _i32, _vp, _i64, _i32, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp]),
-    "dcr_paged_prefill_workspace_bytes": (_sz, [_i32] * 8),
+    "dcr_paged_prefill_workspace_bytes": (_sz, [_i32] * 6),
     "dcr_paged_prefill": (_i32, [_vp, _i64, _i64, _vp, _vp, _i32] + [_i64] * 6 + [
         _i32, _i32, _vp, _i64, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _vp,
         _vp, _vp, _sz, _vp]),
-    "dcr_paged_shared_workspace_bytes": (_sz, [_i32] * 7),
+    "dcr_paged_shared_workspace_bytes": (_sz, [_i32] * 6),
     "dcr_paged_shared_attend": (_i32, [_vp, _i64, _i64, _vp, _vp, _i32] + [_i64] * 6 + [
         _i32, _i32, _vp, _i64, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _i32, _f32, _i32, _vp,
         _vp, _vp, _sz, _vp]),

@@ -57,12 +57,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     return r
 
 
-def paged_prefill_workspace_bytes(T: int, B: int, H: int, H_kv: int, D: int, max_slots: int,
-                                  window: int = 0, dtype: torch.dtype = torch.bfloat16) -> int:
-    """Bytes :func:`paged_prefill` needs for T tokens of B sequences (max_slots = max_pages *
-    page_size)."""
-    return int(_lib.load().dcr_paged_prefill_workspace_bytes(_lib.DTYPE_CODES[dtype], T, B, H, H_kv, D,
-                                                             max_slots, window))
+def paged_prefill_workspace_bytes(T: int, B: int, H: int, H_kv: int, D: int,
+                                  dtype: torch.dtype = torch.bfloat16) -> int:
+    """Bytes :func:`paged_prefill` needs for T tokens of B sequences."""
+    return int(_lib.load().dcr_paged_prefill_workspace_bytes(_lib.DTYPE_CODES[dtype], T, B, H, H_kv, D))
 
 
 def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -88,10 +86,10 @@ def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
 
 
 def paged_shared_workspace_bytes(B: int, groups: int, H: int, H_kv: int, D: int,
-                                 max_slots: int, dtype: torch.dtype = torch.bfloat16) -> int:
-    """Bytes :func:`paged_shared_attention` needs (max_slots = max_pages * page_size)."""
-    return int(_lib.load().dcr_paged_shared_workspace_bytes(_lib.DTYPE_CODES[dtype], B, groups, H,
-                                                            H_kv, D, max_slots))
+                                 dtype: torch.dtype = torch.bfloat16) -> int:
+    """Bytes :func:`paged_shared_attention` needs."""
+    return int(_lib.load().dcr_paged_shared_workspace_bytes(_lib.DTYPE_CODES[dtype], B, groups, H, H_kv,
+                                                            D))
 
 
 def paged_shared_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,

@@ -460,10 +460,9 @@ int dcr_paged_attend(const void* q, int64_t q_stride_b, int64_t q_stride_h, cons
                      float* weights, int64_t w_stride_b, int64_t w_stride_h, void* workspace,
                      size_t workspace_bytes, void* stream);
 
-/* Bytes of workspace dcr_paged_prefill needs for T tokens of B sequences (max_slots = max_pages *
- * page_size); it need not be initialised. 0: invalid shape. */
-size_t dcr_paged_prefill_workspace_bytes(int dtype, int T, int B, int H, int H_kv, int D, int max_slots,
-                                         int window);
+/* Bytes of workspace dcr_paged_prefill needs for T tokens of B sequences; it need not be initialised.
+ * 0: invalid shape. */
+size_t dcr_paged_prefill_workspace_bytes(int dtype, int T, int B, int H, int H_kv, int D);
 
 /* Attention of many new tokens per sequence: tokens starts[b] .. starts[b + 1] - 1 (starts [B + 1],
  * ascending within [0, T]) of q [T, H, D] are the last of sequence b's lengths[b] slots, whose keys
@@ -485,7 +484,7 @@ int dcr_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, con
                       size_t workspace_bytes, void* stream);
 
 /* Bytes of workspace dcr_paged_shared_attend needs; it need not be initialised. 0: invalid shape. */
-size_t dcr_paged_shared_workspace_bytes(int dtype, int B, int groups, int H, int H_kv, int D, int max_slots);
+size_t dcr_paged_shared_workspace_bytes(int dtype, int B, int groups, int H, int H_kv, int D);
 
 /* dcr_paged_attend (without weights) where sequences hold the same pages in their first slots, which
  * are then read once for all of them: sequences groups[p] .. groups[p + 1] - 1 (groups [n_groups + 1],

@@ -8,8 +8,8 @@ import sys
 import pytest
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
-from test_capi_paged import (ALIGN, APPEND, ATTEND, B, D, DTYPE, H, H_KV, MAX_PAGES, NULL, P,  # noqa: E402
-                             PAGE, POOL_REFUSALS, SHAPE, WORKSPACE, _names, _pool_strides, lib)  # noqa: F401
+from test_capi_paged import (ALIGN, APPEND, ATTEND, B, D, DTYPE, H, H_KV, NULL, P,  # noqa: E402
+                             POOL_REFUSALS, SHAPE, WORKSPACE, _names, _pool_strides, lib)  # noqa: F401
 
 T = 5
 PREFILL = dict(ATTEND, q_stride_t=H * D, starts=P, T=T, causal=1, o=P << 1)
@@ -63,12 +63,11 @@ def test_refused(lib, func, base, change, status):  # noqa: F811
 
 
 def test_workspace_sizes(lib):  # noqa: F811
-    slots = MAX_PAGES * PAGE
-    assert lib.dcr_paged_prefill_workspace_bytes(0, T, B, H, H_KV, D, slots, 0) > 0
-    assert lib.dcr_paged_prefill_workspace_bytes(0, T, B, 7, H_KV, D, slots, 0) == 0
-    assert lib.dcr_paged_prefill_workspace_bytes(0, T, B, H, H_KV, 96, slots, 0) == 0
-    assert lib.dcr_paged_shared_workspace_bytes(0, B, 1, H, H_KV, D, slots) > 0
-    assert lib.dcr_paged_shared_workspace_bytes(0, B, 0, H, H_KV, D, slots) == 0
+    assert lib.dcr_paged_prefill_workspace_bytes(0, T, B, H, H_KV, D) > 0
+    assert lib.dcr_paged_prefill_workspace_bytes(0, T, B, 7, H_KV, D) == 0
+    assert lib.dcr_paged_prefill_workspace_bytes(0, T, B, H, H_KV, 96) == 0
+    assert lib.dcr_paged_shared_workspace_bytes(0, B, 1, H, H_KV, D) > 0
+    assert lib.dcr_paged_shared_workspace_bytes(0, B, 0, H, H_KV, D) == 0
 
 
 def test_frequencies():
