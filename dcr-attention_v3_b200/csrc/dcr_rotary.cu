@@ -67,14 +67,6 @@ struct RotaryPlace {
   int64_t position;
 };
 
-template <typename T>
-__device__ __forceinline__ uint4 ro_round(const float (&f)[ElemTraits<T>::kPerChunk]) {
-  float2 x[ElemTraits<T>::kPerChunk / 2];
-#pragma unroll
-  for (int e = 0; e < ElemTraits<T>::kPerChunk / 2; ++e) x[e] = make_float2(f[2 * e], f[2 * e + 1]);
-  return ap_round<T>(x);
-}
-
 template <bool Paged>
 __device__ __forceinline__ RotaryPlace ro_place(const RotaryParams& p, int t) {
   RotaryPlace r;
@@ -106,17 +98,18 @@ __device__ __forceinline__ RotaryPlace ro_place(const RotaryParams& p, int t) {
   return r;
 }
 
-// cos and sin of every token of the CTA, times the factor.
+// cos and sin of every token of the CTA, times the factor: cosines [tokens][rot / 2], then sines.
 __device__ __forceinline__ void ro_angles(const RotaryParams& p, const RotaryPlace* place, int tokens,
-                                          float2* turn) {
-  const int half = p.rot / 2;
-  for (int i = threadIdx.x; i < tokens * half; i += kRoThreads) {
+                                          float* turn) {
+  const int half = p.rot / 2, n = tokens * half;
+  for (int i = threadIdx.x; i < n; i += kRoThreads) {
     const int t = i / half, f = i - t * half;
     const double turns = static_cast<double>(place[t].position) *
                          (static_cast<double>(p.inv_freq[f]) * 0.15915494309189533577);
     float s, c;
     sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
-    turn[i] = make_float2(c * p.factor, s * p.factor);
+    turn[i] = c * p.factor;
+    turn[n + i] = s * p.factor;
   }
 }
 
@@ -140,107 +133,151 @@ __device__ __forceinline__ T* ro_target(const RotaryParams& p, const RotaryPlace
   }
 }
 
-// The two chunks of item i of a row.
-__device__ __forceinline__ int2 ro_chunks(const RotaryParams& p, int i, int n) {
-  const int turned = p.rot / (2 * n);
-  if (i < turned && !p.interleaved) return make_int2(i, i + turned);
+// The two chunks of item i of a row, the first `turned` items of which are rotated.
+__device__ __forceinline__ int2 ro_chunks(int i, int turned, int interleaved) {
+  if (i < turned && !interleaved) return make_int2(i, i + turned);
   return make_int2(2 * i, 2 * i + 1);
 }
+
+// An item of the CTA: part of a row of a token. Items are kRoThreads apart.
+struct RotaryItem {
+  int part, row, t;
+  __device__ __forceinline__ void next(int parts, int rows) {
+    part += kRoThreads % parts;
+    row += kRoThreads / parts;
+    if (part >= parts) {
+      part -= parts;
+      ++row;
+    }
+    while (row >= rows) {
+      row -= rows;
+      ++t;
+    }
+  }
+};
 
 template <typename T, bool Paged>
 __global__ void __launch_bounds__(kRoThreads) rotary_kernel(const RotaryParams p) {
   constexpr int N = ElemTraits<T>::kPerChunk;
-  extern __shared__ __align__(16) float2 ro_turn[];
+  extern __shared__ __align__(16) float ro_turn[];
   __shared__ RotaryPlace place[kRoMaxTokens];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
   const int t0 = blockIdx.x * p.per_cta;
   const int tokens = min(p.per_cta, p.T - t0);
   const int rows = p.H + (Paged ? 2 : 1) * p.H_kv;
-  const int total = tokens * rows * p.parts;
+  const int parts = p.parts, turned = p.rot / (2 * N);
   uint4 x[kRoSteps][2];
-  auto load = [&](int first) {
+  RotaryItem at[kRoSteps];
+  RotaryItem last;  // the item after those loaded
+  last.part = static_cast<int>(threadIdx.x) % parts;
+  last.row = static_cast<int>(threadIdx.x) / parts;
+  last.t = last.row / rows;
+  last.row -= last.t * rows;
+  auto load = [&]() {
 #pragma unroll
     for (int i = 0; i < kRoSteps; ++i) {
-      const int item = first + i * kRoThreads;
-      if (item < total) {
-        const int part = item % p.parts, row = item / p.parts % rows, t = item / (p.parts * rows);
-        const uint4* src = reinterpret_cast<const uint4*>(ro_source<T, Paged>(p, t0 + t, row));
-        const int2 ch = ro_chunks(p, part, N);
+      at[i] = last;
+      if (last.t < tokens) {
+        const uint4* src = reinterpret_cast<const uint4*>(ro_source<T, Paged>(p, t0 + last.t, last.row));
+        const int2 ch = ro_chunks(last.part, turned, p.interleaved);
         x[i][0] = __ldcs(src + ch.x);
         x[i][1] = __ldcs(src + ch.y);
+        last.next(parts, rows);
       } else {
         x[i][0] = x[i][1] = make_uint4(0u, 0u, 0u, 0u);
       }
     }
   };
-  load(threadIdx.x);
+  load();
+  const bool norms = Paged && (p.qw != nullptr || p.kw != nullptr);
+  __shared__ __align__(16) float weight[Paged ? 2 : 1][Paged ? 128 : 4];
+  if (norms && threadIdx.x < p.D / N * 2) {
+    const int k = threadIdx.x >= p.D / N, ch = threadIdx.x - k * (p.D / N);
+    const void* w = k ? p.kw : p.qw;
+    float g[N];
+    if (w != nullptr) {
+      ap_load<T, N>(w, ch * N, g);
+#pragma unroll
+      for (int e = 0; e < N; ++e) weight[k][ch * N + e] = g[e];
+    }
+  }
   if (threadIdx.x < tokens) place[threadIdx.x] = ro_place<Paged>(p, t0 + threadIdx.x);
   __syncthreads();
   ro_angles(p, place, tokens, ro_turn);
   __syncthreads();
+  const int rounds = (tokens * rows * parts + kRoSteps * kRoThreads - 1) / (kRoSteps * kRoThreads);
 #pragma unroll 1
-  for (int first = threadIdx.x; first - static_cast<int>(threadIdx.x) < total;
-       first += kRoSteps * kRoThreads) {
-    if (first != static_cast<int>(threadIdx.x)) load(first);
+  for (int round = 0; round < rounds; ++round) {
+    if (round > 0) load();
 #pragma unroll
     for (int i = 0; i < kRoSteps; ++i) {
-      const int item = first + i * kRoThreads;
-      const bool in = item < total;
-      const int part = item % p.parts, row = in ? item / p.parts % rows : 0;
-      const int t = in ? item / (p.parts * rows) : 0;
-      const int2 ch = ro_chunks(p, part, N);
+      const int part = at[i].part, t = at[i].t, row = at[i].row;
+      const bool in = t < tokens;
+      const int2 ch = ro_chunks(part, turned, p.interleaved);
       const bool value = Paged && row >= p.H + p.H_kv;
-      float f[2][N];
-      ElemTraits<T>::widen(x[i][0], f[0]);
-      ElemTraits<T>::widen(x[i][1], f[1]);
-      const void* w = Paged && !value ? (row < p.H ? p.qw : p.kw) : nullptr;
-      if (Paged && (p.qw != nullptr || p.kw != nullptr)) {  // all lanes of a row take part
-        float ss = 0.0f;
+      float2 f[2][N / 2];
 #pragma unroll
-        for (int e = 0; e < N; ++e) ss = fmaf(f[0][e], f[0][e], fmaf(f[1][e], f[1][e], ss));
-        for (int o = p.parts / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (w != nullptr) {
+      for (int h = 0; h < 2; ++h) {
+        float y[N];
+        ElemTraits<T>::widen(x[i][h], y);
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e) f[h][e] = make_float2(y[2 * e], y[2 * e + 1]);
+      }
+      const float2 zero = make_float2(0.0f, 0.0f);
+      const bool normed = Paged && !value && (row < p.H ? p.qw : p.kw) != nullptr;
+      if (norms) {  // all lanes of a row take part
+        float2 s2 = zero;
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e) s2 = ffma2(f[0][e], f[0][e], ffma2(f[1][e], f[1][e], s2));
+        float ss = s2.x + s2.y;
+        for (int o = parts / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (normed) {
           const float rs = rsqrtf(ss / p.D + p.eps);
-          float g[2][N];
-          ap_load<T, N>(w, ch.x * N, g[0]);
-          ap_load<T, N>(w, ch.y * N, g[1]);
 #pragma unroll
-          for (int e = 0; e < N; ++e) {
-            f[0][e] *= rs * g[0][e];
-            f[1][e] *= rs * g[1][e];
+          for (int h = 0; h < 2; ++h) {
+            const float4* g = reinterpret_cast<const float4*>(weight[row >= p.H] + (h ? ch.y : ch.x) * N);
+#pragma unroll
+            for (int e = 0; e < N / 4; ++e) {
+              const float4 w = g[e];
+              f[h][2 * e] = ffma2(f[h][2 * e], ffma2(make_float2(w.x, w.y), make_float2(rs, rs), zero), zero);
+              f[h][2 * e + 1] = ffma2(f[h][2 * e + 1], ffma2(make_float2(w.z, w.w), make_float2(rs, rs), zero), zero);
+            }
           }
         }
       }
       if (!in) continue;
-      if (!value && part < p.rot / (2 * N)) {
-        const float2* turn = ro_turn + t * (p.rot / 2) + part * N;
-        if (p.interleaved) {
+      if (!value && part < turned) {
+        const float* cs = ro_turn + t * (p.rot / 2) + part * N;
+        const float* sn = cs + tokens * (p.rot / 2);
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+        for (int e = 0; e < N / 4; ++e) {
+          const float4 c = reinterpret_cast<const float4*>(cs)[e], s = reinterpret_cast<const float4*>(sn)[e];
+          if (p.interleaved) {  // the pairs 4 e .. 4 e + 3 of the two chunks
+            const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-            for (int e = 0; e < N; e += 2) {
-              const float2 cs = turn[(h * N + e) / 2];
-              const float a = f[h][e], b = f[h][e + 1];
-              f[h][e] = a * cs.x - b * cs.y;
-              f[h][e + 1] = b * cs.x + a * cs.y;
+            for (int k = 0; k < 4; ++k) {
+              float2& y = f[(4 * e + k) / (N / 2)][(4 * e + k) % (N / 2)];
+              y = ffma2(y, make_float2(cc[k], cc[k]), ffma2(make_float2(-y.y, y.x), make_float2(ss[k], ss[k]), zero));
             }
-        } else {
+          } else {
 #pragma unroll
-          for (int e = 0; e < N; ++e) {
-            const float2 cs = turn[e];
-            const float a = f[0][e], b = f[1][e];
-            f[0][e] = a * cs.x - b * cs.y;
-            f[1][e] = b * cs.x + a * cs.y;
+            for (int k = 0; k < 2; ++k) {
+              const float2 ck = k ? make_float2(c.z, c.w) : make_float2(c.x, c.y);
+              const float2 sk = k ? make_float2(s.z, s.w) : make_float2(s.x, s.y);
+              const float2 a = f[0][2 * e + k], b = f[1][2 * e + k];
+              f[0][2 * e + k] = ffma2(a, ck, ffma2(make_float2(-b.x, -b.y), sk, zero));
+              f[1][2 * e + k] = ffma2(b, ck, ffma2(a, sk, zero));
+            }
           }
         }
       }
       T* dst = ro_target<T, Paged>(p, place[t], t0 + t, row);
       if (dst == nullptr) continue;
       // what no arithmetic touched is stored as it was read
-      const bool same = value || (w == nullptr && part >= p.rot / (2 * N));
-      __stcs(reinterpret_cast<uint4*>(dst) + ch.x, same ? x[i][0] : ro_round<T>(f[0]));
-      __stcs(reinterpret_cast<uint4*>(dst) + ch.y, same ? x[i][1] : ro_round<T>(f[1]));
+      const bool same = value || (!normed && part >= turned);
+      __stcs(reinterpret_cast<uint4*>(dst) + ch.x, same ? x[i][0] : ap_round<T>(f[0]));
+      __stcs(reinterpret_cast<uint4*>(dst) + ch.y, same ? x[i][1] : ap_round<T>(f[1]));
       if (Paged && part == 0 && row >= p.H && !value) {
         const int h = row - p.H;
         if (p.weights != nullptr) p.weights[place[t].b * p.wsb + h * p.wsh + place[t].slot] = 0.0f;
@@ -254,7 +291,7 @@ __global__ void __launch_bounds__(kRoThreads) rotary_kernel(const RotaryParams p
 // Element by element, a warp a row: any even number of rotated elements.
 template <typename T, bool Paged>
 __global__ void __launch_bounds__(kRoThreads) rotary_any_kernel(const RotaryParams p) {
-  extern __shared__ __align__(16) float2 ro_turn[];
+  extern __shared__ __align__(16) float ro_turn[];
   __shared__ RotaryPlace place[kRoMaxTokens];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
@@ -292,10 +329,10 @@ __global__ void __launch_bounds__(kRoThreads) rotary_any_kernel(const RotaryPara
     if (!value)
       for (int f = lane; f < half; f += 32) {
         const int i = p.interleaved ? 2 * f : f, j = p.interleaved ? 2 * f + 1 : f + half;
-        const float2 cs = ro_turn[t * half + f];
+        const float c = ro_turn[t * half + f], s = ro_turn[(tokens + t) * half + f];
         const float a = normed(i), b = normed(j);
-        ElemTraits<T>::store(dst, i, a * cs.x - b * cs.y);
-        ElemTraits<T>::store(dst, j, b * cs.x + a * cs.y);
+        ElemTraits<T>::store(dst, i, a * c - b * s);
+        ElemTraits<T>::store(dst, j, b * c + a * s);
       }
     if (dst != src || w != nullptr)
       for (int e = (value ? 0 : p.rot) + lane; e < p.D; e += 32) {
@@ -324,7 +361,7 @@ static int ro_launch(RotaryParams p, bool in_place, cudaStream_t s) {
   if (per > kRoMaxTokens) per = kRoMaxTokens;
   if (per < 1) per = 1;
   p.per_cta = per;
-  const size_t smem = static_cast<size_t>(per) * (p.rot / 2) * sizeof(float2);
+  const size_t smem = static_cast<size_t>(per) * p.rot * sizeof(float);
   const dim3 grid((p.T + per - 1) / per);
   const cudaError_t e = launch_dependent(whole ? rotary_kernel<T, Paged> : rotary_any_kernel<T, Paged>,
                                          grid, dim3(kRoThreads), smem, s, 1, p);
