@@ -6,7 +6,8 @@ and processed logits.
 :class:`~dcr_b200.paged_cache.PagedKVCache`: sequences of unequal lengths in one batch, a cache that
 grows by pages and, with a budget, forgets the slots that drew the least attention. Per layer and
 step: a norm, the q/k/v GEMM, query/key norms (``qk_norm``) with rotation and append in one launch,
-attention over the pages, o_proj and the MLP. :meth:`PagedLlamaDecoder.generate` is the loop around
+attention over the pages, o_proj and the MLP. Prompts go in whole or in chunks, beside sequences that
+run already, and on a common prefix that is computed and held once. :meth:`PagedLlamaDecoder.generate` is the loop around
 it with penalties, bias and grammar masks on the logits. The reference decodes equal sequences
 greedily over one contiguous cache (tests/kernel/test_m1_acceptance.py:198).
 """
@@ -27,9 +28,13 @@ from dcr_b200.paged_cache import PagedKVCache
 class PagedLlamaDecoder(torch.nn.Module):
     """``model``'s weights over paged caches. ``qk_norm``: every layer RMS-norms its query and key
     heads before the rotation, with its own weights ``q_norm[i]`` and ``k_norm[i]`` (ones at first;
-    a checkpoint's go there). ``max_positions``: rows of the position tables."""
+    a checkpoint's go there). ``max_positions``: rows of the position tables. ``inv_freq`` (fp32 ``[r /
+    2]``): rotate by these frequencies instead of the model's tables, with ``interleaved`` pairs and an
+    amplitude ``rotary_factor`` if wanted (:func:`~dcr_b200.kernel.cuda.rotary.rotary`)."""
 
-    def __init__(self, model: DCRLlamaDecoder, *, qk_norm: bool = False, max_positions: int = 32768):
+    def __init__(self, model: DCRLlamaDecoder, *, qk_norm: bool = False, max_positions: int = 32768,
+                 inv_freq: Optional[torch.Tensor] = None, interleaved: bool = False,
+                 rotary_factor: float = 1.0):
         super().__init__()
         require(model.fast, "the paged decoder runs the packed projections of fast models")
         self.model, self.qk_norm = model, qk_norm
@@ -38,6 +43,10 @@ class PagedLlamaDecoder(torch.nn.Module):
             torch.nn.Parameter(torch.ones(HEAD_DIM, **kw)) for _ in model.layers if qk_norm)
         self.q_norm, self.k_norm = norms(), norms()
         self.cos, self.sin = (t.contiguous() for t in model.rope_table(max_positions))
+        require(inv_freq is not None or (not interleaved and rotary_factor == 1.0),
+                "interleaved pairs and an amplitude go with inv_freq")
+        self.inv_freq = None if inv_freq is None else inv_freq.to(model.device, torch.float32).contiguous()
+        self.interleaved, self.rotary_factor = interleaved, rotary_factor
 
     def new_cache(self, batch: int, pages: int, max_slots: int, **kw) -> PagedKVCache:
         """A cache for this model (keywords as :class:`PagedKVCache`)."""
@@ -48,7 +57,7 @@ class PagedLlamaDecoder(torch.nn.Module):
         """Refuses, before the cache changes, tokens past the position table."""
         require(len(new_tokens) == cache.batch, f"{cache.batch} sequences expected")
         for b, n in enumerate(new_tokens):
-            require(n == 0 or cache.host_seen[b] + n <= self.cos.shape[0],
+            require(n == 0 or self.inv_freq is not None or cache.host_seen[b] + n <= self.cos.shape[0],
                     f"sequence {b} would reach position {cache.host_seen[b] + n} of a table of "
                     f"{self.cos.shape[0]}")
 
@@ -66,34 +75,56 @@ class PagedLlamaDecoder(torch.nn.Module):
             q = qkv[:, :nq].view(T, cfg.heads, HEAD_DIM)
             k = qkv[:, nq:nq + nk].view(T, cfg.kv_heads, HEAD_DIM)
             v = qkv[:, nq + nk:].view(T, cfg.kv_heads, HEAD_DIM)
-            q = cache.append(i, q, k, v, self.cos, self.sin, eps=eps,
-                             q_weight=self.q_norm[i] if self.qk_norm else None,
-                             k_weight=self.k_norm[i] if self.qk_norm else None)
+            norms = dict(eps=eps, q_weight=self.q_norm[i] if self.qk_norm else None,
+                         k_weight=self.k_norm[i] if self.qk_norm else None)
+            if self.inv_freq is None:
+                q = cache.append(i, q, k, v, self.cos, self.sin, **norms)
+            else:
+                q = cache.append_rotary(i, q, k, v, self.inv_freq, interleaved=self.interleaved,
+                                        factor=self.rotary_factor, **norms)
             a = layer.self_attn.o_proj(attend(i, q).reshape(T, nq))
             h, x = add_rmsnorm(h, a, layer.post_attention_layernorm.weight, eps)
             delta = layer.down_proj(silu_mul_packed(F.linear(x, layer._gate_up)))
         return add_rmsnorm(h, delta, self.model.norm.weight, self.model.norm.eps)[1]
 
     @torch.no_grad()
-    def prefill(self, prompts: Sequence[Sequence[int]], cache: PagedKVCache) -> torch.Tensor:
-        """Feeds one prompt per sequence into an empty cache (an empty prompt leaves its sequence
-        idle); returns the logits [batch, vocab] after each prompt's last token (zeros for idle
-        sequences). Attention within a prompt is causal SDPA over its rows. In a cache with a budget,
-        attention weights begin to accumulate with the decode steps; a prompt over the budget, which
-        is evicted before its first step attends, begins with those of its last token."""
+    def prefill(self, prompts: Sequence[Sequence[int]], cache: PagedKVCache, *,
+                prefix: Optional[Sequence[int]] = None) -> torch.Tensor:
+        """Feeds the next tokens of each sequence (none: it stays idle) behind what the cache holds of
+        it: whole prompts, or chunks of them, beside sequences that are further. Returns the logits
+        [batch, vocab] after each one's last token (zeros for idle sequences). A ``prefix`` precedes
+        every prompt of an empty cache: it is computed once, and its full pages are held once. In a
+        cache with a budget, attention weights begin to accumulate with the decode steps; a sequence
+        over the budget, which is evicted before its next step attends, begins with those of its
+        last token."""
         require(len(prompts) == cache.batch, f"{cache.batch} prompts expected")
-        require(not any(cache.host_lengths), "prefill expects an empty cache")
         lengths = [len(p) for p in prompts]
         require(sum(lengths) > 0, "at least one prompt must hold a token")
         vocab = self.model.cfg.vocab
-        require(all(0 <= t < vocab for p in prompts for t in p), f"prompt ids must be in [0, {vocab})")
+        require(all(0 <= t < vocab for p in (*prompts, prefix or ()) for t in p),
+                f"prompt ids must be in [0, {vocab})")
+        if prefix:
+            require(not any(cache.host_lengths), "a prefix expects an empty cache")
+            require(cache.budget is None, "a cache with a budget shares no prefix")
+            whole = [len(prefix) + n if n else 0 for n in lengths]
+            self._check_positions(cache, whole)
+            require(max(whole) <= cache.max_slots, f"{max(whole)} tokens in {cache.max_slots} slots")
+            live = [b for b, n in enumerate(lengths) if n]
+            shared = len(prefix) // cache.page_size * (len(live) - 1)
+            pages = sum(-(-n // cache.page_size) for n in whole) - shared
+            require(pages <= len(cache.free_pages), f"{pages} pages needed, {len(cache.free_pages)} free")
+            self.prefill([prefix if b == live[0] else [] for b in range(cache.batch)], cache)
+            cache.fork(live[0], live[1:])
         self._check_positions(cache, lengths)
+        if cache.over_budget():
+            cache.evict()
         cache.reserve(lengths)
         flat = torch.tensor([t for p in prompts for t in p], dtype=torch.int64).to(self.model.device)
         begins = [sum(lengths[:b]) for b in range(len(lengths))]
         over = last_rows = None
-        if cache.budget is not None and max(lengths) > cache.budget:
-            over = torch.tensor([n if n > cache.budget else 0 for n in lengths],
+        held = [h if n else 0 for h, n in zip(cache.host_lengths, lengths)]
+        if cache.budget is not None and max(held) > cache.budget:
+            over = torch.tensor([h if h > cache.budget else 0 for h in held],
                                 dtype=torch.int32).to(self.model.device)
             last_rows = torch.tensor([begins[b] + n - 1 if n else 0
                                       for b, n in enumerate(lengths)]).to(self.model.device)
@@ -101,15 +132,7 @@ class PagedLlamaDecoder(torch.nn.Module):
         def attend(i, q):
             if over is not None:
                 cache.weigh(i, q[last_rows], over)
-            o = torch.empty_like(q)
-            for b, n in enumerate(lengths):
-                if n:
-                    K, V = cache.gather(i, b)
-                    rows = slice(begins[b], begins[b] + n)
-                    o[rows] = F.scaled_dot_product_attention(
-                        q[rows].transpose(0, 1)[None], K[None], V[None], is_causal=True,
-                        enable_gqa=True)[0].transpose(0, 1)
-            return o
+            return cache.prefill_attend(i, q)
 
         x = self._layers(flat, cache, attend)
         logits = torch.zeros(cache.batch, self.model.cfg.vocab, dtype=x.dtype, device=x.device)
@@ -153,8 +176,9 @@ class PagedLlamaDecoder(torch.nn.Module):
                  presence: Optional[torch.Tensor] = None,
                  frequency: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                  allowed: Optional[Callable[[List[List[int]]], Optional[torch.Tensor]]] = None,
-                 stop: Optional[int] = None) -> List[List[int]]:
-        """Greedy generation of up to ``max_new`` tokens after each prompt, which must not be empty.
+                 stop: Optional[int] = None, prefix: Optional[Sequence[int]] = None) -> List[List[int]]:
+        """Greedy generation of up to ``max_new`` tokens after each prompt, which must not be empty;
+        a ``prefix`` precedes all of them and is computed and held once (:meth:`prefill`).
 
         The penalties, ``bias`` and mask are those of
         :func:`~dcr_b200.kernel.cuda.logits.process_logits`; ``allowed(generated)`` returns a step's
@@ -163,16 +187,17 @@ class PagedLlamaDecoder(torch.nn.Module):
         require(len(prompts) == cache.batch, f"{cache.batch} prompts expected")
         require(max_new > 0 and all(len(p) > 0 for p in prompts), "prompts must hold a token each")
         B, dev = cache.batch, self.model.device
-        width = max(len(p) for p in prompts) + max_new
+        whole = [[*(prefix or ()), *p] for p in prompts]
+        width = max(len(p) for p in whole) + max_new
         history = torch.full((B, width), -1, dtype=torch.int64)
-        for b, p in enumerate(prompts):
-            history[b, :len(p)] = torch.tensor(list(p), dtype=torch.int64)
+        for b, p in enumerate(whole):
+            history[b, :len(p)] = torch.tensor(p, dtype=torch.int64)
         history = history.to(dev)
-        n_prompt = torch.tensor([len(p) for p in prompts], dtype=torch.int32).to(dev)
+        n_prompt = torch.tensor([len(p) for p in whole], dtype=torch.int32).to(dev)
         n_tok = n_prompt.clone()
         out: List[List[int]] = [[] for _ in range(B)]
         live = [True] * B
-        logits = self.prefill(prompts, cache)
+        logits = self.prefill(prompts, cache, prefix=prefix)
         for i in range(max_new):
             mask = None if allowed is None else allowed(out)
             _, token = process_logits(logits, tokens=history, token_lengths=n_tok,

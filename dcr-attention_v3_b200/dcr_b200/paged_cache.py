@@ -5,7 +5,9 @@ the start; :class:`PagedKVCache` hands out pages of ``page_size`` slots as seque
 them back when a sequence ends or its slots are evicted, and keeps one page table for all layers
 (a page number means the same page of every layer's pool). With a ``budget`` it also keeps, per
 layer, the accumulated attention weight and the position of every slot, and evicts what is over
-the budget (``paged_evict``). The reference concatenates one contiguous cache per layer
+the budget (``paged_evict``). Without one, sequences may share the pages of a common prefix
+(:meth:`PagedKVCache.fork`), which attention then reads once for them
+(``paged_shared_attention``). The reference concatenates one contiguous cache per layer
 (dcr_attention/models/llama/compat.py:208-254) and has no counterpart.
 
 The host knows every length, so page handling never waits for the device; lengths, slots and
@@ -19,7 +21,8 @@ import torch
 
 from dcr_b200.kernel.cuda._common import HEAD_DIM, check_dtype, require
 from dcr_b200.kernel.cuda.paged import (PAGED_HEAD_DIMS, paged_append, paged_attention,
-                                        paged_evict)
+                                        paged_evict, paged_prefill, paged_rotary_append,
+                                        paged_shared_attention)
 
 
 class PagedKVCache:
@@ -55,6 +58,8 @@ class PagedKVCache:
         self.lengths = torch.zeros(batch, **i32)     # cached slots
         self.seen = torch.zeros(batch, **i32)        # positions so far
         self.queried = torch.zeros(batch, **i32)     # lengths of the sequences that grew last, else 0
+        self.starts = torch.zeros(batch + 1, **i32)  # where each one's tokens reserved last begin
+        self.groups = self.prefix = None             # sequences that share pages (fork)
         self.weights = self.pos = None
         if budget is not None:
             tables = (batch, H_kv, self.max_pages * page_size)
@@ -67,6 +72,7 @@ class PagedKVCache:
         self.host_seen = [0] * batch
         self._grew = [False] * batch                 # the sequences that reserved a token last
         self.host_pages: List[List[int]] = [[] for _ in range(batch)]
+        self._holders = [0] * pages                  # sequences that hold each page
         self._tokens = None  # (seq, slots, positions) of the tokens reserved last
 
     # ------------------------------------------------------------------------------- host side
@@ -83,6 +89,29 @@ class PagedKVCache:
         for b in rows:
             held = self.host_pages[b]
             to_device(self.page_table[b], held + [-1] * (self.max_pages - len(held)))
+        if rows and max(self._holders, default=0) < 2:
+            self.groups = self.prefix = None
+        elif rows:
+            groups, prefix = self.shared_groups()
+            self.groups = torch.tensor(groups, dtype=torch.int32).to(self.device)
+            self.prefix = torch.tensor(prefix, dtype=torch.int32).to(self.device)
+
+    def shared_groups(self):
+        """(groups, prefix), as :func:`paged_shared_attention` takes them: neighbouring sequences whose
+        first pages are the same ones, and the slots in them."""
+        groups, prefix, lead = [0], [0] * self.batch, 0
+        for b in range(1, self.batch):
+            first, held = self.host_pages[lead], self.host_pages[b]
+            same = 0
+            while same < min(len(first), len(held)) and first[same] == held[same]:
+                same += 1
+            if same == 0:
+                groups.append(b)
+                lead = b
+            else:
+                prefix[b] = same * self.page_size
+                prefix[lead] = max(prefix[lead], prefix[b])
+        return groups + [self.batch], prefix
 
     def _resize(self, b: int, length: int) -> bool:
         """Gives sequence b the pages of `length` slots; True if they changed."""
@@ -90,8 +119,12 @@ class PagedKVCache:
         before = len(held)
         while len(held) < need:
             held.append(self.free_pages.pop())
+            self._holders[held[-1]] = 1
         while len(held) > need:
-            self.free_pages.append(held.pop())
+            page = held.pop()
+            self._holders[page] -= 1
+            if self._holders[page] == 0:
+                self.free_pages.append(page)
         self.host_lengths[b] = length
         return len(held) != before
 
@@ -116,6 +149,8 @@ class PagedKVCache:
         self._grew = [n > 0 for n in new_tokens]
         self._publish(changed)
         i32 = dict(dtype=torch.int32)
+        begins = [sum(new_tokens[:b]) for b in range(self.batch + 1)]
+        self.starts = torch.tensor(begins, **i32).to(self.device)
         self._tokens = tuple(torch.tensor(x, **i32).to(self.device) for x in (seq, slots, positions))
         return len(seq)
 
@@ -124,6 +159,32 @@ class PagedKVCache:
         self._resize(b, 0)
         self.host_seen[b], self._grew[b] = 0, False
         self._publish([b])
+
+    def fork(self, b: int, others: Sequence[int]) -> None:
+        """Gives the empty sequences ``others`` what sequence b holds: its full pages are shared, the
+        last one, if it is not full, is copied. A page goes back to the pool with the last sequence
+        that holds it. Refuses, changing nothing, where the pool runs out of pages."""
+        require(self.budget is None, "a cache with a budget shares no pages")
+        require(0 <= b < self.batch and self.host_lengths[b] > 0, f"sequence {b} holds nothing")
+        require(len(set(others)) == len(others) and
+                all(0 <= o < self.batch and o != b and self.host_lengths[o] == 0 for o in others),
+                "others must be different empty sequences")
+        n, pages = self.host_lengths[b], self.host_pages[b]
+        full = n // self.page_size
+        copies = len(others) if n % self.page_size else 0
+        require(copies <= len(self.free_pages), f"{copies} pages needed, {len(self.free_pages)} free")
+        for o in others:
+            self.host_pages[o] = pages[:full]
+            for page in pages[:full]:
+                self._holders[page] += 1
+            self._resize(o, n)
+            self.host_seen[o] = self.host_seen[b]
+            self._grew[o] = False
+        if copies:
+            to = torch.tensor([self.host_pages[o][-1] for o in others], device=self.device)
+            for pool in self.k + self.v:
+                pool[to] = pool[pages[full]].clone()
+        self._publish(others)
 
     def over_budget(self) -> bool:
         """Whether some sequence holds ``budget + slack`` slots or more."""
@@ -142,10 +203,34 @@ class PagedKVCache:
                             eps=eps, weights=None if self.weights is None else self.weights[layer],
                             pos=None if self.pos is None else self.pos[layer])
 
+    def append_rotary(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                      inv_freq: torch.Tensor, *, interleaved: bool = False, factor: float = 1.0,
+                      q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                      eps: float = 1e-5) -> torch.Tensor:
+        """:meth:`append` with the rotation of :func:`paged_rotary_append`: from frequencies, in any
+        layout."""
+        require(self._tokens is not None, "reserve() comes before append_rotary()")
+        seq, slots, positions = self._tokens
+        return paged_rotary_append(q, k, v, inv_freq, positions, self.k[layer], self.v[layer],
+                                   self.page_table, slots, seq=seq, interleaved=interleaved, factor=factor,
+                                   q_weight=q_weight, k_weight=k_weight, eps=eps,
+                                   weights=None if self.weights is None else self.weights[layer],
+                                   pos=None if self.pos is None else self.pos[layer])
+
+    def prefill_attend(self, layer: int, q: torch.Tensor, *, window: int = 0) -> torch.Tensor:
+        """O ``[tokens, H, D]`` of the tokens reserved last, each over its sequence's slots up to its own.
+        No attention weights are accumulated (:meth:`weigh`)."""
+        require(self._tokens is not None, "reserve() comes before prefill_attend()")
+        return paged_prefill(q, self.k[layer], self.v[layer], self.page_table, self.lengths, self.starts,
+                             window=window)
+
     def attend(self, layer: int, q: torch.Tensor, *, window: int = 0) -> torch.Tensor:
         """O ``[batch, H, D]`` of one query row per sequence over the layer's cached slots; with a
         budget the slots' attention weights are accumulated. A sequence that reserved no token last
-        gets zeros and accumulates nothing."""
+        gets zeros and accumulates nothing. Pages that neighbouring sequences share are read once."""
+        if self.groups is not None:
+            return paged_shared_attention(q, self.k[layer], self.v[layer], self.page_table, self.queried,
+                                          self.groups, self.prefix, window=window)
         return paged_attention(q, self.k[layer], self.v[layer], self.page_table, self.queried,
                                window=window,
                                weights=None if self.weights is None else self.weights[layer])
