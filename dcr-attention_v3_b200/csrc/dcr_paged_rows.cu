@@ -107,9 +107,10 @@ constexpr int kRowsMaxParts = 64;
 constexpr int kRowsMinPart = 4;  // tiles of 128 slots: smaller parts gain nothing, larger ones idle SMs
 
 // Finds this CTA's rows and their limits. A unit is a KV head's tile of BM rows of a segment. Where
-// units are many (pieces = 0) blockIdx.x is one, tiles from the last to the first, since a causal
-// segment's last rows see most. Else units are cut into parts of at most a number of slots, the least
-// for which all parts are no more than the grid. False: nothing to do.
+// units are many (pieces = 0) blockIdx.x is one: heads of a tile side by side, a segment's tiles from the
+// last to the first, since a causal segment's last rows see most, and segments (of up to 64) from the
+// one that sees most on, so that the grid ends on short units. Else units are cut into parts of at most
+// a number of slots, the least for which all parts are no more than the grid. False: nothing to do.
 template <int BM>
 __device__ __forceinline__ bool rows_begin(const RowsParams& p, RowsUnit& u, int2* limits) {
   const int lane = threadIdx.x & 31;
@@ -144,6 +145,61 @@ __device__ __forceinline__ bool rows_begin(const RowsParams& p, RowsUnit& u, int
       }
       chunk = max(1, most);
     }
+    if (lane == 0) u.rows = 0;
+    __syncwarp();
+    auto take = [&](int s, int tok0, int ntok, int parts, int unit, int split) {
+      const int tile = unit / p.H_kv;
+      u.seg = s;
+      u.tok0 = tok0;
+      u.ntok = ntok;
+      u.len = p.prefix == nullptr ? checked_length(p.c, p.lengths[s]) : 0;
+      u.hk = unit - tile * p.H_kv;
+      u.split = split;
+      u.parts = parts;
+      u.row0 = tile * BM;
+      u.rows = min(BM, ntok * p.G - u.row0);
+      u.lo_min = u.hi_min = INT32_MAX;
+      u.lo_max = u.hi_max = 0;
+    };
+    const int want = blockIdx.x;
+    // with K segments a lane: this lane's, if it has the unit
+    auto sorted = [&](auto k) {
+      constexpr int K = decltype(k)::value;
+      int tok0[K], ntok[K], weight[K], n[K], before[K] = {};
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        const int s = lane * K + j;
+        tok0[j] = ntok[j] = weight[j] = 0;
+        if (s < p.nseg) {
+          rows_segment(p, s, tok0[j], ntok[j]);
+          weight[j] = rows_weight(p, s, tok0[j], ntok[j]);
+        }
+        n[j] = tiles_of(ntok[j]);
+      }
+      const int lanes = (p.nseg + K - 1) / K;
+#pragma unroll 4
+      for (int o = 0; o < lanes; ++o)
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+          const int w = __shfl_sync(0xffffffffu, weight[i], o), m = __shfl_sync(0xffffffffu, n[i], o);
+#pragma unroll
+          for (int j = 0; j < K; ++j)
+            if (w > weight[j] || (w == weight[j] && o * K + i < lane * K + j)) before[j] += m;
+        }
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        const int at = want - before[j];
+        if (at >= 0 && at < n[j]) {
+          const int tile = at / p.H_kv;  // from the last
+          take(lane * K + j, tok0[j], ntok[j], 1, n[j] - (tile + 1) * p.H_kv + (at - tile * p.H_kv), 0);
+        }
+      }
+    };
+    if (p.pieces == 0 && p.nseg <= 32) {
+      sorted(std::integral_constant<int, 1>());
+    } else if (p.pieces == 0 && p.nseg <= 64) {
+      sorted(std::integral_constant<int, 2>());
+    } else {
     auto parts_of = [&](int s, int tok0, int ntok) {
       return p.pieces > 0 ? (rows_weight(p, s, tok0, ntok) + chunk - 1) / chunk : 1;
     };
@@ -161,13 +217,6 @@ __device__ __forceinline__ bool rows_begin(const RowsParams& p, RowsUnit& u, int
       const int y = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += y;
     }
-    int want = blockIdx.x;
-    if (p.pieces == 0) {  // the order of tiles reversed, heads of a tile side by side
-      const int tile = want / p.H_kv;
-      want = __shfl_sync(0xffffffffu, upto, 31) - (tile + 1) * p.H_kv + (want - tile * p.H_kv);
-    }
-    if (lane == 0) u.rows = 0;
-    __syncwarp();
     int before = upto - mine;
     if (want >= before && want < upto) {
       for (int s = lane * per;; ++s) {
@@ -178,20 +227,11 @@ __device__ __forceinline__ bool rows_begin(const RowsParams& p, RowsUnit& u, int
           before += n;
           continue;
         }
-        const int unit = (want - before) / parts, tile = unit / p.H_kv;
-        u.seg = s;
-        u.tok0 = tok0;
-        u.ntok = ntok;
-        u.len = p.prefix == nullptr ? checked_length(p.c, p.lengths[s]) : 0;
-        u.hk = unit - tile * p.H_kv;
-        u.split = want - before - unit * parts;
-        u.parts = parts;
-        u.row0 = tile * BM;
-        u.rows = min(BM, ntok * p.G - u.row0);
-        u.lo_min = u.hi_min = INT32_MAX;
-        u.lo_max = u.hi_max = 0;
+        const int unit = (want - before) / parts;
+        take(s, tok0, ntok, parts, unit, want - before - unit * parts);
         break;
       }
+    }
     }
   }
   __syncthreads();
