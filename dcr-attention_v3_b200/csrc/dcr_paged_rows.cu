@@ -39,6 +39,7 @@ struct RowsParams {
   const int32_t* starts;   // [nseg + 1] tokens of each segment
   const int32_t* prefix;   // shared: [T]; prefill: null
   int T, nseg, H, H_kv, G;
+  FastDiv of_G;            // rows to tokens
   int pieces;              // CTAs that units are cut up for (0: a unit is one CTA's)
   int window, causal;
   float scale2;            // scale * log2(e)
@@ -78,7 +79,7 @@ __device__ __forceinline__ void rows_segment(const RowsParams& p, int s, int& to
 
 // Row r's slots [x, y).
 __device__ __forceinline__ int2 rows_limits(const RowsParams& p, const RowsUnit& u, int r) {
-  const int i = (u.row0 + r) / p.G;
+  const int i = static_cast<int>(p.of_G.div(u.row0 + r));
   if (p.prefix != nullptr) {
     const int len = checked_length(p.c, p.lengths[u.tok0 + i]);
     return make_int2(p.window > 0 ? max(0, len - p.window) : 0, min(len, p.prefix[u.tok0 + i]));
@@ -334,7 +335,6 @@ __global__ void __launch_bounds__(kRfThreads) rows_fma_kernel(const RowsParams p
   __shared__ int2 limits[kRfRows];
   __shared__ int64_t koff[kRfSlots], voff[kRfSlots];
   __shared__ int flag[kRfSlots];  // 1: mapped; 2: V not finite
-  __shared__ int bad;
   float* qt = rf_smem;
   float* kt = qt + D * W;
   float* vs = kt + D * W;
@@ -344,10 +344,10 @@ __global__ void __launch_bounds__(kRfThreads) rows_fma_kernel(const RowsParams p
   if (!rows_begin<kRfRows>(p, u, limits)) return;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   for (int i = threadIdx.x; i < kRfRows * C; i += kRfThreads) {
-    const int r = i / C, ch = i - r * C;
+    const int r = i % kRfRows, ch = i / kRfRows;  // neighbouring lanes, neighbouring rows: see below
     float f[N] = {};
     if (r < u.rows) {
-      const int t = (u.row0 + r) / p.G, g = u.row0 + r - t * p.G;
+      const int t = static_cast<int>(p.of_G.div(u.row0 + r)), g = u.row0 + r - t * p.G;
       const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) +
                                                         (u.tok0 + t) * p.qst + (u.hk * p.G + g) * p.qsh);
       ElemTraits<T>::widen(src[ch], f);
@@ -373,13 +373,20 @@ __global__ void __launch_bounds__(kRfThreads) rows_fma_kernel(const RowsParams p
     __syncthreads();
     if (threadIdx.x < kRfSlots)
       flag[threadIdx.x] = rows_slot(p, u, j0 + threadIdx.x, koff[threadIdx.x], voff[threadIdx.x]);
-    if (threadIdx.x == 0) bad = 0;
     __syncthreads();
+    // K by neighbouring rows: its elements go to neighbouring words of the transposed tile then
+    for (int i = threadIdx.x; i < kRfSlots * C; i += kRfThreads) {
+      const int j = i % kRfSlots, ch = i / kRfSlots;
+      float f[N] = {};
+      if (flag[j] & 1)
+        ElemTraits<T>::widen(reinterpret_cast<const uint4*>(static_cast<const T*>(p.c.k) + koff[j])[ch], f);
+#pragma unroll
+      for (int e = 0; e < N; ++e) kt[(ch * N + e) * W + j] = f[e];
+    }
     for (int i = threadIdx.x; i < kRfSlots * C; i += kRfThreads) {
       const int j = i / C, ch = i - j * C;
-      float f[N] = {}, x[N] = {};
+      float x[N] = {};
       if (flag[j] & 1) {
-        ElemTraits<T>::widen(reinterpret_cast<const uint4*>(static_cast<const T*>(p.c.k) + koff[j])[ch], f);
         ElemTraits<T>::widen(reinterpret_cast<const uint4*>(static_cast<const T*>(p.c.v) + voff[j])[ch], x);
         if (!whole) {
           bool fine = true;
@@ -389,14 +396,9 @@ __global__ void __launch_bounds__(kRfThreads) rows_fma_kernel(const RowsParams p
               fine = false;
               x[e] = 0.0f;
             }
-          if (!fine) {
-            atomicOr(&flag[j], 2);
-            bad = 1;
-          }
+          if (!fine) atomicOr(&flag[j], 2);
         }
       }
-#pragma unroll
-      for (int e = 0; e < N; ++e) kt[(ch * N + e) * W + j] = f[e];
 #pragma unroll
       for (int e = 0; e < N; e += 4)
         *reinterpret_cast<float4*>(vs + j * D + ch * N + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
@@ -420,6 +422,7 @@ __global__ void __launch_bounds__(kRfThreads) rows_fma_kernel(const RowsParams p
       seen |= (flag[4 * tx + e] & 1) << e;
       spoilt |= (flag[4 * tx + e] >> 1) << e;
     }
+    float weight[4][4];  // [slot][row]
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float z[4] = {s[i][0].x, s[i][0].y, s[i][1].x, s[i][1].y};
@@ -443,15 +446,20 @@ __global__ void __launch_bounds__(kRfThreads) rows_fma_kernel(const RowsParams p
       for (int e = 0; e < 2 * E; ++e) o[i][e] = make_float2(o[i][e].x * a, o[i][e].y * a);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float w = rows_exp2(z[e] - base);
-        l[i] += w;
-        pt[(4 * tx + e) * W + 4 * ty + i] = w;
+        weight[e][i] = rows_exp2(z[e] - base);
+        l[i] += weight[e][i];
       }
     }
+    // slot 4 tx + e in row 16 e + tx, so that the lanes' words lie in different banks
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      *reinterpret_cast<float4*>(pt + (16 * e + tx) * W + 4 * ty) =
+          make_float4(weight[e][0], weight[e][1], weight[e][2], weight[e][3]);
     __syncthreads();
 #pragma unroll 4
-    for (int j = 0; j < kRfSlots; ++j) {
-      const float4 a = *reinterpret_cast<const float4*>(pt + j * W + 4 * ty);
+    for (int k = 0; k < kRfSlots; ++k) {
+      const int j = k % 16 * 4 + k / 16;
+      const float4 a = *reinterpret_cast<const float4*>(pt + k * W + 4 * ty);
       const float w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
       for (int x = 0; x < E; ++x) {
@@ -474,7 +482,7 @@ __global__ void __launch_bounds__(kRfThreads) rows_fma_kernel(const RowsParams p
     }
     const int r = 4 * ty + i;
     if (r >= u.rows) continue;
-    const int t = (u.row0 + r) / p.G, g = u.row0 + r - t * p.G;
+    const int t = static_cast<int>(p.of_G.div(u.row0 + r)), g = u.row0 + r - t * p.G;
     const int64_t row = static_cast<int64_t>(u.tok0 + t) * p.H + u.hk * p.G + g;
     const float nan = __int_as_float(0x7fffffff);
     if (rows_in_parts(p, u)) {
@@ -934,7 +942,7 @@ __device__ __forceinline__ void rows_tc_write(const RowsParams& p, RowsTcShared&
   }
   const bool in = r < u.rows;
   const int rr = in ? u.row0 + r : 0;
-  const int t = rr / p.G, g = rr - t * p.G;
+  const int t = static_cast<int>(p.of_G.div(rr)), g = rr - t * p.G;
   const int64_t row = static_cast<int64_t>(u.tok0 + t) * p.H + u.hk * p.G + g;
   const float nan = __int_as_float(0x7fffffff);
   const float spoil = in && sh.spoilt[r] ? nan : 1.0f;
@@ -999,7 +1007,7 @@ __global__ void __launch_bounds__(RowsTc<D, Twin>::kThreads, 1) rows_tc_kernel(c
   const int tid = threadIdx.x, n = tiles.y - tiles.x;
   if (n <= 0) {  // no row of this part sees a slot
     for (int r = tid; r < u.rows; r += S::kThreads) {
-      const int t = (u.row0 + r) / p.G, g = u.row0 + r - t * p.G;
+      const int t = static_cast<int>(p.of_G.div(u.row0 + r)), g = u.row0 + r - t * p.G;
       const int64_t row = static_cast<int64_t>(u.tok0 + t) * p.H + u.hk * p.G + g;
       if (rows_in_parts(p, u)) {
         p.part_ml[rows_place<S::kRows>(p, u, r, row)] = make_float2(-INFINITY, 0.0f);
@@ -1014,6 +1022,25 @@ __global__ void __launch_bounds__(RowsTc<D, Twin>::kThreads, 1) rows_tc_kernel(c
     return;
   }
   const int blocks = Twin || u.rows > 128 ? 2 : 1;
+  // q on its way: a block's rows are brought in by its threads, with Twin half of them by each block's
+  constexpr int C = D / 8, kQRows = Twin ? 64 : 128, kQSteps = kQRows * C / 128;
+  auto q_row = [&](int i) { return (tid % 128 + i * 128) / C + tid / 128 * kQRows; };
+  auto q_place = [&](int i) {
+    const int r = q_row(i), ch = tid % C;
+    return reinterpret_cast<uint4*>(q + r / 128 * S::kTile + (ch >> 3) * S::kPanel + r % 128 * 128 +
+                                    (((ch & 7) ^ (r & 7)) << 4));
+  };
+  if (tid / 128 < blocks && tid < S::kLoad0) {
+#pragma unroll
+    for (int i = 0; i < kQSteps; ++i) {
+      const bool in = q_row(i) < u.rows;
+      const int rr = in ? u.row0 + q_row(i) : 0;
+      const int t = static_cast<int>(p.of_G.div(rr)), g = rr - t * p.G;
+      cp_async_16(q_place(i), static_cast<const T*>(p.q) + (u.tok0 + t) * p.qst + (u.hk * p.G + g) * p.qsh + tid % C * 8,
+                  in ? 16u : 0u);
+    }
+    cp_async_commit();
+  }
   if (tid == S::kMma) {
     mbar_init(&sh.q_full, blocks * 128);
     for (int x = 0; x < 2; ++x) {
@@ -1041,23 +1068,13 @@ __global__ void __launch_bounds__(RowsTc<D, Twin>::kThreads, 1) rows_tc_kernel(c
   if (tid < S::kLoad0) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSoftmax));
     if (tid / 128 < blocks) {
-      // the block's rows of q; with Twin each block brings in half of them
-      constexpr int C = D / 8, kRowsHere = Twin ? 64 : 128;
-      const int r0 = tid / 128 * kRowsHere;
-      const uint32_t flip = p.scale2 < 0.0f ? 0x80008000u : 0u;
-#pragma unroll 4
-      for (int i = tid % 128; i < kRowsHere * C; i += 128) {
-        const int r = r0 + i / C, ch = i % C, rr = u.row0 + r;
-        uint4 w = make_uint4(0u, 0u, 0u, 0u);
-        if (r < u.rows && p.scale2 != 0.0f) {
-          const int t = rr / p.G, g = rr - t * p.G;
-          w = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (u.tok0 + t) * p.qst +
-                                             (u.hk * p.G + g) * p.qsh)[ch];
-          w = make_uint4(w.x ^ flip, w.y ^ flip, w.z ^ flip, w.w ^ flip);
+      cp_async_wait<0>();
+      if (p.scale2 <= 0.0f)
+        for (int i = 0; i < kQSteps; ++i) {
+          uint4* at = q_place(i);
+          const uint32_t keep = p.scale2 < 0.0f ? 0xffffffffu : 0u, flip = keep & 0x80008000u;
+          *at = make_uint4((at->x & keep) ^ flip, (at->y & keep) ^ flip, (at->z & keep) ^ flip, (at->w & keep) ^ flip);
         }
-        *reinterpret_cast<uint4*>(q + r / 128 * S::kTile + (ch >> 3) * S::kPanel + r % 128 * 128 +
-                                  (((ch & 7) ^ (r & 7)) << 4)) = w;
-      }
       fence_proxy_async_smem();
       mbar_arrive(&sh.q_full);
       float2 state = make_float2(-INFINITY, 0.0f);
@@ -1351,6 +1368,7 @@ int dcr_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, con
   p.H = H;
   p.H_kv = H_kv;
   p.G = H / H_kv;
+  p.of_G = FastDiv::make(static_cast<uint32_t>(p.G));
   p.window = window;
   p.causal = causal != 0;
   p.scale2 = scale * kLog2e;
@@ -1438,6 +1456,7 @@ int dcr_paged_shared_attend(const void* q, int64_t q_stride_b, int64_t q_stride_
   p.H = H;
   p.H_kv = H_kv;
   p.G = G;
+  p.of_G = FastDiv::make(static_cast<uint32_t>(G));
   p.window = window;
   p.causal = 0;
   p.scale2 = own.scale2;
