@@ -310,162 +310,172 @@ __device__ __forceinline__ bool rows_slot(const RowsParams& p, const RowsUnit& u
 __device__ __forceinline__ bool rows_finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
 // ---------------------------------------------------------------------------------------
-// fp32 rows: 64 query rows against tiles of 64 slots with fp32 FMAs, 256 threads of 4 x 4 scores
-// and 4 x D / 16 output elements each. Q and K lie transposed in shared memory, so a step of the
-// inner loop reads four neighbouring rows and four neighbouring slots in two 16-byte reads for
-// 8 packed FMAs.
+// fp32 rows: 128 query rows against tiles of 64 slots with fp32 FMAs, 128 threads of 8 x 8 scores and 8 x
+// D / 8 output elements each. Q and K lie transposed in shared memory, so a step of the inner loop
+// reads eight neighbouring rows and eight slots in four 16-byte reads for 64 FMAs; with 4 x 4 a thread
+// shared memory, not the FMAs, set the pace (314 us for the case below). V comes by cp.async while the
+// scores are computed.
 // ---------------------------------------------------------------------------------------
-constexpr int kRfRows = 64, kRfSlots = 64, kRfThreads = 256;
+constexpr int kRfRows = 128, kRfSlots = 64, kRfThreads = 128;
 
 template <int D>
 struct RowsFma {
-  static constexpr int kPad = 4;
-  static constexpr int W = kRfRows + kPad;
-  static constexpr int kQ = D * W * 4, kK = D * W * 4, kV = kRfSlots * D * 4, kP = kRfSlots * W * 4;
-  static constexpr int kSmem = kQ + kK + kV + kP;
+  static constexpr int WQ = kRfRows + 4, WK = kRfSlots + 4;  // words of a transposed row
+  static constexpr int kSmem = 4 * (D * WQ + D * WK + kRfSlots * D + kRfSlots * WQ);
 };
 
-template <typename T, int D>
+template <int D>
 __global__ void __launch_bounds__(kRfThreads) rows_fma_kernel(const RowsParams p) {
   using S = RowsFma<D>;
-  constexpr int W = S::W, N = ElemTraits<T>::kPerChunk, C = D / N;
-  constexpr int E = D / 64;  // groups of 4 output dims a thread
+  constexpr int WQ = S::WQ, WK = S::WK, C = D / 4, E = D / 32;  // chunks of a row; groups of 4 output dims
   extern __shared__ __align__(16) float rf_smem[];
   __shared__ RowsUnit u;
   __shared__ int2 limits[kRfRows];
   __shared__ int64_t koff[kRfSlots], voff[kRfSlots];
   __shared__ int flag[kRfSlots];  // 1: mapped; 2: V not finite
   float* qt = rf_smem;
-  float* kt = qt + D * W;
-  float* vs = kt + D * W;
+  float* kt = qt + D * WQ;
+  float* vs = kt + D * WK;
   float* pt = vs + kRfSlots * D;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
   if (!rows_begin<kRfRows>(p, u, limits)) return;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
+  // Q and K by neighbouring rows: their elements go to neighbouring words of the transposed tile then
   for (int i = threadIdx.x; i < kRfRows * C; i += kRfThreads) {
-    const int r = i % kRfRows, ch = i / kRfRows;  // neighbouring lanes, neighbouring rows: see below
-    float f[N] = {};
+    const int r = i % kRfRows, ch = i / kRfRows;
+    float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (r < u.rows) {
       const int t = static_cast<int>(p.of_G.div(u.row0 + r)), g = u.row0 + r - t * p.G;
-      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) +
-                                                        (u.tok0 + t) * p.qst + (u.hk * p.G + g) * p.qsh);
-      ElemTraits<T>::widen(src[ch], f);
+      f = reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + (u.tok0 + t) * p.qst +
+                                          (u.hk * p.G + g) * p.qsh)[ch];
     }
-#pragma unroll
-    for (int e = 0; e < N; ++e) qt[(ch * N + e) * W + r] = f[e];
+    float* at = qt + 4 * ch * WQ + r;
+    at[0] = f.x, at[WQ] = f.y, at[2 * WQ] = f.z, at[3 * WQ] = f.w;
   }
-  float2 o[4][2 * E] = {};
-  float m[4], l[4];
-  bool poison[4] = {};
-  int2 lim[4];
+  float2 o[8][2 * E] = {};
+  float m[8], l[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 8; ++i) {
     m[i] = -INFINITY;
     l[i] = 0.0f;
-    lim[i] = limits[4 * ty + i];
   }
+  unsigned poison = 0;  // a bit a row
   const int2 tiles = rows_tiles<kRfSlots>(p, u);
 #pragma unroll 1
   for (int t = tiles.x; t < tiles.y; ++t) {
     const int j0 = t * kRfSlots;
-    const bool whole = j0 >= u.lo_max && j0 + kRfSlots <= u.hi_min;
+    const bool seen = j0 >= u.lo_max && j0 + kRfSlots <= u.hi_min;  // whole, by every row
     __syncthreads();
     if (threadIdx.x < kRfSlots)
       flag[threadIdx.x] = rows_slot(p, u, j0 + threadIdx.x, koff[threadIdx.x], voff[threadIdx.x]);
     __syncthreads();
-    // K by neighbouring rows: its elements go to neighbouring words of the transposed tile then
-    for (int i = threadIdx.x; i < kRfSlots * C; i += kRfThreads) {
-      const int j = i % kRfSlots, ch = i / kRfSlots;
-      float f[N] = {};
-      if (flag[j] & 1)
-        ElemTraits<T>::widen(reinterpret_cast<const uint4*>(static_cast<const T*>(p.c.k) + koff[j])[ch], f);
-#pragma unroll
-      for (int e = 0; e < N; ++e) kt[(ch * N + e) * W + j] = f[e];
-    }
+#pragma unroll 4
     for (int i = threadIdx.x; i < kRfSlots * C; i += kRfThreads) {
       const int j = i / C, ch = i - j * C;
-      float x[N] = {};
-      if (flag[j] & 1) {
-        ElemTraits<T>::widen(reinterpret_cast<const uint4*>(static_cast<const T*>(p.c.v) + voff[j])[ch], x);
-        if (!whole) {
-          bool fine = true;
-#pragma unroll
-          for (int e = 0; e < N; ++e)
-            if (!rows_finite(x[e])) {
-              fine = false;
-              x[e] = 0.0f;
-            }
-          if (!fine) atomicOr(&flag[j], 2);
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < N; e += 4)
-        *reinterpret_cast<float4*>(vs + j * D + ch * N + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+      cp_async_16(vs + j * D + ch * 4, static_cast<const float*>(p.c.v) + voff[j] + ch * 4, flag[j] ? 16u : 0u);
+    }
+    cp_async_commit();
+#pragma unroll 4
+    for (int i = threadIdx.x; i < kRfSlots * C; i += kRfThreads) {
+      const int j = i % kRfSlots, ch = i / kRfSlots;
+      float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (flag[j]) f = reinterpret_cast<const float4*>(static_cast<const float*>(p.c.k) + koff[j])[ch];
+      float* at = kt + 4 * ch * WK + j;
+      at[0] = f.x, at[WK] = f.y, at[2 * WK] = f.z, at[3 * WK] = f.w;
     }
     __syncthreads();
-    float2 s[4][2] = {};  // [row][slot pair]
-#pragma unroll 8
+    float2 s[8][4] = {};  // [row][slots 4 tx, 4 tx + 2, 32 + 4 tx, 34 + 4 tx and the next one]
+#pragma unroll 4
     for (int d = 0; d < D; ++d) {
-      const float4 a = *reinterpret_cast<const float4*>(qt + d * W + 4 * ty);
-      const float4 b = *reinterpret_cast<const float4*>(kt + d * W + 4 * tx);
-      const float q[4] = {a.x, a.y, a.z, a.w};
-      const float2 k[2] = {make_float2(b.x, b.y), make_float2(b.z, b.w)};
+      const float4 a0 = *reinterpret_cast<const float4*>(qt + d * WQ + 8 * ty);
+      const float4 a1 = *reinterpret_cast<const float4*>(qt + d * WQ + 8 * ty + 4);
+      const float4 b0 = *reinterpret_cast<const float4*>(kt + d * WK + 4 * tx);
+      const float4 b1 = *reinterpret_cast<const float4*>(kt + d * WK + 32 + 4 * tx);
+      const float q[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
+      const float2 k[4] = {make_float2(b0.x, b0.y), make_float2(b0.z, b0.w), make_float2(b1.x, b1.y),
+                           make_float2(b1.z, b1.w)};
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) s[i][e] = ffma2(make_float2(q[i], q[i]), k[e], s[i][e]);
+        for (int e = 0; e < 4; ++e) s[i][e] = ffma2(make_float2(q[i], q[i]), k[e], s[i][e]);
     }
-    int seen = 0, spoilt = 0;
+    cp_async_wait<0>();
+    if (!seen) {  // a thread's own copies
+      for (int i = threadIdx.x; i < kRfSlots * C; i += kRfThreads) {
+        float* x = vs + i / C * D + i % C * 4;
+        bool fine = true;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      seen |= (flag[4 * tx + e] & 1) << e;
-      spoilt |= (flag[4 * tx + e] >> 1) << e;
+        for (int e = 0; e < 4; ++e)
+          if (!rows_finite(x[e])) {
+            fine = false;
+            x[e] = 0.0f;
+          }
+        if (!fine) atomicOr(&flag[i / C], 2);
+      }
+      __syncthreads();
     }
-    float weight[4][4];  // [slot][row]
+    auto slot = [&](int e) { return e < 4 ? 4 * tx + e : 28 + 4 * tx + e; };
+    unsigned held = 0, spoilt = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float z[4] = {s[i][0].x, s[i][0].y, s[i][1].x, s[i][1].y};
+    for (int e = 0; e < 8; ++e) {
+      held |= static_cast<unsigned>(flag[slot(e)] & 1) << e;
+      spoilt |= static_cast<unsigned>(flag[slot(e)] >> 1) << e;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      unsigned in = held;
+      if (!seen) {
+        const int2 lim = limits[8 * ty + i];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (j0 + slot(e) < lim.x || j0 + slot(e) >= lim.y) in &= ~(1u << e);
+        if ((in & spoilt) != 0) poison |= 1u << i;
+      }
       float top = -INFINITY;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int j = j0 + 4 * tx + e;
-        const bool in = ((seen >> e) & 1) && j >= lim[i].x && j < lim[i].y;
-        z[e] = in ? z[e] * p.scale2 : -INFINITY;
-        if (in && ((spoilt >> e) & 1)) poison[i] = true;
-        top = fmaxf(top, z[e]);
+        s[i][e].x = (in >> (2 * e)) & 1u ? s[i][e].x * p.scale2 : -INFINITY;
+        s[i][e].y = (in >> (2 * e + 1)) & 1u ? s[i][e].y * p.scale2 : -INFINITY;
+        top = fmaxf(top, fmaxf(s[i][e].x, s[i][e].y));
       }
 #pragma unroll
-      for (int x = 8; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      for (int x = 4; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
       const float mn = fmaxf(m[i], top);
-      const float a = m[i] == -INFINITY ? 0.0f : rows_exp2(m[i] - mn);
-      const float base = mn == -INFINITY ? 0.0f : mn;
-      m[i] = mn;
-      l[i] *= a;
+      if (mn > m[i]) {
+        const float a = m[i] == -INFINITY ? 0.0f : rows_exp2(m[i] - mn);
+        m[i] = mn;
+        l[i] *= a;
 #pragma unroll
-      for (int e = 0; e < 2 * E; ++e) o[i][e] = make_float2(o[i][e].x * a, o[i][e].y * a);
+        for (int e = 0; e < 2 * E; ++e) o[i][e] = make_float2(o[i][e].x * a, o[i][e].y * a);
+      }
+      const float base = mn == -INFINITY ? 0.0f : mn;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        weight[e][i] = rows_exp2(z[e] - base);
-        l[i] += weight[e][i];
+        s[i][e] = make_float2(rows_exp2(s[i][e].x - base), rows_exp2(s[i][e].y - base));
+        l[i] += s[i][e].x + s[i][e].y;
       }
     }
-    // slot 4 tx + e in row 16 e + tx, so that the lanes' words lie in different banks
+    // the weights of slot(e) in row 8 e + tx, so that the lanes' words lie in different banks
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      *reinterpret_cast<float4*>(pt + (16 * e + tx) * W + 4 * ty) =
-          make_float4(weight[e][0], weight[e][1], weight[e][2], weight[e][3]);
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {
+        auto w = [&](int r) { return e % 2 ? s[r][e / 2].y : s[r][e / 2].x; };
+        *reinterpret_cast<float4*>(pt + (8 * e + tx) * WQ + 8 * ty + i) = make_float4(w(i), w(i + 1), w(i + 2), w(i + 3));
+      }
     __syncthreads();
-#pragma unroll 4
+#pragma unroll 2
     for (int k = 0; k < kRfSlots; ++k) {
-      const int j = k % 16 * 4 + k / 16;
-      const float4 a = *reinterpret_cast<const float4*>(pt + k * W + 4 * ty);
-      const float w[4] = {a.x, a.y, a.z, a.w};
+      const int j = k < 32 ? k % 8 * 4 + k / 8 : 28 + k % 8 * 4 + k / 8;
+      const float4 a0 = *reinterpret_cast<const float4*>(pt + k * WQ + 8 * ty);
+      const float4 a1 = *reinterpret_cast<const float4*>(pt + k * WQ + 8 * ty + 4);
+      const float w[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
 #pragma unroll
       for (int x = 0; x < E; ++x) {
-        const float4 b = *reinterpret_cast<const float4*>(vs + j * D + 64 * x + 4 * tx);
+        const float4 b = *reinterpret_cast<const float4*>(vs + j * D + 32 * x + 4 * tx);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 8; ++i) {
           o[i][2 * x] = ffma2(make_float2(w[i], w[i]), make_float2(b.x, b.y), o[i][2 * x]);
           o[i][2 * x + 1] = ffma2(make_float2(w[i], w[i]), make_float2(b.z, b.w), o[i][2 * x + 1]);
         }
@@ -473,42 +483,29 @@ __global__ void __launch_bounds__(kRfThreads) rows_fma_kernel(const RowsParams p
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    int spoilt = poison[i];
+  for (int x = 4; x >= 1; x >>= 1) poison |= __shfl_xor_sync(0xffffffffu, poison, x);
 #pragma unroll
-    for (int x = 8; x >= 1; x >>= 1) {
-      l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
-      spoilt |= __shfl_xor_sync(0xffffffffu, spoilt, x);
-    }
-    const int r = 4 * ty + i;
+  for (int i = 0; i < 8; ++i) {
+#pragma unroll
+    for (int x = 4; x >= 1; x >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
+    const int r = 8 * ty + i;
     if (r >= u.rows) continue;
     const int t = static_cast<int>(p.of_G.div(u.row0 + r)), g = u.row0 + r - t * p.G;
     const int64_t row = static_cast<int64_t>(u.tok0 + t) * p.H + u.hk * p.G + g;
-    const float nan = __int_as_float(0x7fffffff);
-    if (rows_in_parts(p, u)) {
-      const int64_t at = rows_place<kRfRows>(p, u, r, row);
-      if (tx == 0) p.part_ml[at] = make_float2(m[i], l[i]);
-      if (l[i] == 0.0f) continue;  // not read
-#pragma unroll
-      for (int x = 0; x < E; ++x)
-        *reinterpret_cast<float4*>(p.part_o + at * D + 64 * x + 4 * tx) =
-            spoilt ? make_float4(nan, nan, nan, nan)
-                   : make_float4(o[i][2 * x].x, o[i][2 * x].y, o[i][2 * x + 1].x, o[i][2 * x + 1].y);
-      continue;
-    }
-    if (p.part_of != nullptr && tx == 0) p.part_of[row] = make_int2(0, 0);
-    const float inv = l[i] == 0.0f ? 0.0f : spoilt ? nan : 1.0f / l[i];
-    T* dst = static_cast<T*>(p.o) + row * D;
+    const bool parts = rows_in_parts(p, u);
+    const int64_t at = parts ? rows_place<kRfRows>(p, u, r, row) : row;
+    if (!parts && p.part_of != nullptr) p.part_of[row] = make_int2(0, 0);
+    const float spoil = (poison >> i) & 1u ? __int_as_float(0x7fffffff) : 1.0f;
+    const float by = l[i] == 0.0f ? 0.0f : parts ? spoil : spoil / l[i];
+    float* dst = (parts ? p.part_o : static_cast<float*>(p.o)) + at * D + 4 * tx;
 #pragma unroll
     for (int x = 0; x < E; ++x) {
-      const int d = 64 * x + 4 * tx;
-      ElemTraits<T>::store(dst, d, o[i][2 * x].x * inv);
-      ElemTraits<T>::store(dst, d + 1, o[i][2 * x].y * inv);
-      ElemTraits<T>::store(dst, d + 2, o[i][2 * x + 1].x * inv);
-      ElemTraits<T>::store(dst, d + 3, o[i][2 * x + 1].y * inv);
+      const float2 c = o[i][2 * x], d = o[i][2 * x + 1];
+      *reinterpret_cast<float4*>(dst + 32 * x) = make_float4(c.x * by, c.y * by, d.x * by, d.y * by);
     }
-    if (tx == 0 && p.lse != nullptr)
-      p.lse[row] = l[i] == 0.0f ? -INFINITY : (m[i] + log2f(l[i])) * kLn2;
+    if (tx != 0) continue;
+    if (parts) p.part_ml[at] = make_float2(m[i], l[i]);
+    else if (p.lse != nullptr) p.lse[row] = l[i] == 0.0f ? -INFINITY : (m[i] + log2f(l[i])) * kLn2;
   }
 }
 
@@ -1182,9 +1179,10 @@ static RowsPlan rows_plan(int dtype, int T, int nseg, int H_kv, int G, bool shar
   r.bm = !tc ? kRfRows : rows > 128ll * nseg ? 256 : 128;
   // every segment adds one tile of rows at most that is not full
   const int64_t units = (rows / r.bm + (nseg < rows ? nseg : rows)) * H_kv;
-  // units are cut up where the grid has more than one CTA for each
+  // Units are cut up where the grid has more than one CTA for each; fp32 ones, whose longest would set the
+  // pace (a tile takes 4 us), up to 4 CTAs an SM.
   const int64_t slots = static_cast<int64_t>(tc ? 1 : 4) * device_sm_count();
-  r.pieces = units <= slots && (shared || 2 * units <= slots) ? static_cast<int>(slots) : 0;
+  r.pieces = units <= slots && (shared || !tc || 2 * units <= slots) ? static_cast<int>(slots) : 0;
   r.units = units;
   r.ctas = r.pieces > 0 ? r.pieces : units;
   return r;
@@ -1258,7 +1256,7 @@ static bool rows_map(CUtensorMap* map, const PagePool& c, const void* base, int6
 template <typename T, int D, int Parts>
 static int rows_launch(const RowsParams& params, const RowsPlan& plan, cudaStream_t s) {
   if constexpr (sizeof(T) == 4) {
-    return rows_launch_as(rows_fma_kernel<T, D>, kRfThreads, RowsFma<D>::kSmem, plan, s, params);
+    return rows_launch_as(rows_fma_kernel<D>, kRfThreads, RowsFma<D>::kSmem, plan, s, params);
   } else {
     RowsParams p = params;
     RowsMaps maps = {};
