@@ -20,6 +20,23 @@
 // Shared: the prefix is read once for a group instead of once for each of its sequences. Each
 // sequence's own slots go through dcr_paged_attend.cu's kernels into fp32 rows; the parts' (m, l, o)
 // are joined by rows_join_kernel, as are those of a run that is split over several CTAs.
+//
+// Bound: with many rows the exponentials, 16 a cycle and SM, which take 1024 cycles for 128 x 128 scores,
+// as long as both products at D = 128 and twice as long at D = 64; with few rows K and V, read once.
+// Measured (calls one after another in a CUDA graph; a tile of 256 rows and 128 slots takes 3100 to 3250
+// cycles, of which 2080 are what its exponentials need, the rest waits for scores and their loads, and
+// a CTA's beginning and end 14000): 2048 tokens on 32768 slots, 32 heads of 128 on 8, f16 (1.13 TFLOP):
+// 1.03 to 1.16 ms by the card's power, 0.98 to 1.1 PFLOP/s; six prompts of 740 to 8192 tokens, heads of
+// 64, bf16 (0.66 TFLOP): 1.10 ms, 600 TFLOP/s; 48 sequences of 2 to 5 drafted tokens, window 8191, f16
+// (556 MB): 139 us, 4.0 TB/s; 18 sequences of 5 tokens on 16000 slots, heads of 128 (1.2 GB): 178 us, 6.6
+// TB/s; 45 samples of three documents of 7700 to 32768 slots, 64 heads of 128 on 8, f16 (398 MB): 109 us;
+// three prompts of 236 to 1499 slots in fp32: 237 us, 25 TFLOP/s.
+// Tried and not kept: a whole tile's scores at once (1264 us for the six prompts, each step waits for
+// its scores then; in halves 1256, before K and V came by the tensor map); the next half's scores loaded
+// before this one's exponentials (1427 instead of 1221); an eighth, a quarter or a third of the
+// exponentials as polynomials on the FMA pipe (1203, 1235 and more instead of 1221, and 1076, 1162
+// instead of 1041 for the heads of 128); turns between the two blocks for the exponentials (1368
+// instead of 1220); few rows four times over for shorter steps (no gain: loads set their pace).
 #include <cuda.h>
 #include <math.h>
 
@@ -312,9 +329,9 @@ __device__ __forceinline__ bool rows_finite(float x) { return fabsf(x) <= 3.4028
 // ---------------------------------------------------------------------------------------
 // fp32 rows: 128 query rows against tiles of 64 slots with fp32 FMAs, 128 threads of 8 x 8 scores and 8 x
 // D / 8 output elements each. Q and K lie transposed in shared memory, so a step of the inner loop
-// reads eight neighbouring rows and eight slots in four 16-byte reads for 64 FMAs; with 4 x 4 a thread
-// shared memory, not the FMAs, set the pace (314 us for the case below). V comes by cp.async while the
-// scores are computed.
+// reads eight neighbouring rows and eight slots in four 16-byte reads for 64 FMAs; V comes by cp.async while the scores are
+// computed. Measured: three prompts of 236 to 1499 slots, 16 heads of 64: 237 us, 344 without cutting
+// long units up; 64 rows and 4 x 4 scores a thread, four reads for 32 FMAs, took 314.
 // ---------------------------------------------------------------------------------------
 constexpr int kRfRows = 128, kRfSlots = 64, kRfThreads = 128;
 
@@ -512,20 +529,21 @@ __global__ void __launch_bounds__(kRfThreads) rows_fma_kernel(const RowsParams p
 // ---------------------------------------------------------------------------------------
 // 16-bit rows: two blocks of 128 query rows against tiles of 128 slots on the tensor cores.
 //
-// Warps: four per block of rows for the softmax, a row a thread; four that bring K and V in, a
-// slot's address a thread; one that issues the products. Per tile and block S = Q K^T goes to tensor
-// memory, the softmax warps read their rows, keep the running base and sum (m, l) and write the
-// weights P back over S, and O += P V accumulates in tensor memory with P as its A operand. K and V
-// tiles take turns in a ring that the loaders fill by 16-byte cp.async: any page size and stride, slots
-// that are not valid filled with zeros and never read. With two blocks the tensor cores and the loaders
-// serve one while the softmax warps of the other compute.
+// Warps: two groups of four for the softmax, a row a thread; two groups of two that bring in K and V; two
+// that issue the products, one for each softmax group. S = Q K^T of 64 slots goes to one of a group's
+// two buffers in tensor memory; the softmax warps read their rows, keep the running base and sum (m, l)
+// and write the weights P back over S; O += P V accumulates in tensor memory with P as its A operand.
+// While a group computes on one buffer, S of the next 64 slots is made in the other. K and V tiles take
+// turns in a ring. Where segments have more than 128 rows on average a CTA takes 256, a block for each
+// group; else (Twin) 128, whose tiles the groups halve between them, and join what they hold at the
+// end: one group alone would wait on its own chain of steps, at 13 bytes of K and V a cycle and SM.
 //
 // The base is raised only when a row's score is 8 above the largest it was set by, so O is rescaled
-// for few tiles, and never while a product on it runs: S of a tile is only seen complete after the
-// products before it. In f16 the base stays 7 below the maximum, so that small weights keep their
-// bits (2^-24 of 2^7). A weight enters the second product rounded to 16 bits, half a step of
-// which is off by as much as the output's own rounding, and averages out over the slots; with Parts =
-// 2 its remainder goes in as well, in a second product.
+// for few steps, and then when the product of the step before is done. In f16 the base stays 7 below the
+// maximum, so that small weights keep their bits (2^-24 of 2^7). A weight enters the second product
+// rounded to 16 bits, which is off by half a step at most, as the output's own rounding, and averages
+// out over the slots (errors against 64 bits as those of fp32 weights to 5%); with Parts = 2, for
+// shared prefixes, which are bound by their loads, its remainder goes in as well, in a second product.
 // ---------------------------------------------------------------------------------------
 constexpr int kTcSlots = 128;
 

@@ -15,7 +15,13 @@
 // Bound: the rows, read and written once. A CTA takes a few tokens: their angles, once for all heads,
 // go to shared memory while the first rows are on their way. A lane takes two 16-byte chunks that
 // hold whole pairs: chunks r/2 elements apart, or neighbours. Where r is not a multiple of two chunks
-// a warp takes a row element by element.
+// a warp takes a row element by element (106 us for 8191 tokens of 40 heads of 80, 20 elements of each
+// turned, a sixth of the memory's rate).
+// Measured (in a CUDA graph): 16381 tokens of 32 + 8 heads of 128, f16 (336 MB): 65.6 us, 5.1 TB/s; the
+// same with the values of 8 more heads into pages, norms, and 96 elements of each head turned in
+// neighbouring pairs, bf16 (403 MB): 109 us, 3.7 TB/s (whole heads in halves: 92), bound by the
+// instructions, 300 for 32 bytes a lane, at five to seven CTAs an SM; 48 tokens: 2.2 and 4.4 us. With items
+// found by divisions and arithmetic that is not packed these took 75 and 121 us.
 #include <type_traits>
 
 #include "dcr_internal.h"

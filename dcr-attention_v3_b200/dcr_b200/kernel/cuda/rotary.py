@@ -1,9 +1,8 @@
 """Position rotation of query and key heads from frequencies (csrc/dcr_rotary.cu).
 
-The model's own step (csrc/dcr_rotary.cu's neighbours, :func:`~dcr_b200.kernel.cuda.paged.paged_append`
-and the decode prologue) rotates whole heads in halves by tables of cosines and sines, as HF
-apply_rotary_pos_emb (dcr_attention/models/llama/attention.py:395). :func:`rotary` takes the
-frequencies instead: halves or neighbours paired, the whole head or its first part, any position
+:func:`~dcr_b200.kernel.cuda.paged.paged_append` and the decode prologue rotate whole heads in halves by
+tables of cosines and sines, as HF apply_rotary_pos_emb
+(dcr_attention/models/llama/attention.py:395). :func:`rotary` takes the frequencies instead: halves or neighbours paired, the whole head or its first part, any position
 without a table, an amplitude. :func:`rotary_frequencies` makes frequencies and amplitude for the
 usual scalings to longer contexts. Arguments are checked in csrc/dcr_torch.cpp, as the paged
 operators'.
