@@ -46,7 +46,8 @@ def attend(q, k_pages, v_pages, rows, lo, hi, *, scale=None, weight_unit=None):
                 o[t0:t1, heads] = torch.einsum("tgn,nd->tgd", p, blank)
                 lse[t0:t1, heads] = s
                 z0 = torch.where(seen, z, 0.0)
-                dz = torch.where(seen, scale * torch.einsum("tgd,nd->tgn", x.abs(), k.abs()), 0.0)
+                # the products enter with their absolute sizes, the scale with its own (it may be negative)
+                dz = torch.where(seen, abs(scale) * torch.einsum("tgd,nd->tgn", x.abs(), k.abs()), 0.0)
                 dz = dz.amax(-1) * (D + 4) * EPS + 4 * EPS * z0.abs().amax(-1)
                 rel = 2 * dz + (n + 48) * 2 * EPS
                 rel_o = rel + (weight_unit or 0.0)
