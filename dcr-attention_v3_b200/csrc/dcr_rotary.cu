@@ -17,11 +17,12 @@
 // hold whole pairs: chunks r/2 elements apart, or neighbours. Where r is not a multiple of two chunks
 // a warp takes a row element by element (106 us for 8191 tokens of 40 heads of 80, 20 elements of each
 // turned, a sixth of the memory's rate).
-// Measured (in a CUDA graph): 16381 tokens of 32 + 8 heads of 128, f16 (336 MB): 65.6 us, 5.1 TB/s; the
+// Measured (in a CUDA graph): 16381 tokens of 32 + 8 heads of 128, f16 (336 MB): 54.3 us, 6.2 TB/s; the
 // same with the values of 8 more heads into pages, norms, and 96 elements of each head turned in
-// neighbouring pairs, bf16 (403 MB): 109 us, 3.7 TB/s (whole heads in halves: 92), bound by the
-// instructions, 300 for 32 bytes a lane, at five to seven CTAs an SM; 48 tokens: 2.2 and 4.4 us. With items
-// found by divisions and arithmetic that is not packed these took 75 and 121 us.
+// neighbouring pairs, bf16 (403 MB): 97 us, 4.2 TB/s (whole heads in halves: 89), bound by instructions and
+// the five to seven CTAs that fit an SM; 48 tokens: 2.2 and 4.3 us. With items found by divisions and
+// arithmetic that is not packed these took 75 and 121 us; loading each item's successor as soon as it
+// was used (95 registers) 59 and 106; six items in flight 62 and 127.
 #include <type_traits>
 
 #include "dcr_internal.h"
@@ -162,7 +163,7 @@ struct RotaryItem {
   }
 };
 
-template <typename T, bool Paged>
+template <typename T, bool Paged, bool Interleaved, bool Norms>
 __global__ void __launch_bounds__(kRoThreads) rotary_kernel(const RotaryParams p) {
   constexpr int N = ElemTraits<T>::kPerChunk;
   extern __shared__ __align__(16) float ro_turn[];
@@ -186,7 +187,7 @@ __global__ void __launch_bounds__(kRoThreads) rotary_kernel(const RotaryParams p
       at[i] = last;
       if (last.t < tokens) {
         const uint4* src = reinterpret_cast<const uint4*>(ro_source<T, Paged>(p, t0 + last.t, last.row));
-        const int2 ch = ro_chunks(last.part, turned, p.interleaved);
+        const int2 ch = ro_chunks(last.part, turned, Interleaved);
         x[i][0] = __ldcs(src + ch.x);
         x[i][1] = __ldcs(src + ch.y);
         last.next(parts, rows);
@@ -196,9 +197,8 @@ __global__ void __launch_bounds__(kRoThreads) rotary_kernel(const RotaryParams p
     }
   };
   load();
-  const bool norms = Paged && (p.qw != nullptr || p.kw != nullptr);
-  __shared__ __align__(16) float weight[Paged ? 2 : 1][Paged ? 128 : 4];
-  if (norms && threadIdx.x < p.D / N * 2) {
+  __shared__ __align__(16) float weight[Norms ? 2 : 1][Norms ? 128 : 4];
+  if (Norms && threadIdx.x < p.D / N * 2) {
     const int k = threadIdx.x >= p.D / N, ch = threadIdx.x - k * (p.D / N);
     const void* w = k ? p.kw : p.qw;
     float g[N];
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(kRoThreads) rotary_kernel(const RotaryParams p
     for (int i = 0; i < kRoSteps; ++i) {
       const int part = at[i].part, t = at[i].t, row = at[i].row;
       const bool in = t < tokens;
-      const int2 ch = ro_chunks(part, turned, p.interleaved);
+      const int2 ch = ro_chunks(part, turned, Interleaved);
       const bool value = Paged && row >= p.H + p.H_kv;
       float2 f[2][N / 2];
 #pragma unroll
@@ -231,8 +231,8 @@ __global__ void __launch_bounds__(kRoThreads) rotary_kernel(const RotaryParams p
         for (int e = 0; e < N / 2; ++e) f[h][e] = make_float2(y[2 * e], y[2 * e + 1]);
       }
       const float2 zero = make_float2(0.0f, 0.0f);
-      const bool normed = Paged && !value && (row < p.H ? p.qw : p.kw) != nullptr;
-      if (norms) {  // all lanes of a row take part
+      const bool normed = Norms && !value && (row < p.H ? p.qw : p.kw) != nullptr;
+      if constexpr (Norms) {  // all lanes of a row take part
         float2 s2 = zero;
 #pragma unroll
         for (int e = 0; e < N / 2; ++e) s2 = ffma2(f[0][e], f[0][e], ffma2(f[1][e], f[1][e], s2));
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(kRoThreads) rotary_kernel(const RotaryParams p
 #pragma unroll
         for (int e = 0; e < N / 4; ++e) {
           const float4 c = reinterpret_cast<const float4*>(cs)[e], s = reinterpret_cast<const float4*>(sn)[e];
-          if (p.interleaved) {  // the pairs 4 e .. 4 e + 3 of the two chunks
+          if constexpr (Interleaved) {  // the pairs 4 e .. 4 e + 3 of the two chunks
             const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -360,8 +360,11 @@ static int ro_launch(RotaryParams p, bool in_place, cudaStream_t s) {
   const bool whole = p.D % (2 * N) == 0 && p.rot % (2 * N) == 0;
   p.parts = (in_place ? p.rot : p.D) / (2 * N);
   const int rows = p.H + (Paged ? 2 : 1) * p.H_kv;
-  // enough tokens for every thread to have kRoSteps items, few enough to fill the SMs
-  int per = whole ? kRoSteps * kRoThreads / (rows * p.parts) : 4;
+  // Tokens a CTA: for a few rounds of kRoSteps items a thread, since a CTA's beginning (places, angles) costs
+  // as much as a round (1, 2 and 4 rounds: 58.3, 54.3 and 54.8 us for the first case above, 108.5, 100.6
+  // and 96.8 for the second), few enough to fill the SMs.
+  constexpr int kRounds = Paged ? 4 : 2;
+  int per = whole ? kRounds * kRoSteps * kRoThreads / (rows * p.parts) : 4;
   const int spread = p.T / (4 * device_sm_count());
   if (per > spread) per = spread;
   if (per > kRoMaxTokens) per = kRoMaxTokens;
@@ -369,8 +372,13 @@ static int ro_launch(RotaryParams p, bool in_place, cudaStream_t s) {
   p.per_cta = per;
   const size_t smem = static_cast<size_t>(per) * p.rot * sizeof(float);
   const dim3 grid((p.T + per - 1) / per);
-  const cudaError_t e = launch_dependent(whole ? rotary_kernel<T, Paged> : rotary_any_kernel<T, Paged>,
-                                         grid, dim3(kRoThreads), smem, s, 1, p);
+  const bool norms = Paged && (p.qw != nullptr || p.kw != nullptr);
+  auto kernel = rotary_any_kernel<T, Paged>;
+  if (whole && norms)
+    kernel = p.interleaved ? rotary_kernel<T, Paged, true, Paged> : rotary_kernel<T, Paged, false, Paged>;
+  else if (whole)
+    kernel = p.interleaved ? rotary_kernel<T, Paged, true, false> : rotary_kernel<T, Paged, false, false>;
+  const cudaError_t e = launch_dependent(kernel, grid, dim3(kRoThreads), smem, s, 1, p);
   return e == cudaSuccess ? DCR_OK : DCR_ERR_CUDA;
 }
 
