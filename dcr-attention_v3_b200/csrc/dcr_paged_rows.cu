@@ -218,38 +218,35 @@ __device__ __forceinline__ bool rows_begin(const RowsParams& p, RowsUnit& u, int
     } else if (p.pieces == 0 && p.nseg <= 64) {
       sorted(std::integral_constant<int, 2>());
     } else {
-    auto parts_of = [&](int s, int tok0, int ntok) {
-      return p.pieces > 0 ? (rows_weight(p, s, tok0, ntok) + chunk - 1) / chunk : 1;
-    };
-    int mine = 0;
-    for (int j = 0; j < per; ++j) {
-      const int s = lane * per + j;
-      int tok0, ntok;
-      if (s >= p.nseg) break;
-      rows_segment(p, s, tok0, ntok);
-      mine += tiles_of(ntok) * parts_of(s, tok0, ntok);
-    }
-    int upto = mine;
+      auto parts_of = [&](int s, int tok0, int ntok) {
+        return p.pieces > 0 ? (rows_weight(p, s, tok0, ntok) + chunk - 1) / chunk : 1;
+      };
+      int mine = 0;
+      for (int j = 0; j < per; ++j) {
+        const int s = lane * per + j;
+        int tok0, ntok;
+        if (s >= p.nseg) break;
+        rows_segment(p, s, tok0, ntok);
+        mine += tiles_of(ntok) * parts_of(s, tok0, ntok);
+      }
+      int upto = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += y;
-    }
-    int before = upto - mine;
-    if (want >= before && want < upto) {
-      for (int s = lane * per;; ++s) {
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+      }
+      int before = upto - mine;
+      for (int s = lane * per; want >= before && want < upto && s < p.nseg; ++s) {
         int tok0, ntok;
         rows_segment(p, s, tok0, ntok);
         const int parts = parts_of(s, tok0, ntok), n = tiles_of(ntok) * parts;
-        if (want >= before + n) {
-          before += n;
-          continue;
+        if (want < before + n) {
+          const int unit = (want - before) / parts;
+          take(s, tok0, ntok, parts, unit, want - before - unit * parts);
+          break;
         }
-        const int unit = (want - before) / parts;
-        take(s, tok0, ntok, parts, unit, want - before - unit * parts);
-        break;
+        before += n;
       }
-    }
     }
   }
   __syncthreads();

@@ -4,8 +4,8 @@
 // arguments and marshalling them through ctypes cost as much again: with the checks in Python a
 // call took 17 to 30 us of host time, from here it took 11 to 13 (now 6 to 12, outputs allocated).
 // So their argument checks, output
-// allocations and the call of the C ABI live here; kernel/cuda/paged.py and logits.py give them
-// their names, keywords and documentation.
+// allocations and the call of the C ABI live here; kernel/cuda/paged.py, rotary.py and logits.py give
+// them their names, keywords and documentation.
 //
 // Every function takes its arguments by position, checks them (AssertionError for shapes, dtypes,
 // layouts and values, RuntimeError for tensors that are not on a CUDA device), runs on the current
