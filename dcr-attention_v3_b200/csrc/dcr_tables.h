@@ -70,6 +70,14 @@ inline bool rows_meet(const void* from, int64_t stride_n, int64_t stride_h, cons
                      TableSpan(to, n, heads, D, heads * D, D, element));
 }
 
+// Whether contiguous output rows [n, heads, D] reach into strided rows [n, from_heads, D] that they are
+// not computed from, as a step's keys and values.
+inline bool rows_reach(const void* from, int64_t stride_n, int64_t stride_h, int64_t from_heads,
+                       const void* to, int64_t n, int64_t heads, int64_t D, int64_t element) {
+  return tables_meet(TableSpan(from, n, from_heads, D, stride_n, stride_h, element),
+                     TableSpan(to, n, heads, D, heads * D, D, element));
+}
+
 // Whether rows [B, V] processed into rows of other strides or another address would be read after
 // they are written. In place, row for row, is fine.
 inline bool logits_meet(const void* from, int64_t from_stride, const void* to, int64_t to_stride,

@@ -203,6 +203,15 @@ void check_apart(PyObject* out, const at::Tensor& o, const Rows& q, const Pool& 
     refuse("out must be q itself (contiguous) or share no memory with it");
 }
 
+// Refuses an output that reaches into the keys or values that are appended beside it.
+void check_apart_kv(PyObject* out, const at::Tensor& o, const Rows& k, const Rows& v, const Pool& p, int64_t tokens,
+                    int64_t heads) {
+  if (out == Py_None) return;
+  for (const Rows* x : {&k, &v})
+    if (dcr::rows_reach(x->data, x->st, x->sh, p.H_kv, o.data_ptr(), tokens, heads, p.D, o.element_size()))
+      refuse("out must share no memory with k or v");
+}
+
 // The caller's workspace (checked) or a fresh one from torch's allocator.
 at::Tensor scratch(PyObject* o, size_t bytes, int device) {
   if (o == Py_None)
@@ -514,6 +523,7 @@ PyObject* rotary_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const c10::cuda::OptionalCUDAGuard guard(p.k->device());
     const at::Tensor o = output(a[17], {T, H, p.D}, p.k->options());
     check_apart(a[17], o, q, p, T, H);
+    check_apart_kv(a[17], o, k, v, p, T, H);
     if (T > 0) {
       const int st = dcr_paged_rotary_append(
           q.data, q.st, q.sh, k.data, k.st, k.sh, v.data, v.st, v.sh, qw, kw,

@@ -565,7 +565,8 @@ int dcr_rotary(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void
                int64_t qo_stride_h, void* k_out, int64_t ko_stride_t, int64_t ko_stride_h,
                void* stream);
 
-/* dcr_paged_append with that rotation in place of the tables' (any position is valid). */
+/* dcr_paged_append with that rotation in place of the tables' (any position is valid). q_out shares no
+ * memory with k or v. */
 int dcr_paged_rotary_append(
     const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
     int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h,
