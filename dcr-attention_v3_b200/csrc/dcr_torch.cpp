@@ -419,6 +419,7 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const c10::cuda::OptionalCUDAGuard guard(p.k->device());
     const at::Tensor o = output(a[16], {T, H, p.D}, p.k->options());
     check_apart(a[16], o, q, p, T, H);
+    check_apart_kv(a[16], o, k, v, p, T, H);
     if (T > 0) {
       const int st = dcr_paged_append(
           q.data, q.st, q.sh, k.data, k.st, k.sh, v.data, v.st, v.sh, qw, kw,

@@ -450,7 +450,8 @@ size_t dcr_paged_workspace_bytes(int B, int H, int H_kv, int D, int max_slots, i
  * h_kv * w_stride_h + slot], max_pages * page_size slots) is increased by every slot's
  * softmax weight, summed over the KV head's query heads in a fixed order. A row with no valid
  * slot gets O = 0 and lse = -inf; a score of -inf counts as a masked slot. O may be q itself
- * where q is contiguous, else it shares no memory with it; so q_out of dcr_paged_append. */
+ * where q is contiguous, else it shares no memory with it; so q_out of dcr_paged_append,
+ * which shares none with k and v either. */
 int dcr_paged_attend(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k_pages,
                      const void* v_pages, int dtype, int64_t k_stride_p, int64_t k_stride_h,
                      int64_t k_stride_s, int64_t v_stride_p, int64_t v_stride_h,
@@ -565,8 +566,7 @@ int dcr_rotary(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void
                int64_t qo_stride_h, void* k_out, int64_t ko_stride_t, int64_t ko_stride_h,
                void* stream);
 
-/* dcr_paged_append with that rotation in place of the tables' (any position is valid). q_out shares no
- * memory with k or v. */
+/* dcr_paged_append with that rotation in place of the tables' (any position is valid). */
 int dcr_paged_rotary_append(
     const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
     int64_t k_stride_h, const void* v, int64_t v_stride_t, int64_t v_stride_h,

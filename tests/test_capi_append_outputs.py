@@ -8,7 +8,7 @@ import sys
 import pytest
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
-from test_capi_paged import B, D, H, H_KV, SHAPE, _names, lib  # noqa: E402,F401
+from test_capi_paged import APPEND, B, D, H, H_KV, SHAPE, _names, lib  # noqa: E402,F401
 from test_capi_paged_edges import P, QKV  # noqa: E402
 from test_capi_prompts import ROTARY_APPEND  # noqa: E402
 
@@ -46,3 +46,8 @@ def _check(lib, func, base, change, refused):  # noqa: F811
 @pytest.mark.parametrize("change,refused", CASES, ids=str)
 def test_rotary_append(lib, change, refused):  # noqa: F811
     _check(lib, "dcr_paged_rotary_append", ROTARY_APPEND, change, refused)
+
+
+@pytest.mark.parametrize("change,refused", CASES, ids=str)
+def test_append(lib, change, refused):  # noqa: F811
+    _check(lib, "dcr_paged_append", APPEND, change, refused)

@@ -41,3 +41,8 @@ def _refused(func):
 def test_rotary_append():
     from dcr_b200.kernel.cuda import paged_rotary_append
     _refused(paged_rotary_append)
+
+
+def test_append():
+    from dcr_b200.kernel.cuda import paged_append
+    _refused(paged_append)
