@@ -147,6 +147,7 @@ const char* dcr_status_string(int status) {
     case DCR_ERR_DEVICE_TIMEOUT: return "device: a bounded wait expired";
     case DCR_ERR_NOALLOC_LIMIT:
       return "shape needs more scratch than dcr_decode_noalloc's 16 MiB array; use dcr_decode";
+    case DCR_ERR_OVERLAP: return "an output reaches into keys or values that are read beside it";
     case DCR_ERR_DEVICE_INDEX: return "device: an index outside [0, N) was skipped";
     case DCR_ERR_DEVICE_SHARD:
       return "device: sharded selection saw inconsistent global histograms (k_eff >= total N?)";

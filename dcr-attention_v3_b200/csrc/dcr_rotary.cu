@@ -520,11 +520,11 @@ int dcr_paged_rotary_append(
       (pos != nullptr && (p_stride_b < 0 || p_stride_h < 0 ||
                           !rows_apart(n_seq, H_kv, max_slots, p_stride_b, p_stride_h))))
     return DCR_ERR_SHAPE;
+  if (rows_meet(q, q_stride_t, q_stride_h, q_out, T, H, D, 16 / per16)) return DCR_ERR_SHAPE;
   // queries written over keys or values that another warp has yet to read would end in the cache
-  if (rows_meet(q, q_stride_t, q_stride_h, q_out, T, H, D, 16 / per16) ||
-      rows_reach(k, k_stride_t, k_stride_h, H_kv, q_out, T, H, D, 16 / per16) ||
+  if (rows_reach(k, k_stride_t, k_stride_h, H_kv, q_out, T, H, D, 16 / per16) ||
       rows_reach(v, v_stride_t, v_stride_h, H_kv, q_out, T, H, D, 16 / per16))
-    return DCR_ERR_SHAPE;
+    return DCR_ERR_OVERLAP;
   RotaryParams p = {};
   p.q = q;
   p.k = k;

@@ -28,6 +28,7 @@ DCR_ERR_WORKSPACE = 6
 DCR_ERR_CUDA = 7
 DCR_ERR_DEVICE_TIMEOUT = 8
 DCR_ERR_NOALLOC_LIMIT = 9
+DCR_ERR_OVERLAP = 10
 DCR_ERR_DEVICE_INDEX = 16
 DCR_ERR_DEVICE_SHARD = 32
 IPC_HANDLE_BYTES = 64

@@ -67,6 +67,7 @@ typedef enum dcr_status {
   DCR_ERR_CUDA = 7,             /* a CUDA runtime call failed                         */
   DCR_ERR_DEVICE_TIMEOUT = 8,   /* device status: a bounded wait expired              */
   DCR_ERR_NOALLOC_LIMIT = 9,    /* shape needs more than DCR_NOALLOC_SCRATCH_BYTES    */
+  DCR_ERR_OVERLAP = 10,         /* queries would be written over the keys or values  */
   DCR_ERR_DEVICE_INDEX = 16,    /* device status: an index outside [0, N) was skipped */
   DCR_ERR_DEVICE_SHARD = 32     /* device status: sharded selection found the global
                                    histograms inconsistent (fewer than k_eff keys over
@@ -451,7 +452,7 @@ size_t dcr_paged_workspace_bytes(int B, int H, int H_kv, int D, int max_slots, i
  * softmax weight, summed over the KV head's query heads in a fixed order. A row with no valid
  * slot gets O = 0 and lse = -inf; a score of -inf counts as a masked slot. O may be q itself
  * where q is contiguous, else it shares no memory with it; so q_out of dcr_paged_append,
- * which shares none with k and v either. */
+ * which shares none with k and v either (DCR_ERR_OVERLAP). */
 int dcr_paged_attend(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k_pages,
                      const void* v_pages, int dtype, int64_t k_stride_p, int64_t k_stride_h,
                      int64_t k_stride_s, int64_t v_stride_p, int64_t v_stride_h,
