@@ -93,21 +93,37 @@ class PagedKVCache:
             self.groups = self.prefix = None
         elif rows:
             groups, prefix = self.shared_groups()
+            if not any(prefix):  # the sequences that share are no neighbours
+                self.groups = self.prefix = None
+                return
             self.groups = torch.tensor(groups, dtype=torch.int32).to(self.device)
             self.prefix = torch.tensor(prefix, dtype=torch.int32).to(self.device)
 
+    def _shares(self, b: int) -> bool:
+        """Whether another sequence holds sequence b's first page."""
+        held = self.host_pages[b]
+        return bool(held) and self._holders[held[0]] > 1
+
     def shared_groups(self):
         """(groups, prefix), as :func:`paged_shared_attention` takes them: neighbouring sequences whose
-        first pages are the same ones, and the slots in them."""
-        groups, prefix, lead = [0], [0] * self.batch, 0
-        for b in range(1, self.batch):
-            first, held = self.host_pages[lead], self.host_pages[b]
+        first pages are the same ones, and the slots in them. A sequence that shares nothing, since it has
+        ended, waits or grew from a prompt of its own, does not part its neighbours: it stays in their
+        group with a prefix of 0. The pages are the group's first sequence's, so those before the first
+        that shares are alone."""
+        groups, prefix, lead = [0], [0] * self.batch, None
+        for b in range(self.batch):
             same = 0
-            while same < min(len(first), len(held)) and first[same] == held[same]:
-                same += 1
+            if self._shares(b):
+                first, held = self.host_pages[b if lead is None else lead], self.host_pages[b]
+                while lead is not None and same < min(len(first), len(held)) and first[same] == held[same]:
+                    same += 1
+                if same == 0:
+                    lead = b
+            elif lead is not None:
+                continue
             if same == 0:
-                groups.append(b)
-                lead = b
+                if b > 0:
+                    groups.append(b)
             else:
                 prefix[b] = same * self.page_size
                 prefix[lead] = max(prefix[lead], prefix[b])

@@ -1,0 +1,100 @@
+"""Groups of sequences that share pages (CPU): they outlive the sequences that end, wait or begin
+among them."""
+from __future__ import annotations
+
+import os
+import sys
+
+import pytest
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+from test_paged_prompts_host import _cache, _check  # noqa: E402
+
+
+def _forked(batch, slots=32, **kw):
+    c = _cache(**{**dict(batch=batch, pages=200, max_slots=64), **kw})
+    c.reserve([slots] + [0] * (batch - 1))
+    c.fork(0, list(range(1, batch)))
+    return c
+
+
+def _same(c, groups, prefix):
+    _check(c, 200)
+    assert c.groups.tolist() == groups and c.prefix.tolist() == prefix
+
+
+def test_sequences_that_end_do_not_part_the_others():
+    c = _forked(5)
+    _same(c, [0, 5], [32] * 5)
+    c.release(1), c.release(3)
+    _same(c, [0, 5], [32, 0, 32, 0, 32])
+    c.release(4)
+    _same(c, [0, 5], [32, 0, 32, 0, 0])
+    c.release(0)  # the last holder shares with nobody
+    _check_none(c)
+
+
+def _check_none(c):
+    assert c.groups is None and c.prefix is None
+
+
+@pytest.mark.parametrize("gone", [(10, 20, 30), (1, 2, 3), (62, 63), (5, 60)])
+def test_a_batch_stays_one_group(gone):
+    c = _forked(64)
+    for b in gone:
+        c.release(b)
+    _same(c, [0, 64], [0 if b in gone else 32 for b in range(64)])
+
+
+def test_a_group_that_lost_its_first():
+    c = _forked(6)
+    c.release(0), c.release(3)
+    _same(c, [0, 1, 6], [0, 32, 32, 0, 32, 32])
+
+
+def test_a_prompt_of_its_own_in_the_place_of_one_that_ended():
+    c = _forked(5)
+    c.release(2)
+    c.reserve([1, 1, 20, 1, 1])
+    _same(c, [0, 5], [32, 32, 0, 32, 32])
+    c.reserve([9, 0, 1, 0, 9])
+    _same(c, [0, 5], [32, 32, 0, 32, 32])
+    c.fork(0, [])
+    _same(c, [0, 5], [32, 32, 0, 32, 32])
+
+
+def test_two_prefixes_side_by_side():
+    c = _cache(batch=7, pages=200, max_slots=64)
+    c.reserve([0, 32, 0, 0, 24, 0, 0])
+    c.fork(1, [2, 3])
+    c.fork(4, [5, 6])
+    _same(c, [0, 1, 4, 7], [0, 32, 32, 32, 24, 24, 24])
+    c.release(2), c.release(5)
+    _same(c, [0, 1, 4, 7], [0, 32, 0, 32, 24, 0, 24])
+    c.release(4)  # the second group's last holder is alone
+    _same(c, [0, 1, 7], [0, 32, 0, 32, 0, 0, 0])
+
+
+def test_holders_that_are_no_neighbours():
+    c = _cache(batch=4, pages=200, max_slots=64)
+    c.reserve([16, 16, 0, 0])
+    c.fork(0, [2])
+    c.fork(1, [3])  # 0 and 2, 1 and 3
+    assert max(c._holders) == 2
+    _check_none(c)
+    c.release(1)
+    _same(c, [0, 4], [16, 0, 16, 0])
+
+
+def test_an_idle_sequence_among_prompts_on_a_prefix(monkeypatch):
+    import torch
+    from dcr_b200.models.llama import paged as module
+    from test_paged_edges_host import _decoder
+    decoder = _decoder(100)
+    cache = decoder.new_cache(4, 200, 64, page_size=8)
+    monkeypatch.setattr(module.PagedLlamaDecoder, "_layers",
+                        lambda self, tokens, cache, attend: torch.zeros(tokens.shape[0], 128))
+    decoder.prefill([[1], [], [2, 3], [4]], cache, prefix=[5] * 17)
+    _same(cache, [0, 4], [16, 0, 16, 16])
+    decoder.prefill([[], [6] * 9, [], []], cache)
+    _same(cache, [0, 4], [16, 0, 16, 16])
