@@ -73,6 +73,7 @@ class PagedKVCache:
         self._grew = [False] * batch                 # the sequences that reserved a token last
         self.host_pages: List[List[int]] = [[] for _ in range(batch)]
         self._holders = [0] * pages                  # sequences that hold each page
+        self._shared = 0                             # pages that several hold
         self._tokens = None  # (seq, slots, positions) of the tokens reserved last
 
     # ------------------------------------------------------------------------------- host side
@@ -89,20 +90,33 @@ class PagedKVCache:
         for b in rows:
             held = self.host_pages[b]
             to_device(self.page_table[b], held + [-1] * (self.max_pages - len(held)))
-        if rows and max(self._holders, default=0) < 2:
+
+    def _regroup(self) -> None:
+        """Publishes the groups that share pages. What sequences share changes when one is forked or
+        released: a page that one grows into is its own, so its prefix stays what it is."""
+        groups, prefix = self.shared_groups()
+        if not any(prefix):  # nobody shares, or no neighbours do
             self.groups = self.prefix = None
-        elif rows:
-            groups, prefix = self.shared_groups()
-            if not any(prefix):  # the sequences that share are no neighbours
-                self.groups = self.prefix = None
-                return
-            self.groups = torch.tensor(groups, dtype=torch.int32).to(self.device)
-            self.prefix = torch.tensor(prefix, dtype=torch.int32).to(self.device)
+            return
+        self.groups = torch.tensor(groups, dtype=torch.int32).to(self.device)
+        self.prefix = torch.tensor(prefix, dtype=torch.int32).to(self.device)
 
     def _shares(self, b: int) -> bool:
         """Whether another sequence holds sequence b's first page."""
         held = self.host_pages[b]
         return bool(held) and self._holders[held[0]] > 1
+
+    def _common(self, a: int, b: int) -> int:
+        """First pages that sequences a and b both hold, by bisection: with one they hold all before it."""
+        x, y = self.host_pages[a], self.host_pages[b]
+        least, most = 0, min(len(x), len(y))
+        while least < most:
+            mid = (least + most + 1) // 2
+            if x[mid - 1] == y[mid - 1]:
+                least = mid
+            else:
+                most = mid - 1
+        return least
 
     def shared_groups(self):
         """(groups, prefix), as :func:`paged_shared_attention` takes them: neighbouring sequences whose
@@ -114,9 +128,7 @@ class PagedKVCache:
         for b in range(self.batch):
             same = 0
             if self._shares(b):
-                first, held = self.host_pages[b if lead is None else lead], self.host_pages[b]
-                while lead is not None and same < min(len(first), len(held)) and first[same] == held[same]:
-                    same += 1
+                same = 0 if lead is None else self._common(lead, b)
                 if same == 0:
                     lead = b
             elif lead is not None:
@@ -141,6 +153,8 @@ class PagedKVCache:
             self._holders[page] -= 1
             if self._holders[page] == 0:
                 self.free_pages.append(page)
+            elif self._holders[page] == 1:
+                self._shared -= 1
         self.host_lengths[b] = length
         return len(held) != before
 
@@ -172,9 +186,12 @@ class PagedKVCache:
 
     def release(self, b: int) -> None:
         """Ends sequence b: its pages go back to the pool."""
+        shared = self._shared
         self._resize(b, 0)
         self.host_seen[b], self._grew[b] = 0, False
         self._publish([b])
+        if shared:
+            self._regroup()
 
     def fork(self, b: int, others: Sequence[int]) -> None:
         """Gives the empty sequences ``others`` what sequence b holds: its full pages are shared, the
@@ -193,6 +210,7 @@ class PagedKVCache:
             self.host_pages[o] = pages[:full]
             for page in pages[:full]:
                 self._holders[page] += 1
+                self._shared += self._holders[page] == 2
             self._resize(o, n)
             self.host_seen[o] = self.host_seen[b]
             self._grew[o] = False
@@ -201,6 +219,7 @@ class PagedKVCache:
             for pool in self.k + self.v:
                 pool[to] = pool[pages[full]].clone()
         self._publish(others)
+        self._regroup()
 
     def over_budget(self) -> bool:
         """Whether some sequence holds ``budget + slack`` slots or more."""

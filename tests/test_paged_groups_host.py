@@ -98,3 +98,55 @@ def test_an_idle_sequence_among_prompts_on_a_prefix(monkeypatch):
     _same(cache, [0, 4], [16, 0, 16, 16])
     decoder.prefill([[], [6] * 9, [], []], cache)
     _same(cache, [0, 4], [16, 0, 16, 16])
+
+
+def _moments(c, steps, monkeypatch):
+    """Grows every sequence, and fails where that looks for shared pages or walks the pool."""
+    class Unwalked(list):
+        def __iter__(self):
+            raise AssertionError("every page of the pool is looked at")
+    c._holders = Unwalked(c._holders)
+    with monkeypatch.context() as m:
+        m.setattr(c, "shared_groups", lambda: pytest.fail("shared pages are looked for"))
+        for _ in range(steps):
+            c.reserve([1] * c.batch)
+    c._holders = list.copy(c._holders)
+
+
+def test_sequences_that_grow_look_for_no_shared_pages(monkeypatch):
+    c = _forked(8)
+    _moments(c, 20, monkeypatch)
+    _same(c, [0, 8], [32] * 8)
+    c.release(3)
+    c.reserve([0, 0, 0, 9, 0, 0, 0, 0])
+    _moments(c, 9, monkeypatch)
+    _same(c, [0, 8], [0 if b == 3 else 32 for b in range(8)])
+
+
+def test_a_cache_that_shares_nothing_looks_for_nothing(monkeypatch):
+    c = _cache(batch=4, pages=200, max_slots=64)
+    _moments(c, 20, monkeypatch)
+    with monkeypatch.context() as m:
+        m.setattr(c, "shared_groups", lambda: pytest.fail("shared pages are looked for"))
+        c.release(1)
+    _check_none(c)
+
+
+def test_prefixes_of_any_length():
+    """Forks of forks that parted at several places."""
+    for slots in (1, 7, 8, 9, 16, 63, 64):
+        c = _forked(4, slots)
+        n = slots // 8 * 8
+        if n == 0:
+            _check_none(c)
+            continue
+        _same(c, [0, 4], [n] * 4)
+    c = _cache(batch=6, pages=200, max_slots=160)
+    c.reserve([8, 0, 0, 0, 0, 0])
+    for b in range(1, 6):  # each goes on behind the one before it
+        c.fork(b - 1, [b])
+        c.reserve([0] * b + [16] + [0] * (5 - b))
+    _same(c, [0, 6], [8] * 6)
+    c.release(0)
+    _same(c, [0, 1, 6], [0, 24, 24, 24, 24, 24])
+    assert c._shared == len({p for p in range(200) if c._holders[p] > 1})
