@@ -15,6 +15,7 @@ positions are also on the device, where the kernels read them.
 """
 from __future__ import annotations
 
+from itertools import accumulate
 from typing import List, Optional, Sequence
 
 import torch
@@ -59,7 +60,9 @@ class PagedKVCache:
         self.seen = torch.zeros(batch, **i32)        # positions so far
         self.queried = torch.zeros(batch, **i32)     # lengths of the sequences that grew last, else 0
         self.starts = torch.zeros(batch + 1, **i32)  # where each one's tokens reserved last begin
-        self.groups = self.prefix = None             # sequences that share pages (fork)
+        self._begins = [0] * (batch + 1)             # starts, as published
+        self.groups = self.prefix = None             # sequences that share pages (fork), of the next two
+        self._groups, self._prefix = torch.zeros(batch + 1, **i32), torch.zeros(batch, **i32)
         self.weights = self.pos = None
         if budget is not None:
             tables = (batch, H_kv, self.max_pages * page_size)
@@ -77,19 +80,20 @@ class PagedKVCache:
         self._tokens = None  # (seq, slots, positions) of the tokens reserved last
 
     # ------------------------------------------------------------------------------- host side
+    def _to_device(self, dst: torch.Tensor, values: Sequence[int]) -> None:
+        """Copies values into dst in the current stream's order, without waiting for it."""
+        src = torch.tensor(values, dtype=torch.int32)
+        pinned = self.device.type == "cuda"
+        dst.copy_(src.pin_memory() if pinned else src, non_blocking=pinned)
+
     def _publish(self, rows: Sequence[int]) -> None:
         """Copies the host's lengths and the page table's given rows to the device."""
-        pinned = self.device.type == "cuda"
-
-        def to_device(dst, values):
-            src = torch.tensor(values, dtype=torch.int32)
-            dst.copy_(src.pin_memory() if pinned else src, non_blocking=pinned)
-        to_device(self.lengths, self.host_lengths)
-        to_device(self.seen, self.host_seen)
-        to_device(self.queried, [n if g else 0 for n, g in zip(self.host_lengths, self._grew)])
+        self._to_device(self.lengths, self.host_lengths)
+        self._to_device(self.seen, self.host_seen)
+        self._to_device(self.queried, [n if g else 0 for n, g in zip(self.host_lengths, self._grew)])
         for b in rows:
             held = self.host_pages[b]
-            to_device(self.page_table[b], held + [-1] * (self.max_pages - len(held)))
+            self._to_device(self.page_table[b], held + [-1] * (self.max_pages - len(held)))
 
     def _regroup(self) -> None:
         """Publishes the groups that share pages. What sequences share changes when one is forked or
@@ -98,8 +102,9 @@ class PagedKVCache:
         if not any(prefix):  # nobody shares, or no neighbours do
             self.groups = self.prefix = None
             return
-        self.groups = torch.tensor(groups, dtype=torch.int32).to(self.device)
-        self.prefix = torch.tensor(prefix, dtype=torch.int32).to(self.device)
+        self._to_device(self._prefix, prefix)
+        self.groups, self.prefix = self._groups[:len(groups)], self._prefix
+        self._to_device(self.groups, groups)
 
     def _shares(self, b: int) -> bool:
         """Whether another sequence holds sequence b's first page."""
@@ -179,8 +184,10 @@ class PagedKVCache:
         self._grew = [n > 0 for n in new_tokens]
         self._publish(changed)
         i32 = dict(dtype=torch.int32)
-        begins = [sum(new_tokens[:b]) for b in range(self.batch + 1)]
-        self.starts = torch.tensor(begins, **i32).to(self.device)
+        begins = [0, *accumulate(new_tokens)]
+        if begins != self._begins:  # the same from one decode step to the next
+            self._to_device(self.starts, begins)
+            self._begins = begins
         self._tokens = tuple(torch.tensor(x, **i32).to(self.device) for x in (seq, slots, positions))
         return len(seq)
 

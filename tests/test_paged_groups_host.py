@@ -150,3 +150,33 @@ def test_prefixes_of_any_length():
     c.release(0)
     _same(c, [0, 1, 6], [0, 24, 24, 24, 24, 24])
     assert c._shared == len({p for p in range(200) if c._holders[p] > 1})
+
+
+def test_what_kernels_read_stays_where_it_is():
+    """Starts, groups and prefixes are written in place, as lengths are, so that a captured call reads the
+    present ones."""
+    c = _forked(5)
+    starts, groups, prefix = c.starts, c.groups, c.prefix
+    for new in ([1] * 5, [1] * 5, [0, 3, 1, 0, 1], [1] * 5, [0] * 5):
+        c.reserve(new)
+        assert c.starts is starts and starts.tolist() == [sum(new[:b]) for b in range(6)]
+    c.release(2)
+    assert c.groups.data_ptr() == groups.data_ptr() and c.prefix is prefix
+    _same(c, [0, 5], [32, 32, 0, 32, 32])
+    for b in (0, 1, 3):
+        c.release(b)
+    _check_none(c)
+    c.fork(4, [0, 1, 2])
+    assert c.groups.data_ptr() == groups.data_ptr() and c.prefix is prefix
+    _same(c, [0, 5], [32, 32, 32, 0, 32])
+
+
+def test_starts_are_copied_when_they_change_only():
+    c = _cache(batch=3, pages=200, max_slots=64)
+    c.reserve([1, 1, 1])
+    starts = c.starts
+    starts.fill_(-7)
+    c.reserve([1, 1, 1])
+    assert c.starts is starts and (starts == -7).all()
+    c.reserve([1, 0, 1])
+    assert starts.tolist() == [0, 1, 1, 2]
