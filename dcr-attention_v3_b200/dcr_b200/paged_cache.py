@@ -75,6 +75,8 @@ class PagedKVCache:
         self.host_seen = [0] * batch
         self._grew = [False] * batch                 # the sequences that reserved a token last
         self.host_pages: List[List[int]] = [[] for _ in range(batch)]
+        self._mapped = [0] * batch                   # pages of each one in the page table
+        self._intact = [0] * batch                   # the first of these that it still holds
         self._holders = [0] * pages                  # sequences that hold each page
         self._shared = 0                             # pages that several hold
         self._tokens = None  # (seq, slots, positions) of the tokens reserved last
@@ -87,13 +89,16 @@ class PagedKVCache:
         dst.copy_(src.pin_memory() if pinned else src, non_blocking=pinned)
 
     def _publish(self, rows: Sequence[int]) -> None:
-        """Copies the host's lengths and the page table's given rows to the device."""
+        """Copies the host's lengths and what changed in the page table's given rows to the device."""
         self._to_device(self.lengths, self.host_lengths)
         self._to_device(self.seen, self.host_seen)
         self._to_device(self.queried, [n if g else 0 for n, g in zip(self.host_lengths, self._grew)])
         for b in rows:
-            held = self.host_pages[b]
-            self._to_device(self.page_table[b], held + [-1] * (self.max_pages - len(held)))
+            held, first = self.host_pages[b], self._intact[b]
+            last = max(len(held), self._mapped[b])
+            if first < last:
+                self._to_device(self.page_table[b, first:last], held[first:] + [-1] * (last - len(held)))
+            self._mapped[b] = self._intact[b] = len(held)
 
     def _regroup(self) -> None:
         """Publishes the groups that share pages. What sequences share changes when one is forked or
@@ -160,6 +165,7 @@ class PagedKVCache:
                 self.free_pages.append(page)
             elif self._holders[page] == 1:
                 self._shared -= 1
+        self._intact[b] = min(self._intact[b], len(held))
         self.host_lengths[b] = length
         return len(held) != before
 

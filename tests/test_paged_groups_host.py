@@ -180,3 +180,38 @@ def test_starts_are_copied_when_they_change_only():
     assert c.starts is starts and (starts == -7).all()
     c.reserve([1, 0, 1])
     assert starts.tolist() == [0, 1, 1, 2]
+
+
+def test_a_step_copies_the_entries_of_its_new_pages():
+    """Whatever comes and goes, the page table follows; what did not change in it is not copied."""
+    import random
+    rng = random.Random(5)
+    c = _cache(batch=5, pages=200, max_slots=320)
+    c.reserve([300, 0, 0, 0, 0])
+    c.fork(0, [3])
+    c.page_table[0, :37].fill_(-9)  # a step's new page is entry 38
+    c.reserve([8, 0, 0, 0, 0])
+    assert (c.page_table[0, :37] == -9).all() and c.page_table[0, 38] == c.host_pages[0][38]
+    c.release(0)
+    for _ in range(60):
+        b, others = rng.randrange(5), [o for o in range(5) if c.host_lengths[o] == 0]
+        if c.host_lengths[b] and rng.random() < 0.4:
+            c.release(b)
+        elif c.host_lengths[b] and rng.random() < 0.5:
+            c.fork(b, others)
+        else:
+            c.reserve([min(rng.randrange(20), 320 - n) if rng.random() < 0.6 else 0 for n in c.host_lengths])
+        if c.groups is not None or max(c._holders) < 2:
+            _check(c, 200)
+        for s in range(5):
+            assert c.page_table[s].tolist() == c.host_pages[s] + [-1] * (40 - len(c.host_pages[s]))
+
+
+def test_evicted_pages_leave_the_table():
+    c = _cache(batch=2, pages=200, max_slots=64, budget=16, sinks=1, recent=2)
+    c.reserve([60, 20])
+    changed = [b for b in range(2) if c._resize(b, 16)]
+    c._resize(0, 30)  # other pages in the places of those that left
+    c._publish(changed)
+    for s in range(2):
+        assert c.page_table[s].tolist() == c.host_pages[s] + [-1] * (8 - len(c.host_pages[s]))
