@@ -105,20 +105,37 @@ __device__ __forceinline__ int2 rows_limits(const RowsParams& p, const RowsUnit&
   return make_int2(p.window > 0 ? max(0, x + 1 - p.window) : 0, p.causal ? x + 1 : u.len);
 }
 
-// Tiles of 128 slots that a segment's rows may see, by its first token: how units are cut up goes by
-// them, not what they see.
-__device__ __forceinline__ int rows_weight(const RowsParams& p, int s, int tok0, int ntok) {
-  if (ntok == 0) return 0;
-  int hi, lo = 0;
-  if (p.prefix != nullptr) {
-    const int len = checked_length(p.c, p.lengths[tok0]);
-    hi = min(len, p.prefix[tok0]);
-    if (p.window > 0) lo = len - p.window;
-  } else {
+// Tiles of 128 slots that a segment's rows may see: how units are cut up goes by them, not what they
+// see. A shared segment's are those from the first slot that any of its tokens sees to the last, since the
+// first token may wait (a length of 0) or share less than the others. Every `step`th token from `first` on
+// is looked at.
+__device__ __forceinline__ int2 rows_span(const RowsParams& p, int s, int tok0, int ntok, int first, int step) {
+  int lo = INT32_MAX, hi = 0;
+  if (p.prefix == nullptr) {
     hi = checked_length(p.c, p.lengths[s]);
-    if (p.window > 0) lo = hi - ntok + 1 - p.window;
+    lo = p.window > 0 ? max(0, hi - ntok + 1 - p.window) : 0;
+  } else {
+    for (int t = tok0 + first; t < tok0 + ntok; t += step) {
+      const int len = checked_length(p.c, p.lengths[t]);
+      const int a = p.window > 0 ? max(0, len - p.window) : 0, b = min(len, p.prefix[t]);
+      if (a >= b) continue;
+      lo = min(lo, a);
+      hi = max(hi, b);
+    }
   }
-  return max(1, (hi - max(lo, 0) + 127) / 128);
+  return make_int2(lo, hi);
+}
+
+__device__ __forceinline__ int rows_tiles_of(int2 span, int ntok) {
+  return ntok == 0 ? 0 : span.x < span.y ? (span.y - span.x + 127) / 128 : 1;
+}
+
+// The weights of shared segments, found once by the whole CTA, a warp a segment.
+constexpr int kRowsWeights = 640;  // segments; of the others every thread looks at all tokens
+
+__device__ __forceinline__ int rows_weight(const RowsParams& p, const int* found, int s, int tok0, int ntok) {
+  if (p.prefix != nullptr && s < kRowsWeights) return found[s];
+  return rows_tiles_of(rows_span(p, s, tok0, ntok, 0, 1), ntok);
 }
 
 constexpr int kRowsMaxParts = 64;
@@ -131,7 +148,19 @@ constexpr int kRowsMinPart = 4;  // tiles of 128 slots: smaller parts gain nothi
 // a number of slots, the least for which all parts are no more than the grid. False: nothing to do.
 template <int BM>
 __device__ __forceinline__ bool rows_begin(const RowsParams& p, RowsUnit& u, int2* limits) {
+  __shared__ int found[kRowsWeights];
   const int lane = threadIdx.x & 31;
+  if (p.prefix != nullptr) {
+    for (int s = threadIdx.x >> 5; s < min(p.nseg, kRowsWeights); s += blockDim.x >> 5) {
+      int tok0, ntok;
+      rows_segment(p, s, tok0, ntok);
+      int2 span = rows_span(p, s, tok0, ntok, lane, 32);
+      span.x = __reduce_min_sync(0xffffffffu, span.x);
+      span.y = __reduce_max_sync(0xffffffffu, span.y);
+      if (lane == 0) found[s] = rows_tiles_of(span, ntok);
+    }
+    __syncthreads();
+  }
   if (threadIdx.x < 32) {
     const int per = (p.nseg + 31) >> 5;
     auto tiles_of = [&](int ntok) { return (ntok * p.G + BM - 1) / BM * p.H_kv; };  // units of a segment
@@ -143,7 +172,7 @@ __device__ __forceinline__ bool rows_begin(const RowsParams& p, RowsUnit& u, int
         int tok0, ntok;
         if (s >= p.nseg) break;
         rows_segment(p, s, tok0, ntok);
-        most = max(most, rows_weight(p, s, tok0, ntok));
+        most = max(most, rows_weight(p, found, s, tok0, ntok));
       }
       most = __reduce_max_sync(0xffffffffu, most);
       int least = min(most, max(kRowsMinPart, (most + kRowsMaxParts - 1) / kRowsMaxParts));
@@ -155,7 +184,7 @@ __device__ __forceinline__ bool rows_begin(const RowsParams& p, RowsUnit& u, int
           int tok0, ntok;
           if (s >= p.nseg) break;
           rows_segment(p, s, tok0, ntok);
-          n += tiles_of(ntok) * ((rows_weight(p, s, tok0, ntok) + mid - 1) / mid);
+          n += tiles_of(ntok) * ((rows_weight(p, found, s, tok0, ntok) + mid - 1) / mid);
         }
         n = __reduce_add_sync(0xffffffffu, n);
         if (n > p.pieces) least = mid + 1;
@@ -190,7 +219,7 @@ __device__ __forceinline__ bool rows_begin(const RowsParams& p, RowsUnit& u, int
         tok0[j] = ntok[j] = weight[j] = 0;
         if (s < p.nseg) {
           rows_segment(p, s, tok0[j], ntok[j]);
-          weight[j] = rows_weight(p, s, tok0[j], ntok[j]);
+          weight[j] = rows_weight(p, found, s, tok0[j], ntok[j]);
         }
         n[j] = tiles_of(ntok[j]);
       }
@@ -219,7 +248,7 @@ __device__ __forceinline__ bool rows_begin(const RowsParams& p, RowsUnit& u, int
       sorted(std::integral_constant<int, 2>());
     } else {
       auto parts_of = [&](int s, int tok0, int ntok) {
-        return p.pieces > 0 ? (rows_weight(p, s, tok0, ntok) + chunk - 1) / chunk : 1;
+        return p.pieces > 0 ? (rows_weight(p, found, s, tok0, ntok) + chunk - 1) / chunk : 1;
       };
       int mine = 0;
       for (int j = 0; j < per; ++j) {
