@@ -79,7 +79,7 @@ struct RowsUnit {
   int seg, tok0, ntok, len;  // the segment, its tokens; prefill: its sequence's length
   int hk, split, parts;      // this CTA's part of the slots
   int row0, rows;            // first row in the segment and their number (0: nothing to do)
-  int lo_min, lo_max, hi_min, hi_max;  // over the rows
+  int lo_min, lo_max, hi_min, hi_max;  // over the rows that see a slot
 };
 
 // The tokens of segment s; an inverted or outlying pair of starts raises the status.
@@ -285,10 +285,12 @@ __device__ __forceinline__ bool rows_begin(const RowsParams& p, RowsUnit& u, int
     const bool in = r < u.rows;
     const int2 x = in ? rows_limits(p, u, r) : make_int2(0, 0);
     limits[r] = x;
-    const bool sees = in && x.x < x.y;  // else it widens nothing, but no tile is seen whole
+    // A row that sees nothing (a sequence that waits) does not count: a tile that all others see is whole
+    // for them. Its own scores are hidden wherever it stands, and its sum of 0 makes its output 0.
+    const bool sees = in && x.x < x.y;
     const int a = __reduce_min_sync(0xffffffffu, sees ? x.x : INT32_MAX);
-    const int b = __reduce_max_sync(0xffffffffu, in ? x.x : 0);
-    const int c = __reduce_min_sync(0xffffffffu, in ? x.y : INT32_MAX);
+    const int b = __reduce_max_sync(0xffffffffu, sees ? x.x : 0);
+    const int c = __reduce_min_sync(0xffffffffu, sees ? x.y : INT32_MAX);
     const int d = __reduce_max_sync(0xffffffffu, sees ? x.y : 0);
     if (lane == 0) {
       atomicMin(&u.lo_min, a);
@@ -408,7 +410,7 @@ __global__ void __launch_bounds__(kRfThreads) rows_fma_kernel(const RowsParams p
 #pragma unroll 1
   for (int t = tiles.x; t < tiles.y; ++t) {
     const int j0 = t * kRfSlots;
-    const bool seen = j0 >= u.lo_max && j0 + kRfSlots <= u.hi_min;  // whole, by every row
+    const bool seen = j0 >= u.lo_max && j0 + kRfSlots <= u.hi_min;  // whole, by every row that sees any
     __syncthreads();
     if (threadIdx.x < kRfSlots)
       flag[threadIdx.x] = rows_slot(p, u, j0 + threadIdx.x, koff[threadIdx.x], voff[threadIdx.x]);
@@ -468,8 +470,8 @@ __global__ void __launch_bounds__(kRfThreads) rows_fma_kernel(const RowsParams p
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       unsigned in = held;
-      if (!seen) {
-        const int2 lim = limits[8 * ty + i];
+      const int2 lim = limits[8 * ty + i];
+      if (!seen || (lim.x >= lim.y && 8 * ty + i < u.rows)) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (j0 + slot(e) < lim.x || j0 + slot(e) >= lim.y) in &= ~(1u << e);
@@ -539,11 +541,12 @@ __global__ void __launch_bounds__(kRfThreads) rows_fma_kernel(const RowsParams p
     const int64_t at = parts ? rows_place<kRfRows>(p, u, r, row) : row;
     if (!parts && p.part_of != nullptr) p.part_of[row] = make_int2(0, 0);
     const float spoil = (poison >> i) & 1u ? __int_as_float(0x7fffffff) : 1.0f;
-    const float by = l[i] == 0.0f ? 0.0f : parts ? spoil : spoil / l[i];
+    const bool none = l[i] == 0.0f;  // its o may be 0 times a value that is not finite
+    const float by = none ? 0.0f : parts ? spoil : spoil / l[i];
     float* dst = (parts ? p.part_o : static_cast<float*>(p.o)) + at * D + 4 * tx;
 #pragma unroll
     for (int x = 0; x < E; ++x) {
-      const float2 c = o[i][2 * x], d = o[i][2 * x + 1];
+      const float2 c = none ? make_float2(0.0f, 0.0f) : o[i][2 * x], d = none ? c : o[i][2 * x + 1];
       *reinterpret_cast<float4*>(dst + 32 * x) = make_float4(c.x * by, c.y * by, d.x * by, d.y * by);
     }
     if (tx != 0) continue;
@@ -695,7 +698,7 @@ __device__ __forceinline__ void rows_tc_load(const RowsParams& p, const RowsMaps
 #pragma unroll 1
   for (int t = 0; t < n; ++t) {
     const int j0 = (tiles.x + t) * kTcSlots;
-    const bool seen = j0 >= u.lo_max && j0 + kTcSlots <= u.hi_min;  // whole, by every row
+    const bool seen = j0 >= u.lo_max && j0 + kTcSlots <= u.hi_min;  // whole, by every row that sees any
     int page[2], in[2];
     unsigned held[2];
 #pragma unroll
@@ -865,6 +868,8 @@ __device__ __forceinline__ bool rows_tc_softmax(const RowsParams& p, RowsTcShare
   const uint32_t s_at = sh.tmem + lane0 + x * 128, o_at = sh.tmem + lane0 + 256 + x * D;
   const int2 lim = sh.limits[r];
   const bool idle = (r & ~31) >= u.rows;  // no row of this warp is one
+  // a row that sees nothing, of tiles that are whole for the others either
+  const bool blind = __any_sync(0xffffffffu, r < u.rows && lim.x >= lim.y);
   float& m = state.x;
   float& l = state.y;
   bool fine = true;
@@ -895,7 +900,7 @@ __device__ __forceinline__ bool rows_tc_softmax(const RowsParams& p, RowsTcShare
         whole = whole && words[w] == 0xffffffffu;
       }
       tc_load_wait(s);
-      if (!whole) {
+      if (!whole || blind) {
 #pragma unroll
         for (int w = 0; w < 2; ++w) words[w] &= rows_bits(lim.x - j0 - 32 * w, lim.y - j0 - 32 * w);
         rows_hide(s, words);

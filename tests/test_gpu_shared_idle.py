@@ -52,6 +52,21 @@ def test_a_group_whose_first_sequence_sees_little_is_cut_up(dt, change):
     assert less <= 3 * whole and _status() == 0
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("idle", [0, 7])
+def test_a_sequence_that_waits_leaves_whole_tiles_whole(dt, idle):
+    """With its row among the limits no tile of the prefix came by tensor-map copies, and each was masked and
+    searched for values that are not finite: twice the time. 1.4 is halfway on a logarithm."""
+    from dcr_b200.kernel.cuda import paged_shared_attention
+    k, v, table, n, prefix, groups = _make_shared([16], [32768], [64] * 16, 8, 32, 128, DT[dt], 1)
+    q = torch.randn(16, 64, 128, generator=_gen(2), device=DEV).to(DT[dt])
+
+    def time_of(n):
+        args = (q, k, v, table, _i32(n), _i32(groups), _i32(prefix))
+        return _time(lambda: paged_shared_attention(*args))
+    assert time_of([0 if b == idle else x for b, x in enumerate(n)]) <= 1.4 * time_of(n) and _status() == 0
+
+
 def _check_idle(members, prefixes, owns, idle, H, H_kv, page, D, dt, *, window=0, seed=0, spoil=None):
     """Some sequences wait; a value or key in the prefix that is not finite spoils none of them."""
     from dcr_b200.kernel.cuda import paged_shared_attention
