@@ -95,8 +95,8 @@ class PagedLlamaDecoder(torch.nn.Module):
         [batch, vocab] after each one's last token (zeros for idle sequences). A ``prefix`` precedes
         every prompt of an empty cache: it is computed once, and its full pages are held once. In a
         cache with a budget, attention weights begin to accumulate with the decode steps; a sequence
-        over the budget, which is evicted before its next step attends, begins with those of its
-        last token."""
+        over the budget, which may be evicted before its next step attends, begins with those of its
+        last token (of its prompt's last chunk, where no eviction comes between the chunks)."""
         require(len(prompts) == cache.batch, f"{cache.batch} prompts expected")
         lengths = [len(p) for p in prompts]
         require(sum(lengths) > 0, "at least one prompt must hold a token")
@@ -122,8 +122,13 @@ class PagedLlamaDecoder(torch.nn.Module):
         flat = torch.tensor([t for p in prompts for t in p], dtype=torch.int64).to(self.model.device)
         begins = [sum(lengths[:b]) for b in range(len(lengths))]
         over = last_rows = None
+        provisional = []
         held = [h if n else 0 for h, n in zip(cache.host_lengths, lengths)]
+        if cache.budget is not None:
+            cache.withdraw([b for b, n in enumerate(lengths) if n])  # more of their prompts follows
         if cache.budget is not None and max(held) > cache.budget:
+            if not cache.over_budget():  # else they are evicted next, with these weights
+                provisional = [b for b, h in enumerate(held) if h > cache.budget]
             over = torch.tensor([h if h > cache.budget else 0 for h in held],
                                 dtype=torch.int32).to(self.model.device)
             last_rows = torch.tensor([begins[b] + n - 1 if n else 0
@@ -131,7 +136,7 @@ class PagedLlamaDecoder(torch.nn.Module):
 
         def attend(i, q):
             if over is not None:
-                cache.weigh(i, q[last_rows], over)
+                cache.weigh(i, q[last_rows], over, provisional=provisional)
             return cache.prefill_attend(i, q)
 
         x = self._layers(flat, cache, attend)

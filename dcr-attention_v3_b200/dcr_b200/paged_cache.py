@@ -69,6 +69,7 @@ class PagedKVCache:
             f32 = dict(dtype=torch.float32, device=self.device)
             self.weights = [torch.zeros(tables, **f32) for _ in range(layers)]
             self.pos = [torch.zeros(tables, **i32) for _ in range(layers)]
+            self._provisional = {}  # sequence: its layers' weights before a prompt's last token counted
             self._spare_weights, self._spare_pos = torch.zeros(tables, **f32), torch.zeros(tables, **i32)
         self.free_pages = list(range(pages - 1, -1, -1))
         self.host_lengths = [0] * batch
@@ -201,6 +202,8 @@ class PagedKVCache:
         """Ends sequence b: its pages go back to the pool."""
         shared = self._shared
         self._resize(b, 0)
+        if self.budget is not None:
+            self._provisional.pop(b, None)
         self.host_seen[b], self._grew[b] = 0, False
         self._publish([b])
         if shared:
@@ -279,16 +282,31 @@ class PagedKVCache:
         if self.groups is not None:
             return paged_shared_attention(q, self.k[layer], self.v[layer], self.page_table, self.queried,
                                           self.groups, self.prefix, window=window)
+        if self.budget is not None and self._provisional:
+            for b in [b for b in self._provisional if self._grew[b]]:
+                del self._provisional[b]  # its prompt is over
         return paged_attention(q, self.k[layer], self.v[layer], self.page_table, self.queried,
                                window=window,
                                weights=None if self.weights is None else self.weights[layer])
 
-    def weigh(self, layer: int, q: torch.Tensor, lengths: torch.Tensor) -> None:
+    def weigh(self, layer: int, q: torch.Tensor, lengths: torch.Tensor, *,
+              provisional: Sequence[int] = ()) -> None:
         """Accumulates the attention weights of one query row per sequence over its first
-        ``lengths[b]`` slots (int32 on the device; 0: none) in the layer's table, and nothing else."""
+        ``lengths[b]`` slots (int32 on the device; 0: none) in the layer's table, and nothing else. Those
+        of ``provisional`` sequences can be taken back until they attend or an eviction goes by them
+        (:meth:`withdraw`)."""
         require(self.budget is not None, "this cache has no budget")
+        for b in provisional:
+            self._provisional.setdefault(b, {})[layer] = self.weights[layer][b].clone()
         paged_attention(q, self.k[layer], self.v[layer], self.page_table, lengths,
                         weights=self.weights[layer])
+
+    def withdraw(self, sequences: Sequence[int]) -> None:
+        """Takes back the provisional weights of these sequences, where they have any."""
+        require(self.budget is not None, "this cache has no budget")
+        for b in sequences:
+            for layer, before in self._provisional.pop(b, {}).items():
+                self.weights[layer][b].copy_(before)
 
     def gather(self, layer: int, b: int):
         """(K, V) ``[H_kv, length, D]`` of sequence b, copied out of its pages."""
@@ -306,6 +324,7 @@ class PagedKVCache:
                         weights_out=self._spare_weights, pos_out=self._spare_pos)
             self.weights[i], self._spare_weights = self._spare_weights, self.weights[i]
             self.pos[i], self._spare_pos = self._spare_pos, self.pos[i]
+        self._provisional.clear()
         if max(self.host_lengths) > self.budget:
             self._tokens = None
         changed = [b for b, n in enumerate(self.host_lengths)
