@@ -80,6 +80,7 @@ struct RowsUnit {
   int hk, split, parts;      // this CTA's part of the slots
   int row0, rows;            // first row in the segment and their number (0: nothing to do)
   int lo_min, lo_max, hi_min, hi_max;  // over the rows that see a slot
+  int blind;                 // some row sees none
 };
 
 // The tokens of segment s; an inverted or outlying pair of starts raises the status.
@@ -106,36 +107,36 @@ __device__ __forceinline__ int2 rows_limits(const RowsParams& p, const RowsUnit&
 }
 
 // Tiles of 128 slots that a segment's rows may see: how units are cut up goes by them, not what they
-// see. A shared segment's are those from the first slot that any of its tokens sees to the last, since the
-// first token may wait (a length of 0) or share less than the others. Every `step`th token from `first` on
-// is looked at.
-__device__ __forceinline__ int2 rows_span(const RowsParams& p, int s, int tok0, int ntok, int first, int step) {
-  int lo = INT32_MAX, hi = 0;
-  if (p.prefix == nullptr) {
-    hi = checked_length(p.c, p.lengths[s]);
-    lo = p.window > 0 ? max(0, hi - ntok + 1 - p.window) : 0;
-  } else {
-    for (int t = tok0 + first; t < tok0 + ntok; t += step) {
-      const int len = checked_length(p.c, p.lengths[t]);
-      const int a = p.window > 0 ? max(0, len - p.window) : 0, b = min(len, p.prefix[t]);
-      if (a >= b) continue;
-      lo = min(lo, a);
-      hi = max(hi, b);
-    }
-  }
-  return make_int2(lo, hi);
-}
-
-__device__ __forceinline__ int rows_tiles_of(int2 span, int ntok) {
-  return ntok == 0 ? 0 : span.x < span.y ? (span.y - span.x + 127) / 128 : 1;
-}
-
-// The weights of shared segments, found once by the whole CTA, a warp a segment.
-constexpr int kRowsWeights = 640;  // segments; of the others every thread looks at all tokens
+// see. A shared segment's are found by the whole CTA beforehand, those from the first slot that any of its
+// tokens sees to the last, since its first token may wait (a length of 0) or share less than the others.
+constexpr int kRowsWeights = 640;  // shared segments; those past them (no call with so many is cut up) count 1
 
 __device__ __forceinline__ int rows_weight(const RowsParams& p, const int* found, int s, int tok0, int ntok) {
-  if (p.prefix != nullptr && s < kRowsWeights) return found[s];
-  return rows_tiles_of(rows_span(p, s, tok0, ntok, 0, 1), ntok);
+  if (ntok == 0) return 0;
+  if (p.prefix != nullptr) return s < kRowsWeights ? found[s] : 1;
+  const int hi = checked_length(p.c, p.lengths[s]);
+  const int lo = p.window > 0 ? hi - ntok + 1 - p.window : 0;
+  return max(1, (hi - max(lo, 0) + 127) / 128);
+}
+
+// The weights of shared segments, a warp a segment.
+__device__ __forceinline__ void rows_find_weights(const RowsParams& p, int* found) {
+  const int lane = threadIdx.x & 31, cap = p.c.max_pages * static_cast<int>(p.c.page.d);
+#pragma unroll 1
+  for (int s = threadIdx.x >> 5; s < min(p.nseg, kRowsWeights); s += blockDim.x >> 5) {
+    int tok0, ntok, lo = INT32_MAX, hi = 0;
+    rows_segment(p, s, tok0, ntok);
+#pragma unroll 4
+    for (int t = tok0 + lane; t < tok0 + ntok; t += 32) {
+      const int len = min(p.lengths[t], cap), b = min(len, p.prefix[t]);
+      const int a = p.window > 0 ? max(0, len - p.window) : 0;
+      lo = min(lo, a < b ? a : INT32_MAX);
+      hi = max(hi, a < b ? b : 0);
+    }
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    if (lane == 0) found[s] = lo < hi ? (hi - lo + 127) / 128 : 1;
+  }
 }
 
 constexpr int kRowsMaxParts = 64;
@@ -151,14 +152,7 @@ __device__ __forceinline__ bool rows_begin(const RowsParams& p, RowsUnit& u, int
   __shared__ int found[kRowsWeights];
   const int lane = threadIdx.x & 31;
   if (p.prefix != nullptr) {
-    for (int s = threadIdx.x >> 5; s < min(p.nseg, kRowsWeights); s += blockDim.x >> 5) {
-      int tok0, ntok;
-      rows_segment(p, s, tok0, ntok);
-      int2 span = rows_span(p, s, tok0, ntok, lane, 32);
-      span.x = __reduce_min_sync(0xffffffffu, span.x);
-      span.y = __reduce_max_sync(0xffffffffu, span.y);
-      if (lane == 0) found[s] = rows_tiles_of(span, ntok);
-    }
+    rows_find_weights(p, found);
     __syncthreads();
   }
   if (threadIdx.x < 32) {
@@ -206,7 +200,7 @@ __device__ __forceinline__ bool rows_begin(const RowsParams& p, RowsUnit& u, int
       u.row0 = tile * BM;
       u.rows = min(BM, ntok * p.G - u.row0);
       u.lo_min = u.hi_min = INT32_MAX;
-      u.lo_max = u.hi_max = 0;
+      u.lo_max = u.hi_max = u.blind = 0;
     };
     const int want = blockIdx.x;
     // with K segments a lane: this lane's, if it has the unit
@@ -286,12 +280,13 @@ __device__ __forceinline__ bool rows_begin(const RowsParams& p, RowsUnit& u, int
     const int2 x = in ? rows_limits(p, u, r) : make_int2(0, 0);
     limits[r] = x;
     // A row that sees nothing (a sequence that waits) does not count: a tile that all others see is whole
-    // for them. Its own scores are hidden wherever it stands, and its sum of 0 makes its output 0.
+    // for them. What is computed in its place is dropped in the end.
     const bool sees = in && x.x < x.y;
     const int a = __reduce_min_sync(0xffffffffu, sees ? x.x : INT32_MAX);
     const int b = __reduce_max_sync(0xffffffffu, sees ? x.x : 0);
     const int c = __reduce_min_sync(0xffffffffu, sees ? x.y : INT32_MAX);
     const int d = __reduce_max_sync(0xffffffffu, sees ? x.y : 0);
+    if (in && !sees) u.blind = 1;
     if (lane == 0) {
       atomicMin(&u.lo_min, a);
       atomicMax(&u.lo_max, b);
@@ -470,8 +465,8 @@ __global__ void __launch_bounds__(kRfThreads) rows_fma_kernel(const RowsParams p
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       unsigned in = held;
-      const int2 lim = limits[8 * ty + i];
-      if (!seen || (lim.x >= lim.y && 8 * ty + i < u.rows)) {
+      if (!seen) {
+        const int2 lim = limits[8 * ty + i];
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (j0 + slot(e) < lim.x || j0 + slot(e) >= lim.y) in &= ~(1u << e);
@@ -535,13 +530,17 @@ __global__ void __launch_bounds__(kRfThreads) rows_fma_kernel(const RowsParams p
     for (int x = 4; x >= 1; x >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
     const int r = 8 * ty + i;
     if (r >= u.rows) continue;
+    if (limits[r].x >= limits[r].y) {  // it sees nothing
+      m[i] = -INFINITY;
+      l[i] = 0.0f;
+    }
     const int t = static_cast<int>(p.of_G.div(u.row0 + r)), g = u.row0 + r - t * p.G;
     const int64_t row = static_cast<int64_t>(u.tok0 + t) * p.H + u.hk * p.G + g;
     const bool parts = rows_in_parts(p, u);
     const int64_t at = parts ? rows_place<kRfRows>(p, u, r, row) : row;
     if (!parts && p.part_of != nullptr) p.part_of[row] = make_int2(0, 0);
     const float spoil = (poison >> i) & 1u ? __int_as_float(0x7fffffff) : 1.0f;
-    const bool none = l[i] == 0.0f;  // its o may be 0 times a value that is not finite
+    const bool none = l[i] == 0.0f;  // what is in its o may be anything
     const float by = none ? 0.0f : parts ? spoil : spoil / l[i];
     float* dst = (parts ? p.part_o : static_cast<float*>(p.o)) + at * D + 4 * tx;
 #pragma unroll
@@ -868,8 +867,6 @@ __device__ __forceinline__ bool rows_tc_softmax(const RowsParams& p, RowsTcShare
   const uint32_t s_at = sh.tmem + lane0 + x * 128, o_at = sh.tmem + lane0 + 256 + x * D;
   const int2 lim = sh.limits[r];
   const bool idle = (r & ~31) >= u.rows;  // no row of this warp is one
-  // a row that sees nothing, of tiles that are whole for the others either
-  const bool blind = __any_sync(0xffffffffu, r < u.rows && lim.x >= lim.y);
   float& m = state.x;
   float& l = state.y;
   bool fine = true;
@@ -900,7 +897,7 @@ __device__ __forceinline__ bool rows_tc_softmax(const RowsParams& p, RowsTcShare
         whole = whole && words[w] == 0xffffffffu;
       }
       tc_load_wait(s);
-      if (!whole || blind) {
+      if (!whole) {
 #pragma unroll
         for (int w = 0; w < 2; ++w) words[w] &= rows_bits(lim.x - j0 - 32 * w, lim.y - j0 - 32 * w);
         rows_hide(s, words);
@@ -1121,10 +1118,15 @@ __global__ void __launch_bounds__(RowsTc<D, Twin>::kThreads, 1) rows_tc_kernel(c
           const uint32_t keep = p.scale2 < 0.0f ? 0xffffffffu : 0u, flip = keep & 0x80008000u;
           *at = make_uint4((at->x & keep) ^ flip, (at->y & keep) ^ flip, (at->z & keep) ^ flip, (at->w & keep) ^ flip);
         }
+      if (u.blind != 0)  // zeros for rows that see nothing, so that they raise no base of their warp's
+        for (int i = 0; i < kQSteps; ++i)
+          if (sh.limits[q_row(i)].x >= sh.limits[q_row(i)].y) *q_place(i) = make_uint4(0u, 0u, 0u, 0u);
       fence_proxy_async_smem();
       mbar_arrive(&sh.q_full);
       float2 state = make_float2(-INFINITY, 0.0f);
       const bool fine = rows_tc_softmax<T, D, Twin, Parts>(p, sh, tiles, scale2, state);
+      const int2 lim = sh.limits[tid % 128 + (Twin ? 0 : tid / 128 * 128)];
+      if (lim.x >= lim.y) state = make_float2(-INFINITY, 0.0f);  // it sees nothing
       rows_tc_write<T, D, Twin>(p, sh, reinterpret_cast<float*>(ring), state, fine);
     }
   } else if (tid < S::kMma) {
