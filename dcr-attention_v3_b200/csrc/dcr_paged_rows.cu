@@ -80,7 +80,6 @@ struct RowsUnit {
   int hk, split, parts;      // this CTA's part of the slots
   int row0, rows;            // first row in the segment and their number (0: nothing to do)
   int lo_min, lo_max, hi_min, hi_max;  // over the rows that see a slot
-  int blind;                 // some row sees none
 };
 
 // The tokens of segment s; an inverted or outlying pair of starts raises the status.
@@ -200,7 +199,7 @@ __device__ __forceinline__ bool rows_begin(const RowsParams& p, RowsUnit& u, int
       u.row0 = tile * BM;
       u.rows = min(BM, ntok * p.G - u.row0);
       u.lo_min = u.hi_min = INT32_MAX;
-      u.lo_max = u.hi_max = u.blind = 0;
+      u.lo_max = u.hi_max = 0;
     };
     const int want = blockIdx.x;
     // with K segments a lane: this lane's, if it has the unit
@@ -286,7 +285,6 @@ __device__ __forceinline__ bool rows_begin(const RowsParams& p, RowsUnit& u, int
     const int b = __reduce_max_sync(0xffffffffu, sees ? x.x : 0);
     const int c = __reduce_min_sync(0xffffffffu, sees ? x.y : INT32_MAX);
     const int d = __reduce_max_sync(0xffffffffu, sees ? x.y : 0);
-    if (in && !sees) u.blind = 1;
     if (lane == 0) {
       atomicMin(&u.lo_min, a);
       atomicMax(&u.lo_max, b);
@@ -1118,15 +1116,14 @@ __global__ void __launch_bounds__(RowsTc<D, Twin>::kThreads, 1) rows_tc_kernel(c
           const uint32_t keep = p.scale2 < 0.0f ? 0xffffffffu : 0u, flip = keep & 0x80008000u;
           *at = make_uint4((at->x & keep) ^ flip, (at->y & keep) ^ flip, (at->z & keep) ^ flip, (at->w & keep) ^ flip);
         }
-      if (u.blind != 0)  // zeros for rows that see nothing, so that they raise no base of their warp's
-        for (int i = 0; i < kQSteps; ++i)
-          if (sh.limits[q_row(i)].x >= sh.limits[q_row(i)].y) *q_place(i) = make_uint4(0u, 0u, 0u, 0u);
       fence_proxy_async_smem();
       mbar_arrive(&sh.q_full);
-      float2 state = make_float2(-INFINITY, 0.0f);
-      const bool fine = rows_tc_softmax<T, D, Twin, Parts>(p, sh, tiles, scale2, state);
+      // a row that sees nothing begins at a base that no score is above, so that it raises none of its warp's
       const int2 lim = sh.limits[tid % 128 + (Twin ? 0 : tid / 128 * 128)];
-      if (lim.x >= lim.y) state = make_float2(-INFINITY, 0.0f);  // it sees nothing
+      const bool blind = lim.x >= lim.y;
+      float2 state = make_float2(blind ? INFINITY : -INFINITY, 0.0f);
+      const bool fine = rows_tc_softmax<T, D, Twin, Parts>(p, sh, tiles, scale2, state);
+      if (blind) state = make_float2(-INFINITY, 0.0f);
       rows_tc_write<T, D, Twin>(p, sh, reinterpret_cast<float*>(ring), state, fine);
     }
   } else if (tid < S::kMma) {
