@@ -63,6 +63,8 @@ class PagedKVCache:
         self._begins = [0] * (batch + 1)             # starts, as published
         self.groups = self.prefix = None             # sequences that share pages (fork), of the next two
         self._groups, self._prefix = torch.zeros(batch + 1, **i32), torch.zeros(batch, **i32)
+        self._spans = torch.zeros(batch + 1, **i32)  # groups without those that share nothing
+        self._host_spans: List[int] = []
         self.weights = self.pos = None
         if budget is not None:
             tables = (batch, H_kv, self.max_pages * page_size)
@@ -111,6 +113,10 @@ class PagedKVCache:
         self._to_device(self._prefix, prefix)
         self.groups, self.prefix = self._groups[:len(groups)], self._prefix
         self._to_device(self.groups, groups)
+        # What attend passes: a group that shares nothing joins the one before it, or those before the first
+        # that shares are one, since a call of many groups does not cut their prefixes up.
+        self._host_spans = [0, *(b for b in groups[1:-1] if prefix[b]), self.batch]
+        self._to_device(self._spans[:len(self._host_spans)], self._host_spans)
 
     def _shares(self, b: int) -> bool:
         """Whether another sequence holds sequence b's first page."""
@@ -281,7 +287,7 @@ class PagedKVCache:
         gets zeros and accumulates nothing. Pages that neighbouring sequences share are read once."""
         if self.groups is not None:
             return paged_shared_attention(q, self.k[layer], self.v[layer], self.page_table, self.queried,
-                                          self.groups, self.prefix, window=window)
+                                          self._spans[:len(self._host_spans)], self.prefix, window=window)
         if self.budget is not None and self._provisional:
             for b in [b for b in self._provisional if self._grew[b]]:
                 del self._provisional[b]  # its prompt is over

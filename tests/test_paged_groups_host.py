@@ -215,3 +215,35 @@ def test_evicted_pages_leave_the_table():
     c._publish(changed)
     for s in range(2):
         assert c.page_table[s].tolist() == c.host_pages[s] + [-1] * (8 - len(c.host_pages[s]))
+
+
+@pytest.mark.parametrize("gone,spans", [((0,), [0, 1, 64]), (tuple(range(40)), [0, 40, 64]), ((63,), [0, 64]),
+                                        ((), [0, 64])])
+def test_sequences_before_the_first_that_shares_are_one_span(gone, spans, monkeypatch):
+    """A batch whose first sequences ended is two groups in a call, not one for each of them."""
+    import torch
+    from dcr_b200 import paged_cache
+    got = []
+    monkeypatch.setattr(paged_cache, "paged_shared_attention", lambda *a, **kw: got.append(a))
+    c = _forked(64)
+    for b in gone:
+        c.release(b)
+    c.attend(0, torch.zeros(64, 2, 64))
+    groups, prefix = got[0][5], got[0][6]
+    assert groups.tolist() == spans and prefix.tolist() == [0 if b in gone else 32 for b in range(64)]
+
+
+def test_spans_of_several_prefixes(monkeypatch):
+    import torch
+    from dcr_b200 import paged_cache
+    got = []
+    monkeypatch.setattr(paged_cache, "paged_shared_attention", lambda *a, **kw: got.append(a[5].tolist()))
+    c = _cache(batch=9, pages=200, max_slots=64)
+    c.reserve([9, 0, 32, 0, 16, 0, 0, 24, 0])
+    c.fork(2, [3])
+    c.fork(4, [6])  # 5 waits
+    c.fork(7, [8])
+    c.attend(0, torch.zeros(9, 2, 64))
+    c.release(4)  # 6 shares with nobody
+    c.attend(0, torch.zeros(9, 2, 64))
+    assert got == [[0, 2, 4, 7, 9], [0, 2, 7, 9]]
