@@ -6,7 +6,7 @@ them back when a sequence ends or its slots are evicted, and keeps one page tabl
 (a page number means the same page of every layer's pool). With a ``budget`` it also keeps, per
 layer, the accumulated attention weight and the position of every slot, and evicts what is over
 the budget (``paged_evict``). Without one, sequences may share the pages of a common prefix
-(:meth:`PagedKVCache.fork`), which attention then reads once for them
+(:meth:`PagedKVCache.fork`), which attention then reads once for them where that pays
 (``paged_shared_attention``). The reference concatenates one contiguous cache per layer
 (dcr_attention/models/llama/compat.py:208-254) and has no counterpart.
 
@@ -24,6 +24,15 @@ from dcr_b200.kernel.cuda._common import HEAD_DIM, check_dtype, require
 from dcr_b200.kernel.cuda.paged import (PAGED_HEAD_DIMS, paged_append, paged_attention,
                                         paged_evict, paged_prefill, paged_rotary_append,
                                         paged_shared_attention)
+
+
+# Bytes of keys and values that the shared call has to save a layer for :meth:`PagedKVCache.attend` to take
+# it instead of the plain one, by the bytes of an element. It has a fixed cost of its own (the prefix's
+# kernel, parts and a join beside the own slots' kernels). Measured on cold pools, plain -> shared: in 16 bits
+# 51 MB 18 -> 31 us, 101 MB 27 -> 36, 126 MB 29 -> 24 to 36 -> 49, 201 MB 41 -> 40, 252 MB 47 -> 30 to 53 ->
+# 53, 528 MB 90 -> 43, 2.1 GB 310 -> 57 (32 query heads of 64 or 64 of 128, on 4 and 8, 2 to 64 sequences); in 32 bits,
+# bound by arithmetic, 503 MB 121 -> 198, 1.0 GB 137 -> 162 to 230 -> 141, 2.1 GB 275 -> 172.
+SHARED_BYTES = {2: 200e6, 4: 1e9}
 
 
 class PagedKVCache:
@@ -64,7 +73,9 @@ class PagedKVCache:
         self.groups = self.prefix = None             # sequences that share pages (fork), of the next two
         self._groups, self._prefix = torch.zeros(batch + 1, **i32), torch.zeros(batch, **i32)
         self._spans = torch.zeros(batch + 1, **i32)  # groups without those that share nothing
-        self._host_spans: List[int] = []
+        self._host_spans, self._host_prefix = [0, batch], [0] * batch
+        self._saved = {}                             # by window: bytes that sharing saves a call, as it stands
+        self.shared_bytes = SHARED_BYTES[dtype.itemsize]
         self.weights = self.pos = None
         if budget is not None:
             tables = (batch, H_kv, self.max_pages * page_size)
@@ -93,6 +104,7 @@ class PagedKVCache:
 
     def _publish(self, rows: Sequence[int]) -> None:
         """Copies the host's lengths and what changed in the page table's given rows to the device."""
+        self._saved = {}
         self._to_device(self.lengths, self.host_lengths)
         self._to_device(self.seen, self.host_seen)
         self._to_device(self.queried, [n if g else 0 for n, g in zip(self.host_lengths, self._grew)])
@@ -107,6 +119,7 @@ class PagedKVCache:
         """Publishes the groups that share pages. What sequences share changes when one is forked or
         released: a page that one grows into is its own, so its prefix stays what it is."""
         groups, prefix = self.shared_groups()
+        self._saved = {}
         if not any(prefix):  # nobody shares, or no neighbours do
             self.groups = self.prefix = None
             return
@@ -116,6 +129,7 @@ class PagedKVCache:
         # What attend passes: a group that shares nothing joins the one before it, or those before the first
         # that shares are one, since a call of many groups does not cut their prefixes up.
         self._host_spans = [0, *(b for b in groups[1:-1] if prefix[b]), self.batch]
+        self._host_prefix = prefix
         self._to_device(self._spans[:len(self._host_spans)], self._host_spans)
 
     def _shares(self, b: int) -> bool:
@@ -157,6 +171,17 @@ class PagedKVCache:
                 prefix[b] = same * self.page_size
                 prefix[lead] = max(prefix[lead], prefix[b])
         return groups + [self.batch], prefix
+
+    def _shared_call_pays(self, window: int) -> bool:
+        """Whether reading the shared pages once for the sequences that grew last saves so much."""
+        if window not in self._saved:
+            n, slots = [x if g else 0 for x, g in zip(self.host_lengths, self._grew)], 0
+            for a, b in zip(self._host_spans, self._host_spans[1:]):
+                seen = [max(0, min(self._host_prefix[s], n[s]) - (max(0, n[s] - window) if window else 0))
+                        for s in range(a, b)]
+                slots += sum(seen) - max(seen)
+            self._saved[window] = slots * 2 * self.H_kv * self.D * self.dtype.itemsize
+        return self._saved[window] >= self.shared_bytes
 
     def _resize(self, b: int, length: int) -> bool:
         """Gives sequence b the pages of `length` slots; True if they changed."""
@@ -284,8 +309,9 @@ class PagedKVCache:
     def attend(self, layer: int, q: torch.Tensor, *, window: int = 0) -> torch.Tensor:
         """O ``[batch, H, D]`` of one query row per sequence over the layer's cached slots; with a
         budget the slots' attention weights are accumulated. A sequence that reserved no token last
-        gets zeros and accumulates nothing. Pages that neighbouring sequences share are read once."""
-        if self.groups is not None:
+        gets zeros and accumulates nothing. Pages that neighbouring sequences share are read once where that
+        saves ``shared_bytes``."""
+        if self.groups is not None and self._shared_call_pays(window):
             return paged_shared_attention(q, self.k[layer], self.v[layer], self.page_table, self.queried,
                                           self._spans[:len(self._host_spans)], self.prefix, window=window)
         if self.budget is not None and self._provisional:

@@ -226,6 +226,7 @@ def test_sequences_before_the_first_that_shares_are_one_span(gone, spans, monkey
     got = []
     monkeypatch.setattr(paged_cache, "paged_shared_attention", lambda *a, **kw: got.append(a))
     c = _forked(64)
+    c.shared_bytes = 0
     for b in gone:
         c.release(b)
     c.attend(0, torch.zeros(64, 2, 64))
@@ -239,6 +240,7 @@ def test_spans_of_several_prefixes(monkeypatch):
     got = []
     monkeypatch.setattr(paged_cache, "paged_shared_attention", lambda *a, **kw: got.append(a[5].tolist()))
     c = _cache(batch=9, pages=200, max_slots=64)
+    c.shared_bytes = 0
     c.reserve([9, 0, 32, 0, 16, 0, 0, 24, 0])
     c.fork(2, [3])
     c.fork(4, [6])  # 5 waits
@@ -247,3 +249,38 @@ def test_spans_of_several_prefixes(monkeypatch):
     c.release(4)  # 6 shares with nobody
     c.attend(0, torch.zeros(9, 2, 64))
     assert got == [[0, 2, 4, 7, 9], [0, 2, 7, 9]]
+
+
+def test_the_shared_call_is_taken_where_it_saves_enough(monkeypatch):
+    """2 KV heads of 64 in fp32: 1024 bytes a slot; 32 shared slots of each sequence but one."""
+    import torch
+    from dcr_b200 import paged_cache
+    got = []
+    monkeypatch.setattr(paged_cache, "paged_shared_attention", lambda *a, **kw: got.append("shared"))
+    monkeypatch.setattr(paged_cache, "paged_attention", lambda *a, **kw: got.append("plain"))
+    c, q = _forked(9), torch.zeros(9, 2, 64)
+
+    def call(window=0):
+        c.attend(0, q, window=window)
+        return got.pop()
+    assert c.shared_bytes == 1e9 and _cache(dtype=torch.float16).shared_bytes == 2e8
+    c.reserve([1] * 9)
+    assert call() == "plain"
+    c.shared_bytes = 8 * 32 * 1024
+    assert call() == "shared"
+    assert call(33) == "shared" and call(32) == "plain" and call(1) == "plain" and call(1000) == "shared"
+    c.reserve([1] * 8 + [0])           # the last one waits
+    assert call() == "plain"
+    c.shared_bytes = 7 * 32 * 1024
+    assert call() == "shared" and call(34) == "shared" and call(33) == "plain"
+    c.reserve([0] + [1] * 8)           # the first one does
+    assert call() == "shared"
+    c.release(0)
+    assert call() == "shared"
+    c.release(4)
+    assert call() == "plain"
+    c.shared_bytes = 6 * 32 * 1024
+    assert call() == "shared"
+    for b in (1, 2, 3, 5, 6, 7):
+        c.release(b)
+    assert c.groups is None and call() == "plain"
