@@ -113,3 +113,15 @@ def test_more_groups_than_weights_are_kept_of():
     """Groups of one, most of which wait."""
     B = 700
     _check_idle([1] * B, [48] * B, [3] * B, [b for b in range(B) if b % 7], 1, 1, 16, 64, torch.bfloat16, seed=5)
+
+
+@pytest.mark.parametrize("dt,groups,D", [("bf16", 24, 64), ("f16", 40, 128), ("bf16", 70, 64), ("f32", 80, 64)])
+@pytest.mark.parametrize("window", [0, 200])
+def test_more_units_than_are_cut_up(dt, groups, D, window):
+    """Groups times KV heads past the SMs (four times past them in fp32): a CTA a unit, a place a row; up to 64
+    groups by what they see, more in their order."""
+    members = [1 + g % 3 for g in range(groups)]
+    B = sum(members)
+    idle = [b for b in range(B) if b % 11 == 4]
+    _check_idle(members, [16 * (1 + g * 7 % 30) for g in range(groups)], [1 + b % 40 for b in range(B)], idle, 16, 8,
+                16, D, DT[dt], window=window, seed=6)
