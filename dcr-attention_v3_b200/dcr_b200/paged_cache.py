@@ -243,7 +243,8 @@ class PagedKVCache:
     def fork(self, b: int, others: Sequence[int]) -> None:
         """Gives the empty sequences ``others`` what sequence b holds: its full pages are shared, the
         last one, if it is not full, is copied. A page goes back to the pool with the last sequence
-        that holds it. Refuses, changing nothing, where the pool runs out of pages."""
+        that holds it. What was reserved last has to be appended in every layer before. Refuses, changing
+        nothing, where the pool runs out of pages."""
         require(self.budget is None, "a cache with a budget shares no pages")
         require(0 <= b < self.batch and self.host_lengths[b] > 0, f"sequence {b} holds nothing")
         require(len(set(others)) == len(others) and

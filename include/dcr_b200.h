@@ -472,10 +472,10 @@ size_t dcr_paged_prefill_workspace_bytes(int dtype, int T, int B, int H, int H_k
  * lengths[b] - n + i (causal != 0; else all lengths[b]) and, with window > 0 (causal only), of these
  * the last `window`. O [T, H, D] and lse [T, H] (or NULL) as dcr_paged_attend, with fp32 statistics
  * and sums; in bf16 and f16 the weights enter the second product rounded to 16 bits. Rows of q that
- * belong to no sequence are not touched in O and lse; a token before the sequence's first slot (n >
- * lengths[b]) sees nothing and gets 0 and -inf. A value that is not finite spoils elements of the rows
- * that see it (all of them, or its own only), and no other rows. O may be q itself where q is contiguous, else it shares no memory
- * with it. */
+ * belong to no sequence are not touched in O and lse. With causal a token before the sequence's first
+ * slot (n > lengths[b]) sees nothing and gets 0 and -inf; without it sees all slots, as the others do.
+ * A value that is not finite spoils elements of the rows that see it (all of them, or its own only),
+ * and no other rows. O may be q itself where q is contiguous, else it shares no memory with it. */
 int dcr_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_pages,
                       const void* v_pages, int dtype, int64_t k_stride_p, int64_t k_stride_h,
                       int64_t k_stride_s, int64_t v_stride_p, int64_t v_stride_h,
