@@ -28,9 +28,9 @@
 // a CTA's beginning and end 14000): 2048 tokens on 32768 slots, 32 heads of 128 on 8, f16 (1.13 TFLOP):
 // 1.03 to 1.16 ms by the card's power, 0.98 to 1.1 PFLOP/s; six prompts of 740 to 8192 tokens, heads of
 // 64, bf16 (0.66 TFLOP): 1.10 ms, 600 TFLOP/s; 48 sequences of 2 to 5 drafted tokens, window 8191, f16
-// (556 MB): 139 us, 4.0 TB/s; 18 sequences of 5 tokens on 16000 slots, heads of 128 (1.2 GB): 178 us, 6.6
-// TB/s; 45 samples of three documents of 7700 to 32768 slots, 64 heads of 128 on 8, f16 (398 MB): 109 us;
-// three prompts of 236 to 1499 slots in fp32: 237 us, 25 TFLOP/s.
+// (556 MB): 136 us, 4.1 TB/s; sequences of 5 tokens on 16000 slots, heads of 128, 8 of them 95 us, 9 (72
+// CTAs) 135, 18 (a full wave, 1.2 GB) 178, 19 309; 45 samples of three documents of 7700 to 32768 slots, 64
+// heads of 128 on 8, f16 (398 MB): 108 us; three prompts of 236 to 1499 slots in fp32: 237 us, 25 TFLOP/s.
 // Tried and not kept: a whole tile's scores at once (1264 us for the six prompts, each step waits for
 // its scores then; in halves 1256, before K and V came by the tensor map); the next half's scores loaded
 // before this one's exponentials (1427 instead of 1221); an eighth, a quarter or a third of the
@@ -567,9 +567,15 @@ __global__ void __launch_bounds__(kRfThreads) rows_fma_kernel(const RowsParams p
 // The base is raised only when a row's score is 8 above the largest it was set by, so O is rescaled
 // for few steps, and then when the product of the step before is done. In f16 the base stays 7 below the
 // maximum, so that small weights keep their bits (2^-24 of 2^7). A weight enters the second product
-// rounded to 16 bits, which is off by half a step at most, as the output's own rounding, and averages
-// out over the slots (errors against 64 bits as those of fp32 weights to 5%); with Parts = 2, for
-// shared prefixes, which are bound by their loads, its remainder goes in as well, in a second product.
+// rounded to 16 bits, off by half a step at most, as the output's own rounding. Errors against 64 bits are
+// 1.02 to 1.06 times those of fp32 weights for the prompts above, and the square root of 2 times where a row's
+// weights are alike and its values have no mean, so that both errors are as large (1200 tokens on 2048 to
+// 32768 slots: f16 0.00029 instead of 0.00021, bf16 0.00235 instead of 0.00166). With Parts = 2 a weight's
+// remainder goes in as well, in a second product: for shared prefixes, which are bound by their loads. Prompts
+// would take 4 to 25% longer (the six 1278 us, the chunk 1246, the drafted tokens 146) for the errors of fp32
+// weights, but for the chunk, whose error is that of its sums. Those are of 32 bits and lose a little with each
+// product of 16 slots, as if truncated: a row's output is 3.5e-5 of itself too small behind 32768 slots, and
+// 1.3e-4 behind 131072.
 // ---------------------------------------------------------------------------------------
 constexpr int kTcSlots = 128;
 
@@ -1228,7 +1234,10 @@ static RowsPlan rows_plan(int dtype, int T, int nseg, int H_kv, int G, bool shar
   // every segment adds one tile of rows at most that is not full
   const int64_t units = (rows / r.bm + (nseg < rows ? nseg : rows)) * H_kv;
   // Units are cut up where the grid has more than one CTA for each; fp32 ones, whose longest would set the
-  // pace (a tile takes 4 us), up to 4 CTAs an SM.
+  // pace (a tile takes 4 us), up to 4 CTAs an SM. A 16-bit prompt's where it has two: with fewer most units
+  // stay whole, and the call pays for parts and join (10 to 16 sequences on 16000 slots, 8 KV heads of 64: 124 us
+  // whole, 129 cut; on 2000 slots 23 and 27; 9 sequences, whose units are counted as 80 and are 72, would
+  // gain: 125 whole, 75 cut).
   const int64_t slots = static_cast<int64_t>(tc ? 1 : 4) * device_sm_count();
   r.pieces = units <= slots && (shared || !tc || 2 * units <= slots) ? static_cast<int>(slots) : 0;
   r.units = units;

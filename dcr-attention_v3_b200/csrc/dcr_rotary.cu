@@ -19,8 +19,10 @@
 // turned, a sixth of the memory's rate).
 // Measured (in a CUDA graph): 16381 tokens of 32 + 8 heads of 128, f16 (336 MB): 54.3 us, 6.2 TB/s; the
 // same with the values of 8 more heads into pages, norms, and 96 elements of each head turned in
-// neighbouring pairs, bf16 (403 MB): 97 us, 4.2 TB/s (whole heads in halves: 89), bound by instructions and
-// the five to seven CTAs that fit an SM; 48 tokens: 2.2 and 4.3 us. With items found by divisions and
+// neighbouring pairs, bf16 (403 MB): 97 us, 4.2 TB/s (whole heads in halves: 91), bound by instructions: the
+// place, angle, weight and pair of each row part are worked out by itself. The append by tables, whose warps hold
+// angle and weight as two factors for all rows of a token, takes 68 us for whole heads in halves. 48 tokens: 2.2
+// and 4.3 us. With items found by divisions and
 // arithmetic that is not packed these took 75 and 121 us; loading each item's successor as soon as it
 // was used (95 registers) 59 and 106; six items in flight 62 and 127.
 #include <type_traits>
