@@ -1125,8 +1125,8 @@ __global__ void __launch_bounds__(RowsTc<D, Twin>::kThreads, 1) rows_tc_kernel(c
       fence_proxy_async_smem();
       mbar_arrive(&sh.q_full);
       // a row that sees nothing begins at a base that no score is above, so that it raises none of its warp's
-      const int2 lim = sh.limits[tid % 128 + (Twin ? 0 : tid / 128 * 128)];
-      const bool blind = lim.x >= lim.y;
+      const int r = tid % 128 + (Twin ? 0 : tid / 128 * 128);
+      const bool blind = r < u.rows && sh.limits[r].x >= sh.limits[r].y;
       float2 state = make_float2(blind ? INFINITY : -INFINITY, 0.0f);
       const bool fine = rows_tc_softmax<T, D, Twin, Parts>(p, sh, tiles, scale2, state);
       if (blind) state = make_float2(-INFINITY, 0.0f);
