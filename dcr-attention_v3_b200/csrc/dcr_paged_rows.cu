@@ -143,8 +143,9 @@ constexpr int kRowsMinPart = 4;  // tiles of 128 slots: smaller parts gain nothi
 
 // Finds this CTA's rows and their limits. A unit is a KV head's tile of BM rows of a segment. Where
 // units are many (pieces = 0) blockIdx.x is one: heads of a tile side by side, a segment's tiles from the
-// last to the first, since a causal segment's last rows see most, and segments (of up to 64) from the
-// one that sees most on, so that the grid ends on short units. Else units are cut into parts of at most
+// last to the first, since a causal segment's last rows see most, and segments from the one that sees
+// most on, so that the grid ends on short units (up to 64 segments, two a lane; the units of more are so many
+// that the grid's end is a small part of it). Else units are cut into parts of at most
 // a number of slots, the least for which all parts are no more than the grid. False: nothing to do.
 template <int BM>
 __device__ __forceinline__ bool rows_begin(const RowsParams& p, RowsUnit& u, int2* limits) {

@@ -326,9 +326,11 @@ class PagedKVCache:
               provisional: Sequence[int] = ()) -> None:
         """Accumulates the attention weights of one query row per sequence over its first
         ``lengths[b]`` slots (int32 on the device; 0: none) in the layer's table, and nothing else. Those
-        of ``provisional`` sequences can be taken back until they attend or an eviction goes by them
-        (:meth:`withdraw`)."""
+        of ``provisional`` sequences can be taken back (:meth:`withdraw`) until they attend, an eviction
+        goes by them or others are accumulated that cannot."""
         require(self.budget is not None, "this cache has no budget")
+        if not provisional:
+            self._provisional.clear()
         for b in provisional:
             self._provisional.setdefault(b, {})[layer] = self.weights[layer][b].clone()
         paged_attention(q, self.k[layer], self.v[layer], self.page_table, lengths,

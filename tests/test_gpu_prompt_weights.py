@@ -79,6 +79,18 @@ def test_a_sequence_in_the_range_is_evicted_by_its_last_token():
             assert kept == {0, 28, 29} | {1 + x for x in order[:21]}
 
 
+def test_other_weights_settle_what_was_provisional():
+    from dcr_b200.models.llama.paged import PagedLlamaDecoder
+    paged = PagedLlamaDecoder(_model(), max_positions=256)
+    cache = _feed(paged, (20,))
+    q = torch.randn(2, 4, 128, device=DEV)[..., :cache.D].contiguous()
+    for i in range(2):
+        cache.weigh(i, q, torch.tensor([30, 0], dtype=torch.int32, device=DEV))
+    paged.prefill([[3], []], cache)
+    for i in range(2):  # the last token's, these and the new last token's
+        assert (cache.weights[i][0, :, :31].sum() - 4 * 3).abs() < 1e-3
+
+
 def test_refused_chunks_take_nothing_back():
     from dcr_b200.models.llama.paged import PagedLlamaDecoder
     paged = PagedLlamaDecoder(_model(), max_positions=256)
